@@ -108,6 +108,20 @@ def _declare(L):
                                          vp, vp, vp, vp, vp, vp]),
         "bc2n_structure_heads_bwd": (i, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i, c.c_int64,
                                          c.c_int64, cs, vp, vp]),
+        "bc2n_logprobs_save_bytes": (sz, [c.c_int64]),
+        "bc2n_logprobs_work_bytes": (sz, [i, c.c_int64, i, i]),
+        "bc2n_logprobs_fwd": (i, [vp, i, vp, c.c_int64, c.c_int64, i, vp, i, i] + [vp] * 6),
+        "bc2n_logprobs_bwd": (i, [vp, i, vp, c.c_int64, c.c_int64, i, vp, i, i] + [vp] * 6
+                              + [c.c_int64]),
+        "bc2n_logprobs_grad": (i, [vp, i, vp, c.c_int64, c.c_int64, i, vp, i] + [vp] * 5
+                               + [c.c_int64, vp]),
+        "bc2n_grad_list": (vp, [i, vp, vp, vp, vp]),
+        "bc2n_adam_list": (vp, [i] + [vp] * 10),
+        "bc2n_list_free": (i, [vp]),
+        "bc2n_list_work_bytes": (sz, [vp]),
+        "bc2n_grad_norm": (i, [vp, vp, vp, vp]),
+        "bc2n_grad_clip": (i, [vp, vp, f, vp, vp]),
+        "bc2n_adam_step": (i, [vp, vp] + [c.c_double] * 5 + [c.c_int64, c.c_double, vp, vp, vp]),
         "bc2n_dropout_table": (i, [vp, vp, i, i, u32, u32, f]),
         "bc2n_bernoulli_bits": (i, [vp, vp, c.c_long, u32, u32, f]),
         "bc2n_stack_keys": (i, [vp, vp, i, vp]),

@@ -9,7 +9,10 @@
 #include "heads.h"
 #include "designstep.h"
 #include "confidence.h"
+#include "logprobs.h"
+#include "optim.h"
 
+#include <cmath>
 #include <cstdio>
 #include <map>
 #include <tuple>
@@ -1142,6 +1145,218 @@ int bc2n_confidence_bwd(void* stream, const float* plddt_logits, const float* pa
     confidence_bwd(as_stream(stream), plddt_logits, pae_logits, expres_logits, seq_mask,
                    interface_asym, N, save, d_plddt, d_pae, d_ptm, d_iptm, d_iptm_per_residue,
                    d_expres_ca, d_plddt_logits, d_pae_logits, d_expres_logits);
+  });
+}
+
+namespace {
+LogProbs lp_operands(int dtype, const void* logits, int64_t ld, int64_t rows, int classes,
+                     const void* targets, int target_bits) {
+  need(dtype == BC2N_F32 || dtype == BC2N_F16 || dtype == BC2N_BF16, "logprobs: bad dtype");
+  need(rows >= 0 && rows < (int64_t(1) << 31), "logprobs: bad number of rows");
+  need(classes > 0 && classes <= (1 << 28), "logprobs: bad number of classes");
+  need(ld >= classes, "logprobs: the row stride is below the number of classes");
+  need(!targets || target_bits == 32 || target_bits == 64, "logprobs: targets are i32 or i64");
+  need(rows == 0 || logits, "null operand");
+  LogProbs a;
+  a.dtype = dtype;
+  a.x = logits;
+  a.ld = ld;
+  a.rows = rows;
+  a.V = classes;
+  a.target = targets;
+  a.target64 = target_bits == 64;
+  return a;
+}
+void lp_top(LogProbs& a, int top) {
+  need(top >= 0 && top <= LP_MAX_TOP && top <= a.V,
+       "logprobs: top must be 0..32 and at most the number of classes");
+  a.K = top;
+}
+void lp_gradient(LogProbs& a, void* d_logits, int64_t d_ld) {
+  need(a.rows == 0 || d_logits, "null output");
+  need(d_ld >= a.V, "logprobs: the gradient's row stride is below the number of classes");
+  need(d_logits != a.x || d_ld == a.ld, "logprobs: a gradient in place has the logits' row stride");
+  a.d = d_logits;
+  a.d_ld = d_ld;
+}
+TensorList& list_of(void* list) {
+  TensorList* l = reinterpret_cast<TensorList*>(list);
+  need(l && l->magic == TensorList::MAGIC, "list: not a list of tensors");
+  return *l;
+}
+bool known_type(int t) { return t == BC2N_F32 || t == BC2N_F16 || t == BC2N_BF16; }
+}  // namespace
+
+size_t bc2n_logprobs_save_bytes(int64_t rows) { return rows > 0 ? (size_t)rows * 16 : 0; }
+
+size_t bc2n_logprobs_work_bytes(int dtype, int64_t rows, int classes, int top) {
+  size_t n = 0;
+  guarded([&] {
+    LogProbs a = lp_operands(dtype, &n, classes, rows, classes, nullptr, 0);
+    lp_top(a, top);
+    n = logprobs_work_bytes(dtype, rows, classes, top);
+  });
+  return n;
+}
+
+int bc2n_logprobs_fwd(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows,
+                      int classes, const void* targets, int target_bits, int top, float* logp,
+                      float* entropy, float* top_logp, int32_t* top_index, void* save,
+                      void* work) {
+  return guarded([&] {
+    LogProbs a = lp_operands(dtype, logits, ld, rows, classes, targets, target_bits);
+    lp_top(a, top);
+    need(!logp || targets, "logprobs: logp needs targets");
+    need(top == 0 || rows == 0 || (top_logp && top_index), "null output");
+    need(work || logprobs_work_bytes(dtype, rows, classes, top) == 0, "logprobs: null work");
+    a.logp = logp;
+    a.entropy = entropy;
+    a.top_logp = top_logp;
+    a.top_index = top_index;
+    a.save = reinterpret_cast<float*>(save);
+    logprobs_fwd(as_stream(stream), a, work);
+  });
+}
+
+int bc2n_logprobs_bwd(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows,
+                      int classes, const void* targets, int target_bits, int top,
+                      const int32_t* top_index, const void* save, const float* d_logp,
+                      const float* d_entropy, const float* d_top_logp, void* d_logits,
+                      int64_t d_ld) {
+  return guarded([&] {
+    LogProbs a = lp_operands(dtype, logits, ld, rows, classes, targets, target_bits);
+    lp_top(a, top);
+    lp_gradient(a, d_logits, d_ld);
+    need(rows == 0 || save, "null operand");
+    need(!d_logp || targets, "logprobs: d_logp needs targets");
+    need(!d_top_logp || (top > 0 && top_index), "logprobs: d_top_logp needs top_index");
+    a.top_index = const_cast<int32_t*>(top_index);
+    a.save = reinterpret_cast<float*>(const_cast<void*>(save));
+    a.d_logp = d_logp;
+    a.d_entropy = d_entropy;
+    a.d_top = d_top_logp;
+    logprobs_bwd(as_stream(stream), a);
+  });
+}
+
+int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows,
+                       int classes, const void* targets, int target_bits, const float* d_logp,
+                       const float* d_entropy, float* logp, float* entropy, void* d_logits,
+                       int64_t d_ld, void* work) {
+  return guarded([&] {
+    LogProbs a = lp_operands(dtype, logits, ld, rows, classes, targets, target_bits);
+    lp_gradient(a, d_logits, d_ld);
+    need((!logp && !d_logp) || targets, "logprobs: logp needs targets");
+    need(work || logprobs_work_bytes(dtype, rows, classes, 0) == 0, "logprobs: null work");
+    a.logp = logp;
+    a.entropy = entropy;
+    a.d_logp = d_logp;
+    a.d_entropy = d_entropy;
+    logprobs_grad(as_stream(stream), a, work);
+  });
+}
+
+void* bc2n_grad_list(int count, const void* const* grads, const int64_t* sizes, const int* dtypes,
+                     void* const* out) {
+  TensorList* l = nullptr;
+  guarded([&] {
+    need(count >= 0 && (count == 0 || (grads && sizes && dtypes)), "list: null operand");
+    std::vector<ListEntry> e((size_t)count);
+    for (int i = 0; i < count; ++i) {
+      need(known_type(dtypes[i]), "list: bad dtype");
+      e[i].g = grads[i];
+      e[i].n = sizes[i];
+      e[i].g_type = dtypes[i];
+      if (out) {
+        need(out[i] || sizes[i] == 0, "list: null output");
+        e[i].g_out = out[i];
+      }
+    }
+    l = new TensorList(std::move(e), out != nullptr, false);
+  });
+  return l;
+}
+
+void* bc2n_adam_list(int count, const int64_t* sizes, const void* const* params,
+                     const int* param_dtypes, const void* const* grads, const int* grad_dtypes,
+                     const float* const* avg, const float* const* avg_sq, void* const* params_out,
+                     float* const* avg_out, float* const* avg_sq_out) {
+  TensorList* l = nullptr;
+  guarded([&] {
+    need(count >= 0 && (count == 0 || (sizes && params && param_dtypes && grads && grad_dtypes &&
+                                       avg && avg_sq && params_out && avg_out && avg_sq_out)),
+         "list: null operand");
+    std::vector<ListEntry> e((size_t)count);
+    for (int i = 0; i < count; ++i) {
+      need(known_type(param_dtypes[i]) && known_type(grad_dtypes[i]), "list: bad dtype");
+      e[i].n = sizes[i];
+      e[i].g = grads[i];
+      e[i].g_type = grad_dtypes[i];
+      e[i].p = params[i];
+      e[i].p_type = param_dtypes[i];
+      e[i].m = avg[i];
+      e[i].v = avg_sq[i];
+      e[i].p_out = params_out[i];
+      e[i].m_out = avg_out[i];
+      e[i].v_out = avg_sq_out[i];
+    }
+    l = new TensorList(std::move(e), false, true);
+  });
+  return l;
+}
+
+int bc2n_list_free(void* list) {
+  return guarded([&] {
+    if (list) delete &list_of(list);
+  });
+}
+
+size_t bc2n_list_work_bytes(void* list) {
+  size_t n = 0;
+  guarded([&] { n = list_of(list).work_bytes(); });
+  return n;
+}
+
+int bc2n_grad_norm(void* stream, void* list, float* norm, void* work) {
+  return guarded([&] {
+    TensorList& l = list_of(list);
+    need(norm && work, "null operand");
+    grad_norm(as_stream(stream), l, norm, work);
+  });
+}
+
+int bc2n_grad_clip(void* stream, void* list, float max_norm, float* norm, void* work) {
+  return guarded([&] {
+    TensorList& l = list_of(list);
+    need(l.clips, "grad_clip: the list has no outputs");
+    need(max_norm > 0.f, "grad_clip: max_norm must be positive");
+    need(work, "null operand");
+    grad_clip(as_stream(stream), l, max_norm, norm, work);
+  });
+}
+
+int bc2n_adam_step(void* stream, void* list, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, int64_t step, double max_norm, const float* scalars,
+                   float* norm, void* work) {
+  return guarded([&] {
+    TensorList& l = list_of(list);
+    need(l.adam, "adam_step: not a list of parameters");
+    need(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adam_step: betas must be in [0, 1)");
+    need(eps > 0, "adam_step: eps must be positive");
+    need(weight_decay >= 0, "adam_step: weight_decay must not be negative");
+    need(scalars || (step >= 1 && std::isfinite(lr)), "adam_step: step counts from 1, lr is finite");
+    need(max_norm >= 0, "adam_step: max_norm must be positive, or 0 for none");
+    need(work, "null operand");
+    AdamScalars s;
+    s.lr = lr;
+    s.beta1 = beta1;
+    s.beta2 = beta2;
+    s.eps = eps;
+    s.decay = weight_decay;
+    s.step = step;
+    s.max_norm = max_norm;
+    s.device = scalars;
+    adam_step(as_stream(stream), l, s, norm, work);
   });
 }
 

@@ -745,6 +745,252 @@ class Confidence:
         return d
 
 
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # BC2N_F32, _F16, _BF16
+
+
+def _current(t, what):
+    """t on the device that the calls go to: the current one."""
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: expected a tensor on the current device, got {t.device}")
+    return t
+
+
+class LogProbs:
+    """Log-probabilities of given classes, entropies and the `top` most likely
+    classes of rows of logits, and their gradient (bc2n_logprobs_*).
+
+    logits [..., classes] f32, f16 or bf16, any row stride; targets [...] i32
+    or i64 with a negative one for a row to leave out (its outputs and gradient
+    are zero whatever its logits hold), or None for entropies and alternatives
+    alone.  Outputs are f32, top_index i32 (-1 where there is none)."""
+
+    def __init__(self, top=0):
+        if not 0 <= top <= 32:
+            raise ValueError("top must be 0..32")
+        self.top = int(top)
+
+    @staticmethod
+    def _rows(t, what):
+        """(tensor, its row stride) of [..., classes] as rows."""
+        if t.dim() == 0 or t.dtype not in _DTYPES:
+            raise ValueError(f"{what}: expected float32, float16 or bfloat16 [..., classes], got "
+                             f"{t.dtype} {tuple(t.shape)}")
+        _current(t, what)
+        v = t.shape[-1]
+        if t.is_contiguous():
+            return t, v
+        if t.dim() > 2:
+            try:
+                t = t.view(-1, v)
+            except RuntimeError:
+                raise ValueError(f"{what}: the leading dimensions have no one stride") from None
+        if t.stride(-1) != 1 and v > 1:
+            raise ValueError(f"{what}: a row's elements must be contiguous")
+        return t, (t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else v)
+
+    def _operands(self, logits, targets):
+        x, ld = self._rows(logits, "logits")
+        v, lead = logits.shape[-1], logits.shape[:-1]
+        rows = logits.numel() // v if v else 0
+        bits = 32
+        if targets is not None:
+            if targets.dtype not in (torch.int32, torch.int64) or targets.shape != lead:
+                raise ValueError(f"targets: expected int32 or int64 {tuple(lead)}, got "
+                                 f"{targets.dtype} {tuple(targets.shape)}")
+            bits = 64 if targets.dtype == torch.int64 else 32
+            _current(targets, "targets")
+        return (_DTYPES[x.dtype], x.data_ptr(), ld, rows, v, _ptr(targets), bits), rows, v, lead
+
+    @staticmethod
+    def _cotangent(t, shape, what):
+        if t is not None:
+            _f32(t, shape, what)
+            _current(t, what)
+        return _ptr(t)
+
+    @staticmethod
+    def _work(code, rows, v, top, device):
+        n = lib().bc2n_logprobs_work_bytes(code, rows, v, top)
+        return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+    def _gradient(self, logits, out):
+        if out is None:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if out.dtype != logits.dtype or out.shape != logits.shape:
+            raise ValueError(f"out: expected {logits.dtype} {tuple(logits.shape)}, got {out.dtype} "
+                             f"{tuple(out.shape)}")
+        o, ld = self._rows(out, "out")
+        return out, o.data_ptr(), ld
+
+    def forward(self, logits, targets=None):
+        """-> ((logp, entropy, top_logp, top_index), save); logp is None without
+        targets, the last two with top=0."""
+        operands, rows, v, lead = self._operands(logits, targets)
+        dev = logits.device
+        e = lambda *sh: torch.empty(*sh, dtype=torch.float32, device=dev)
+        logp = e(lead) if targets is not None else None
+        entropy, save = e(lead), e(rows, 4)
+        top_logp = e(*lead, self.top) if self.top else None
+        top_index = torch.empty(*lead, self.top, dtype=torch.int32, device=dev) if self.top else None
+        work = self._work(operands[0], rows, v, self.top, dev)
+        check(lib().bc2n_logprobs_fwd(_stream(), *operands, self.top, _ptr(logp), _ptr(entropy),
+                                      _ptr(top_logp), _ptr(top_index), _ptr(save), _ptr(work)))
+        return (logp, entropy, top_logp, top_index), save
+
+    def backward(self, cts, logits, targets, top_index, save, out=None):
+        """cts = (d_logp, d_entropy, d_top_logp), any None -> d_logits (in `out`
+        where given, which may be logits itself)"""
+        operands, rows, v, lead = self._operands(logits, targets)
+        if tuple(save.shape) != (rows, 4):
+            raise ValueError(f"save: expected the forward's of {rows} rows, got {tuple(save.shape)}")
+        if top_index is not None and (top_index.dtype != torch.int32
+                                      or tuple(top_index.shape) != (*lead, self.top)):
+            raise ValueError(f"top_index: expected int32 {(*lead, self.top)}")
+        c = [self._cotangent(t, sh, n) for t, sh, n in zip(
+            cts, (lead, lead, (*lead, self.top)), ("d_logp", "d_entropy", "d_top_logp"))]
+        out, o, ld = self._gradient(logits, out)
+        check(lib().bc2n_logprobs_bwd(_stream(), *operands, self.top, _ptr(top_index), _ptr(save),
+                                      *c, o, ld))
+        return out
+
+    def value_and_grad(self, logits, targets, d_logp=None, d_entropy=None, out=None):
+        """((logp, entropy), d_logits) in one call, for cotangents known
+        beforehand (a likelihood with given weights); no alternatives."""
+        operands, rows, v, lead = self._operands(logits, targets)
+        dev = logits.device
+        c = [self._cotangent(t, lead, n) for t, n in ((d_logp, "d_logp"), (d_entropy, "d_entropy"))]
+        out, o, ld = self._gradient(logits, out)
+        logp = torch.empty(lead, dtype=torch.float32, device=dev) if targets is not None else None
+        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+        work = self._work(operands[0], rows, v, 0, dev)
+        check(lib().bc2n_logprobs_grad(_stream(), *operands, *c, _ptr(logp), _ptr(entropy), o, ld,
+                                       _ptr(work)))
+        return (logp, entropy), out
+
+
+class _TensorList:
+    """A list of the C ABI over tensors, which it keeps alive and takes to
+    stay where they are."""
+
+    def __init__(self, handle, tensors):
+        if not handle:
+            check(1)
+        self.handle, self.tensors = handle, tensors
+        self.device = next((t.device for t in tensors), torch.device("cuda"))
+        self.work_bytes = lib().bc2n_list_work_bytes(handle)
+
+    def __del__(self):
+        if getattr(self, "handle", None):
+            lib().bc2n_list_free(self.handle)
+            self.handle = None
+
+    @staticmethod
+    def _checked(tensors, like, what, dtypes):
+        tensors = list(tensors)
+        if len(tensors) != len(like):
+            raise ValueError(f"{what}: expected {len(like)} tensors, got {len(tensors)}")
+        for t, g in zip(tensors, like):
+            if t.shape != g.shape or t.dtype not in dtypes or not t.is_contiguous():
+                raise ValueError(f"{what}: expected a contiguous {tuple(g.shape)} of "
+                                 f"{', '.join(map(str, dtypes))}, got {t.dtype} {tuple(t.shape)}")
+            _current(t, what)
+        return tensors
+
+    @staticmethod
+    def _pointers(tensors):
+        return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+    @staticmethod
+    def _types(tensors):
+        return (ctypes.c_int * len(tensors))(*[_DTYPES[t.dtype] for t in tensors])
+
+    @staticmethod
+    def _sizes(tensors):
+        return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+
+    def _scratch(self):
+        if self.device.index is not None and self.device.index != torch.cuda.current_device():
+            raise ValueError(f"the list is on {self.device}, which is not the current device")
+        return (torch.empty(1, dtype=torch.float32, device=self.device),
+                torch.empty(self.work_bytes, dtype=torch.uint8, device=self.device))
+
+
+class GradientClip(_TensorList):
+    """The global 2-norm of a list of gradients (f32, f16 or bf16, contiguous),
+    and the gradients scaled to at most a given norm, into `out` or in place
+    (bc2n_grad_norm, bc2n_grad_clip).  Made once for tensors that stay where
+    they are; many tensors cost the launches of one."""
+
+    def __init__(self, grads, out=None):
+        grads = list(grads)
+        self._checked(grads, grads, "grads", tuple(_DTYPES))
+        out = grads if out is None else self._checked(out, grads, "out", tuple(_DTYPES))
+        for g, o in zip(grads, out):
+            if g.dtype != o.dtype:
+                raise ValueError(f"out: expected {g.dtype}, got {o.dtype}")
+        super().__init__(lib().bc2n_grad_list(len(grads), self._pointers(grads), self._sizes(grads),
+                                              self._types(grads), self._pointers(out)),
+                         [*grads, *out])
+
+    def norm(self):
+        """-> f32 [1] on the device"""
+        norm, work = self._scratch()
+        check(lib().bc2n_grad_norm(_stream(), self.handle, _ptr(norm), _ptr(work)))
+        return norm
+
+    def clip(self, max_norm):
+        """Scales by max_norm / norm where the norm is not below max_norm (a copy
+        into `out` elsewhere) -> the norm before, f32 [1] on the device"""
+        norm, work = self._scratch()
+        check(lib().bc2n_grad_clip(_stream(), self.handle, float(max_norm), _ptr(norm), _ptr(work)))
+        return norm
+
+
+class Adam(_TensorList):
+    """An Adam step with decoupled weight decay over lists of parameters and
+    gradients (f32, f16 or bf16, contiguous) and their f32 moments, in place or
+    into out = (params, exp_avg, exp_avg_sq) (bc2n_adam_step)."""
+
+    def __init__(self, params, grads, exp_avg, exp_avg_sq, out=None, betas=(0.9, 0.999), eps=1e-8,
+                 weight_decay=0.0):
+        params, f32 = list(params), (torch.float32,)
+        self._checked(params, params, "params", tuple(_DTYPES))
+        grads = self._checked(grads, params, "grads", tuple(_DTYPES))
+        avg = self._checked(exp_avg, params, "exp_avg", f32)
+        avg_sq = self._checked(exp_avg_sq, params, "exp_avg_sq", f32)
+        p2, a2, s2 = (params, avg, avg_sq) if out is None else out
+        p2 = self._checked(p2, params, "out", tuple(_DTYPES))
+        for p, o in zip(params, p2):
+            if p.dtype != o.dtype:
+                raise ValueError(f"out: expected {p.dtype}, got {o.dtype}")
+        a2 = self._checked(a2, params, "out", f32)
+        s2 = self._checked(s2, params, "out", f32)
+        self.betas, self.eps, self.weight_decay = tuple(map(float, betas)), float(eps), float(weight_decay)
+        ptr = self._pointers
+        super().__init__(lib().bc2n_adam_list(len(params), self._sizes(params), ptr(params),
+                                              self._types(params), ptr(grads), self._types(grads),
+                                              ptr(avg), ptr(avg_sq), ptr(p2), ptr(a2), ptr(s2)),
+                         [*params, *grads, *avg, *avg_sq, *p2, *a2, *s2])
+
+    def step(self, step, lr, max_norm=None, scalars=None):
+        """Step number `step` (from 1).  max_norm: the gradients clipped to that
+        global norm first -> their norm before, f32 [1] on the device (None
+        without).  scalars: f32 [2] on the device, lr and step in place of the
+        arguments."""
+        norm, work = self._scratch()
+        if max_norm is None:
+            norm = None
+        elif not max_norm > 0:
+            raise ValueError("max_norm must be positive")
+        if scalars is not None:
+            _f32(scalars, (2,), "scalars")
+            _current(scalars, "scalars")
+        check(lib().bc2n_adam_step(_stream(), self.handle, float(lr), *self.betas, self.eps,
+                                   self.weight_decay, int(step), float(max_norm or 0.0),
+                                   _ptr(scalars), _ptr(norm), _ptr(work)))
+        return norm
+
+
 def dropout_table(rows, channels, key, rate, device="cuda"):
     """[rows, channels] keep/keep_rate table from a JAX key (k0, k1)."""
     tbl = torch.empty(rows, channels, dtype=torch.float32, device=device)

@@ -607,6 +607,96 @@ int bc2n_confidence_bwd(void* stream, const float* plddt_logits, const float* pa
                         float* d_plddt_logits, float* d_pae_logits, float* d_expres_logits);
 
 /* ------------------------------------------------------------------------
+ * Log-probabilities of given classes (next to the confidence metrics: the
+ * likelihood terms of a design loss over distogram, PAE, pLDDT or sequence
+ * logits, and of any other categorical output).  No reference counterpart.
+ * logits [rows][classes] of BC2N_F32, BC2N_F16 or BC2N_BF16, row stride ld >=
+ * classes elements; targets i32 or i64 (target_bits) [rows] or NULL.  Per row
+ * x with target t, p = softmax(x):
+ *   logp = log p_t, entropy = -sum_j p_j log p_j, and for the `top` largest
+ *   logits (ties to the lowest class; top 0..32) top_index and top_logp =
+ *   log p, both [rows][top], in descending order.
+ * All outputs f32 (top_index i32); sums and statistics are f32.  logp and
+ * entropy may be NULL (not wanted).
+ *   - A negative target leaves its row out: its logits have no effect (they
+ *     may hold anything), its outputs and gradient are 0, its indices -1.
+ *   - A logit of -inf has probability 0 (a target there: logp -inf); a row of
+ *     -inf alone has log-probabilities -inf, entropy 0 and gradient 0.
+ *   - A NaN or +inf makes its row's outputs and gradient NaN, its indices -1.
+ *   - A target >= classes makes its row's logp and its gradient NaN.
+ * save (NULL: no backward follows) is bc2n_logprobs_save_bytes(rows) bytes,
+ * 16-byte aligned, written by fwd and read by bwd; work is a scratch buffer of
+ * bc2n_logprobs_work_bytes() bytes, 16-byte aligned, for the time of the call
+ * (NULL where that is 0; -- 0 with a message in bc2n_last_error() on bad
+ * arguments).
+ * bwd: cotangents d_logp [rows], d_entropy [rows], d_top_logp [rows][top]
+ * (any may be NULL; the last needs the forward's top_index) -> d_logits of
+ * the logits' type, row stride d_ld, rounded once; d_logits may be logits
+ * itself with d_ld = ld, and overlaps them in no other way.
+ * grad: forward and backward in one call for cotangents known beforehand
+ * (a weighted likelihood), the logits read once where a row stays on chip.
+ * ---------------------------------------------------------------------- */
+enum { BC2N_F32 = 0, BC2N_F16 = 1, BC2N_BF16 = 2 };
+size_t bc2n_logprobs_save_bytes(int64_t rows);
+size_t bc2n_logprobs_work_bytes(int dtype, int64_t rows, int classes, int top);
+int bc2n_logprobs_fwd(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows,
+                      int classes, const void* targets, int target_bits, int top, float* logp,
+                      float* entropy, float* top_logp, int32_t* top_index, void* save, void* work);
+int bc2n_logprobs_bwd(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows,
+                      int classes, const void* targets, int target_bits, int top,
+                      const int32_t* top_index, const void* save, const float* d_logp,
+                      const float* d_entropy, const float* d_top_logp, void* d_logits,
+                      int64_t d_ld);
+int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows,
+                       int classes, const void* targets, int target_bits, const float* d_logp,
+                       const float* d_entropy, float* logp, float* entropy, void* d_logits,
+                       int64_t d_ld, void* work);
+
+/* ------------------------------------------------------------------------
+ * Lists of gradients (the designed logits' of several states, a model's
+ * parameters'): global norm, clipping, and the Adam update that takes the
+ * clipped gradients.  No reference counterpart (the reference leaves them to
+ * its optimiser library).
+ * A list is made once for tensors that stay where they are, and holds their
+ * addresses, not their values: count tensors of sizes[i] >= 0 contiguous
+ * elements of BC2N_F32, BC2N_F16 or BC2N_BF16 (moments f32), aligned to one
+ * element.  An output may be its own input (in place); it shares memory with
+ * no other operand, which making the list checks.  Making a list of more than
+ * 32 non-empty tensors allocates and copies a table to the device, waiting for
+ * it (not under graph capture); a list outlives the graphs that captured its
+ * calls.  Freeing one makes no HIP call: its table goes to a later list.  NULL
+ * on error.
+ *   grad_list: grads, and `out` for their clipped values (NULL: norm only).
+ *   adam_list: parameters, gradients, first and second moments, and where the
+ *     updated ones go.
+ * Calls: norm f32[1] = sqrt(sum of all squares), summed in 64 bits in one
+ * order; work is bc2n_list_work_bytes() bytes, 16-byte aligned, for the time
+ * of the call.
+ *   grad_clip: out = g c, c = 1 where norm < max_norm, else max_norm / norm
+ *     (a norm that is NaN makes all of it NaN); norm may be NULL.
+ *   adam_step: with g the gradient times c (max_norm 0: not clipped),
+ *     m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
+ *     p' = p - lr (m' / (1 - beta1^step) / (sqrt(v' / (1 - beta2^step)) + eps)
+ *                  + weight_decay p)
+ *     in f32, rounded once; step counts from 1.  scalars, or NULL: f32[2] on
+ *     the device, lr and step in place of the arguments (a captured graph's
+ *     schedule).  norm (of the gradients before clipping) may be NULL.
+ * ---------------------------------------------------------------------- */
+void* bc2n_grad_list(int count, const void* const* grads, const int64_t* sizes, const int* dtypes,
+                     void* const* out);
+void* bc2n_adam_list(int count, const int64_t* sizes, const void* const* params,
+                     const int* param_dtypes, const void* const* grads, const int* grad_dtypes,
+                     const float* const* avg, const float* const* avg_sq, void* const* params_out,
+                     float* const* avg_out, float* const* avg_sq_out);
+int bc2n_list_free(void* list);
+size_t bc2n_list_work_bytes(void* list);
+int bc2n_grad_norm(void* stream, void* list, float* norm, void* work);
+int bc2n_grad_clip(void* stream, void* list, float max_norm, float* norm, void* work);
+int bc2n_adam_step(void* stream, void* list, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, int64_t step, double max_norm, const float* scalars,
+                   float* norm, void* work);
+
+/* ------------------------------------------------------------------------
  * Dropout with JAX's own bits.  tbl[b*C+c] = keep/keep_rate where
  * keep = jax.random.bernoulli(key, keep_rate, (B, C)), keep_rate =
  * float32(1) - float32(rate); key = (k0, k1) = jax.random.key_data(key).
