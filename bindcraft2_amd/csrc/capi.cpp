@@ -60,6 +60,10 @@ hipStream_t as_stream(void* s) {
   return st;
 }
 
+// For calls that use no library scratch: only their stream orders them, and
+// they record no event (which costs a short call as much as its launch).
+hipStream_t own_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
+
 // after a call: mark the end of its work on its stream
 void end_call() {
   if (!t_call_has_stream) return;
@@ -1184,6 +1188,9 @@ TensorList& list_of(void* list) {
   need(l && l->magic == TensorList::MAGIC, "list: not a list of tensors");
   return *l;
 }
+void list_work(const TensorList& l, const void* work) {
+  need(work || l.work_bytes() == 0, "list: null work");
+}
 bool known_type(int t) { return t == BC2N_F32 || t == BC2N_F16 || t == BC2N_BF16; }
 }  // namespace
 
@@ -1214,7 +1221,7 @@ int bc2n_logprobs_fwd(void* stream, int dtype, const void* logits, int64_t ld, i
     a.top_logp = top_logp;
     a.top_index = top_index;
     a.save = reinterpret_cast<float*>(save);
-    logprobs_fwd(as_stream(stream), a, work);
+    logprobs_fwd(own_stream(stream), a, work);
   });
 }
 
@@ -1235,7 +1242,7 @@ int bc2n_logprobs_bwd(void* stream, int dtype, const void* logits, int64_t ld, i
     a.d_logp = d_logp;
     a.d_entropy = d_entropy;
     a.d_top = d_top_logp;
-    logprobs_bwd(as_stream(stream), a);
+    logprobs_bwd(own_stream(stream), a);
   });
 }
 
@@ -1252,7 +1259,7 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
     a.entropy = entropy;
     a.d_logp = d_logp;
     a.d_entropy = d_entropy;
-    logprobs_grad(as_stream(stream), a, work);
+    logprobs_grad(own_stream(stream), a, work);
   });
 }
 
@@ -1320,8 +1327,9 @@ size_t bc2n_list_work_bytes(void* list) {
 int bc2n_grad_norm(void* stream, void* list, float* norm, void* work) {
   return guarded([&] {
     TensorList& l = list_of(list);
-    need(norm && work, "null operand");
-    grad_norm(as_stream(stream), l, norm, work);
+    need(norm, "null operand");
+    list_work(l, work);
+    grad_norm(own_stream(stream), l, norm, work);
   });
 }
 
@@ -1330,8 +1338,8 @@ int bc2n_grad_clip(void* stream, void* list, float max_norm, float* norm, void* 
     TensorList& l = list_of(list);
     need(l.clips, "grad_clip: the list has no outputs");
     need(max_norm > 0.f, "grad_clip: max_norm must be positive");
-    need(work, "null operand");
-    grad_clip(as_stream(stream), l, max_norm, norm, work);
+    list_work(l, work);
+    grad_clip(own_stream(stream), l, max_norm, norm, work);
   });
 }
 
@@ -1346,7 +1354,7 @@ int bc2n_adam_step(void* stream, void* list, double lr, double beta1, double bet
     need(weight_decay >= 0, "adam_step: weight_decay must not be negative");
     need(scalars || (step >= 1 && std::isfinite(lr)), "adam_step: step counts from 1, lr is finite");
     need(max_norm >= 0, "adam_step: max_norm must be positive, or 0 for none");
-    need(work, "null operand");
+    list_work(l, work);
     AdamScalars s;
     s.lr = lr;
     s.beta1 = beta1;
@@ -1356,7 +1364,7 @@ int bc2n_adam_step(void* stream, void* list, double lr, double beta1, double bet
     s.step = step;
     s.max_norm = max_norm;
     s.device = scalars;
-    adam_step(as_stream(stream), l, s, norm, work);
+    adam_step(own_stream(stream), l, s, norm, work);
   });
 }
 

@@ -24,6 +24,9 @@
 
 #include "../../include/bc2n.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace bc2n {
 
 namespace {
@@ -250,150 +253,228 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LogProbs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Longer rows: a workgroup reads a row, or one of `splits` parts of it, 16
-// bytes a lane and U vectors at a time, with a running maximum a lane (the
-// sums are rescaled once a chunk of U * VN elements).
+// Longer rows: whole workgroups.  A row is the elements before the first
+// 16-byte boundary (`head`), aligned vectors, and what is left behind them;
+// head and rest together are fewer than 16 elements, the `edge`, one a lane of
+// the first wave.  (Aligned vectors: 50 against 56 us for 2047 rows of 50 k
+// binary16 logits that start anywhere.)
 // ---------------------------------------------------------------------------
-constexpr int U = 4;
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float v, Op op) {
+  v = group_reduce<16>(v, op);
+  auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v),
+                                            __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  v = op(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                            __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return op(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_reduce(v, [](float a, float b) { return a + b; });
+}
 
-// A wave's largest elements, the k-th in lane k (index -1: none yet); above
-// `floor` an element belongs to them.  A wave takes its elements in ascending
-// order of index, so a later one equal to the last kept is never better.
+template <class T>
+struct Row {
+  static constexpr int VN = Vec<T>::N;
+  const T* p;
+  int head, nv, edges;  // vector g holds the elements from head + g * VN
+  __device__ __forceinline__ Row(const T* row, int V) : p(row) {
+    const int past = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+    head = min(V, ((16 - past) & 15) / (int)sizeof(T));
+    nv = (V - head) / VN;
+    edges = V - nv * VN;
+  }
+  // index of edge element t < edges
+  __device__ __forceinline__ int edge(int t) const { return t < head ? t : t + nv * VN; }
+  __device__ __forceinline__ u32x4 load(int g) const { return Vec<T>::load(p + head + g * VN); }
+  static __device__ __forceinline__ u32x4 none() {  // -inf
+    constexpr uint32_t w = sizeof(T) == 4 ? 0xff800000u
+                           : std::is_same<T, h16>::value ? 0xfc00fc00u : 0xff80ff80u;
+    return u32x4{w, w, w, w};
+  }
+};
+
+// A chunk: E elements a lane, U vectors apart by the workgroup's width
+constexpr int E = 16;
+
+// vectors base + u * NT + lane below v1, -inf past it
+template <class T, int NT>
+__device__ __forceinline__ void fetch(const Row<T>& r, int base, int v1, u32x4 (&raw)[E / Vec<T>::N]) {
+  constexpr int U = E / Vec<T>::N;
+  const int g = base + (int)threadIdx.x;
+  if (base + U * NT <= v1) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = r.load(g + u * NT);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      raw[u] = Row<T>::none();
+      if (g + u * NT < v1) raw[u] = r.load(g + u * NT);
+    }
+  }
+}
+// Keeps the compiler from holding a vector's f32 values from one use to the
+// next, in twice the registers.
+__device__ __forceinline__ void as_stored(u32x4& v) { asm volatile("" : "+v"(v)); }
+template <int N>
+__device__ __forceinline__ float max_of(const float (&x)[N]) {
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+  return m;
+}
+// a lane's running sums over one more chunk of maximum mx
+template <int N>
+__device__ __forceinline__ void add_chunk(Stat& q, const float (&x)[N], float mx) {
+  if (__any(mx > q.m)) q.raise(fmaxf(q.m, mx));
+#pragma unroll
+  for (int i = 0; i < N; ++i) q.add(x[i]);
+}
+
+__device__ __forceinline__ float read_lane(float v, int lane) {
+  return __builtin_bit_cast(float,
+                            __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+// key of the float just below the one of this key; there is none below -inf
+__device__ __forceinline__ uint32_t key_below(uint32_t k) {
+  return k == 0x80000000u ? k - 2 : k - 1;  // below 0 lies the smallest negative, not -0
+}
+__device__ __forceinline__ float value_of_key(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// A wave's largest elements, the k-th in lane k (index -1: none yet).  An
+// element not above `floor` is not among the row's: the wave has K as large
+// that come before it.  Waves of one row tell each other, through LDS, values
+// that K elements reach (*shared, as a key), so that a wave does not collect
+// what another has better; when they learn it changes only what is collected
+// beside the answer.
 struct TopList {
   float v = NEG_INF;
   int i = -1;
   float floor = NEG_INF;
 
-  // x: this lane's elements of one chunk, vector u starting at index i0 + u *
-  // step; mx: their maximum
-  template <int VN>
-  __device__ __forceinline__ void take(const float (&x)[U * VN], float mx, int i0, int step, int K,
-                                       bool first) {
-    if (!__ballot(mx > floor)) return;
+  __device__ __forceinline__ void insert(float cv, int ci, int K) {
     const int lane = threadIdx.x & 63;
+    const int before = __popcll(__ballot(v > cv) | (__ballot(v == cv) & __ballot(i < ci)));
+    const float pv = dpp_mov<0x138>(v);  // the lane before
+    const int pi = (int)dpp_u32<0x138>((uint32_t)i);
+    v = lane > before ? pv : lane == before ? cv : v;
+    i = lane > before ? pi : lane == before ? ci : i;
+    floor = fmaxf(floor, read_lane(v, K - 1));
+  }
+
+  // x: this lane's elements of one chunk, vector u from index i0 + u * step;
+  // mx: their maximum
+  template <int VN, bool SHARE>
+  __device__ __forceinline__ void take(const float (&x)[E], float mx, int i0, int step, int K,
+                                       bool first, uint32_t* shared) {
+    if (!__any(mx > floor)) return;
+    const int lane = threadIdx.x & 63;
+    if (SHARE) {
+      const uint32_t k = __hip_atomic_load(shared, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (k) floor = fmaxf(floor, value_of_key(key_below(k)));
+      if (!__any(mx > floor)) return;
+    }
+    uint32_t reached = 0;
     if (first) {
       // K lanes hold an element as large as the K-th largest of the lanes'
       // maxima, so nothing below it can stay: without this bound the first
       // chunk would enter the list one by one
       float w = mx, t = NEG_INF;
       for (int k = 0; k < K; ++k) {
-        t = group_max<64>(w);
+        t = wave_max(w);
         const uint64_t b = __ballot(w == t);
         if (b == 0) break;
         if (lane == __ffsll((unsigned long long)b) - 1) w = NEG_INF;
       }
-      if (t > NEG_INF) {  // the float just below
-        const int b = __builtin_bit_cast(int, t);
-        floor = __builtin_bit_cast(float, t > 0.f ? b - 1 : t < 0.f ? b + 1 : (int)0x80000001);
+      if (t > NEG_INF) {
+        reached = order_key(t);
+        floor = fmaxf(floor, value_of_key(key_below(reached)));
       }
     }
+    const float before = floor;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      unsigned want = 0;
-#pragma unroll
-      for (int j = 0; j < VN; ++j) want |= x[u * VN + j] > floor ? 1u << j : 0u;
-      for (uint64_t b = __ballot(want != 0); b; b = __ballot(want != 0)) {
-        const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)b) - 1);
-        const int j = __ffs(want) - 1;
-        float xv = x[u * VN];
-#pragma unroll
-        for (int q = 1; q < VN; ++q)
-          if (j == q) xv = x[u * VN + q];
-        const float cv = __builtin_bit_cast(
-            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, xv), from));
-        const int ci = __builtin_amdgcn_readlane(i0 + u * step + j, from);
-        if (lane == from) want &= want - 1;
-        if (!(cv > floor)) continue;  // the list rose since
-        const int before = __popcll(__ballot(i >= 0 && v >= cv));
-        const float pv = __shfl_up(v, 1, 64);
-        const int pi = __shfl_up(i, 1, 64);
-        if (lane > before) {
-          v = pv;
-          i = pi;
-        } else if (lane == before) {
-          v = cv;
-          i = ci;
-        }
-        floor = fmaxf(floor, __builtin_bit_cast(float, __builtin_amdgcn_readlane(
-                                                           __builtin_bit_cast(int, v), K - 1)));
+    for (int n = 0; n < E; ++n) {
+      // out of order within the chunk, so an equal one may be better
+      for (uint64_t b = __ballot(x[n] >= floor); b; b &= b - 1) {
+        const int from = __ffsll((unsigned long long)b) - 1;
+        const float cv = read_lane(x[n], from);
+        const int ci = __builtin_amdgcn_readlane(i0, from) + n / VN * step + n % VN;
+        if (cv > NEG_INF && cv >= floor) insert(cv, ci, K);  // else the list rose since
       }
+    }
+    if (SHARE) {
+      if (floor > before) reached = order_key(floor);
+      if (reached && lane == 0)
+        __hip_atomic_fetch_max(shared, reached, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+  }
+  // one element a lane, at any index
+  __device__ __forceinline__ void take_edge(float x, int at, int K) {
+    for (uint64_t b = __ballot(x > NEG_INF && x >= floor); b; b &= b - 1) {
+      const int from = __ffsll((unsigned long long)b) - 1;
+      insert(read_lane(x, from), __builtin_amdgcn_readlane(at, from), K);
     }
   }
 };
 
-// The chunk of U vectors a lane at `pos` (VN elements a lane a vector, NT
-// lanes), elements at or past `hi` as -inf
-template <class T, int NT>
-__device__ __forceinline__ void read_chunk(const T* p, int64_t pos, int64_t hi,
-                                           float (&x)[U * Vec<T>::N]) {
-  constexpr int VN = Vec<T>::N;
-  if (pos + (int64_t)U * NT * VN <= hi) {
-    u32x4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = Vec<T>::load(p + pos + (u * NT + (int)threadIdx.x) * VN);
-#pragma unroll
-    for (int u = 0; u < U; ++u) Vec<T>::unpack(raw[u], x + u * VN);
-    return;
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t at = pos + (u * NT + (int)threadIdx.x) * VN;
-    if (at + VN <= hi) {
-      Vec<T>::unpack(Vec<T>::load(p + at), x + u * VN);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VN; ++j) x[u * VN + j] = at + j < hi ? (float)p[at + j] : NEG_INF;
-    }
-  }
+// Sum of a row over a wave's lanes, and over the workgroup's NT, in every lane
+__device__ __forceinline__ Stat join_wave(Stat q) {
+  q.raise(wave_max(q.m));
+  q.s = wave_sum(q.s);
+  q.u = wave_sum(q.u);
+  return q;
 }
-
-// Sum of a part of a row over the workgroup's NT lanes, in every lane
 template <int NT>
 __device__ __forceinline__ Stat join(Stat q, float (*buf)[4]) {
-  q.raise(group_max<64>(q.m));
-  q.s = group_sum<64>(q.s);
-  q.u = group_sum<64>(q.u);
-  const int w = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
+  q = join_wave(q);
+  if constexpr (NT == 64) return q;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (lane == 0) {
     buf[w][0] = q.m;
     buf[w][1] = q.s;
     buf[w][2] = q.u;
   }
   __syncthreads();
-  float m = buf[0][0];
-#pragma unroll
-  for (int i = 1; i < NT / 64; ++i) m = fmaxf(m, buf[i][0]);
-  Stat all;
-  all.m = m;
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) {
-    Stat o;
-    o.m = buf[i][0];
-    o.s = buf[i][1];
-    o.u = buf[i][2];
-    o.raise(m);
-    all.s += o.s;
-    all.u += o.u;
+  Stat o;
+  if (lane < NT / 64) {
+    o.m = buf[lane][0];
+    o.s = buf[lane][1];
+    o.u = buf[lane][2];
   }
-  return all;
+  return join_wave(o);
 }
 
-// Of n candidates (cv, ci; ci < 0: none) in LDS the rank of candidate c among
-// all, by value and then by index
-__device__ __forceinline__ int rank_of(const float* cv, const int* ci, int n, int c) {
-  const float v = cv[c];
-  const int i = ci[c];
+// Candidates in LDS are one word each: the value's order key over the index's
+// complement, so that the larger word is the better candidate; 0: none.
+__device__ __forceinline__ uint64_t candidate(float v, int i) {
+  return i < 0 ? 0 : (uint64_t)order_key(v) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ int index_of(uint64_t c) { return (int)~(uint32_t)c; }
+__device__ __forceinline__ float value_of(uint64_t c) { return value_of_key((uint32_t)(c >> 32)); }
+// how many of the n candidates (n a multiple of 8) are better than c
+__device__ __forceinline__ int rank_of(const uint64_t* cand, int n, uint64_t c) {
   int rank = 0;
-  for (int o = 0; o < n; ++o)
-    rank += ci[o] >= 0 && (cv[o] > v || (cv[o] == v && ci[o] < i));
+  for (int o = 0; o < n; o += 8) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) rank += cand[o + k] > c;
+  }
   return rank;
 }
+constexpr int up8(int n) { return (n + 7) / 8 * 8; }
 
-// Writes the K best of n candidates in LDS as row r's alternatives; where
-// there are fewer than K above -inf, the first -inf elements of the row follow.
+// Writes the K best of n candidates (LDS, zeros behind up to a multiple of 8)
+// as row r's alternatives; where there are fewer than K above -inf, the first
+// -inf elements of the row follow.
 template <class T, int NT>
 __device__ __forceinline__ void write_tops(const LogProbs& a, int64_t r, const RowStat& st,
-                                           const float* cv, const int* ci, int n) {
+                                           const uint64_t* cand, int n) {
   float* ov = a.top_logp + r * a.K;
   int32_t* oi = a.top_index + r * a.K;
   if (is_nan(st.logs)) {
@@ -404,26 +485,25 @@ __device__ __forceinline__ void write_tops(const LogProbs& a, int64_t r, const R
     return;
   }
   for (int c = threadIdx.x; c < n; c += NT) {
-    if (ci[c] < 0) continue;
-    const int k = rank_of(cv, ci, n, c);
+    const uint64_t mine = cand[c];
+    const int k = mine ? rank_of(cand, n, mine) : a.K;
     if (k < a.K) {
-      ov[k] = log_prob(st, cv[c]);
-      oi[k] = ci[c];
+      ov[k] = log_prob(st, value_of(mine));
+      oi[k] = index_of(mine);
     }
   }
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
     int have = 0;
-    for (int c = lane; c < n; c += 64) have += ci[c] >= 0;
-    have = (int)group_sum<64>((float)have);  // at most 1024: exact
+    for (int c = 0; c < n; c += 64) have += __popcll(__ballot(c + lane < n && cand[c + lane] != 0));
     const T* p = reinterpret_cast<const T*>(a.x) + r * a.ld;
-    for (int64_t b = 0; have < a.K && b < a.V; b += 64) {
+    for (int b = 0; have < a.K && b < a.V; b += 64) {
       const bool gone = b + lane < a.V && (float)p[b + lane] == NEG_INF;
       const uint64_t m = __ballot(gone);
       const int k = have + __popcll(m & ((1ull << lane) - 1));
       if (gone && k < a.K) {
         ov[k] = NEG_INF;
-        oi[k] = (int)(b + lane);
+        oi[k] = b + lane;
       }
       have += __popcll(m);
     }
@@ -438,29 +518,29 @@ __device__ __forceinline__ void no_tops(const LogProbs& a, int64_t r, int nt) {
 
 // Parts of rows: their sums and their largest elements
 struct Parts {
-  float4* stat = nullptr;  // [rows][splits]
-  float* v = nullptr;      // [rows][splits][K]
-  int* i = nullptr;
+  float4* stat = nullptr;    // [rows][splits]
+  uint64_t* top = nullptr;   // [rows][splits][K] candidates
 };
 template <class A>
 Parts parts_of(A& c, int64_t rows, int splits, int K) {
   Parts p;
   const size_t n = (size_t)rows * splits;
   p.stat = c.template take<float4>(n);
-  p.v = c.template take<float>(n * (K > 0 ? K : 1));
-  p.i = c.template take<int>(n * (K > 0 ? K : 1));
+  p.top = c.template take<uint64_t>(n * K);
   return p;
 }
 
-constexpr int FWD_NT = 256;
-
-template <class T, bool TOP>
-__global__ __launch_bounds__(FWD_NT) void lp_stream_kernel(LogProbs a, int splits, int64_t part,
-                                                           Parts parts) {
-  constexpr int VN = Vec<T>::N, NT = FWD_NT, NW = NT / 64;
+// A workgroup reads a row, or one of `splits` parts of `part` vectors of it
+// (the first with the edge), a chunk ahead of the one it works on, with a
+// running maximum a lane.
+template <class T, bool TOP, int NT>
+__global__ __launch_bounds__(NT, 8) void lp_stream_kernel(LogProbs a, int splits, int part,
+                                                       Parts parts) {
+  constexpr int VN = Vec<T>::N, NW = NT / 64, U = E / VN;
   __shared__ float buf[NW][4];
-  __shared__ float cv[TOP ? NW * LP_MAX_TOP : 1];
-  __shared__ int ci[TOP ? NW * LP_MAX_TOP : 1];
+  __shared__ uint64_t cand[TOP ? NW * LP_MAX_TOP : 1];
+  __shared__ uint32_t shared;
+  constexpr bool SHARE = TOP && NT > 64;
   const int64_t r = blockIdx.x / splits;
   const int sp = blockIdx.x % splits;
   const int64_t t = target_of(a, r);
@@ -471,66 +551,77 @@ __global__ __launch_bounds__(FWD_NT) void lp_stream_kernel(LogProbs a, int split
     }
     return;
   }
-  const T* p = reinterpret_cast<const T*>(a.x) + r * a.ld;
-  const int64_t lo = sp * part, hi = min((int64_t)a.V, lo + part);
+  const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
+  const int v0 = sp * part, v1 = min(row.nv, v0 + part);
+  const bool edge = sp == 0 && (int)threadIdx.x < row.edges;
+  const int edge_at = edge ? row.edge(threadIdx.x) : -1;
+  const float ex = edge ? (float)row.p[edge_at] : NEG_INF;
   Stat q;
   TopList top;
-  for (int64_t pos = lo; pos < hi; pos += (int64_t)U * NT * VN) {
-    float x[U * VN];
-    read_chunk<T, NT>(p, pos, hi, x);
-    float mx = x[0];
+  u32x4 raw[U];
+  if (v0 < v1) fetch<T, NT>(row, v0, v1, raw);
+  if (SHARE) {
+    if (threadIdx.x == 0) shared = 0;
+    __syncthreads();
+  }
+  for (int base = v0; base < v1; base += U * NT) {
+    float x[E];
 #pragma unroll
-    for (int i = 1; i < U * VN; ++i) mx = fmaxf(mx, x[i]);
-    q.raise(fmaxf(q.m, mx));
-#pragma unroll
-    for (int i = 0; i < U * VN; ++i) q.add(x[i]);
-    if (TOP) top.take<VN>(x, mx, (int)pos + threadIdx.x * VN, NT * VN, a.K, pos == lo);
+    for (int u = 0; u < U; ++u) Vec<T>::unpack(raw[u], x + u * VN);
+    if (base + U * NT < v1) fetch<T, NT>(row, base + U * NT, v1, raw);
+    const float mx = max_of(x);
+    add_chunk(q, x, mx);
+    if (TOP)
+      top.take<VN, SHARE>(x, mx, row.head + (base + (int)threadIdx.x) * VN, NT * VN, a.K,
+                          base == v0, &shared);
+  }
+  if (threadIdx.x < 64 && sp == 0) {
+    const float one[1] = {ex};
+    add_chunk(q, one, ex);
+    if (TOP) top.take_edge(ex, edge_at, a.K);
   }
   if (TOP) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    if (lane < a.K) {
-      cv[w * a.K + lane] = top.v;
-      ci[w * a.K + lane] = top.i;
-    }
+    const int n = NW * a.K;
+    if (lane < a.K) cand[w * a.K + lane] = candidate(top.v, top.i);
+    if ((int)threadIdx.x < up8(n) - n) cand[n + threadIdx.x] = 0;
   }
-  const Stat all = join<NT>(q, buf);  // its barrier also covers cv, ci
+  const Stat all = join<NT>(q, buf);
+  if (TOP && NT == 64) __syncthreads();  // else join's
   if (splits == 1) {
     const RowStat st = finish(all, true);
     if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
-    if (TOP) write_tops<T, NT>(a, r, st, cv, ci, NW * a.K);
+    if (TOP) write_tops<T, NT>(a, r, st, cand, NW * a.K);
     return;
   }
   const int64_t o = r * splits + sp;
   if (threadIdx.x == 0) parts.stat[o] = make_float4(all.m, all.s, all.u, 0.f);
   if (TOP) {
+    // in any order; places that no candidate ranks for are none
     const int n = NW * a.K;
+    uint64_t mine = 0;
     int have = 0;
-    for (int c = 0; c < n; ++c) have += ci[c] >= 0;
-    for (int c = threadIdx.x; c < n; c += NT) {
-      if (ci[c] < 0) continue;
-      const int k = rank_of(cv, ci, n, c);
-      if (k < a.K) {
-        parts.v[o * a.K + k] = cv[c];
-        parts.i[o * a.K + k] = ci[c];
-      }
+    for (int c = 0; c < n; c += 64) {
+      const int lane = threadIdx.x & 63;
+      have += __popcll(__ballot(c + lane < n && cand[c + lane] != 0));
     }
-    for (int k = have + threadIdx.x; k < a.K; k += NT) parts.i[o * a.K + k] = -1;
+    for (int c = threadIdx.x; c < n; c += NT) {
+      mine = cand[c];
+      const int k = mine ? rank_of(cand, n, mine) : a.K;
+      if (k < a.K) parts.top[o * a.K + k] = mine;
+    }
+    for (int k = have + threadIdx.x; k < a.K; k += NT) parts.top[o * a.K + k] = 0;
   }
 }
 
 // Joins the parts of a row.
 constexpr int MAX_SPLITS = 32;
 template <class T>
-__global__ __launch_bounds__(FWD_NT) void lp_join_kernel(LogProbs a, int splits, Parts parts) {
-  __shared__ float cv[MAX_SPLITS * LP_MAX_TOP];
-  __shared__ int ci[MAX_SPLITS * LP_MAX_TOP];
+__global__ __launch_bounds__(256) void lp_join_kernel(LogProbs a, int splits, Parts parts) {
+  __shared__ uint64_t cand[MAX_SPLITS * LP_MAX_TOP];
   const int64_t r = blockIdx.x;
-  const int64_t t = target_of(a, r);
-  if (t < 0) {
-    if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
-    no_tops(a, r, FWD_NT);
-    return;
-  }
+  const int n = splits * a.K;
+  for (int c = threadIdx.x; c < up8(n); c += 256) cand[c] = c < n ? parts.top[r * n + c] : 0;
   const int lane = threadIdx.x & 63;
   Stat q;
   if (lane < splits) {  // each wave by itself
@@ -539,142 +630,248 @@ __global__ __launch_bounds__(FWD_NT) void lp_join_kernel(LogProbs a, int splits,
     q.s = s.y;
     q.u = s.z;
   }
-  q.raise(group_max<64>(q.m));
-  q.s = group_sum<64>(q.s);
-  q.u = group_sum<64>(q.u);
-  const RowStat st = finish(q, true);
-  if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
-  if (a.K > 0) {
-    const int n = splits * a.K;
-    for (int c = threadIdx.x; c < n; c += FWD_NT) {
-      cv[c] = parts.v[r * n + c];
-      ci[c] = parts.i[r * n + c];
-    }
-    __syncthreads();
-    write_tops<T, FWD_NT>(a, r, st, cv, ci, n);
-  }
-}
-
-// The gradient of [lo, hi) of row r from its statistics.  The classes with
-// terms of their own (the target and the alternatives) are computed first, by
-// one wave, and stored last: a row may be written in place.
-template <class T, int NT>
-__device__ __forceinline__ void write_gradient(const LogProbs& a, int64_t r, int64_t t,
-                                               const RowStat& st, int K, int64_t lo, int64_t hi) {
-  constexpr int VN = Vec<T>::N;
-  T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
-  if (st.live == 0.f || t < 0) {
-    const float zero[VN] = {};
-    for (int64_t at = lo + threadIdx.x * VN; at < hi; at += NT * VN) {
-      if (at + VN <= hi) Vec<T>::store(o + at, Vec<T>::pack(zero));
-      else
-        for (int64_t j = at; j < hi; ++j) o[j] = (T)0.f;
-    }
+  const int64_t t = target_of(a, r);
+  if (t < 0) {
+    if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
+    no_tops(a, r, 256);
     return;
   }
-  const T* p = reinterpret_cast<const T*>(a.x) + r * a.ld;
-  const int lane = threadIdx.x & 63;
-  const float g = a.d_logp ? a.d_logp[r] : 0.f;
-  Cotangent c{st.m, st.logs, st.h, g, a.d_entropy ? a.d_entropy[r] : 0.f};
-  // lane k < K: alternative k; lane K: the target
-  int64_t at = -1;
-  float own = 0.f;
-  if (a.d_top && lane < K) {
-    at = a.top_index[r * K + lane];
-    own = a.d_top[r * K + lane];
-  }
-  c.g += group_sum<64>(own);
-  if (lane == K && a.d_logp) {
-    at = t;
-    own = g;
-  }
-  if (a.d_logp && t >= a.V) c.g = __builtin_nanf("");
-  if (a.d_top && a.d_logp) {  // a target among the alternatives has both terms
-    const uint64_t same = __ballot(lane < K && at == t);
-    if (lane < K && at == t) own += g;
-    if (lane == K && same) at = -1;
-  }
-  const bool special = threadIdx.x < 64 && at >= lo && at < hi;
-  T sv = (T)0.f;
-  if (special) sv = (T)(c.at((float)p[at]) + own);
+  const RowStat st = finish(join_wave(q), true);
+  if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
   __syncthreads();
-  for (int64_t pos = lo; pos < hi; pos += (int64_t)U * NT * VN) {
-    float x[U * VN];
-    read_chunk<T, NT>(p, pos, hi, x);
+  if (a.K > 0) write_tops<T, 256>(a, r, st, cand, n);
+}
+
+// zeros over row r's gradient
+template <class T, int NT>
+__device__ __forceinline__ void write_zeros(const LogProbs& a, int64_t r, int64_t lo, int64_t hi) {
+  constexpr int VN = Vec<T>::N;
+  T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
+  for (int64_t at = lo + threadIdx.x * VN; at < hi; at += NT * VN) {
+    if (at + VN <= hi) Vec<T>::store(o + at, u32x4{0, 0, 0, 0});
+    else
+      for (int64_t j = at; j < hi; ++j) o[j] = (T)0.f;
+  }
+}
+
+// The classes of a row with terms of their own, one a lane of each wave:
+// lane k < K alternative k, lane K the target.
+struct Special {
+  int64_t at = -1;  // class, or none
+  float own = 0.f;  // its own terms
+};
+__device__ __forceinline__ Special special_of(const LogProbs& a, int64_t r, int64_t t, int K,
+                                              Cotangent& c) {
+  const int lane = threadIdx.x & 63;
+  Special s;
+  if (a.d_top && lane < K) {
+    s.at = a.top_index[r * K + lane];
+    s.own = a.d_top[r * K + lane];
+  }
+  if (a.d_top) c.g += wave_sum(s.own);
+  if (a.d_logp) {
+    const float g = a.d_logp[r];
+    const uint64_t same = __ballot(lane < K && s.at == t);  // the target among the alternatives
+    if (lane < K && s.at == t) s.own += g;
+    if (lane == K && !same) {
+      s.at = t;
+      s.own = g;
+    }
+    if (t >= a.V) c.g = __builtin_nanf("");
+  }
+  return s;
+}
+__device__ __forceinline__ Cotangent cotangent_of(const LogProbs& a, int64_t r, const RowStat& st) {
+  return Cotangent{st.m, st.logs, st.h, a.d_logp ? a.d_logp[r] : 0.f,
+                   a.d_entropy ? a.d_entropy[r] : 0.f};
+}
+
+// The gradient of vectors [v0, v1) and, where `edge`, the edge of row r from
+// its statistics.  The special classes are computed first, by one wave, and
+// stored last: a row may be written in place.
+template <class T, int NT, bool ONCE>
+__device__ __forceinline__ void write_gradient(const LogProbs& a, int64_t r, int64_t t,
+                                               const RowStat& st, int K, const Row<T>& row, int v0,
+                                               int v1, bool edge) {
+  constexpr int VN = Vec<T>::N, U = E / VN;
+  T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
+  Cotangent c = cotangent_of(a, r, st);
+  const Special sp = special_of(a, r, t, K, c);
+  const int lo = row.head + v0 * VN, hi = row.head + v1 * VN;
+  const bool inside = sp.at >= lo && sp.at < hi;
+  const bool outside = edge && sp.at >= 0 && sp.at < a.V &&
+                       (sp.at < row.head || sp.at >= row.head + row.nv * VN);
+  const bool mine = threadIdx.x < 64 && (inside || outside);
+  T sv = (T)0.f;
+  if (mine) sv = (T)(c.at((float)row.p[sp.at]) + sp.own);
+  __syncthreads();
+  if (edge && (int)threadIdx.x < row.edges) {
+    const int at = row.edge(threadIdx.x);
+    o[at] = (T)c.at((float)row.p[at]);
+  }
+  u32x4 raw[U];
+  if (v0 < v1) fetch<T, NT>(row, v0, v1, raw);
+  for (int base = v0; base < v1; base += U * NT) {
+    float x[E];
 #pragma unroll
-    for (int i = 0; i < U * VN; ++i) x[i] = c.at(x[i]);
+    for (int u = 0; u < U; ++u) Vec<T>::unpack(raw[u], x + u * VN);
+    if (base + U * NT < v1) fetch<T, NT>(row, base + U * NT, v1, raw);
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = c.at(x[i]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t b = pos + (u * NT + (int)threadIdx.x) * VN;
-      if (b + VN <= hi) {
-        Vec<T>::store(o + b, Vec<T>::pack(x + u * VN));
-      } else {
-#pragma unroll
-        for (int j = 0; j < VN; ++j)
-          if (b + j < hi) o[b + j] = (T)x[u * VN + j];
-      }
+      const int g = base + u * NT + (int)threadIdx.x;
+      if (g < v1) Vec<T>::template store<ONCE>(o + row.head + g * VN, Vec<T>::pack(x + u * VN));
     }
   }
   __syncthreads();
-  if (special) o[at] = sv;
+  if (mine) o[sp.at] = sv;
 }
 
-template <class T>
-__global__ __launch_bounds__(FWD_NT) void lp_gradient_kernel(LogProbs a, int splits, int64_t part) {
-  const int64_t r = blockIdx.x / splits, lo = (blockIdx.x % splits) * part;
+constexpr int BWD_NT = 256;
+template <class T, bool ONCE>
+__global__ __launch_bounds__(BWD_NT) void lp_gradient_kernel(LogProbs a, int splits, int part) {
+  const int64_t r = blockIdx.x / splits;
+  const int sp = blockIdx.x % splits;
+  const int64_t t = target_of(a, r);
   const float4 s = reinterpret_cast<const float4*>(a.save)[r];
-  write_gradient<T, FWD_NT>(a, r, target_of(a, r), RowStat{s.x, s.y, s.z, s.w}, a.K, lo,
-                            min((int64_t)a.V, lo + part));
+  const RowStat st{s.x, s.y, s.z, s.w};
+  const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
+  const int v0 = min(row.nv, sp * part), v1 = min(row.nv, v0 + part);
+  if (st.live == 0.f || t < 0) {
+    constexpr int VN = Vec<T>::N;
+    write_zeros<T, BWD_NT>(a, r, sp == 0 ? 0 : row.head + v0 * VN,
+                           sp == splits - 1 ? a.V : row.head + v1 * VN);
+    return;
+  }
+  write_gradient<T, BWD_NT, ONCE>(a, r, t, st, a.K, row, v0, v1, sp == 0);
 }
 
-// A workgroup takes a whole row twice, the second time out of the caches.
-constexpr int BOTH_NT = 1024;
-template <class T>
-__global__ __launch_bounds__(BOTH_NT) void lp_both_kernel(LogProbs a) {
-  constexpr int VN = Vec<T>::N, NT = BOTH_NT;
+// Forward and backward of a row held in the registers of one workgroup: NV
+// vectors a lane.
+template <class T, int NT, int NV, bool ONCE>
+__global__ __launch_bounds__(NT) void lp_block_kernel(LogProbs a) {
+  constexpr int VN = Vec<T>::N;
   __shared__ float buf[NT / 64][4];
   const int64_t r = blockIdx.x;
   const int64_t t = target_of(a, r);
-  Stat q;
-  if (t >= 0) {
-    const T* p = reinterpret_cast<const T*>(a.x) + r * a.ld;
-    for (int64_t pos = 0; pos < a.V; pos += (int64_t)U * NT * VN) {
-      float x[U * VN];
-      read_chunk<T, NT>(p, pos, a.V, x);
-      float mx = x[0];
-#pragma unroll
-      for (int i = 1; i < U * VN; ++i) mx = fmaxf(mx, x[i]);
-      q.raise(fmaxf(q.m, mx));
-#pragma unroll
-      for (int i = 0; i < U * VN; ++i) q.add(x[i]);
-    }
+  if (t < 0) {
+    if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
+    write_zeros<T, NT>(a, r, 0, a.V);
+    return;
   }
-  const RowStat st = finish(join<NT>(q, buf), t >= 0);
+  const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
+  u32x4 raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int g = i * NT + (int)threadIdx.x;
+    raw[i] = Row<T>::none();
+    if (g < row.nv) raw[i] = row.load(g);
+  }
+  const bool edge = (int)threadIdx.x < row.edges;
+  const int edge_at = edge ? row.edge(threadIdx.x) : -1;
+  const float ex = edge ? (float)row.p[edge_at] : NEG_INF;
+  Stat q;
+  q.m = fmaxf(LOWEST, ex);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float x[VN];
+    Vec<T>::unpack(raw[i], x);
+    q.m = fmaxf(q.m, max_of(x));
+    as_stored(raw[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float x[VN];
+    Vec<T>::unpack(raw[i], x);
+#pragma unroll
+    for (int j = 0; j < VN; ++j) q.add(x[j]);
+    as_stored(raw[i]);
+  }
+  q.add(ex);
+  const RowStat st = finish(join<NT>(q, buf), true);
+  if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
+  if (st.live == 0.f) {
+    __syncthreads();  // the target's logit is read before its place is written
+    write_zeros<T, NT>(a, r, 0, a.V);
+    return;
+  }
+  Cotangent c = cotangent_of(a, r, st);
+  const Special sp = special_of(a, r, t, 0, c);
+  const bool mine = threadIdx.x < 64 && sp.at >= 0 && sp.at < a.V;
+  T sv = (T)0.f;
+  if (mine) sv = (T)(c.at((float)row.p[sp.at]) + sp.own);
+  __syncthreads();
+  T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
+  if (edge) o[edge_at] = (T)c.at(ex);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int g = i * NT + (int)threadIdx.x;
+    float x[VN];
+    Vec<T>::unpack(raw[i], x);
+#pragma unroll
+    for (int j = 0; j < VN; ++j) x[j] = c.at(x[j]);
+    if (g < row.nv) Vec<T>::template store<ONCE>(o + row.head + g * VN, Vec<T>::pack(x));
+  }
+  __syncthreads();
+  if (mine) o[sp.at] = sv;
+}
+
+// Rows longer than that: a workgroup takes a whole row twice, the second time
+// out of the caches.
+constexpr int BOTH_NT = 1024;
+template <class T, bool ONCE>
+__global__ __launch_bounds__(BOTH_NT) void lp_both_kernel(LogProbs a) {
+  constexpr int VN = Vec<T>::N, NT = BOTH_NT, U = E / VN;
+  __shared__ float buf[NT / 64][4];
+  const int64_t r = blockIdx.x;
+  const int64_t t = target_of(a, r);
+  if (t < 0) {
+    if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
+    write_zeros<T, NT>(a, r, 0, a.V);
+    return;
+  }
+  const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
+  const bool edge = (int)threadIdx.x < row.edges;
+  const float ex = edge ? (float)row.p[row.edge(threadIdx.x)] : NEG_INF;
+  Stat q;
+  u32x4 raw[U];
+  if (row.nv > 0) fetch<T, NT>(row, 0, row.nv, raw);
+  for (int base = 0; base < row.nv; base += U * NT) {
+    float x[E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec<T>::unpack(raw[u], x + u * VN);
+    if (base + U * NT < row.nv) fetch<T, NT>(row, base + U * NT, row.nv, raw);
+    add_chunk(q, x, max_of(x));
+  }
+  const float one[1] = {ex};
+  add_chunk(q, one, ex);
+  const RowStat st = finish(join<NT>(q, buf), true);
   if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
   __syncthreads();  // the target's logit is read before its place is written
-  write_gradient<T, NT>(a, r, t, st, 0, 0, a.V);
+  if (st.live == 0.f) return write_zeros<T, NT>(a, r, 0, a.V);
+  write_gradient<T, NT, ONCE>(a, r, t, st, 0, row, 0, row.nv, true);
 }
 
 // ---------------------------------------------------------------------------
 // Which kernel
 // ---------------------------------------------------------------------------
-constexpr int ROW_MAX = 1024;  // longest row held by a group of lanes
+constexpr int ROW_MAX = 1024;      // longest row held by a group of lanes
+constexpr int WAVE_MAX = 8192;     // longest row read by one wave
+constexpr int BLOCK_VECS = 8192;   // vectors that one workgroup holds
 
-// Parts a row is read in: as many as fill the card, each at least one chunk
-// of a workgroup.
-int splits_of(int dtype, int64_t rows, int V) {
-  if (V <= ROW_MAX) return 1;
-  const int64_t chunk = (int64_t)U * FWD_NT * (dtype == BC2N_F32 ? 4 : 8);
-  const int64_t fill = (2 * (int64_t)device_cus() + rows - 1) / rows;
-  int64_t s = (V + chunk - 1) / chunk;
-  if (s > fill) s = fill;
-  if (s > MAX_SPLITS) s = MAX_SPLITS;
-  return s < 1 ? 1 : (int)s;
-}
-int64_t part_of(int V, int splits) {
-  // a multiple of 64 elements, so that parts begin like the row
-  const int64_t p = (V + splits - 1) / splits;
-  return (p + 63) / 64 * 64;
+// How a long row is divided among workgroups of 256: into as many parts as
+// fill the card, each at least one chunk.
+struct Split {
+  int splits = 1, part = 0;  // part in vectors
+};
+Split split_of(int dtype, int64_t rows, int V) {
+  const int vn = dtype == BC2N_F32 ? 4 : 8, nv = (V + vn - 1) / vn;
+  const int64_t chunk = (int64_t)E / vn * 256;
+  const int64_t fill = (4 * (int64_t)device_cus() + rows - 1) / rows;
+  int64_t s = std::min<int64_t>({(nv + chunk - 1) / chunk, fill, MAX_SPLITS});
+  if (s < 1 || V <= WAVE_MAX) s = 1;
+  return Split{(int)s, (int)((nv + s - 1) / s)};
 }
 
 void launched() { hip_check(hipGetLastError(), "logprobs launch"); }
@@ -699,40 +896,80 @@ void rows_launch(hipStream_t st, const LogProbs& a) {
   else if constexpr (N == 4) rows_go<T, N, 64, 4, MODE>(st, a);
 }
 
+template <class T, int NT>
+void stream_go(hipStream_t st, const LogProbs& a, const Split& s, const Parts& parts) {
+  const unsigned grid = (unsigned)(a.rows * s.splits);
+  if (a.K > 0) lp_stream_kernel<T, true, NT><<<grid, NT, 0, st>>>(a, s.splits, s.part, parts);
+  else lp_stream_kernel<T, false, NT><<<grid, NT, 0, st>>>(a, s.splits, s.part, parts);
+}
+
 template <class T>
 void fwd(hipStream_t st, const LogProbs& a, void* work) {
   if (a.V <= ROW_MAX) return rows_launch<T, 1>(st, a);
-  const int s = splits_of(a.dtype, a.rows, a.V);
+  const Split s = split_of(a.dtype, a.rows, a.V);
   Parts parts;
-  if (s > 1) {
+  if (s.splits > 1) {
     Carver c(work);
-    parts = parts_of(c, a.rows, s, a.K);
+    parts = parts_of(c, a.rows, s.splits, a.K);
   }
-  const unsigned grid = (unsigned)(a.rows * s);
-  if (a.K > 0) lp_stream_kernel<T, true><<<grid, FWD_NT, 0, st>>>(a, s, part_of(a.V, s), parts);
-  else lp_stream_kernel<T, false><<<grid, FWD_NT, 0, st>>>(a, s, part_of(a.V, s), parts);
-  if (s > 1) lp_join_kernel<T><<<(unsigned)a.rows, FWD_NT, 0, st>>>(a, s, parts);
+  if (a.V <= WAVE_MAX) stream_go<T, 64>(st, a, s, parts);
+  else stream_go<T, 256>(st, a, s, parts);
+  if (s.splits > 1) lp_join_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a, s.splits, parts);
+}
+
+// Logits and gradient of more than half of the Infinity Cache's 256 MiB: the
+// gradient is stored past the caches, which leaves them to the logits (1021
+// rows of 33 k f32, forward and backward: 95 -> 82 us; 30 k of 1.5 k: 113 ->
+// 102).  Smaller ones stay for whoever reads them next.
+template <class F>
+void with_once(const LogProbs& a, F f) {
+  const int64_t bytes = 2 * a.rows * a.V * (a.dtype == BC2N_F32 ? 4 : 2);
+  if (bytes > int64_t(128) << 20) f(std::true_type());
+  else f(std::false_type());
 }
 
 template <class T>
 void bwd(hipStream_t st, const LogProbs& a) {
   if (a.V <= ROW_MAX) return rows_launch<T, 2>(st, a);
-  const int s = splits_of(a.dtype, a.rows, a.V);
-  lp_gradient_kernel<T><<<(unsigned)(a.rows * s), FWD_NT, 0, st>>>(a, s, part_of(a.V, s));
+  const Split s = split_of(a.dtype, a.rows, a.V);
+  const unsigned grid = (unsigned)(a.rows * s.splits);
+  with_once(a, [&](auto once) {
+    lp_gradient_kernel<T, once><<<grid, BWD_NT, 0, st>>>(a, s.splits, s.part);
+  });
+}
+
+// Few rows that no workgroup holds: forward in parts, then backward
+bool in_parts(int dtype, int64_t rows, int V) {
+  return V / (dtype == BC2N_F32 ? 4 : 8) > BLOCK_VECS && rows < device_cus();
+}
+
+template <class T, int NT, int NV>
+void block_go(hipStream_t st, const LogProbs& a) {
+  with_once(a, [&](auto once) {
+    lp_block_kernel<T, NT, NV, once><<<(unsigned)a.rows, NT, 0, st>>>(a);
+  });
 }
 
 template <class T>
 void both(hipStream_t st, const LogProbs& a, void* work) {
   if (a.V <= ROW_MAX) return rows_launch<T, 3>(st, a);
-  if (splits_of(a.dtype, a.rows, a.V) == 1) {
-    lp_both_kernel<T><<<(unsigned)a.rows, BOTH_NT, 0, st>>>(a);
-    return;
+  const int vecs = a.V / Vec<T>::N;
+  if (vecs <= 512) block_go<T, 64, 8>(st, a);
+  else if (vecs <= 1024) block_go<T, 256, 4>(st, a);
+  else if (vecs <= 2048) block_go<T, 256, 8>(st, a);
+  else if (vecs <= 4096) block_go<T, 512, 8>(st, a);
+  else if (vecs <= BLOCK_VECS) block_go<T, 1024, 8>(st, a);
+  else if (!in_parts(a.dtype, a.rows, a.V)) {
+    with_once(a, [&](auto once) {
+      lp_both_kernel<T, once><<<(unsigned)a.rows, BOTH_NT, 0, st>>>(a);
+    });
+  } else {
+    LogProbs b = a;
+    Carver c(work);
+    b.save = c.take<float>(4 * (size_t)a.rows);
+    fwd<T>(st, b, c.p + c.off);
+    bwd<T>(st, b);
   }
-  LogProbs b = a;
-  Carver c(work);
-  b.save = c.take<float>(4 * (size_t)a.rows);
-  fwd<T>(st, b, c.p + c.off);
-  bwd<T>(st, b);
 }
 
 template <class F>
@@ -746,12 +983,11 @@ void by_type(int dtype, F f) {
 }  // namespace
 
 size_t logprobs_work_bytes(int dtype, int64_t rows, int V, int K) {
-  if (rows <= 0) return 0;
-  const int s = splits_of(dtype, rows, V);
-  if (s == 1) return 0;
+  if (rows <= 0 || V <= WAVE_MAX) return 0;
+  const Split s = split_of(dtype, rows, V);
   Sizer z;
-  z.take<float>(4 * (size_t)rows);
-  parts_of(z, rows, s, K);
+  if (s.splits > 1 || in_parts(dtype, rows, V)) z.take<float>(4 * (size_t)rows);
+  if (s.splits > 1) parts_of(z, rows, s.splits, K);
   return z.off;
 }
 

@@ -49,7 +49,7 @@ class TensorList {
   uint32_t magic = MAGIC;
 
   std::vector<ListEntry> entries;  // the non-empty tensors
-  int64_t total = 0, chunk = 0;
+  int64_t total = 0, bytes = 0, chunk = 0;  // elements, of all operands, of a chunk
   uint32_t chunks = 0;
   ListEntry* dev = nullptr;        // device table (beyond LIST_INLINE)
   int32_t* dev_owner = nullptr;    // chunk -> entry

@@ -22,11 +22,17 @@ struct Vec {
   struct __attribute__((packed, aligned(sizeof(T)))) Raw {
     u32x4 v;
   };
+  // ONCE: nontemporal, for what passes by once and would only displace what is
+  // read again
+  template <bool ONCE = false>
   static __device__ __forceinline__ u32x4 load(const T* p) {
-    return global_ptr<const Raw>(p)->v;
+    if constexpr (ONCE) return __builtin_nontemporal_load(&global_ptr<const Raw>(p)->v);
+    else return global_ptr<const Raw>(p)->v;
   }
+  template <bool ONCE = false>
   static __device__ __forceinline__ void store(T* p, u32x4 v) {
-    global_ptr<Raw>(p)->v = v;
+    if constexpr (ONCE) __builtin_nontemporal_store(v, &global_ptr<Raw>(p)->v);
+    else global_ptr<Raw>(p)->v = v;
   }
   static __device__ __forceinline__ void unpack(u32x4 v, float* x) {
     typedef T Tv __attribute__((ext_vector_type(N)));
@@ -51,17 +57,22 @@ struct Few {
   struct __attribute__((packed, aligned(sizeof(T)))) Raw {
     V v;
   };
+  template <bool ONCE>
   static __device__ __forceinline__ void load(const T* p, float* x) {
-    const V v = global_ptr<const Raw>(p)->v;
+    V v;
+    if constexpr (ONCE) v = __builtin_nontemporal_load(&global_ptr<const Raw>(p)->v);
+    else v = global_ptr<const Raw>(p)->v;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = (float)v[i];
   }
   // rounded to nearest even, once
+  template <bool ONCE>
   static __device__ __forceinline__ void store(T* p, const float* x) {
     V v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (T)x[i];
-    global_ptr<Raw>(p)->v = v;
+    if constexpr (ONCE) __builtin_nontemporal_store(v, &global_ptr<Raw>(p)->v);
+    else global_ptr<Raw>(p)->v = v;
   }
 };
 

@@ -24,7 +24,8 @@ def _ptr(t):
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the handle alone: building a torch.cuda.Stream takes longer than a launch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _f32(t, shape, name):
@@ -771,14 +772,14 @@ class LogProbs:
 
     @staticmethod
     def _rows(t, what):
-        """(tensor, its row stride) of [..., classes] as rows."""
+        """(address, row stride) of [..., classes] as rows."""
         if t.dim() == 0 or t.dtype not in _DTYPES:
             raise ValueError(f"{what}: expected float32, float16 or bfloat16 [..., classes], got "
                              f"{t.dtype} {tuple(t.shape)}")
         _current(t, what)
         v = t.shape[-1]
         if t.is_contiguous():
-            return t, v
+            return t.data_ptr(), v
         if t.dim() > 2:
             try:
                 t = t.view(-1, v)
@@ -786,70 +787,91 @@ class LogProbs:
                 raise ValueError(f"{what}: the leading dimensions have no one stride") from None
         if t.stride(-1) != 1 and v > 1:
             raise ValueError(f"{what}: a row's elements must be contiguous")
-        return t, (t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else v)
+        return t.data_ptr(), (t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else v)
 
     def _operands(self, logits, targets):
         x, ld = self._rows(logits, "logits")
-        v, lead = logits.shape[-1], logits.shape[:-1]
+        shape = logits.shape
+        v, lead = shape[-1], shape[:-1]
         rows = logits.numel() // v if v else 0
-        bits = 32
+        t, bits = None, 32
         if targets is not None:
-            if targets.dtype not in (torch.int32, torch.int64) or targets.shape != lead:
-                raise ValueError(f"targets: expected int32 or int64 {tuple(lead)}, got "
-                                 f"{targets.dtype} {tuple(targets.shape)}")
-            bits = 64 if targets.dtype == torch.int64 else 32
-            _current(targets, "targets")
-        return (_DTYPES[x.dtype], x.data_ptr(), ld, rows, v, _ptr(targets), bits), rows, v, lead
+            if targets.dtype == torch.int64:
+                bits = 64
+            elif targets.dtype != torch.int32:
+                raise ValueError(f"targets: expected int32 or int64, got {targets.dtype}")
+            if targets.shape != lead:
+                raise ValueError(f"targets: expected {tuple(lead)}, got {tuple(targets.shape)}")
+            t = self._given(targets, "targets")
+        return (_DTYPES[logits.dtype], x, ld, rows, v, t, bits), rows, v, lead
 
     @staticmethod
-    def _cotangent(t, shape, what):
-        if t is not None:
-            _f32(t, shape, what)
-            _current(t, what)
-        return _ptr(t)
+    def _given(t, what):
+        """The address of a contiguous operand on the current device."""
+        if not _current(t, what).is_contiguous():
+            raise ValueError(f"{what}: expected a contiguous tensor")
+        return t.data_ptr()
+
+    def _cotangent(self, t, shape, what):
+        if t is None:
+            return None
+        _f32(t, shape, what)
+        return self._given(t, what)
 
     @staticmethod
     def _work(code, rows, v, top, device):
+        """(scratch, its address) of a forward; one without any needs none."""
         n = lib().bc2n_logprobs_work_bytes(code, rows, v, top)
-        return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        if n == 0:
+            return None, None
+        work = torch.empty(n, dtype=torch.uint8, device=device)
+        return work, work.data_ptr()
 
     def _gradient(self, logits, out):
         if out is None:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            out = torch.empty_like(logits, memory_format=torch.contiguous_format)
         if out.dtype != logits.dtype or out.shape != logits.shape:
             raise ValueError(f"out: expected {logits.dtype} {tuple(logits.shape)}, got {out.dtype} "
                              f"{tuple(out.shape)}")
-        o, ld = self._rows(out, "out")
-        return out, o.data_ptr(), ld
+        return (out, *self._rows(out, "out"))
 
     def forward(self, logits, targets=None):
         """-> ((logp, entropy, top_logp, top_index), save); logp is None without
         targets, the last two with top=0."""
         operands, rows, v, lead = self._operands(logits, targets)
-        dev = logits.device
-        e = lambda *sh: torch.empty(*sh, dtype=torch.float32, device=dev)
-        logp = e(lead) if targets is not None else None
-        entropy, save = e(lead), e(rows, 4)
-        top_logp = e(*lead, self.top) if self.top else None
-        top_index = torch.empty(*lead, self.top, dtype=torch.int32, device=dev) if self.top else None
-        work = self._work(operands[0], rows, v, self.top, dev)
-        check(lib().bc2n_logprobs_fwd(_stream(), *operands, self.top, _ptr(logp), _ptr(entropy),
-                                      _ptr(top_logp), _ptr(top_index), _ptr(save), _ptr(work)))
+        dev, f32, top = logits.device, torch.float32, self.top
+        logp = top_logp = top_index = a = b = c = None
+        if targets is None:
+            entropy = torch.empty(lead, dtype=f32, device=dev)
+        else:  # empty_like takes half the time that a shape takes
+            logp, entropy = torch.empty_like(targets, dtype=f32), torch.empty_like(targets, dtype=f32)
+            a = logp.data_ptr()
+        save = torch.empty(4 * rows, dtype=f32, device=dev)
+        if top:
+            top_logp = torch.empty((*lead, top), dtype=f32, device=dev)
+            top_index = torch.empty((*lead, top), dtype=torch.int32, device=dev)
+            b, c = top_logp.data_ptr(), top_index.data_ptr()
+        work, w = self._work(operands[0], rows, v, top, dev)
+        check(lib().bc2n_logprobs_fwd(_stream(), *operands, top, a, entropy.data_ptr(), b, c,
+                                      save.data_ptr(), w))
         return (logp, entropy, top_logp, top_index), save
 
     def backward(self, cts, logits, targets, top_index, save, out=None):
         """cts = (d_logp, d_entropy, d_top_logp), any None -> d_logits (in `out`
         where given, which may be logits itself)"""
         operands, rows, v, lead = self._operands(logits, targets)
-        if tuple(save.shape) != (rows, 4):
-            raise ValueError(f"save: expected the forward's of {rows} rows, got {tuple(save.shape)}")
-        if top_index is not None and (top_index.dtype != torch.int32
-                                      or tuple(top_index.shape) != (*lead, self.top)):
-            raise ValueError(f"top_index: expected int32 {(*lead, self.top)}")
-        c = [self._cotangent(t, sh, n) for t, sh, n in zip(
-            cts, (lead, lead, (*lead, self.top)), ("d_logp", "d_entropy", "d_top_logp"))]
+        _f32(save, (4 * rows,), "save")
+        i = None
+        if top_index is not None:
+            if top_index.dtype != torch.int32 or top_index.shape != (*lead, self.top):
+                raise ValueError(f"top_index: expected int32 {(*lead, self.top)}, got "
+                                 f"{top_index.dtype} {tuple(top_index.shape)}")
+            i = self._given(top_index, "top_index")
+        d_logp, d_entropy, d_top = cts
+        c = (self._cotangent(d_logp, lead, "d_logp"), self._cotangent(d_entropy, lead, "d_entropy"),
+             self._cotangent(d_top, (*lead, self.top), "d_top_logp"))
         out, o, ld = self._gradient(logits, out)
-        check(lib().bc2n_logprobs_bwd(_stream(), *operands, self.top, _ptr(top_index), _ptr(save),
+        check(lib().bc2n_logprobs_bwd(_stream(), *operands, self.top, i, self._given(save, "save"),
                                       *c, o, ld))
         return out
 
@@ -857,14 +879,17 @@ class LogProbs:
         """((logp, entropy), d_logits) in one call, for cotangents known
         beforehand (a likelihood with given weights); no alternatives."""
         operands, rows, v, lead = self._operands(logits, targets)
-        dev = logits.device
-        c = [self._cotangent(t, lead, n) for t, n in ((d_logp, "d_logp"), (d_entropy, "d_entropy"))]
+        dev, logp, a = logits.device, None, None
+        c = self._cotangent(d_logp, lead, "d_logp"), self._cotangent(d_entropy, lead, "d_entropy")
         out, o, ld = self._gradient(logits, out)
-        logp = torch.empty(lead, dtype=torch.float32, device=dev) if targets is not None else None
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-        work = self._work(operands[0], rows, v, 0, dev)
-        check(lib().bc2n_logprobs_grad(_stream(), *operands, *c, _ptr(logp), _ptr(entropy), o, ld,
-                                       _ptr(work)))
+        if targets is None:
+            entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+        else:
+            logp = torch.empty_like(targets, dtype=torch.float32)
+            entropy = torch.empty_like(logp)
+            a = logp.data_ptr()
+        work, w = self._work(operands[0], rows, v, 0, dev)
+        check(lib().bc2n_logprobs_grad(_stream(), *operands, *c, a, entropy.data_ptr(), o, ld, w))
         return (logp, entropy), out
 
 
@@ -875,13 +900,13 @@ class _TensorList:
     def __init__(self, handle, tensors):
         if not handle:
             check(1)
-        self.handle, self.tensors = handle, tensors
+        self.handle, self.tensors, self._free = handle, tensors, lib().bc2n_list_free
         self.device = next((t.device for t in tensors), torch.device("cuda"))
         self.work_bytes = lib().bc2n_list_work_bytes(handle)
 
     def __del__(self):
         if getattr(self, "handle", None):
-            lib().bc2n_list_free(self.handle)
+            self._free(self.handle)
             self.handle = None
 
     @staticmethod
@@ -909,10 +934,15 @@ class _TensorList:
         return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
 
     def _scratch(self):
-        if self.device.index is not None and self.device.index != torch.cuda.current_device():
-            raise ValueError(f"the list is on {self.device}, which is not the current device")
-        return (torch.empty(1, dtype=torch.float32, device=self.device),
-                torch.empty(self.work_bytes, dtype=torch.uint8, device=self.device))
+        """(norm, scratch, its address), on the list's device, the current one."""
+        dev = self.device
+        if dev.index is not None and dev.index != torch.cuda.current_device():
+            raise ValueError(f"the list is on {dev}, which is not the current device")
+        norm = torch.empty(1, dtype=torch.float32, device=dev)
+        if self.work_bytes == 0:
+            return norm, None, None
+        work = torch.empty(self.work_bytes, dtype=torch.uint8, device=dev)
+        return norm, work, work.data_ptr()
 
 
 class GradientClip(_TensorList):
@@ -934,15 +964,15 @@ class GradientClip(_TensorList):
 
     def norm(self):
         """-> f32 [1] on the device"""
-        norm, work = self._scratch()
-        check(lib().bc2n_grad_norm(_stream(), self.handle, _ptr(norm), _ptr(work)))
+        norm, work, w = self._scratch()
+        check(lib().bc2n_grad_norm(_stream(), self.handle, norm.data_ptr(), w))
         return norm
 
     def clip(self, max_norm):
         """Scales by max_norm / norm where the norm is not below max_norm (a copy
         into `out` elsewhere) -> the norm before, f32 [1] on the device"""
-        norm, work = self._scratch()
-        check(lib().bc2n_grad_clip(_stream(), self.handle, float(max_norm), _ptr(norm), _ptr(work)))
+        norm, work, w = self._scratch()
+        check(lib().bc2n_grad_clip(_stream(), self.handle, float(max_norm), norm.data_ptr(), w))
         return norm
 
 
@@ -977,7 +1007,7 @@ class Adam(_TensorList):
         global norm first -> their norm before, f32 [1] on the device (None
         without).  scalars: f32 [2] on the device, lr and step in place of the
         arguments."""
-        norm, work = self._scratch()
+        norm, work, w = self._scratch()
         if max_norm is None:
             norm = None
         elif not max_norm > 0:
@@ -987,7 +1017,7 @@ class Adam(_TensorList):
             _current(scalars, "scalars")
         check(lib().bc2n_adam_step(_stream(), self.handle, float(lr), *self.betas, self.eps,
                                    self.weight_decay, int(step), float(max_norm or 0.0),
-                                   _ptr(scalars), _ptr(norm), _ptr(work)))
+                                   _ptr(scalars), _ptr(norm), w))
         return norm
 
 

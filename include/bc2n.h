@@ -17,6 +17,8 @@
  * call records an event on its stream after its last launch and a call on
  * another stream first waits for it, so calls run one after another as on
  * one stream (under graph capture only the capturing stream orders a call).
+ * The log-probability and gradient-list calls use no library scratch and take
+ * no part in this: their stream alone orders them, as any kernel's launch.
  * Calls from several host threads must not overlap.
  *
  * Lengths: N (residues) must be a multiple of 32 -- the reference's caller
@@ -671,7 +673,7 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
  *     updated ones go.
  * Calls: norm f32[1] = sqrt(sum of all squares), summed in 64 bits in one
  * order; work is bc2n_list_work_bytes() bytes, 16-byte aligned, for the time
- * of the call.
+ * of the call (NULL where that is 0: a small list).
  *   grad_clip: out = g c, c = 1 where norm < max_norm, else max_norm / norm
  *     (a norm that is NaN makes all of it NaN); norm may be NULL.
  *   adam_step: with g the gradient times c (max_norm 0: not clipped),

@@ -48,6 +48,7 @@ def test_logprobs_refusals():
     assert b.lib().bc2n_logprobs_work_bytes(7, 4, 64, 0) == 0
     assert b"dtype" in b.lib().bc2n_last_error()
     assert b.lib().bc2n_logprobs_save_bytes(10) == 160
+    assert b.lib().bc2n_logprobs_work_bytes(F16, 9, 8192, 32) == 0
 
 
 def ptrs(*v):
@@ -78,6 +79,9 @@ def test_list_refusals():
     no_list(grad_list([P], [8], out=[P + 4]), b"shares memory")
     no_list(L.bc2n_grad_list(-1, None, None, None, None), b"null")
     h = grad_list([P, P + 16, None], [4, 4, 0], out=[P, P + 16, None])  # neighbours
+    assert h and L.bc2n_list_work_bytes(h) == 0  # a small list needs none
+    L.bc2n_list_free(h)
+    h = grad_list([P, P + 400000, None], [100000, 4, 0], out=[P, P + 400000, None])
     assert h and L.bc2n_list_work_bytes(h) > 0
     refused(L.bc2n_grad_clip(None, h, 0.0, P, P), b"max_norm")
     refused(L.bc2n_grad_clip(None, h, float("nan"), P, P), b"max_norm")
@@ -95,7 +99,9 @@ def test_adam_refusals():
     L = b.lib()
     one = lambda t, v: (t * 1)(v)  # noqa: E731
 
-    def make(p=P, g=2 * P, m=3 * P, v=4 * P, po=P, mo=3 * P, vo=4 * P, pt=F32, gt=F32, n=64):
+    def make(p=P, g=2 * P, m=3 * P, v=4 * P, po=P, mo=3 * P, vo=4 * P, pt=F32, gt=F32, n=64,
+             far=1):
+        p, g, m, v, po, mo, vo = (x and x * far for x in (p, g, m, v, po, mo, vo))
         return L.bc2n_adam_list(1, one(ctypes.c_int64, n), ptrs(p), one(ctypes.c_int, pt), ptrs(g),
                                 one(ctypes.c_int, gt), ptrs(m), ptrs(v), ptrs(po), ptrs(mo), ptrs(vo))
 
@@ -105,6 +111,9 @@ def test_adam_refusals():
     no_list(make(g=P), b"shares memory")
     no_list(make(m=3 * P + 2, mo=3 * P + 2), b"unaligned")
     h = make(pt=BF16, gt=F16, p=P + 2, po=P + 2)
+    assert h and L.bc2n_list_work_bytes(h) == 0
+    L.bc2n_list_free(h)
+    h = make(n=100000, far=100)
     assert h
 
     def step(lr=0.1, b1=0.9, b2=0.99, eps=1e-8, wd=0.0, t=1, mx=0.0, work=P):
