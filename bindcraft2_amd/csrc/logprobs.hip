@@ -97,12 +97,21 @@ __device__ __forceinline__ void write_row(const LogProbs& a, int64_t r, const Ro
   if (a.save) reinterpret_cast<float4*>(a.save)[r] = make_float4(st.m, st.logs, st.h, st.live);
 }
 
-// The gradient at one element without the terms of single classes.
+// The gradient at one element without the terms of single classes:
+// -p (g + e (log p + H)), in units of log 2.
 struct Cotangent {
-  float m, logs, h, g, e;  // g: those of logp and the alternatives together
+  float m, l2;    // log2 of the sum
+  float gh, e2;   // g + e H, e log 2; g with those of the alternatives
+  __device__ __forceinline__ Cotangent(const RowStat& st, float g, float e)
+      : m(st.m), l2(st.logs * LOG2E), gh(fmaf(e, st.h, g)), e2(e * LN2) {}
   __device__ __forceinline__ float at(float x) const {
-    const float lp = (x - m) - logs;
-    return -exp_f(lp) * fmaf(e, fmaxf(lp, FAR) + h, g);
+    const float lp2 = fmaf(x - m, LOG2E, -l2), p = __builtin_amdgcn_exp2f(lp2);
+    return -p * fmaf(e2, fmaxf(lp2, FAR), gh);
+  }
+  template <int N>
+  __device__ __forceinline__ void all(float (&x)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = at(x[i]);
   }
 };
 
@@ -119,20 +128,270 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float value_of_key(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
 }
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// with the other 16-lane row of its pair, with the other half of the wave
+__device__ __forceinline__ uint32_t swap16_max(uint32_t v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return umax(a[0], a[1]);
+}
+__device__ __forceinline__ uint32_t swap32_max(uint32_t v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return umax(a[0], a[1]);
+}
 template <int W>
 __device__ __forceinline__ uint32_t group_umax(uint32_t v) {
   if constexpr (W >= 2) v = umax(v, dpp_u32<DPP_QUAD_1032>(v));
   if constexpr (W >= 4) v = umax(v, dpp_u32<DPP_QUAD_2301>(v));
   if constexpr (W >= 8) v = umax(v, dpp_u32<DPP_ROW_HALF_MIRROR>(v));
   if constexpr (W >= 16) v = umax(v, dpp_u32<DPP_ROW_MIRROR>(v));
-  if constexpr (W >= 32) v = umax(v, (uint32_t)__shfl_xor((int)v, 16, 64));
-  if constexpr (W >= 64) v = umax(v, (uint32_t)__shfl_xor((int)v, 32, 64));
+  if constexpr (W >= 32) v = swap16_max(v);
+  if constexpr (W >= 64) v = swap32_max(v);
   return v;
+}
+
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float v, Op op) {
+  v = group_reduce<16>(v, op);
+  auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v),
+                                            __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  v = op(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                            __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return op(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_reduce(v, [](float a, float b) { return a + b; });
+}
+
+template <int N>
+__device__ __forceinline__ float max_of(const float (&x)[N]) {
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+  return m;
+}
+__device__ __forceinline__ float read_lane(float v, int lane) {
+  return __builtin_bit_cast(float,
+                            __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+// key of the float just below the one of this key; there is none below -inf
+__device__ __forceinline__ uint32_t key_below(uint32_t k) {
+  return k == 0x80000000u ? k - 2 : k - 1;  // below 0 lies the smallest negative, not -0
+}
+
+// A wave's largest elements, the k-th in lane k (index -1: none yet).  An
+// element not above `floor` is not among the row's: the wave has K as large
+// that come before it.  Waves of one row tell each other, through LDS, values
+// that K elements reach (*shared, as a key), so that a wave does not collect
+// what another has better; when they learn it changes only what is collected
+// beside the answer.
+struct TopList {
+  float v = NEG_INF;
+  int i = -1;
+  float floor = NEG_INF;
+
+  __device__ __forceinline__ void insert(float cv, int ci, int K) {
+    const int lane = threadIdx.x & 63;
+    const int before = __popcll(__ballot(v > cv) | (__ballot(v == cv) & __ballot(i < ci)));
+    const float pv = dpp_mov<0x138>(v);  // the lane before
+    const int pi = (int)dpp_u32<0x138>((uint32_t)i);
+    v = lane > before ? pv : lane == before ? cv : v;
+    i = lane > before ? pi : lane == before ? ci : i;
+    floor = fmaxf(floor, read_lane(v, K - 1));
+  }
+
+  // K lanes hold an element as large as the K-th largest of the lanes' maxima
+  // mx, so nothing below it can stay: without this bound the first elements
+  // would enter the list one by one.  Returns its key (0: none).
+  __device__ __forceinline__ uint32_t bound(float mx, int K) {
+    const int lane = threadIdx.x & 63;
+    float t = NEG_INF;
+    for (int k = 0; k < K; ++k) {
+      t = wave_max(mx);
+      const uint64_t b = __ballot(mx == t);
+      if (b == 0) break;
+      if (lane == __ffsll((unsigned long long)b) - 1) mx = NEG_INF;
+    }
+    if (!(t > NEG_INF)) return 0;
+    const uint32_t reached = order_key(t);
+    floor = fmaxf(floor, value_of_key(key_below(reached)));
+    return reached;
+  }
+  // element x of each lane; index(lane) its index
+  template <class F>
+  __device__ __forceinline__ void offer(float x, int K, F index) {
+    // out of order among the lanes' elements, so an equal one may be better
+    for (uint64_t b = __ballot(x >= floor); b; b &= b - 1) {
+      const int from = __ffsll((unsigned long long)b) - 1;
+      const float cv = read_lane(x, from);
+      if (cv > NEG_INF && cv >= floor) insert(cv, index(from), K);  // else the list rose since
+    }
+  }
+
+  // x: this lane's elements of one chunk, vector u from index i0 + u * step;
+  // mx: their maximum
+  template <int VN, bool SHARE, int N>
+  __device__ __forceinline__ void take(const float (&x)[N], float mx, int i0, int step, int K,
+                                       bool first, uint32_t* shared) {
+    if (!__any(mx > floor)) return;
+    if (SHARE) {
+      const uint32_t k = __hip_atomic_load(shared, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (k) floor = fmaxf(floor, value_of_key(key_below(k)));
+      if (!__any(mx > floor)) return;
+    }
+    uint32_t reached = first ? bound(mx, K) : 0;
+    const float before = floor;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      offer(x[n], K, [&](int from) {
+        return __builtin_amdgcn_readlane(i0, from) + n / VN * step + n % VN;
+      });
+    if (SHARE) {
+      if (floor > before) reached = order_key(floor);
+      if (reached && (threadIdx.x & 63) == 0)
+        __hip_atomic_fetch_max(shared, reached, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+  }
+};
+
+// A row's alternative k, by one lane
+__device__ __forceinline__ void write_top(const LogProbs& a, int64_t r, int k, const RowStat& st,
+                                          bool counts, float v, int i) {
+  const bool bad = is_nan(st.logs);
+  a.top_logp[r * a.K + k] = bad ? st.logs : counts ? log_prob(st, v) : 0.f;
+  a.top_index[r * a.K + k] = bad || !counts ? -1 : i;
+}
+
+// Where a row has only `have` < K alternatives above -inf, its first -inf
+// elements follow; by one wave.
+template <class T>
+__device__ __forceinline__ void fill_tops(const LogProbs& a, int64_t r, int have) {
+  const int lane = threadIdx.x & 63;
+  const T* p = reinterpret_cast<const T*>(a.x) + r * a.ld;
+  for (int b = 0; have < a.K && b < a.V; b += 64) {
+    const bool gone = b + lane < a.V && (float)p[b + lane] == NEG_INF;
+    const uint64_t m = __ballot(gone);
+    const int k = have + __popcll(m & ((1ull << lane) - 1));
+    if (gone && k < a.K) {
+      a.top_logp[r * a.K + k] = NEG_INF;
+      a.top_index[r * a.K + k] = b + lane;
+    }
+    have += __popcll(m);
+  }
+}
+
+// 16-bit logits: a key holds an element's order and its index's complement
+// (rows here have at most 1024), so the largest of a group is the next
+// alternative, index and all, and is taken out by comparing keys.
+template <class T, int W, int E>
+__device__ __forceinline__ void tops_by_key(const LogProbs& a, int64_t r, bool mine,
+                                            const RowStat& st, bool counts, uint32_t (&key)[E]) {
+  const int l = threadIdx.x & (W - 1);
+  uint32_t kept = 0;
+  for (int k = 0; k < a.K; ++k) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) best = umax(best, key[i]);
+    best = group_umax<W>(best);
+#pragma unroll
+    for (int i = 0; i < E; ++i) key[i] = key[i] == best ? 0u : key[i];
+    if (l == (k & (W - 1))) kept = best;
+    if ((k & (W - 1)) == W - 1 || k == a.K - 1) {  // W of them together
+      const int at = (k & ~(W - 1)) + l;
+      const uint32_t o = kept >> 16, bits = o & 0x8000u ? o ^ 0x8000u : o ^ 0xffffu;
+      if (mine && at <= k)
+        write_top(a, r, at, st, counts, (float)__builtin_bit_cast(T, (uint16_t)bits),
+                  0xffff - (int)(kept & 0xffffu));
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ uint32_t key16(float x, int i) {
+  const uint32_t b = __builtin_bit_cast(uint16_t, (T)(x + 0.f));
+  return (b & 0x8000u ? b ^ 0xffffu : b ^ 0x8000u) << 16 | (0xffffu - (uint32_t)i);
+}
+
+// f32 logits: each lane's elements in descending order, equal ones as they
+// were (neighbours change places); the largest first element of the group is
+// the next alternative, and the lowest lane that has it holds the lowest index.
+template <int W, int E>
+__device__ __forceinline__ void tops_by_lane(const LogProbs& a, int64_t r, bool mine,
+                                             const RowStat& st, bool counts, uint32_t (&key)[E],
+                                             int (&at)[E]) {
+  const int l = threadIdx.x & (W - 1), lane0 = (threadIdx.x & 63) - l;
+  if (a.K == 1) {  // the first of the largest is enough
+#pragma unroll
+    for (int i = 1; i < E; ++i) {
+      const bool more = key[i] > key[0];
+      key[0] = more ? key[i] : key[0];
+      at[0] = more ? at[i] : at[0];
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < E; ++p)
+#pragma unroll
+      for (int i = p & 1; i + 1 < E; i += 2) {
+        const bool swap = key[i] < key[i + 1];
+        const uint32_t x = key[i], y = key[i + 1];
+        const int u = at[i], v = at[i + 1];
+        key[i] = swap ? y : x;
+        key[i + 1] = swap ? x : y;
+        at[i] = swap ? v : u;
+        at[i + 1] = swap ? u : v;
+      }
+  }
+  for (int k = 0; k < a.K; ++k) {
+    const uint32_t top = group_umax<W>(key[0]);
+    const uint64_t b = __ballot(key[0] == top) >> lane0;
+    const int first = W <= 32 ? __ffs((int)b) : __ffsll((unsigned long long)b);
+    if (l == first - 1) {
+      if (mine) write_top(a, r, k, st, counts, value_of_key(top), at[0]);
+#pragma unroll
+      for (int i = 0; i + 1 < E; ++i) {
+        key[i] = key[i + 1];
+        at[i] = at[i + 1];
+      }
+      key[E - 1] = 0;
+    }
+  }
+}
+
+// f32 logits of a row that is a wave's, more than four a lane: a sort of them
+// would cost more than the list (K = 3 of 100 k rows of 500: 79 us).
+template <class T, int VN, int NV>
+__device__ __forceinline__ void tops_by_list(const LogProbs& a, int64_t r, bool mine,
+                                             const RowStat& st, bool counts,
+                                             const float (&x)[VN * NV], const int (&pos)[NV],
+                                             const int (&skip)[NV]) {
+  const int lane = threadIdx.x & 63;
+  TopList top;
+  if (counts && !is_nan(st.logs)) {
+    float y[VN * NV];
+#pragma unroll
+    for (int i = 0; i < VN * NV; ++i) y[i] = i % VN >= skip[i / VN] ? x[i] : NEG_INF;
+    top.bound(max_of(y), a.K);
+#pragma unroll
+    for (int i = 0; i < VN * NV; ++i)
+      top.offer(y[i], a.K, [&](int from) {
+        return __builtin_amdgcn_readlane(pos[i / VN], from) + i % VN;
+      });
+  }
+  if (!mine) return;
+  const bool some = counts && !is_nan(st.logs);
+  if (lane < a.K && (top.i >= 0 || !some)) write_top(a, r, lane, st, counts, top.v, top.i);
+  if (some) fill_tops<T>(a, r, __popcll(__ballot(lane < a.K && top.i >= 0)));
 }
 
 template <class T, int VN, int W, int NV, int MODE>
@@ -175,39 +434,20 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LogProbs a) {
     if (mine && l == 0) write_row<T>(a, r, st, a.target ? t : -1);
 
     if (MODE == 1 && a.K > 0) {
-      uint32_t key[E];
+      if constexpr (sizeof(T) == 4 && E > 4) {
+        tops_by_list<T, VN, NV>(a, r, mine, st, counts, x, pos, skip);
+      } else {
+        uint32_t key[E];
+        int at[E];
 #pragma unroll
-      for (int i = 0; i < E; ++i) key[i] = i % VN >= skip[i / VN] ? order_key(x[i]) : 0u;
-      const int lane0 = (threadIdx.x & 63) - l;
-      for (int k = 0; k < a.K; ++k) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) best = umax(best, key[i]);
-        const uint32_t top = group_umax<W>(best);
-        const uint64_t at = __ballot(best == top) >> lane0;
-        if (l == __ffsll((unsigned long long)at) - 1) {
-          // the first of this lane's elements that holds it
-          int idx = 0;
-          float v = 0.f;
-#pragma unroll
-          for (int i = E - 1; i >= 0; --i)
-            if (key[i] == top) {
-              idx = i;
-              v = x[i];
-            }
-          int where = 0;
-#pragma unroll
-          for (int i = 0; i < E; ++i)
-            if (i == idx) {
-              key[i] = 0u;
-              where = pos[i / VN] + i % VN;
-            }
-          if (mine) {
-            const bool bad = is_nan(st.logs);
-            a.top_logp[r * a.K + k] = bad ? st.logs : counts ? log_prob(st, v) : 0.f;
-            a.top_index[r * a.K + k] = bad || !counts ? -1 : where;
-          }
+        for (int i = 0; i < E; ++i) {
+          at[i] = pos[i / VN] + i % VN;
+          const bool real = i % VN >= skip[i / VN];
+          if constexpr (sizeof(T) == 2) key[i] = real ? key16<T>(x[i], at[i]) : 0u;
+          else key[i] = real ? order_key(x[i]) : 0u;
         }
+        if constexpr (sizeof(T) == 2) tops_by_key<T, W>(a, r, mine, st, counts, key);
+        else tops_by_lane<W>(a, r, mine, st, counts, key, at);
       }
     }
   } else {
@@ -217,10 +457,11 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LogProbs a) {
 
   if constexpr (MODE & 2) {
     const float g = a.d_logp ? a.d_logp[r] : 0.f;
-    Cotangent c{st.m, st.logs, st.h, g, a.d_entropy ? a.d_entropy[r] : 0.f};
+    float all = g;
     if (MODE == 2 && a.d_top)
-      for (int k = 0; k < a.K; ++k) c.g += a.d_top[r * a.K + k];
-    if (a.d_logp && t >= a.V) c.g = __builtin_nanf("");
+      for (int k = 0; k < a.K; ++k) all += a.d_top[r * a.K + k];
+    if (a.d_logp && t >= a.V) all = __builtin_nanf("");
+    const Cotangent c(st, all, a.d_entropy ? a.d_entropy[r] : 0.f);
     float d[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) d[i] = c.at(x[i]);
@@ -259,25 +500,6 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LogProbs a) {
 // the first wave.  (Aligned vectors: 50 against 56 us for 2047 rows of 50 k
 // binary16 logits that start anywhere.)
 // ---------------------------------------------------------------------------
-template <class Op>
-__device__ __forceinline__ float wave_reduce(float v, Op op) {
-  v = group_reduce<16>(v, op);
-  auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v),
-                                            __builtin_bit_cast(uint32_t, v), false, false);
-  const uint32_t a0 = a[0], a1 = a[1];
-  v = op(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
-  auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
-                                            __builtin_bit_cast(uint32_t, v), false, false);
-  const uint32_t b0 = b[0], b1 = b[1];
-  return op(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
-}
-__device__ __forceinline__ float wave_max(float v) {
-  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float wave_sum(float v) {
-  return wave_reduce(v, [](float a, float b) { return a + b; });
-}
-
 template <class T>
 struct Row {
   static constexpr int VN = Vec<T>::N;
@@ -302,32 +524,48 @@ struct Row {
 // A chunk: E elements a lane, U vectors apart by the workgroup's width
 constexpr int E = 16;
 
-// vectors base + u * NT + lane below v1, -inf past it
-template <class T, int NT>
-__device__ __forceinline__ void fetch(const Row<T>& r, int base, int v1, u32x4 (&raw)[E / Vec<T>::N]) {
-  constexpr int U = E / Vec<T>::N;
-  const int g = base + (int)threadIdx.x;
-  if (base + U * NT <= v1) {
+// f(chunk, base) for the chunks of U vectors a lane of [v0, v1): chunk[u] is
+// vector base + u * NT + lane, -inf past v1.  While one is worked on the next
+// is on its way: two buffers that take turns, so that no copy waits for it.
+template <class T, int NT, int U, class F>
+__device__ __forceinline__ void each_chunk(const Row<T>& r, int v0, int v1, F f) {
+  constexpr int STEP = U * NT;
+  const int t = threadIdx.x;
+  u32x4 a[U], b[U];
+  auto fetch = [&](int base, u32x4(&c)[U]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = r.load(g + u * NT);
-  } else {
+    for (int u = 0; u < U; ++u) c[u] = r.load(base + u * NT + t);
+  };
+  const int full = (v1 - v0) / STEP, end = v0 + full * STEP;
+  int base = v0;
+  if (full > 0) {
+    fetch(base, a);
+    for (; base + 2 * STEP < end; base += 2 * STEP) {
+      fetch(base + STEP, b);
+      f(a, base);
+      fetch(base + 2 * STEP, a);
+      f(b, base + STEP);
+    }
+    if (base + STEP < end) {
+      fetch(base + STEP, b);
+      f(a, base);
+      f(b, base + STEP);
+    } else {
+      f(a, base);
+    }
+  }
+  if (end < v1) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      raw[u] = Row<T>::none();
-      if (g + u * NT < v1) raw[u] = r.load(g + u * NT);
+      a[u] = Row<T>::none();
+      if (end + u * NT + t < v1) a[u] = r.load(end + u * NT + t);
     }
+    f(a, end);
   }
 }
 // Keeps the compiler from holding a vector's f32 values from one use to the
 // next, in twice the registers.
 __device__ __forceinline__ void as_stored(u32x4& v) { asm volatile("" : "+v"(v)); }
-template <int N>
-__device__ __forceinline__ float max_of(const float (&x)[N]) {
-  float m = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-  return m;
-}
 // a lane's running sums over one more chunk of maximum mx
 template <int N>
 __device__ __forceinline__ void add_chunk(Stat& q, const float (&x)[N], float mx) {
@@ -336,105 +574,16 @@ __device__ __forceinline__ void add_chunk(Stat& q, const float (&x)[N], float mx
   for (int i = 0; i < N; ++i) q.add(x[i]);
 }
 
-__device__ __forceinline__ float read_lane(float v, int lane) {
-  return __builtin_bit_cast(float,
-                            __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
-}
-// key of the float just below the one of this key; there is none below -inf
-__device__ __forceinline__ uint32_t key_below(uint32_t k) {
-  return k == 0x80000000u ? k - 2 : k - 1;  // below 0 lies the smallest negative, not -0
-}
-__device__ __forceinline__ float value_of_key(uint32_t k) {
-  return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
-}
-
-// A wave's largest elements, the k-th in lane k (index -1: none yet).  An
-// element not above `floor` is not among the row's: the wave has K as large
-// that come before it.  Waves of one row tell each other, through LDS, values
-// that K elements reach (*shared, as a key), so that a wave does not collect
-// what another has better; when they learn it changes only what is collected
-// beside the answer.
-struct TopList {
-  float v = NEG_INF;
-  int i = -1;
-  float floor = NEG_INF;
-
-  __device__ __forceinline__ void insert(float cv, int ci, int K) {
-    const int lane = threadIdx.x & 63;
-    const int before = __popcll(__ballot(v > cv) | (__ballot(v == cv) & __ballot(i < ci)));
-    const float pv = dpp_mov<0x138>(v);  // the lane before
-    const int pi = (int)dpp_u32<0x138>((uint32_t)i);
-    v = lane > before ? pv : lane == before ? cv : v;
-    i = lane > before ? pi : lane == before ? ci : i;
-    floor = fmaxf(floor, read_lane(v, K - 1));
-  }
-
-  // x: this lane's elements of one chunk, vector u from index i0 + u * step;
-  // mx: their maximum
-  template <int VN, bool SHARE>
-  __device__ __forceinline__ void take(const float (&x)[E], float mx, int i0, int step, int K,
-                                       bool first, uint32_t* shared) {
-    if (!__any(mx > floor)) return;
-    const int lane = threadIdx.x & 63;
-    if (SHARE) {
-      const uint32_t k = __hip_atomic_load(shared, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      if (k) floor = fmaxf(floor, value_of_key(key_below(k)));
-      if (!__any(mx > floor)) return;
-    }
-    uint32_t reached = 0;
-    if (first) {
-      // K lanes hold an element as large as the K-th largest of the lanes'
-      // maxima, so nothing below it can stay: without this bound the first
-      // chunk would enter the list one by one
-      float w = mx, t = NEG_INF;
-      for (int k = 0; k < K; ++k) {
-        t = wave_max(w);
-        const uint64_t b = __ballot(w == t);
-        if (b == 0) break;
-        if (lane == __ffsll((unsigned long long)b) - 1) w = NEG_INF;
-      }
-      if (t > NEG_INF) {
-        reached = order_key(t);
-        floor = fmaxf(floor, value_of_key(key_below(reached)));
-      }
-    }
-    const float before = floor;
-#pragma unroll
-    for (int n = 0; n < E; ++n) {
-      // out of order within the chunk, so an equal one may be better
-      for (uint64_t b = __ballot(x[n] >= floor); b; b &= b - 1) {
-        const int from = __ffsll((unsigned long long)b) - 1;
-        const float cv = read_lane(x[n], from);
-        const int ci = __builtin_amdgcn_readlane(i0, from) + n / VN * step + n % VN;
-        if (cv > NEG_INF && cv >= floor) insert(cv, ci, K);  // else the list rose since
-      }
-    }
-    if (SHARE) {
-      if (floor > before) reached = order_key(floor);
-      if (reached && lane == 0)
-        __hip_atomic_fetch_max(shared, reached, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    }
-  }
-  // one element a lane, at any index
-  __device__ __forceinline__ void take_edge(float x, int at, int K) {
-    for (uint64_t b = __ballot(x > NEG_INF && x >= floor); b; b &= b - 1) {
-      const int from = __ffsll((unsigned long long)b) - 1;
-      insert(read_lane(x, from), __builtin_amdgcn_readlane(at, from), K);
-    }
-  }
-};
-
-// Sum of a row over a wave's lanes, and over the workgroup's NT, in every lane
+// Sum of a row over a wave's lanes, and over the workgroup's waves, in every lane
 __device__ __forceinline__ Stat join_wave(Stat q) {
   q.raise(wave_max(q.m));
   q.s = wave_sum(q.s);
   q.u = wave_sum(q.u);
   return q;
 }
-template <int NT>
-__device__ __forceinline__ Stat join(Stat q, float (*buf)[4]) {
+__device__ __forceinline__ Stat join(Stat q, float (*buf)[4], int waves) {
   q = join_wave(q);
-  if constexpr (NT == 64) return q;
+  if (waves == 1) return q;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if (lane == 0) {
     buf[w][0] = q.m;
@@ -443,7 +592,7 @@ __device__ __forceinline__ Stat join(Stat q, float (*buf)[4]) {
   }
   __syncthreads();
   Stat o;
-  if (lane < NT / 64) {
+  if (lane < waves) {
     o.m = buf[lane][0];
     o.s = buf[lane][1];
     o.u = buf[lane][2];
@@ -496,17 +645,7 @@ __device__ __forceinline__ void write_tops(const LogProbs& a, int64_t r, const R
     const int lane = threadIdx.x;
     int have = 0;
     for (int c = 0; c < n; c += 64) have += __popcll(__ballot(c + lane < n && cand[c + lane] != 0));
-    const T* p = reinterpret_cast<const T*>(a.x) + r * a.ld;
-    for (int b = 0; have < a.K && b < a.V; b += 64) {
-      const bool gone = b + lane < a.V && (float)p[b + lane] == NEG_INF;
-      const uint64_t m = __ballot(gone);
-      const int k = have + __popcll(m & ((1ull << lane) - 1));
-      if (gone && k < a.K) {
-        ov[k] = NEG_INF;
-        oi[k] = b + lane;
-      }
-      have += __popcll(m);
-    }
+    fill_tops<T>(a, r, have);
   }
 }
 __device__ __forceinline__ void no_tops(const LogProbs& a, int64_t r, int nt) {
@@ -558,27 +697,25 @@ __global__ __launch_bounds__(NT, 8) void lp_stream_kernel(LogProbs a, int splits
   const float ex = edge ? (float)row.p[edge_at] : NEG_INF;
   Stat q;
   TopList top;
-  u32x4 raw[U];
-  if (v0 < v1) fetch<T, NT>(row, v0, v1, raw);
   if (SHARE) {
     if (threadIdx.x == 0) shared = 0;
     __syncthreads();
   }
-  for (int base = v0; base < v1; base += U * NT) {
+  each_chunk<T, NT, U>(row, v0, v1, [&](const u32x4(&raw)[U], int base) {
     float x[E];
 #pragma unroll
     for (int u = 0; u < U; ++u) Vec<T>::unpack(raw[u], x + u * VN);
-    if (base + U * NT < v1) fetch<T, NT>(row, base + U * NT, v1, raw);
     const float mx = max_of(x);
     add_chunk(q, x, mx);
     if (TOP)
       top.take<VN, SHARE>(x, mx, row.head + (base + (int)threadIdx.x) * VN, NT * VN, a.K,
                           base == v0, &shared);
-  }
+  });
   if (threadIdx.x < 64 && sp == 0) {
     const float one[1] = {ex};
     add_chunk(q, one, ex);
-    if (TOP) top.take_edge(ex, edge_at, a.K);
+    if (TOP)
+      top.offer(ex, a.K, [&](int from) { return __builtin_amdgcn_readlane(edge_at, from); });
   }
   if (TOP) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -586,7 +723,7 @@ __global__ __launch_bounds__(NT, 8) void lp_stream_kernel(LogProbs a, int splits
     if (lane < a.K) cand[w * a.K + lane] = candidate(top.v, top.i);
     if ((int)threadIdx.x < up8(n) - n) cand[n + threadIdx.x] = 0;
   }
-  const Stat all = join<NT>(q, buf);
+  const Stat all = join(q, buf, NT / 64);
   if (TOP && NT == 64) __syncthreads();  // else join's
   if (splits == 1) {
     const RowStat st = finish(all, true);
@@ -643,9 +780,10 @@ __global__ __launch_bounds__(256) void lp_join_kernel(LogProbs a, int splits, Pa
 }
 
 // zeros over row r's gradient
-template <class T, int NT>
+template <class T>
 __device__ __forceinline__ void write_zeros(const LogProbs& a, int64_t r, int64_t lo, int64_t hi) {
   constexpr int VN = Vec<T>::N;
+  const int NT = blockDim.x;
   T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
   for (int64_t at = lo + threadIdx.x * VN; at < hi; at += NT * VN) {
     if (at + VN <= hi) Vec<T>::store(o + at, u32x4{0, 0, 0, 0});
@@ -655,35 +793,35 @@ __device__ __forceinline__ void write_zeros(const LogProbs& a, int64_t r, int64_
 }
 
 // The classes of a row with terms of their own, one a lane of each wave:
-// lane k < K alternative k, lane K the target.
+// lane k < K alternative k, lane K the target.  g: the sum of those terms.
 struct Special {
   int64_t at = -1;  // class, or none
   float own = 0.f;  // its own terms
 };
 __device__ __forceinline__ Special special_of(const LogProbs& a, int64_t r, int64_t t, int K,
-                                              Cotangent& c) {
+                                              float& g) {
   const int lane = threadIdx.x & 63;
   Special s;
   if (a.d_top && lane < K) {
     s.at = a.top_index[r * K + lane];
     s.own = a.d_top[r * K + lane];
   }
-  if (a.d_top) c.g += wave_sum(s.own);
+  g = a.d_top ? wave_sum(s.own) : 0.f;
   if (a.d_logp) {
-    const float g = a.d_logp[r];
+    const float gt = a.d_logp[r];
     const uint64_t same = __ballot(lane < K && s.at == t);  // the target among the alternatives
-    if (lane < K && s.at == t) s.own += g;
+    if (lane < K && s.at == t) s.own += gt;
     if (lane == K && !same) {
       s.at = t;
-      s.own = g;
+      s.own = gt;
     }
-    if (t >= a.V) c.g = __builtin_nanf("");
+    g += t >= a.V ? __builtin_nanf("") : gt;
   }
   return s;
 }
-__device__ __forceinline__ Cotangent cotangent_of(const LogProbs& a, int64_t r, const RowStat& st) {
-  return Cotangent{st.m, st.logs, st.h, a.d_logp ? a.d_logp[r] : 0.f,
-                   a.d_entropy ? a.d_entropy[r] : 0.f};
+__device__ __forceinline__ Cotangent cotangent_of(const LogProbs& a, int64_t r, const RowStat& st,
+                                                  float g) {
+  return Cotangent(st, g, a.d_entropy ? a.d_entropy[r] : 0.f);
 }
 
 // The gradient of vectors [v0, v1) and, where `edge`, the edge of row r from
@@ -695,8 +833,9 @@ __device__ __forceinline__ void write_gradient(const LogProbs& a, int64_t r, int
                                                int v1, bool edge) {
   constexpr int VN = Vec<T>::N, U = E / VN;
   T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
-  Cotangent c = cotangent_of(a, r, st);
-  const Special sp = special_of(a, r, t, K, c);
+  float g;
+  const Special sp = special_of(a, r, t, K, g);
+  const Cotangent c = cotangent_of(a, r, st, g);
   const int lo = row.head + v0 * VN, hi = row.head + v1 * VN;
   const bool inside = sp.at >= lo && sp.at < hi;
   const bool outside = edge && sp.at >= 0 && sp.at < a.V &&
@@ -709,21 +848,17 @@ __device__ __forceinline__ void write_gradient(const LogProbs& a, int64_t r, int
     const int at = row.edge(threadIdx.x);
     o[at] = (T)c.at((float)row.p[at]);
   }
-  u32x4 raw[U];
-  if (v0 < v1) fetch<T, NT>(row, v0, v1, raw);
-  for (int base = v0; base < v1; base += U * NT) {
+  each_chunk<T, NT, U>(row, v0, v1, [&](const u32x4(&raw)[U], int base) {
     float x[E];
 #pragma unroll
     for (int u = 0; u < U; ++u) Vec<T>::unpack(raw[u], x + u * VN);
-    if (base + U * NT < v1) fetch<T, NT>(row, base + U * NT, v1, raw);
-#pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = c.at(x[i]);
+    c.all(x);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int g = base + u * NT + (int)threadIdx.x;
       if (g < v1) Vec<T>::template store<ONCE>(o + row.head + g * VN, Vec<T>::pack(x + u * VN));
     }
-  }
+  });
   __syncthreads();
   if (mine) o[sp.at] = sv;
 }
@@ -740,24 +875,25 @@ __global__ __launch_bounds__(BWD_NT) void lp_gradient_kernel(LogProbs a, int spl
   const int v0 = min(row.nv, sp * part), v1 = min(row.nv, v0 + part);
   if (st.live == 0.f || t < 0) {
     constexpr int VN = Vec<T>::N;
-    write_zeros<T, BWD_NT>(a, r, sp == 0 ? 0 : row.head + v0 * VN,
+    write_zeros<T>(a, r, sp == 0 ? 0 : row.head + v0 * VN,
                            sp == splits - 1 ? a.V : row.head + v1 * VN);
     return;
   }
   write_gradient<T, BWD_NT, ONCE>(a, r, t, st, a.K, row, v0, v1, sp == 0);
 }
 
-// Forward and backward of a row held in the registers of one workgroup: NV
-// vectors a lane.
-template <class T, int NT, int NV, bool ONCE>
-__global__ __launch_bounds__(NT) void lp_block_kernel(LogProbs a) {
+// Forward and backward of a row held in the registers of one workgroup, as wide
+// as the row takes at NV vectors a lane.
+template <class T, int NV, bool ONCE>
+__global__ __launch_bounds__(1024) void lp_block_kernel(LogProbs a) {
   constexpr int VN = Vec<T>::N;
-  __shared__ float buf[NT / 64][4];
+  const int NT = blockDim.x;
+  __shared__ float buf[16][4];
   const int64_t r = blockIdx.x;
   const int64_t t = target_of(a, r);
   if (t < 0) {
     if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
-    write_zeros<T, NT>(a, r, 0, a.V);
+    write_zeros<T>(a, r, 0, a.V);
     return;
   }
   const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
@@ -789,15 +925,16 @@ __global__ __launch_bounds__(NT) void lp_block_kernel(LogProbs a) {
     as_stored(raw[i]);
   }
   q.add(ex);
-  const RowStat st = finish(join<NT>(q, buf), true);
+  const RowStat st = finish(join(q, buf, NT / 64), true);
   if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
   if (st.live == 0.f) {
     __syncthreads();  // the target's logit is read before its place is written
-    write_zeros<T, NT>(a, r, 0, a.V);
+    write_zeros<T>(a, r, 0, a.V);
     return;
   }
-  Cotangent c = cotangent_of(a, r, st);
-  const Special sp = special_of(a, r, t, 0, c);
+  float g;
+  const Special sp = special_of(a, r, t, 0, g);
+  const Cotangent c = cotangent_of(a, r, st, g);
   const bool mine = threadIdx.x < 64 && sp.at >= 0 && sp.at < a.V;
   T sv = (T)0.f;
   if (mine) sv = (T)(c.at((float)row.p[sp.at]) + sp.own);
@@ -809,48 +946,99 @@ __global__ __launch_bounds__(NT) void lp_block_kernel(LogProbs a) {
     const int g = i * NT + (int)threadIdx.x;
     float x[VN];
     Vec<T>::unpack(raw[i], x);
-#pragma unroll
-    for (int j = 0; j < VN; ++j) x[j] = c.at(x[j]);
+    c.all(x);
     if (g < row.nv) Vec<T>::template store<ONCE>(o + row.head + g * VN, Vec<T>::pack(x));
   }
   __syncthreads();
   if (mine) o[sp.at] = sv;
 }
 
-// Rows longer than that: a workgroup takes a whole row twice, the second time
-// out of the caches.
-constexpr int BOTH_NT = 1024;
+// Rows longer than that: what a workgroup can hold of one (half of the CU's
+// registers and LDS, at two workgroups a CU) it reads once, the rest twice,
+// the second time out of the caches.
+// 2048 rows of 131 k bfloat16: nothing held 228 us, registers alone 217, LDS
+// too 210; six vectors a lane in registers 217, a workgroup of 512 250.
+constexpr int BOTH_NT = 1024, BOTH_KEEP = 4, BOTH_LDS = 4;  // vectors a lane
 template <class T, bool ONCE>
-__global__ __launch_bounds__(BOTH_NT) void lp_both_kernel(LogProbs a) {
-  constexpr int VN = Vec<T>::N, NT = BOTH_NT, U = E / VN;
+__global__ __launch_bounds__(BOTH_NT, 8) void lp_both_kernel(LogProbs a) {
+  constexpr int VN = Vec<T>::N, NT = BOTH_NT, U = 2, KEEP = BOTH_KEEP, LDS = BOTH_LDS;
   __shared__ float buf[NT / 64][4];
+  __shared__ u32x4 held[LDS * NT];
   const int64_t r = blockIdx.x;
   const int64_t t = target_of(a, r);
   if (t < 0) {
     if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
-    write_zeros<T, NT>(a, r, 0, a.V);
+    write_zeros<T>(a, r, 0, a.V);
     return;
   }
   const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
-  const bool edge = (int)threadIdx.x < row.edges;
-  const float ex = edge ? (float)row.p[row.edge(threadIdx.x)] : NEG_INF;
+  const int lane = threadIdx.x, rest = min(row.nv, (KEEP + LDS) * NT);
+  const bool edge = lane < row.edges;
+  const int edge_at = edge ? row.edge(lane) : -1;
+  const float ex = edge ? (float)row.p[edge_at] : NEG_INF;
   Stat q;
-  u32x4 raw[U];
-  if (row.nv > 0) fetch<T, NT>(row, 0, row.nv, raw);
-  for (int base = 0; base < row.nv; base += U * NT) {
-    float x[E];
+  auto add = [&](const u32x4(&raw)[U]) {
+    float x[U * VN];
 #pragma unroll
     for (int u = 0; u < U; ++u) Vec<T>::unpack(raw[u], x + u * VN);
-    if (base + U * NT < row.nv) fetch<T, NT>(row, base + U * NT, row.nv, raw);
     add_chunk(q, x, max_of(x));
+  };
+  u32x4 keep[KEEP / U][U];  // vectors [0, KEEP * NT): all there
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) keep[i / U][i % U] = row.load(i * NT + lane);
+#pragma unroll
+  for (int i = 0; i < LDS / U; ++i) {
+    u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int g = (KEEP + i * U + u) * NT + lane;
+      raw[u] = Row<T>::none();
+      if (g < row.nv) raw[u] = row.load(g);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) held[(i * U + u) * NT + lane] = raw[u];
+    add(raw);
   }
+#pragma unroll
+  for (int i = 0; i < KEEP / U; ++i) {
+    add(keep[i]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) as_stored(keep[i][u]);
+  }
+  each_chunk<T, NT, U>(row, rest, row.nv, [&](const u32x4(&raw)[U], int) { add(raw); });
   const float one[1] = {ex};
   add_chunk(q, one, ex);
-  const RowStat st = finish(join<NT>(q, buf), true);
-  if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
-  __syncthreads();  // the target's logit is read before its place is written
-  if (st.live == 0.f) return write_zeros<T, NT>(a, r, 0, a.V);
-  write_gradient<T, NT, ONCE>(a, r, t, st, 0, row, 0, row.nv, true);
+  const RowStat st = finish(join(q, buf, NT / 64), true);
+  if (lane == 0) write_row<T>(a, r, st, a.target ? t : -1);
+  if (st.live == 0.f) {
+    __syncthreads();  // the target's logit is read before its place is written
+    return write_zeros<T>(a, r, 0, a.V);
+  }
+  float g;
+  const Special sp = special_of(a, r, t, 0, g);
+  const Cotangent c = cotangent_of(a, r, st, g);
+  const bool mine = lane < 64 && sp.at >= 0 && sp.at < a.V;
+  T sv = (T)0.f;
+  if (mine) sv = (T)(c.at((float)row.p[sp.at]) + sp.own);
+  __syncthreads();
+  T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
+  if (edge) o[edge_at] = (T)c.at(ex);
+  auto put = [&](u32x4 raw, int v) {
+    float x[VN];
+    Vec<T>::unpack(raw, x);
+    c.all(x);
+    if (v < row.nv) Vec<T>::template store<ONCE>(o + row.head + v * VN, Vec<T>::pack(x));
+  };
+  each_chunk<T, NT, U>(row, rest, row.nv, [&](const u32x4(&raw)[U], int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(raw[u], base + u * NT + lane);
+  });
+#pragma unroll
+  for (int i = 0; i < LDS; ++i) put(held[i * NT + lane], (KEEP + i) * NT + lane);
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) put(keep[i / U][i % U], i * NT + lane);
+  __syncthreads();
+  if (mine) o[sp.at] = sv;
 }
 
 // ---------------------------------------------------------------------------
@@ -858,7 +1046,7 @@ __global__ __launch_bounds__(BOTH_NT) void lp_both_kernel(LogProbs a) {
 // ---------------------------------------------------------------------------
 constexpr int ROW_MAX = 1024;      // longest row held by a group of lanes
 constexpr int WAVE_MAX = 8192;     // longest row read by one wave
-constexpr int BLOCK_VECS = 8192;   // vectors that one workgroup holds
+constexpr int BLOCK_VECS = 8192;   // vectors that one workgroup holds in registers
 
 // How a long row is divided among workgroups of 256: into as many parts as
 // fill the card, each at least one chunk.
@@ -868,7 +1056,7 @@ struct Split {
 Split split_of(int dtype, int64_t rows, int V) {
   const int vn = dtype == BC2N_F32 ? 4 : 8, nv = (V + vn - 1) / vn;
   const int64_t chunk = (int64_t)E / vn * 256;
-  const int64_t fill = (4 * (int64_t)device_cus() + rows - 1) / rows;
+  const int64_t fill = (4 * (int64_t)device_cus() + rows / 2) / rows;
   int64_t s = std::min<int64_t>({(nv + chunk - 1) / chunk, fill, MAX_SPLITS});
   if (s < 1 || V <= WAVE_MAX) s = 1;
   return Split{(int)s, (int)((nv + s - 1) / s)};
@@ -943,10 +1131,11 @@ bool in_parts(int dtype, int64_t rows, int V) {
   return V / (dtype == BC2N_F32 ? 4 : 8) > BLOCK_VECS && rows < device_cus();
 }
 
-template <class T, int NT, int NV>
+template <class T, int NV>
 void block_go(hipStream_t st, const LogProbs& a) {
+  const int vecs = a.V / Vec<T>::N, nt = (vecs + 64 * NV - 1) / (64 * NV) * 64;
   with_once(a, [&](auto once) {
-    lp_block_kernel<T, NT, NV, once><<<(unsigned)a.rows, NT, 0, st>>>(a);
+    lp_block_kernel<T, NV, once><<<(unsigned)a.rows, nt, 0, st>>>(a);
   });
 }
 
@@ -954,11 +1143,8 @@ template <class T>
 void both(hipStream_t st, const LogProbs& a, void* work) {
   if (a.V <= ROW_MAX) return rows_launch<T, 3>(st, a);
   const int vecs = a.V / Vec<T>::N;
-  if (vecs <= 512) block_go<T, 64, 8>(st, a);
-  else if (vecs <= 1024) block_go<T, 256, 4>(st, a);
-  else if (vecs <= 2048) block_go<T, 256, 8>(st, a);
-  else if (vecs <= 4096) block_go<T, 512, 8>(st, a);
-  else if (vecs <= BLOCK_VECS) block_go<T, 1024, 8>(st, a);
+  if (vecs <= BLOCK_VECS / 2) block_go<T, 4>(st, a);
+  else if (vecs <= BLOCK_VECS) block_go<T, 8>(st, a);
   else if (!in_parts(a.dtype, a.rows, a.V)) {
     with_once(a, [&](auto once) {
       lp_both_kernel<T, once><<<(unsigned)a.rows, BOTH_NT, 0, st>>>(a);
