@@ -191,6 +191,24 @@ __device__ __forceinline__ uint32_t key_below(uint32_t k) {
   return k == 0x80000000u ? k - 2 : k - 1;  // below 0 lies the smallest negative, not -0
 }
 
+// Candidates in LDS are one word each: the value's order key over the index's
+// complement, so that the larger word is the better candidate; 0: none.
+__device__ __forceinline__ uint64_t candidate(float v, int i) {
+  return i < 0 ? 0 : (uint64_t)order_key(v) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ int index_of(uint64_t c) { return (int)~(uint32_t)c; }
+__device__ __forceinline__ float value_of(uint64_t c) { return value_of_key((uint32_t)(c >> 32)); }
+// how many of the n candidates (n a multiple of 8) are better than c
+__device__ __forceinline__ int rank_of(const uint64_t* cand, int n, uint64_t c) {
+  int rank = 0;
+  for (int o = 0; o < n; o += 8) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) rank += cand[o + k] > c;
+  }
+  return rank;
+}
+constexpr int up8(int n) { return (n + 7) / 8 * 8; }
+
 // A wave's largest elements, the k-th in lane k (index -1: none yet).  An
 // element not above `floor` is not among the row's: the wave has K as large
 // that come before it.  Waves of one row tell each other, through LDS, values
@@ -218,11 +236,18 @@ struct TopList {
   __device__ __forceinline__ uint32_t bound(float mx, int K) {
     const int lane = threadIdx.x & 63;
     float t = NEG_INF;
-    for (int k = 0; k < K; ++k) {
-      t = wave_max(mx);
-      const uint64_t b = __ballot(mx == t);
-      if (b == 0) break;
-      if (lane == __ffsll((unsigned long long)b) - 1) mx = NEG_INF;
+    if (K <= 6) {  // the largest, K times
+      for (int k = 0; k < K; ++k) {
+        t = wave_max(mx);
+        const uint64_t b = __ballot(mx == t);
+        if (b == 0) break;
+        if (lane == __ffsll((unsigned long long)b) - 1) mx = NEG_INF;
+      }
+    } else {  // the smallest of those that fewer than K are above
+      int above = 0;
+#pragma unroll
+      for (int j = 0; j < 64; ++j) above += read_lane(mx, j) > mx;
+      t = -wave_max(above < K ? -mx : NEG_INF);
     }
     if (!(t > NEG_INF)) return 0;
     const uint32_t reached = order_key(t);
@@ -600,24 +625,6 @@ __device__ __forceinline__ Stat join(Stat q, float (*buf)[4], int waves) {
   return join_wave(o);
 }
 
-// Candidates in LDS are one word each: the value's order key over the index's
-// complement, so that the larger word is the better candidate; 0: none.
-__device__ __forceinline__ uint64_t candidate(float v, int i) {
-  return i < 0 ? 0 : (uint64_t)order_key(v) << 32 | (uint32_t)~i;
-}
-__device__ __forceinline__ int index_of(uint64_t c) { return (int)~(uint32_t)c; }
-__device__ __forceinline__ float value_of(uint64_t c) { return value_of_key((uint32_t)(c >> 32)); }
-// how many of the n candidates (n a multiple of 8) are better than c
-__device__ __forceinline__ int rank_of(const uint64_t* cand, int n, uint64_t c) {
-  int rank = 0;
-  for (int o = 0; o < n; o += 8) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) rank += cand[o + k] > c;
-  }
-  return rank;
-}
-constexpr int up8(int n) { return (n + 7) / 8 * 8; }
-
 // Writes the K best of n candidates (LDS, zeros behind up to a multiple of 8)
 // as row r's alternatives; where there are fewer than K above -inf, the first
 // -inf elements of the row follow.
@@ -683,11 +690,11 @@ __global__ __launch_bounds__(NT, 8) void lp_stream_kernel(LogProbs a, int splits
   const int64_t r = blockIdx.x / splits;
   const int sp = blockIdx.x % splits;
   const int64_t t = target_of(a, r);
-  if (t < 0) {  // left out: not read
-    if (splits == 1) {
-      if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
-      if (TOP) no_tops(a, r, NT);
-    }
+  // left out: not read.  (A part's rows are few, and waiting for the target
+  // first costs each a load's latency: the join leaves them out.)
+  if (splits == 1 && t < 0) {
+    if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
+    if (TOP) no_tops(a, r, NT);
     return;
   }
   const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
@@ -1053,11 +1060,14 @@ constexpr int BLOCK_VECS = 8192;   // vectors that one workgroup holds in regist
 struct Split {
   int splits = 1, part = 0;  // part in vectors
 };
-Split split_of(int dtype, int64_t rows, int V) {
+Split split_of(int dtype, int64_t rows, int V, int K) {
   const int vn = dtype == BC2N_F32 ? 4 : 8, nv = (V + vn - 1) / vn;
   const int64_t chunk = (int64_t)E / vn * 256;
   const int64_t fill = (4 * (int64_t)device_cus() + rows / 2) / rows;
-  int64_t s = std::min<int64_t>({(nv + chunk - 1) / chunk, fill, MAX_SPLITS});
+  // the join ranks splits * K candidates against each other: at most 256 (K =
+  // 20 of 32 rows of 150 k: 32 parts 39 us, 8 parts 24)
+  const int64_t most = K > 0 ? std::min(MAX_SPLITS, std::max(4, 256 / K)) : MAX_SPLITS;
+  int64_t s = std::min<int64_t>({(nv + chunk - 1) / chunk, fill, most});
   if (s < 1 || V <= WAVE_MAX) s = 1;
   return Split{(int)s, (int)((nv + s - 1) / s)};
 }
@@ -1094,7 +1104,7 @@ void stream_go(hipStream_t st, const LogProbs& a, const Split& s, const Parts& p
 template <class T>
 void fwd(hipStream_t st, const LogProbs& a, void* work) {
   if (a.V <= ROW_MAX) return rows_launch<T, 1>(st, a);
-  const Split s = split_of(a.dtype, a.rows, a.V);
+  const Split s = split_of(a.dtype, a.rows, a.V, a.K);
   Parts parts;
   if (s.splits > 1) {
     Carver c(work);
@@ -1119,7 +1129,7 @@ void with_once(const LogProbs& a, F f) {
 template <class T>
 void bwd(hipStream_t st, const LogProbs& a) {
   if (a.V <= ROW_MAX) return rows_launch<T, 2>(st, a);
-  const Split s = split_of(a.dtype, a.rows, a.V);
+  const Split s = split_of(a.dtype, a.rows, a.V, a.K);
   const unsigned grid = (unsigned)(a.rows * s.splits);
   with_once(a, [&](auto once) {
     lp_gradient_kernel<T, once><<<grid, BWD_NT, 0, st>>>(a, s.splits, s.part);
@@ -1170,7 +1180,7 @@ void by_type(int dtype, F f) {
 
 size_t logprobs_work_bytes(int dtype, int64_t rows, int V, int K) {
   if (rows <= 0 || V <= WAVE_MAX) return 0;
-  const Split s = split_of(dtype, rows, V);
+  const Split s = split_of(dtype, rows, V, K);
   Sizer z;
   if (s.splits > 1 || in_parts(dtype, rows, V)) z.take<float>(4 * (size_t)rows);
   if (s.splits > 1) parts_of(z, rows, s.splits, K);
