@@ -1153,6 +1153,10 @@ int bc2n_confidence_bwd(void* stream, const float* plddt_logits, const float* pa
 }
 
 namespace {
+void aligned(const void* p, int to, const char* what) {
+  if (p && reinterpret_cast<uintptr_t>(p) % (uintptr_t)to)
+    throw std::invalid_argument(std::string("unaligned ") + what);
+}
 LogProbs lp_operands(int dtype, const void* logits, int64_t ld, int64_t rows, int classes,
                      const void* targets, int target_bits) {
   need(dtype == BC2N_F32 || dtype == BC2N_F16 || dtype == BC2N_BF16, "logprobs: bad dtype");
@@ -1161,11 +1165,13 @@ LogProbs lp_operands(int dtype, const void* logits, int64_t ld, int64_t rows, in
   need(ld >= classes, "logprobs: the row stride is below the number of classes");
   need(!targets || target_bits == 32 || target_bits == 64, "logprobs: targets are i32 or i64");
   need(rows == 0 || logits, "null operand");
+  aligned(logits, dtype == BC2N_F32 ? 4 : 2, "logits");
+  if (targets) aligned(targets, target_bits / 8, "targets");
   LogProbs a;
   a.dtype = dtype;
   a.x = logits;
   a.ld = ld;
-  a.rows = rows;
+  a.rows = a.total = rows;
   a.V = classes;
   a.target = targets;
   a.target64 = target_bits == 64;
@@ -1180,6 +1186,7 @@ void lp_gradient(LogProbs& a, void* d_logits, int64_t d_ld) {
   need(a.rows == 0 || d_logits, "null output");
   need(d_ld >= a.V, "logprobs: the gradient's row stride is below the number of classes");
   need(d_logits != a.x || d_ld == a.ld, "logprobs: a gradient in place has the logits' row stride");
+  aligned(d_logits, a.dtype == BC2N_F32 ? 4 : 2, "d_logits");
   a.d = d_logits;
   a.d_ld = d_ld;
 }
@@ -1190,6 +1197,11 @@ TensorList& list_of(void* list) {
 }
 void list_work(const TensorList& l, const void* work) {
   need(work || l.work_bytes() == 0, "list: null work");
+  aligned(work, 16, "work");
+}
+hipStream_t list_stream(void* s, TensorList& l) {
+  if (l.dev && capturing(own_stream(s))) l.keep_table();
+  return own_stream(s);
 }
 bool known_type(int t) { return t == BC2N_F32 || t == BC2N_F16 || t == BC2N_BF16; }
 }  // namespace
@@ -1216,6 +1228,8 @@ int bc2n_logprobs_fwd(void* stream, int dtype, const void* logits, int64_t ld, i
     need(!logp || targets, "logprobs: logp needs targets");
     need(top == 0 || rows == 0 || (top_logp && top_index), "null output");
     need(work || logprobs_work_bytes(dtype, rows, classes, top) == 0, "logprobs: null work");
+    aligned(work, 16, "work");
+    aligned(save, 16, "save");
     a.logp = logp;
     a.entropy = entropy;
     a.top_logp = top_logp;
@@ -1235,6 +1249,7 @@ int bc2n_logprobs_bwd(void* stream, int dtype, const void* logits, int64_t ld, i
     lp_top(a, top);
     lp_gradient(a, d_logits, d_ld);
     need(rows == 0 || save, "null operand");
+    aligned(save, 16, "save");
     need(!d_logp || targets, "logprobs: d_logp needs targets");
     need(!d_top_logp || (top > 0 && top_index), "logprobs: d_top_logp needs top_index");
     a.top_index = const_cast<int32_t*>(top_index);
@@ -1255,6 +1270,7 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
     lp_gradient(a, d_logits, d_ld);
     need((!logp && !d_logp) || targets, "logprobs: logp needs targets");
     need(work || logprobs_work_bytes(dtype, rows, classes, 0) == 0, "logprobs: null work");
+    aligned(work, 16, "work");
     a.logp = logp;
     a.entropy = entropy;
     a.d_logp = d_logp;
@@ -1329,7 +1345,7 @@ int bc2n_grad_norm(void* stream, void* list, float* norm, void* work) {
     TensorList& l = list_of(list);
     need(norm, "null operand");
     list_work(l, work);
-    grad_norm(own_stream(stream), l, norm, work);
+    grad_norm(list_stream(stream, l), l, norm, work);
   });
 }
 
@@ -1339,7 +1355,7 @@ int bc2n_grad_clip(void* stream, void* list, float max_norm, float* norm, void* 
     need(l.clips, "grad_clip: the list has no outputs");
     need(max_norm > 0.f, "grad_clip: max_norm must be positive");
     list_work(l, work);
-    grad_clip(own_stream(stream), l, max_norm, norm, work);
+    grad_clip(list_stream(stream, l), l, max_norm, norm, work);
   });
 }
 
@@ -1364,7 +1380,7 @@ int bc2n_adam_step(void* stream, void* list, double lr, double beta1, double bet
     s.step = step;
     s.max_norm = max_norm;
     s.device = scalars;
-    adam_step(own_stream(stream), l, s, norm, work);
+    adam_step(list_stream(stream, l), l, s, norm, work);
   });
 }
 

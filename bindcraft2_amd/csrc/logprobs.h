@@ -15,6 +15,7 @@ struct LogProbs {
   int dtype = 0;  // of x and d: BC2N_F32, BC2N_F16, BC2N_BF16
   const void* x = nullptr;  // [rows][V], row stride ld elements
   int64_t ld = 0, rows = 0;
+  int64_t total = 0;  // rows of the whole call, of which these may be a part
   int V = 0;
   const void* target = nullptr;  // [rows] i32 or (target64) i64; null: none
   int target64 = 0;

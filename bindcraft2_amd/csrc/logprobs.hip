@@ -1118,7 +1118,7 @@ void stream_go(hipStream_t st, const LogProbs& a, const Split& s, const Parts& p
 template <class T>
 void fwd(hipStream_t st, const LogProbs& a, void* work) {
   if (short_row<T>(a.V)) return rows_launch<T, 1>(st, a);
-  const Split s = split_of(a.dtype, a.rows, a.V, a.K);
+  const Split s = split_of(a.dtype, a.total, a.V, a.K);
   Parts parts;
   if (s.splits > 1) {
     Carver c(work);
@@ -1135,7 +1135,7 @@ void fwd(hipStream_t st, const LogProbs& a, void* work) {
 // 102).  Smaller ones stay for whoever reads them next.
 template <class F>
 void with_once(const LogProbs& a, F f) {
-  const int64_t bytes = 2 * a.rows * a.V * (a.dtype == BC2N_F32 ? 4 : 2);
+  const int64_t bytes = 2 * a.total * a.V * (a.dtype == BC2N_F32 ? 4 : 2);
   if (bytes > int64_t(128) << 20) f(std::true_type());
   else f(std::false_type());
 }
@@ -1143,7 +1143,7 @@ void with_once(const LogProbs& a, F f) {
 template <class T>
 void bwd(hipStream_t st, const LogProbs& a) {
   if (short_row<T>(a.V)) return rows_launch<T, 2>(st, a);
-  const Split s = split_of(a.dtype, a.rows, a.V, a.K);
+  const Split s = split_of(a.dtype, a.total, a.V, a.K);
   const unsigned grid = (unsigned)(a.rows * s.splits);
   with_once(a, [&](auto once) {
     lp_gradient_kernel<T, once><<<grid, BWD_NT, 0, st>>>(a, s.splits, s.part);
@@ -1169,7 +1169,7 @@ void both(hipStream_t st, const LogProbs& a, void* work) {
   const int vecs = a.V / Vec<T>::N;
   if (vecs <= BLOCK_VECS / 2) block_go<T, 4>(st, a);
   else if (vecs <= BLOCK_VECS) block_go<T, 8>(st, a);
-  else if (!in_parts(a.dtype, a.rows, a.V)) {
+  else if (!in_parts(a.dtype, a.total, a.V)) {
     with_once(a, [&](auto once) {
       lp_both_kernel<T, once><<<(unsigned)a.rows, BOTH_NT, 0, st>>>(a);
     });
@@ -1201,22 +1201,58 @@ size_t logprobs_work_bytes(int dtype, int64_t rows, int V, int K) {
   return z.off;
 }
 
+namespace {
+
+// rows [r0, r0 + n) of a call
+LogProbs slice(const LogProbs& a, int64_t r0, int64_t n) {
+  const int64_t w = a.dtype == BC2N_F32 ? 4 : 2;
+  auto bytes = [](auto*& p, int64_t by) {
+    typedef std::remove_reference_t<decltype(p)> P;
+    if (p) p = (P)((uintptr_t)p + (uintptr_t)by);
+  };
+  LogProbs b = a;
+  b.rows = n;
+  bytes(b.x, r0 * a.ld * w);
+  bytes(b.d, r0 * a.d_ld * w);
+  bytes(b.target, r0 * (a.target64 ? 8 : 4));
+  for (auto** p : {&b.logp, &b.entropy}) bytes(*p, r0 * 4);
+  for (auto** p : {&b.d_logp, &b.d_entropy}) bytes(*p, r0 * 4);
+  bytes(b.top_logp, r0 * a.K * 4);
+  bytes(b.top_index, r0 * a.K * 4);
+  bytes(b.d_top, r0 * a.K * 4);
+  bytes(b.save, r0 * 16);
+  return b;
+}
+
+// A grid holds fewer than 2^32 threads, at most 1024 of them a row here.
+constexpr int64_t SLICE = int64_t(1) << 21;
+template <class F>
+void by_slices(const LogProbs& a, F f) {
+  for (int64_t r = 0; r < a.rows; r += SLICE)
+    f(a.rows <= SLICE ? a : slice(a, r, std::min(SLICE, a.rows - r)));
+}
+
+}  // namespace
+
 void logprobs_fwd(hipStream_t st, const LogProbs& a, void* work) {
-  if (a.rows == 0) return;
-  KTimed t("logprobs.fwd", st);
-  by_type(a.dtype, [&](auto v) { fwd<decltype(v)>(st, a, work); });
+  by_slices(a, [&](const LogProbs& b) {
+    KTimed t("logprobs.fwd", st);
+    by_type(a.dtype, [&](auto v) { fwd<decltype(v)>(st, b, work); });
+  });
 }
 
 void logprobs_bwd(hipStream_t st, const LogProbs& a) {
-  if (a.rows == 0) return;
-  KTimed t("logprobs.bwd", st);
-  by_type(a.dtype, [&](auto v) { bwd<decltype(v)>(st, a); });
+  by_slices(a, [&](const LogProbs& b) {
+    KTimed t("logprobs.bwd", st);
+    by_type(a.dtype, [&](auto v) { bwd<decltype(v)>(st, b); });
+  });
 }
 
 void logprobs_grad(hipStream_t st, const LogProbs& a, void* work) {
-  if (a.rows == 0) return;
-  KTimed t("logprobs.grad", st);
-  by_type(a.dtype, [&](auto v) { both<decltype(v)>(st, a, work); });
+  by_slices(a, [&](const LogProbs& b) {
+    KTimed t("logprobs.grad", st);
+    by_type(a.dtype, [&](auto v) { both<decltype(v)>(st, b, work); });
+  });
 }
 
 }  // namespace bc2n

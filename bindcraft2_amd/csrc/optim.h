@@ -45,6 +45,10 @@ class TensorList {
   const bool clips;  // its gradients have outputs
   const bool adam;   // it has parameters and their moments
 
+  // For a call captured into a graph: the graph may outlive the list, so the
+  // list's table is never given to another.
+  void keep_table() { kept_ = true; }
+
   static constexpr uint32_t MAGIC = 0x6c747362;
   uint32_t magic = MAGIC;
 
@@ -56,6 +60,7 @@ class TensorList {
 
  private:
   DeviceBlock block_;
+  bool kept_ = false;
 };
 
 struct AdamScalars {

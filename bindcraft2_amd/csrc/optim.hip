@@ -420,6 +420,7 @@ TensorList::TensorList(std::vector<ListEntry> all, bool clips_, bool adam_)
   for (size_t i = 0; i < all.size(); ++i) {
     ListEntry& e = all[i];
     const std::string at = "tensor " + std::to_string(i);
+    if (all.size() > (size_t(1) << 22)) throw std::invalid_argument("list: too many tensors");
     if (e.n < 0) throw std::invalid_argument("list: " + at + " has a negative size");
     if (e.n > (int64_t(1) << 40)) throw std::invalid_argument("list: " + at + " is too large");
     if (e.n == 0) continue;
@@ -491,7 +492,7 @@ TensorList::TensorList(std::vector<ListEntry> all, bool clips_, bool adam_)
 
 TensorList::~TensorList() {
   magic = 0;
-  if (block_.p) tables().give(block_);
+  if (block_.p && !kept_) tables().give(block_);
 }
 
 size_t TensorList::work_bytes() const {

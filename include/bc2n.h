@@ -665,9 +665,8 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
  * element.  An output may be its own input (in place); it shares memory with
  * no other operand, which making the list checks.  Making a list of more than
  * 32 non-empty tensors allocates and copies a table to the device, waiting for
- * it (not under graph capture); a list outlives the graphs that captured its
- * calls.  Freeing one makes no HIP call: its table goes to a later list.  NULL
- * on error.
+ * it (not under graph capture).  Freeing one makes no HIP call: its table goes
+ * to a later list, unless a call was captured into a graph.  NULL on error.
  *   grad_list: grads, and `out` for their clipped values (NULL: norm only).
  *   adam_list: parameters, gradients, first and second moments, and where the
  *     updated ones go.

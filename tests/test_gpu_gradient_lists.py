@@ -238,6 +238,27 @@ def test_lists_streams_and_graphs(cuda, name):
         torch.cuda.synchronize()
 
 
+def test_graph_of_a_list_that_is_gone(cuda):
+    """A captured call's table is not given to a later list."""
+    grads, _ = make(LISTS["table"], 3)
+    outs = [torch.zeros_like(g) for g in grads]
+    h = ops.GradientClip(grads, out=outs)
+    norm = h.clip(0.25)
+    want = [o.clone() for o in outs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = h.clip(0.25)
+    del h
+    others = [ops.GradientClip([torch.ones(7, device="cuda") for _ in range(k)]) for k in (40, 500)]
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, norm) and all(torch.equal(o, w) for o, w in zip(outs, want))
+        assert [o.norm().item() for o in others] == pytest.approx([(7 * k) ** 0.5 for k in (40, 500)])
+
+
 def test_bad_lists(cuda):
     f = lambda n: torch.randn(n, device="cuda")  # noqa: E731
     a, b = f(64), f(64)

@@ -225,6 +225,27 @@ def test_rows_far_apart(cuda):
     verify(y.contiguous(), None, 4, out)
 
 
+@pytest.mark.parametrize("v,dtype", [(8, "f32"), (1100, "bf16")])
+def test_more_rows_than_one_launch_takes(cuda, v, dtype):
+    """2^21 rows and a few: each row as the same row in a call of few."""
+    print(f"many rows v={v} {dtype}", flush=True)
+    rows = 2 ** 21 + 5
+    x, g = logits(64, v, TYPES[dtype], v)
+    x = x.repeat(rows // 64 + 1, 1)[:rows]
+    t = torch.randint(v, (64,), generator=g, device="cuda").repeat(rows // 64 + 1)[:rows]
+    dl, de = (torch.randn(64, generator=g, device="cuda").repeat(rows // 64 + 1)[:rows] for _ in range(2))
+    op = ops.LogProbs(3)
+    out, save = op.forward(x, t)
+    d = op.backward((dl, de, out[2]), x, t, out[3], save)
+    verify(x[:64], t[:64], 3, [o[:64] for o in out], d[:64], (dl[:64], de[:64], out[2][:64]))
+    period = lambda o: torch.equal(o[64:], o[:-64])  # noqa: E731
+    assert all(period(o) for o in (*out, d))
+    del d
+    (lp, en), d = ops.LogProbs().value_and_grad(x, t, dl, de)
+    verify(x[:64], t[:64], 0, (lp[:64], en[:64], None, None), d[:64], (dl[:64], de[:64], None))
+    assert period(d) and period(lp) and period(en)
+
+
 @pytest.mark.parametrize("rows,v", [(300, 64), (2, 40000), (700, 4000)])
 def test_same_bits_streams_and_graphs(cuda, rows, v):
     """The same bits every time, on another stream, and from a captured graph

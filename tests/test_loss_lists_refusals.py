@@ -36,6 +36,12 @@ def test_logprobs_refusals():
     refused(fwd(top=-1), b"top")
     refused(fwd(v=3, top=4, tl=P, ti=P), b"top")
     refused(fwd(top=2, tl=P), b"null")
+    refused(fwd(x=P + 2), b"unaligned")
+    refused(fwd(t=P + 4), b"unaligned")
+    refused(fwd(save=P + 8), b"unaligned")
+    refused(fwd(work=P + 8), b"unaligned")
+    refused(bwd(d=P + 1), b"unaligned")
+    refused(bwd(save=P + 4), b"unaligned")
     refused(bwd(d=None), b"null")
     refused(bwd(dld=63), b"stride")
     refused(bwd(d=P, ld=64, dld=65), b"in place")
