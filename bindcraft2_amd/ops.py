@@ -914,11 +914,13 @@ class _TensorList:
         tensors = list(tensors)
         if len(tensors) != len(like):
             raise ValueError(f"{what}: expected {len(like)} tensors, got {len(tensors)}")
+        here = torch.cuda.current_device() if tensors else None
         for t, g in zip(tensors, like):
             if t.shape != g.shape or t.dtype not in dtypes or not t.is_contiguous():
                 raise ValueError(f"{what}: expected a contiguous {tuple(g.shape)} of "
                                  f"{', '.join(map(str, dtypes))}, got {t.dtype} {tuple(t.shape)}")
-            _current(t, what)
+            if t.get_device() != here:
+                _current(t, what)
         return tensors
 
     @staticmethod

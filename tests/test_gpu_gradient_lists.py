@@ -238,6 +238,29 @@ def test_lists_streams_and_graphs(cuda, name):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("count", [3, 50])
+def test_lists_beyond_the_caches(cuda, count):
+    """Operands of more than 256 MiB, entries with the launch and in the table."""
+    print(f"large lists {count}", flush=True)
+    sizes = [36_000_000 // count + 7 * k for k in range(count)]
+    grads, buffers = make(sizes, 3, (torch.float32,))
+    outs, out_buffers = make(sizes, 4, (torch.float32,))
+    norm = exact_norm(grads)
+    assert abs(ops.GradientClip(grads, out=outs).clip(0.5).item() - norm) <= 3 * HALF * norm
+    for o, g in zip(outs, grads):
+        rounded(o, g.double() * (0.5 / norm), "large")
+    assert untouched(buffers) and untouched(out_buffers)
+    sizes = [12_000_000 // count + 7 * k for k in range(count)]
+    for types in (((torch.float32,), (torch.float32,)), (TYPES, TYPES[1:] + TYPES[:1])):
+        state, buffers = adam_state(sizes, 11, *types)
+        outs, out_buffers = adam_state(sizes, 31, *types)
+        norm = exact_norm(state[1])
+        h = ops.Adam(*state, out=(outs[0], outs[2], outs[3]), weight_decay=0.01)
+        assert abs(h.step(5, 0.01, max_norm=0.5).item() - norm) <= 3 * HALF * norm
+        check_adam(state, (outs[0], outs[2], outs[3]), 0.5 / norm, 5, 0.01, 0.9, 0.999, 1e-8, 0.01)
+        assert all(untouched(b) for b in (*buffers, *out_buffers))
+
+
 def test_graph_of_a_list_that_is_gone(cuda):
     """A captured call's table is not given to a later list."""
     grads, _ = make(LISTS["table"], 3)

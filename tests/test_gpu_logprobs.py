@@ -94,16 +94,8 @@ def test_number_of_alternatives(cuda, top, rows, v):
     through(x, t, top, g)
 
 
-WIDTHS = [20, 64, 700, 3001, 20000]
-
-
-@pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("v", WIDTHS)
-def test_special_rows(cuda, v, dtype):
-    """Rows with nothing allowed, one class allowed, the type's lowest and
-    largest values, NaN, infinities; the target on each side; left out."""
-    print(f"special rows v={v} {dtype}", flush=True)
-    t, f = TYPES[dtype], torch.finfo(TYPES[dtype])
+def special(v, t):
+    f = torch.finfo(t)
     x, g = logits(16, v, t, v)
     at = torch.randint(v, (16,), generator=g, device="cuda", dtype=torch.int32)
     x[0] = -math.inf
@@ -132,6 +124,19 @@ def test_special_rows(cuda, v, dtype):
     x[13] = f.max
     x[13, 0] = f.min
     x[14, 0] = -math.inf
+    return x, at, g
+
+
+WIDTHS = [20, 64, 700, 3001, 20000]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", WIDTHS)
+def test_special_rows(cuda, v, dtype):
+    """Rows with nothing allowed, one class allowed, the type's lowest and
+    largest values, NaN, infinities; the target on each side; left out."""
+    print(f"special rows v={v} {dtype}", flush=True)
+    x, at, g = special(v, TYPES[dtype])
     for targets in (at, at.long(), None):
         op = ops.LogProbs(5)
         out, save = op.forward(x, targets)
@@ -143,6 +148,47 @@ def test_special_rows(cuda, v, dtype):
     verify(x, at, 5, out, op.backward((dl, None, None), x, at, out[3], save), (dl, None, None))
     (logp, entropy), d = op.value_and_grad(x, at, dl, de)
     verify(x, at, 0, (logp, entropy, None, None), d, (dl, de, None))
+
+
+@pytest.mark.parametrize("rows,v,dtype", [(272, 33003, "f32"), (272, 66001, "bf16"), (256, 65544, "f16"),
+                                          (600, 33100, "f32"), (2500, 9001, "f32"), (3000, 700, "f32")])
+def test_rows_beyond_a_workgroup_and_the_caches(cuda, rows, v, dtype):
+    """Rows of which a workgroup holds a part, every sixteenth a special one;
+    logits and gradient of more than the caches keep; in place."""
+    print(f"large rows={rows} v={v} {dtype}", flush=True)
+    t = TYPES[dtype]
+    x, g = logits(rows, v, t, v)
+    at = torch.randint(v, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    odd, odd_at, _ = special(v, t)
+    x[:16], at[:16] = odd, odd_at
+    x[rows - 16:], at[rows - 16:] = odd, odd_at
+    dl, de = (torch.randn(rows, generator=g, device="cuda") for _ in range(2))
+    dt = torch.randn(rows, 3, generator=g, device="cuda")
+    op = ops.LogProbs(3)
+    out, save = op.forward(x, at)
+    verify(x, at, 3, out, op.backward((dl, de, dt), x, at, out[3], save), (dl, de, dt))
+    (logp, entropy), d = op.value_and_grad(x, at, dl, de)
+    verify(x, at, 0, (logp, entropy, None, None), d, (dl, de, None))
+    y = x.clone()
+    op.value_and_grad(y, at, dl, de, out=y)
+    assert torch.equal(y.nan_to_num(nan=3.0), d.nan_to_num(nan=3.0))
+
+
+@pytest.mark.parametrize("v", [33, 3001, 70000])
+def test_without_targets(cuda, v):
+    """Entropies and alternatives alone, and their gradients."""
+    x, g = logits(5, v, torch.float32, v)
+    de, dt = torch.randn(5, generator=g, device="cuda"), torch.randn(5, 6, generator=g, device="cuda")
+    op = ops.LogProbs(6)
+    out, save = op.forward(x)
+    assert out[0] is None
+    verify(x, None, 6, out, op.backward((None, de, dt), x, None, out[3], save), (None, de, dt))
+    verify(x, None, 6, out, op.backward((None, de, None), x, None, None, save), (None, de, None))
+    verify(x, None, 6, out, op.backward((None, None, dt), x, None, out[3], save), (None, None, dt))
+    (logp, entropy), d = op.value_and_grad(x, None, None, de)
+    assert logp is None
+    verify(x, None, 0, (None, entropy, None, None), d, (None, de, None))
+    assert (op.value_and_grad(x, None)[1] == 0).all()
 
 
 @pytest.mark.parametrize("v", WIDTHS)
