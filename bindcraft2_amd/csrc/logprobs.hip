@@ -14,8 +14,16 @@
 // a target at or past V makes its row's log-probability and gradient NaN.
 //
 // Rows are independent and every element is read once and (gradient) written
-// once, a few operations a byte, so memory bounds all of it: the kernels only
-// have to keep enough 16-byte loads in flight and the row on chip.
+// once, a few operations a byte, so memory bounds most of it: the kernels have
+// to keep enough 16-byte loads in flight and the row on chip.  A read-only pass
+// reaches 6.2 to 6.9 TB/s on this card, a copy 5.0 to 6.5.  16-bit logits come
+// near the vector units' rate too (ten operations an element, one of them a
+// quarter-rate exp2), and alternatives cost instructions by their number.
+// Measured (bytes read and written once over the time):
+//   forward, f32:  262 k rows of 64 4.9 TB/s, 50 k of 1000 5.1, 4084 of 33 k 5.9
+//   forward, binary16: 2047 rows of 50 k 4.8 TB/s, with five alternatives 4.1
+//   with gradient: 262 k of 64 f32 4.6 TB/s, 50 k of 1000 f32 5.7, 5000 of 20 k
+//   bfloat16 4.4, 2048 of 131 k bfloat16 4.9
 #include "logprobs.h"
 
 #include "common.h"
@@ -681,7 +689,7 @@ Parts parts_of(A& c, int64_t rows, int splits, int K) {
 // running maximum a lane.
 template <class T, bool TOP, int NT>
 __global__ __launch_bounds__(NT, 8) void lp_stream_kernel(LogProbs a, int splits, int part,
-                                                       Parts parts) {
+                                                          Parts parts) {
   constexpr int VN = Vec<T>::N, NW = NT / 64, U = E / VN;
   __shared__ float buf[NW][4];
   __shared__ uint64_t cand[TOP ? NW * LP_MAX_TOP : 1];
@@ -883,7 +891,7 @@ __global__ __launch_bounds__(BWD_NT) void lp_gradient_kernel(LogProbs a, int spl
   if (st.live == 0.f || t < 0) {
     constexpr int VN = Vec<T>::N;
     write_zeros<T>(a, r, sp == 0 ? 0 : row.head + v0 * VN,
-                           sp == splits - 1 ? a.V : row.head + v1 * VN);
+                   sp == splits - 1 ? a.V : row.head + v1 * VN);
     return;
   }
   write_gradient<T, BWD_NT, ONCE>(a, r, t, st, a.K, row, v0, v1, sp == 0);
@@ -1052,7 +1060,7 @@ __global__ __launch_bounds__(BOTH_NT, 8) void lp_both_kernel(LogProbs a) {
 // Which kernel
 // ---------------------------------------------------------------------------
 constexpr int ROW_VECS = 128;      // vectors that a group of lanes holds
-constexpr int WAVE_MAX = 8192;     // longest row read by one wave
+constexpr int PART_MIN = 8192;     // longest row that is always read whole
 constexpr int BLOCK_VECS = 8192;   // vectors that one workgroup holds in registers
 
 template <class T>
@@ -1073,7 +1081,7 @@ Split split_of(int dtype, int64_t rows, int V, int K) {
   // 20 of 32 rows of 150 k: 32 parts 39 us, 8 parts 24)
   const int64_t most = K > 0 ? std::min(MAX_SPLITS, std::max(4, 256 / K)) : MAX_SPLITS;
   int64_t s = std::min<int64_t>({(nv + chunk - 1) / chunk, fill, most});
-  if (s < 1 || V <= WAVE_MAX) s = 1;
+  if (s < 1 || V <= PART_MIN) s = 1;
   return Split{(int)s, (int)((nv + s - 1) / s)};
 }
 
@@ -1124,7 +1132,12 @@ void fwd(hipStream_t st, const LogProbs& a, void* work) {
     Carver c(work);
     parts = parts_of(c, a.rows, s.splits, a.K);
   }
-  if (a.V <= WAVE_MAX) stream_go<T, 64>(st, a, s, parts);
+  // A wave by itself collects its row's alternatives once, and joins nothing,
+  // where rows enough fill the card with waves: five alternatives of 2048 rows
+  // of 8000 bfloat16 15.5 us against 17.5, 8000 rows of 5003 28 against 47; of
+  // 256 rows of 8000 11.5 against 8.3.
+  const bool waves = a.V <= 2048 || (a.V <= PART_MIN && a.total >= 6 * (int64_t)device_cus());
+  if (waves) stream_go<T, 64>(st, a, s, parts);
   else stream_go<T, 256>(st, a, s, parts);
   if (s.splits > 1) lp_join_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a, s.splits, parts);
 }
@@ -1193,7 +1206,7 @@ void by_type(int dtype, F f) {
 }  // namespace
 
 size_t logprobs_work_bytes(int dtype, int64_t rows, int V, int K) {
-  if (rows <= 0 || V <= WAVE_MAX) return 0;
+  if (rows <= 0 || V <= PART_MIN) return 0;
   const Split s = split_of(dtype, rows, V, K);
   Sizer z;
   if (s.splits > 1 || in_parts(dtype, rows, V)) z.take<float>(4 * (size_t)rows);
