@@ -10,7 +10,10 @@
 // tensors' sizes, so a list of thousands costs the launches of one tensor.
 // The squares are summed in f64: an f32 gradient's square can pass f32's
 // range, and the chunks' sums are added in one fixed order, so a norm is the
-// same every time.
+// same every time.  (Its cost is hidden: a read-only pass with f32 squares is
+// as long.)  Measured on 4080 tensors of 88 M f32 elements: the squares' pass
+// 60 us (5.9 TB/s), the clipping's 108 (6.5, part of it read from the Infinity
+// Cache), Adam's 437 (5.6); a copy reaches 5.0 to 6.5 TB/s on this card.
 #include "optim.h"
 
 #include "common.h"

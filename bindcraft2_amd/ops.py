@@ -751,7 +751,7 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # BC2N_F32, _
 
 def _current(t, what):
     """t on the device that the calls go to: the current one."""
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():  # -1: on the host
         raise ValueError(f"{what}: expected a tensor on the current device, got {t.device}")
     return t
 
@@ -773,9 +773,6 @@ class LogProbs:
     @staticmethod
     def _rows(t, what):
         """(address, row stride) of [..., classes] as rows."""
-        if t.dim() == 0 or t.dtype not in _DTYPES:
-            raise ValueError(f"{what}: expected float32, float16 or bfloat16 [..., classes], got "
-                             f"{t.dtype} {tuple(t.shape)}")
         _current(t, what)
         v = t.shape[-1]
         if t.is_contiguous():
@@ -790,8 +787,11 @@ class LogProbs:
         return t.data_ptr(), (t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else v)
 
     def _operands(self, logits, targets):
+        code, shape = _DTYPES.get(logits.dtype), logits.shape
+        if code is None or not shape:
+            raise ValueError(f"logits: expected float32, float16 or bfloat16 [..., classes], got "
+                             f"{logits.dtype} {tuple(shape)}")
         x, ld = self._rows(logits, "logits")
-        shape = logits.shape
         v, lead = shape[-1], shape[:-1]
         rows = logits.numel() // v if v else 0
         t, bits = None, 32
@@ -803,7 +803,7 @@ class LogProbs:
             if targets.shape != lead:
                 raise ValueError(f"targets: expected {tuple(lead)}, got {tuple(targets.shape)}")
             t = self._given(targets, "targets")
-        return (_DTYPES[logits.dtype], x, ld, rows, v, t, bits), rows, v, lead
+        return (code, x, ld, rows, v, t, bits), rows, v, lead
 
     @staticmethod
     def _given(t, what):

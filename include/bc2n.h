@@ -679,7 +679,8 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
  *     m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
  *     p' = p - lr (m' / (1 - beta1^step) / (sqrt(v' / (1 - beta2^step)) + eps)
  *                  + weight_decay p)
- *     in f32, rounded once; step counts from 1.  scalars, or NULL: f32[2] on
+ *     in f32, rounded once; step counts from 1.  A norm that is NaN makes all
+ *     of it NaN.  scalars, or NULL: f32[2] on
  *     the device, lr and step in place of the arguments (a captured graph's
  *     schedule).  norm (of the gradients before clipping) may be NULL.
  * ---------------------------------------------------------------------- */
