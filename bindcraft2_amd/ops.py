@@ -818,15 +818,6 @@ class LogProbs:
         _f32(t, shape, what)
         return self._given(t, what)
 
-    @staticmethod
-    def _work(code, rows, v, top, device):
-        """(scratch, its address) of a forward; one without any needs none."""
-        n = lib().bc2n_logprobs_work_bytes(code, rows, v, top)
-        if n == 0:
-            return None, None
-        work = torch.empty(n, dtype=torch.uint8, device=device)
-        return work, work.data_ptr()
-
     def _gradient(self, logits, out):
         if out is None:
             out = torch.empty_like(logits, memory_format=torch.contiguous_format)
@@ -846,21 +837,25 @@ class LogProbs:
         else:  # empty_like takes half the time that a shape takes
             logp, entropy = torch.empty_like(targets, dtype=f32), torch.empty_like(targets, dtype=f32)
             a = logp.data_ptr()
-        save = torch.empty(4 * rows, dtype=f32, device=dev)
+        # the scratch of few long rows lies behind the save-set: one allocation less
+        scratch = lib().bc2n_logprobs_work_bytes(operands[0], rows, v, top)
+        save = torch.empty(4 * rows + scratch // 4, dtype=f32, device=dev)
         if top:
             top_logp = torch.empty((*lead, top), dtype=f32, device=dev)
             top_index = torch.empty((*lead, top), dtype=torch.int32, device=dev)
             b, c = top_logp.data_ptr(), top_index.data_ptr()
-        work, w = self._work(operands[0], rows, v, top, dev)
-        check(lib().bc2n_logprobs_fwd(_stream(), *operands, top, a, entropy.data_ptr(), b, c,
-                                      save.data_ptr(), w))
+        at = save.data_ptr()
+        check(lib().bc2n_logprobs_fwd(_stream(), *operands, top, a, entropy.data_ptr(), b, c, at,
+                                      at + 16 * rows if scratch else None))
         return (logp, entropy, top_logp, top_index), save
 
     def backward(self, cts, logits, targets, top_index, save, out=None):
         """cts = (d_logp, d_entropy, d_top_logp), any None -> d_logits (in `out`
         where given, which may be logits itself)"""
         operands, rows, v, lead = self._operands(logits, targets)
-        _f32(save, (4 * rows,), "save")
+        if save.dtype != torch.float32 or save.dim() != 1 or save.numel() < 4 * rows:
+            raise ValueError(f"save: expected the forward's of {rows} rows, got {save.dtype} "
+                             f"{tuple(save.shape)}")
         i = None
         if top_index is not None:
             if top_index.dtype != torch.int32 or top_index.shape != (*lead, self.top):
@@ -888,8 +883,10 @@ class LogProbs:
             logp = torch.empty_like(targets, dtype=torch.float32)
             entropy = torch.empty_like(logp)
             a = logp.data_ptr()
-        work, w = self._work(operands[0], rows, v, 0, dev)
-        check(lib().bc2n_logprobs_grad(_stream(), *operands, *c, a, entropy.data_ptr(), o, ld, w))
+        scratch = lib().bc2n_logprobs_work_bytes(operands[0], rows, v, 0)
+        work = torch.empty(scratch, dtype=torch.uint8, device=dev) if scratch else None
+        check(lib().bc2n_logprobs_grad(_stream(), *operands, *c, a, entropy.data_ptr(), o, ld,
+                                       _ptr(work)))
         return (logp, entropy), out
 
 
