@@ -1186,7 +1186,17 @@ void lp_gradient(LogProbs& a, void* d_logits, int64_t d_ld) {
   need(a.rows == 0 || d_logits, "null output");
   need(d_ld >= a.V, "logprobs: the gradient's row stride is below the number of classes");
   need(d_logits != a.x || d_ld == a.ld, "logprobs: a gradient in place has the logits' row stride");
-  aligned(d_logits, a.dtype == BC2N_F32 ? 4 : 2, "d_logits");
+  const int64_t w = a.dtype == BC2N_F32 ? 4 : 2;
+  aligned(d_logits, (int)w, "d_logits");
+  if (d_logits != a.x && a.rows > 0) {
+    // apart, or columns of one buffer that no class shares
+    const intptr_t x = reinterpret_cast<intptr_t>(a.x), d = reinterpret_cast<intptr_t>(d_logits);
+    const bool apart = d >= x + ((a.rows - 1) * a.ld + a.V) * w ||
+                       x >= d + ((a.rows - 1) * d_ld + a.V) * w;
+    const int64_t column = (((d - x) / w) % a.ld + a.ld) % a.ld;
+    need(apart || (d_ld == a.ld && column >= a.V && column + a.V <= a.ld),
+         "logprobs: the gradient overlaps the logits");
+  }
   a.d = d_logits;
   a.d_ld = d_ld;
 }

@@ -29,6 +29,7 @@ constexpr int LIST_INLINE = 32;  // tensors whose entries go with the launch
 struct DeviceBlock {
   char* p = nullptr;
   size_t n = 0;
+  int device = 0;
 };
 
 // A list as the kernels take it: cut into chunks of at most `chunk` elements

@@ -335,8 +335,10 @@ struct Tables {
   std::vector<DeviceBlock> free;
   DeviceBlock take(size_t n) {
     std::lock_guard<std::mutex> lk(mu);
+    int dev = 0;
+    BC2N_HIP(hipGetDevice(&dev));
     for (size_t i = 0; i < free.size(); ++i)
-      if (free[i].n >= n) {
+      if (free[i].n >= n && free[i].device == dev) {
         // a launch that reads the old table may still be queued
         BC2N_HIP(hipDeviceSynchronize());
         const DeviceBlock b = free[i];
@@ -346,6 +348,7 @@ struct Tables {
     DeviceBlock b;
     BC2N_HIP(hipMalloc(reinterpret_cast<void**>(&b.p), n));
     b.n = n;
+    b.device = dev;
     return b;
   }
   void give(DeviceBlock b) {

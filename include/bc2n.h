@@ -618,8 +618,9 @@ int bc2n_confidence_bwd(void* stream, const float* plddt_logits, const float* pa
  *   logp = log p_t, entropy = -sum_j p_j log p_j, and for the `top` largest
  *   logits (ties to the lowest class; top 0..32) top_index and top_logp =
  *   log p, both [rows][top], in descending order.
- * All outputs f32 (top_index i32); sums and statistics are f32.  logp and
- * entropy may be NULL (not wanted).
+ * All outputs f32 (top_index i32); sums and statistics are f32, added in an
+ * order that goes by the shape and the rows' alignment to 16 bytes alone.
+ * logp and entropy may be NULL (not wanted).
  *   - A negative target leaves its row out: its logits have no effect (they
  *     may hold anything), its outputs and gradient are 0, its indices -1.
  *   - A logit of -inf has probability 0 (a target there: logp -inf); a row of
@@ -634,7 +635,8 @@ int bc2n_confidence_bwd(void* stream, const float* plddt_logits, const float* pa
  * bwd: cotangents d_logp [rows], d_entropy [rows], d_top_logp [rows][top]
  * (any may be NULL; the last needs the forward's top_index) -> d_logits of
  * the logits' type, row stride d_ld, rounded once; d_logits may be logits
- * itself with d_ld = ld, and overlaps them in no other way.
+ * itself with d_ld = ld, or other columns of their buffer with d_ld = ld, and
+ * otherwise shares no memory with them.
  * grad: forward and backward in one call for cotangents known beforehand
  * (a weighted likelihood), the logits read once where a row stays on chip.
  * ---------------------------------------------------------------------- */

@@ -241,6 +241,24 @@ def test_strides_and_what_lies_between(cuda, v, dtype):
     assert torch.equal(third[~gap], one.flatten())
 
 
+@pytest.mark.parametrize("v", [20, 999, 4001])
+def test_gradient_beside_the_logits(cuda, v):
+    """Logits and gradient as columns of one buffer."""
+    x, g = logits(9, v, torch.float32, v)
+    buf = torch.full((9, 2 * v + 3), 11.0, device="cuda")
+    buf[:, :v] = x
+    t = torch.randint(v, (9,), generator=g, device="cuda")
+    dl = torch.randn(9, generator=g, device="cuda")
+    (lp, en), d = ops.LogProbs().value_and_grad(buf[:, :v], t, dl, out=buf[:, v + 1:2 * v + 1])
+    assert torch.equal(buf[:, :v], x)
+    # (not the bits of the same rows elsewhere: a sum's order goes by a row's
+    # alignment to 16 bytes)
+    verify(x, t, 0, (lp, en, None, None), d, (dl, None, None))
+    assert (buf[:, v] == 11).all() and (buf[:, 2 * v + 1:] == 11).all()
+    with pytest.raises(NativeError, match="overlaps"):
+        ops.LogProbs().value_and_grad(buf[:, :v], t, dl, out=buf[:, 1:v + 1])
+
+
 def test_leading_dimensions_and_empty(cuda):
     x = torch.randn(4, 5, 64, device="cuda")
     t = torch.randint(64, (4, 5), device="cuda")

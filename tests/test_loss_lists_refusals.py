@@ -45,6 +45,13 @@ def test_logprobs_refusals():
     refused(bwd(d=None), b"null")
     refused(bwd(dld=63), b"stride")
     refused(bwd(d=P, ld=64, dld=65), b"in place")
+    refused(bwd(d=P + 2), b"overlaps")
+    refused(bwd(d=P + 2 * 64 * 3 + 2 * 63), b"overlaps")  # the last row's last class
+    refused(bwd(x=P + 2 * 64, d=P), b"overlaps")
+    refused(bwd(ld=200, d=P + 2 * 63, dld=200), b"overlaps")
+    refused(bwd(ld=200, d=P + 2 * 150, dld=200), b"overlaps")  # into the next row
+    refused(bwd(ld=200, d=P + 2 * 100, dld=201), b"overlaps")
+    refused(bwd(ld=200, d=P + 2 * 64, dld=200, save=None), b"null")  # columns beside: taken
     refused(bwd(save=None), b"null")
     refused(bwd(t=None), b"targets")
     refused(bwd(h=P), b"top_index")
