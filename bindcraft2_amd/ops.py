@@ -892,7 +892,8 @@ class LogProbs:
 
 class _TensorList:
     """A list of the C ABI over tensors, which it keeps alive and takes to
-    stay where they are."""
+    stay where they are: it holds their addresses, so what a call returns in a
+    new tensor (a backward's gradient) is copied into the list's."""
 
     def __init__(self, handle, tensors):
         if not handle:
