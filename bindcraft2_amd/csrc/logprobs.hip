@@ -11,7 +11,8 @@
 // (g, e, h the cotangents of logp, H and top k).  A row with t < 0 is left
 // out (zeros, indices -1); a row of -inf alone has log-probabilities -inf,
 // entropy and gradient 0; a NaN or +inf makes its row NaN and its indices -1;
-// a target at or past V makes its row's log-probability and gradient NaN.
+// a target at or past V makes its row's log-probability and gradient NaN,
+// whichever cotangents are given.
 //
 // Rows are independent and every element is read once and (gradient) written
 // once, a few operations a byte, so memory bounds most of it: the kernels have
@@ -52,6 +53,9 @@ __device__ __forceinline__ int64_t target_of(const LogProbs& a, int64_t r) {
   return a.target64 ? reinterpret_cast<const int64_t*>(a.target)[r]
                     : (int64_t) reinterpret_cast<const int32_t*>(a.target)[r];
 }
+// A target past the classes makes its row's gradient NaN, whatever the
+// cotangents and the logits.  (Without targets t is 0.)
+__device__ __forceinline__ bool past_classes(const LogProbs& a, int64_t t) { return t >= a.V; }
 
 // m, s, u of a part of a row
 struct Stat {
@@ -493,7 +497,6 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LogProbs a) {
     float all = g;
     if (MODE == 2 && a.d_top)
       for (int k = 0; k < a.K; ++k) all += a.d_top[r * a.K + k];
-    if (a.d_logp && t >= a.V) all = __builtin_nanf("");
     const Cotangent c(st, all, a.d_entropy ? a.d_entropy[r] : 0.f);
     float d[E];
 #pragma unroll
@@ -513,11 +516,13 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LogProbs a) {
       }
     }
     T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
+    const bool past = past_classes(a, t), one = past || st.live == 0.f || !counts;
+    const float all_of = past ? __builtin_nanf("") : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int j = 0; j < VN; ++j)
-        if (st.live == 0.f || !counts) d[i * VN + j] = 0.f;
+        if (one) d[i * VN + j] = all_of;
       if (mine && skip[i] < VN) {
         if constexpr (VN == 1) o[pos[i]] = (T)d[i];
         else Vec<T>::store(o + pos[i], Vec<T>::pack(d + i * VN));
@@ -794,16 +799,22 @@ __global__ __launch_bounds__(256) void lp_join_kernel(LogProbs a, int splits, Pa
   if (a.K > 0) write_tops<T, 256>(a, r, st, cand, n);
 }
 
-// zeros over row r's gradient
+// One value over [lo, hi) of row r's gradient: NaN for a target past the
+// classes, else zero.
 template <class T>
-__device__ __forceinline__ void write_zeros(const LogProbs& a, int64_t r, int64_t lo, int64_t hi) {
+__device__ __forceinline__ void write_one(const LogProbs& a, int64_t r, int64_t t, int64_t lo,
+                                          int64_t hi) {
   constexpr int VN = Vec<T>::N;
   const int NT = blockDim.x;
   T* o = reinterpret_cast<T*>(a.d) + r * a.d_ld;
+  float x[VN];
+#pragma unroll
+  for (int i = 0; i < VN; ++i) x[i] = past_classes(a, t) ? __builtin_nanf("") : 0.f;
+  const u32x4 v = Vec<T>::pack(x);
   for (int64_t at = lo + threadIdx.x * VN; at < hi; at += NT * VN) {
-    if (at + VN <= hi) Vec<T>::store(o + at, u32x4{0, 0, 0, 0});
+    if (at + VN <= hi) Vec<T>::store(o + at, v);
     else
-      for (int64_t j = at; j < hi; ++j) o[j] = (T)0.f;
+      for (int64_t j = at; j < hi; ++j) o[j] = (T)x[0];
   }
 }
 
@@ -830,7 +841,7 @@ __device__ __forceinline__ Special special_of(const LogProbs& a, int64_t r, int6
       s.at = t;
       s.own = gt;
     }
-    g += t >= a.V ? __builtin_nanf("") : gt;
+    g += gt;
   }
   return s;
 }
@@ -888,10 +899,10 @@ __global__ __launch_bounds__(BWD_NT) void lp_gradient_kernel(LogProbs a, int spl
   const RowStat st{s.x, s.y, s.z, s.w};
   const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
   const int v0 = min(row.nv, sp * part), v1 = min(row.nv, v0 + part);
-  if (st.live == 0.f || t < 0) {
+  if (st.live == 0.f || t < 0 || past_classes(a, t)) {
     constexpr int VN = Vec<T>::N;
-    write_zeros<T>(a, r, sp == 0 ? 0 : row.head + v0 * VN,
-                   sp == splits - 1 ? a.V : row.head + v1 * VN);
+    write_one<T>(a, r, t, sp == 0 ? 0 : row.head + v0 * VN,
+                 sp == splits - 1 ? a.V : row.head + v1 * VN);
     return;
   }
   write_gradient<T, BWD_NT, ONCE>(a, r, t, st, a.K, row, v0, v1, sp == 0);
@@ -908,7 +919,7 @@ __global__ __launch_bounds__(1024) void lp_block_kernel(LogProbs a) {
   const int64_t t = target_of(a, r);
   if (t < 0) {
     if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
-    write_zeros<T>(a, r, 0, a.V);
+    write_one<T>(a, r, t, 0, a.V);
     return;
   }
   const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
@@ -942,9 +953,9 @@ __global__ __launch_bounds__(1024) void lp_block_kernel(LogProbs a) {
   q.add(ex);
   const RowStat st = finish(join(q, buf, NT / 64), true);
   if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
-  if (st.live == 0.f) {
+  if (st.live == 0.f || past_classes(a, t)) {
     __syncthreads();  // the target's logit is read before its place is written
-    write_zeros<T>(a, r, 0, a.V);
+    write_one<T>(a, r, t, 0, a.V);
     return;
   }
   float g;
@@ -983,7 +994,7 @@ __global__ __launch_bounds__(BOTH_NT, 8) void lp_both_kernel(LogProbs a) {
   const int64_t t = target_of(a, r);
   if (t < 0) {
     if (threadIdx.x == 0) write_row<T>(a, r, finish(Stat(), false), -1);
-    write_zeros<T>(a, r, 0, a.V);
+    write_one<T>(a, r, t, 0, a.V);
     return;
   }
   const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
@@ -1025,9 +1036,9 @@ __global__ __launch_bounds__(BOTH_NT, 8) void lp_both_kernel(LogProbs a) {
   add_chunk(q, one, ex);
   const RowStat st = finish(join(q, buf, NT / 64), true);
   if (lane == 0) write_row<T>(a, r, st, a.target ? t : -1);
-  if (st.live == 0.f) {
+  if (st.live == 0.f || past_classes(a, t)) {
     __syncthreads();  // the target's logit is read before its place is written
-    return write_zeros<T>(a, r, 0, a.V);
+    return write_one<T>(a, r, t, 0, a.V);
   }
   float g;
   const Special sp = special_of(a, r, t, 0, g);

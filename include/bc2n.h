@@ -626,7 +626,8 @@ int bc2n_confidence_bwd(void* stream, const float* plddt_logits, const float* pa
  *   - A logit of -inf has probability 0 (a target there: logp -inf); a row of
  *     -inf alone has log-probabilities -inf, entropy 0 and gradient 0.
  *   - A NaN or +inf makes its row's outputs and gradient NaN, its indices -1.
- *   - A target >= classes makes its row's logp and its gradient NaN.
+ *   - A target >= classes makes its row's logp and its gradient NaN (whichever
+ *     cotangents are given; in a row of -inf alone too).
  * save (NULL: no backward follows) is bc2n_logprobs_save_bytes(rows) bytes,
  * 16-byte aligned, written by fwd and read by bwd; work is a scratch buffer of
  * bc2n_logprobs_work_bytes() bytes, 16-byte aligned, for the time of the call
