@@ -1005,8 +1005,8 @@ class Adam(_TensorList):
     def step(self, step, lr, max_norm=None, scalars=None):
         """Step number `step` (from 1).  max_norm: the gradients clipped to that
         global norm first -> their norm before, f32 [1] on the device (None
-        without).  scalars: f32 [2] on the device, lr and step in place of the
-        arguments."""
+        without).  scalars: contiguous f32 [2] on the device, lr and step in place
+        of the arguments."""
         norm, work, w = self._scratch()
         if max_norm is None:
             norm = None
@@ -1014,7 +1014,8 @@ class Adam(_TensorList):
             raise ValueError("max_norm must be positive")
         if scalars is not None:
             _f32(scalars, (2,), "scalars")
-            _current(scalars, "scalars")
+            if not _current(scalars, "scalars").is_contiguous():
+                raise ValueError("scalars: lr and step have to lie side by side")
         check(lib().bc2n_adam_step(_stream(), self.handle, float(lr), *self.betas, self.eps,
                                    self.weight_decay, int(step), float(max_norm or 0.0),
                                    _ptr(scalars), _ptr(norm), w))
