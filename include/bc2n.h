@@ -682,10 +682,13 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
  *     m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
  *     p' = p - lr (m' / (1 - beta1^step) / (sqrt(v' / (1 - beta2^step)) + eps)
  *                  + weight_decay p)
- *     in f32, rounded once; step counts from 1.  A norm that is NaN makes all
- *     of it NaN.  scalars, or NULL: f32[2] on
- *     the device, lr and step in place of the arguments (a captured graph's
- *     schedule).  norm (of the gradients before clipping) may be NULL.
+ *     in f32, rounded once; step counts from 1.  The scalars have to be f32's:
+ *     refused are an eps that rounds to 0 or is not finite, and an lr whose
+ *     quotient by 1 - beta1^step or product with weight_decay is past its
+ *     range.  A norm that is NaN makes all of it NaN.  scalars, or NULL: f32[2]
+ *     on the device, lr and step in place of the arguments (a captured graph's
+ *     schedule; its values are not checked).  norm (of the gradients before
+ *     clipping) may be NULL.
  * ---------------------------------------------------------------------- */
 void* bc2n_grad_list(int count, const void* const* grads, const int64_t* sizes, const int* dtypes,
                      void* const* out);
