@@ -407,11 +407,12 @@ __device__ __forceinline__ void tops_by_lane(const LogProbs& a, int64_t r, bool 
 
 // f32 logits of a row that is a wave's, more than four a lane: a sort of them
 // would cost more than the list (K = 3 of 100 k rows of 500: 79 us).
-template <class T, int VN, int NV>
+template <class T, int VN, int W, int NV>
 __device__ __forceinline__ void tops_by_list(const LogProbs& a, int64_t r, bool mine,
                                              const RowStat& st, bool counts,
                                              const float (&x)[VN * NV], const int (&pos)[NV],
                                              const int (&skip)[NV]) {
+  static_assert(W == 64, "the list is a whole wave's, of one row");
   const int lane = threadIdx.x & 63;
   TopList top;
   if (counts && !is_nan(st.logs)) {
@@ -470,21 +471,24 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LogProbs a) {
     st = finish(q, counts);
     if (mine && l == 0) write_row<T>(a, r, st, a.target ? t : -1);
 
-    if (MODE == 1 && a.K > 0) {
-      if constexpr (sizeof(T) == 4 && E > 4) {
-        tops_by_list<T, VN, NV>(a, r, mine, st, counts, x, pos, skip);
-      } else {
-        uint32_t key[E];
-        int at[E];
+    // two vectors a lane by fewer than 64 lanes: without alternatives alone
+    if constexpr (MODE == 1 && (NV == 1 || W == 64)) {
+      if (a.K > 0) {
+        if constexpr (sizeof(T) == 4 && E > 4) {
+          tops_by_list<T, VN, W, NV>(a, r, mine, st, counts, x, pos, skip);
+        } else {
+          uint32_t key[E];
+          int at[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          at[i] = pos[i / VN] + i % VN;
-          const bool real = i % VN >= skip[i / VN];
-          if constexpr (sizeof(T) == 2) key[i] = real ? key16<T>(x[i], at[i]) : 0u;
-          else key[i] = real ? order_key(x[i]) : 0u;
+          for (int i = 0; i < E; ++i) {
+            at[i] = pos[i / VN] + i % VN;
+            const bool real = i % VN >= skip[i / VN];
+            if constexpr (sizeof(T) == 2) key[i] = real ? key16<T>(x[i], at[i]) : 0u;
+            else key[i] = real ? order_key(x[i]) : 0u;
+          }
+          if constexpr (sizeof(T) == 2) tops_by_key<T, W>(a, r, mine, st, counts, key);
+          else tops_by_lane<W>(a, r, mine, st, counts, key, at);
         }
-        if constexpr (sizeof(T) == 2) tops_by_key<T, W>(a, r, mine, st, counts, key);
-        else tops_by_lane<W>(a, r, mine, st, counts, key, at);
       }
     }
   } else {
@@ -1113,12 +1117,14 @@ void rows_launch(hipStream_t st, const LogProbs& a) {
   // joins: V = 64 f32 with gradient 32.8 -> 29.3 us, forward 17.2 -> 14.1 (262 k
   // rows); four (64 bytes between a lane's stores and the next's) 38.  With
   // alternatives one: they cost by the elements of a lane.
-  if (MODE == 1 && a.K > 0) {
-    if (vecs <= 4) return rows_go<T, N, 4, 1, MODE>(st, a);
-    if (vecs <= 8) return rows_go<T, N, 8, 1, MODE>(st, a);
-    if (vecs <= 16) return rows_go<T, N, 16, 1, MODE>(st, a);
-    if (vecs <= 32) return rows_go<T, N, 32, 1, MODE>(st, a);
-    if (vecs <= 64) return rows_go<T, N, 64, 1, MODE>(st, a);
+  if constexpr (MODE == 1) {
+    if (a.K > 0) {
+      if (vecs <= 4) return rows_go<T, N, 4, 1, MODE>(st, a);
+      if (vecs <= 8) return rows_go<T, N, 8, 1, MODE>(st, a);
+      if (vecs <= 16) return rows_go<T, N, 16, 1, MODE>(st, a);
+      if (vecs <= 32) return rows_go<T, N, 32, 1, MODE>(st, a);
+      if (vecs <= 64) return rows_go<T, N, 64, 1, MODE>(st, a);
+    }
   }
   if (vecs <= 8) rows_go<T, N, 4, 2, MODE>(st, a);
   else if (vecs <= 16) rows_go<T, N, 8, 2, MODE>(st, a);
