@@ -18,3 +18,9 @@ def cuda():
     if not torch.cuda.is_available():
         pytest.skip("no GPU")
     return torch.device("cuda")
+
+
+def pytest_collection_modifyitems(items):
+    """First what looks at the library before any call has failed: the tests
+    of refusals leave their messages."""
+    items.sort(key=lambda item: item.name != "test_host_only_calls")
