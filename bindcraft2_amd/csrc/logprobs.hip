@@ -847,6 +847,7 @@ __device__ __forceinline__ Special special_of(const LogProbs& a, int64_t r, int6
     }
     g += gt;
   }
+  if (past_classes(a, t)) g = __builtin_nanf("");
   return s;
 }
 __device__ __forceinline__ Cotangent cotangent_of(const LogProbs& a, int64_t r, const RowStat& st,
@@ -903,7 +904,7 @@ __global__ __launch_bounds__(BWD_NT) void lp_gradient_kernel(LogProbs a, int spl
   const RowStat st{s.x, s.y, s.z, s.w};
   const Row<T> row(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
   const int v0 = min(row.nv, sp * part), v1 = min(row.nv, v0 + part);
-  if (st.live == 0.f || t < 0 || past_classes(a, t)) {
+  if (st.live == 0.f || t < 0) {
     constexpr int VN = Vec<T>::N;
     write_one<T>(a, r, t, sp == 0 ? 0 : row.head + v0 * VN,
                  sp == splits - 1 ? a.V : row.head + v1 * VN);
@@ -957,7 +958,7 @@ __global__ __launch_bounds__(1024) void lp_block_kernel(LogProbs a) {
   q.add(ex);
   const RowStat st = finish(join(q, buf, NT / 64), true);
   if (threadIdx.x == 0) write_row<T>(a, r, st, a.target ? t : -1);
-  if (st.live == 0.f || past_classes(a, t)) {
+  if (st.live == 0.f) {
     __syncthreads();  // the target's logit is read before its place is written
     write_one<T>(a, r, t, 0, a.V);
     return;
@@ -1040,7 +1041,7 @@ __global__ __launch_bounds__(BOTH_NT, 8) void lp_both_kernel(LogProbs a) {
   add_chunk(q, one, ex);
   const RowStat st = finish(join(q, buf, NT / 64), true);
   if (lane == 0) write_row<T>(a, r, st, a.target ? t : -1);
-  if (st.live == 0.f || past_classes(a, t)) {
+  if (st.live == 0.f) {
     __syncthreads();  // the target's logit is read before its place is written
     return write_one<T>(a, r, t, 0, a.V);
   }
