@@ -19,8 +19,13 @@
 // to keep enough 16-byte loads in flight and the row on chip.  A read-only pass
 // reaches 6.2 to 6.9 TB/s on this card, a copy 5.0 to 6.5.  16-bit logits come
 // near the vector units' rate too (ten operations an element, one of them a
-// quarter-rate exp2), and alternatives cost instructions by their number.
-// Measured (bytes read and written once over the time):
+// quarter-rate exp2), and alternatives cost instructions by their number, for
+// longer rows also by the logits' order: where they rise along the classes,
+// every element enters a wave's list (one that falls, or random ones, leave it
+// to the first chunk's bound).  Five alternatives of 2047 rows of 50 k binary16:
+// random 47 us, falling 40, rising 706; eight of 4 rows of 131 k bfloat16: 12,
+// 39, 36.
+// Measured on random logits (bytes read and written once over the time):
 //   forward, f32:  262 k rows of 64 4.9 TB/s, 50 k of 1000 5.1, 4084 of 33 k 5.9
 //   forward, binary16: 2047 rows of 50 k 4.8 TB/s, with five alternatives 4.1
 //   with gradient: 262 k of 64 f32 4.6 TB/s, 50 k of 1000 f32 5.7, 5000 of 20 k
@@ -1117,7 +1122,11 @@ void rows_launch(hipStream_t st, const LogProbs& a) {
   // Two vectors a lane keep more loads in flight and halve the lanes that a sum
   // joins: V = 64 f32 with gradient 32.8 -> 29.3 us, forward 17.2 -> 14.1 (262 k
   // rows); four (64 bytes between a lane's stores and the next's) 38.  With
-  // alternatives one: they cost by the elements of a lane.
+  // alternatives one, for the least time of few rows with two or three (50 k of
+  // 64 f32: two 6.8 against 7.3 us, eight 10.0 against 9.5).  Many rows would
+  // gain from two there as well (262 k of 64 f32: one alternative 21.8 against
+  // 19.7 us, eight 37.4 against 32.7; 100 k of 500 bfloat16: 45 against 37, 77
+  // against 62), which this rule does not take.
   if constexpr (MODE == 1) {
     if (a.K > 0) {
       if (vecs <= 4) return rows_go<T, N, 4, 1, MODE>(st, a);

@@ -34,9 +34,15 @@ constexpr int NT = 256;          // threads of a chunk's workgroup
 constexpr int64_t CHUNK = 8192;  // elements of a chunk, at least
 constexpr uint32_t MANY = 16384; // chunks of a list beyond which they grow
 constexpr int ONE_NT = 1024;     // threads of a small list's one workgroup
-// elements of a small list.  One workgroup against three launches, in a graph:
-// clip of 24 k elements 7.5 against 8.7 us, of 61 k 13.1 against 9.5; Adam of
-// 4.5 k 7.3 against 10.8 us, of 16 k 12.2 against 10.7
+// elements of a small list.  One workgroup against three launches, in a graph,
+// one tensor of f32: clip of 4480 elements 3.6 against 7.0 us, of 32 k 5.6
+// against 7.6, of 61 k 9.2 against 8.0; clipped Adam of 4480 4.6 against 9.2, of
+// 16 k 8.3 against 11.9.  Three tensors: clip of 12 k 5.3 against 8.0, of 33 k
+// 7.3 against 7.9; clipped Adam of 12 k 7.6 against 9.2.  The workgroup takes a
+// list's tensors one after another, so it falls behind from six to eight of them
+// (six of 1000: clip 6.3 against 6.7 us, clipped Adam 8.6 against 7.1; eight 7.7
+// against 6.8 and 10.7 against 7.2; 32 of 100 22.5 against 6.8 and 36 against
+// 7.2): this rule, by elements alone, is for lists of a few states.
 constexpr int64_t SMALL_CLIP = 32768, SMALL_ADAM = 12288;
 // The Infinity Cache holds 256 MiB.  A list whose operands pass it goes by it
 // once (nontemporal loads and stores) and, after the norm, from its end: what

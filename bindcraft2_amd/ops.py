@@ -949,7 +949,8 @@ class GradientClip(_TensorList):
     """The global 2-norm of a list of gradients (f32, f16 or bf16, contiguous),
     and the gradients scaled to at most a given norm, into `out` or in place
     (bc2n_grad_norm, bc2n_grad_clip).  Made once for tensors that stay where
-    they are; many tensors cost the launches of one."""
+    they are; many tensors cost the launches of one.  Making it costs more
+    than a call: 4080 tensors 2 to 3 ms."""
 
     def __init__(self, grads, out=None):
         grads = list(grads)
@@ -979,7 +980,8 @@ class GradientClip(_TensorList):
 class Adam(_TensorList):
     """An Adam step with decoupled weight decay over lists of parameters and
     gradients (f32, f16 or bf16, contiguous) and their f32 moments, in place or
-    into out = (params, exp_avg, exp_avg_sq) (bc2n_adam_step)."""
+    into out = (params, exp_avg, exp_avg_sq) (bc2n_adam_step).  Made once, like
+    GradientClip (4080 parameters: 9 to 10 ms)."""
 
     def __init__(self, params, grads, exp_avg, exp_avg_sq, out=None, betas=(0.9, 0.999), eps=1e-8,
                  weight_decay=0.0):
