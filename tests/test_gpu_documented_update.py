@@ -17,7 +17,8 @@ HALF = 2.0 ** -24
 def documented():
     """The one Python block of the documents that makes an Adam list."""
     text = "".join(open(p, encoding="utf-8").read() for p in sorted(glob.glob(os.path.join(ROOT, "*.md"))))
-    blocks = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "ops.Adam(" in b]
+    blocks = re.findall(r"```python\n(from bindcraft2_amd import ops\n.*?)```", text, re.S)
+    blocks = [b for b in blocks if "ops.Adam(" in b]
     assert len(blocks) == 1
     return blocks[0]
 
