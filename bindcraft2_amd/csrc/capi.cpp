@@ -1376,7 +1376,8 @@ int bc2n_adam_step(void* stream, void* list, double lr, double beta1, double bet
     TensorList& l = list_of(list);
     need(l.adam, "adam_step: not a list of parameters");
     need(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adam_step: betas must be in [0, 1)");
-    need((float)eps > 0 && std::isfinite((float)eps), "adam_step: eps must be positive and finite in f32");
+    need((float)eps > 0 && std::isfinite((float)eps),
+         "adam_step: eps must be positive and finite in f32");
     need(weight_decay >= 0 && std::isfinite(weight_decay),
          "adam_step: weight_decay must be finite and not negative");
     need(scalars || (step >= 1 && std::isfinite(lr)), "adam_step: step counts from 1, lr is finite");

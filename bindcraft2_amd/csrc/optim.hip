@@ -549,7 +549,7 @@ void adam_step(hipStream_t st, const TensorList& l, const AdamScalars& s, float*
     schedule(sa.host, s.lr, (double)s.step, s.beta1, s.beta2, s.decay);
     if (!std::isfinite(sa.host.lr) || !std::isfinite(sa.host.decay))
       throw std::invalid_argument(
-          "adam_step: the learning rate over 1 - beta1^step, or by weight_decay, is past f32's range");
+          "adam_step: the learning rate over 1 - beta1^step, or by weight_decay, is past f32");
   }
   const AdamArgs aa{(float)s.beta1, (float)(1 - s.beta1), (float)s.beta2, (float)(1 - s.beta2),
                     (float)s.eps};
