@@ -34,6 +34,7 @@ def lib():
 def _declare(L):
     c = ctypes
     vp, i, f, u32, sz, cs = c.c_void_p, c.c_int, c.c_float, c.c_uint32, c.c_size_t, c.c_char_p
+    heads = [vp, c.c_int64, c.c_int64]  # an operand of heads: address, token and head strides
     L.bc2n_last_error.restype = cs
     L.bc2n_abi_version.restype = i
     sigs = {
@@ -115,6 +116,19 @@ def _declare(L):
                               + [c.c_int64]),
         "bc2n_logprobs_grad": (i, [vp, i, vp, c.c_int64, c.c_int64, i, vp, i] + [vp] * 5
                                + [c.c_int64, vp]),
+        "bc2n_headnorm_fwd": (i, [vp, i, c.c_int64] + [i] * 5 + heads * 2 + [vp, i, vp, vp, vp, i, f]
+                              + heads * 2),
+        "bc2n_headnorm_work_bytes": (sz, [c.c_int64, i]),
+        "bc2n_headnorm_bwd": (i, [vp, i, c.c_int64] + [i] * 5 + heads * 4 + [vp, i, vp, vp, vp, i, f]
+                              + heads * 2 + [vp] * 3),
+        "bc2n_attention_fwd_work_bytes": (sz, [i, i, i, c.c_int64, c.c_int64, i, i, i]),
+        "bc2n_attention_bwd_work_bytes": (sz, [i, i, i, c.c_int64, c.c_int64, i, i, i]),
+        "bc2n_attention_fwd": (i, [vp, i, i, i, c.c_int64, c.c_int64, i, i, i, f] + [vp] * 4 + heads * 3
+                               + [i] + heads + [vp, vp]),
+        "bc2n_attention_bwd": (i, [vp, i, i, i, c.c_int64, c.c_int64, i, i, i, f] + [vp] * 4 + heads * 5
+                               + [vp, i] + heads * 3 + [vp]),
+        "bc2n_sample": (i, [vp, i, vp, c.c_int64, c.c_int64, i, vp, c.c_double, vp, c.c_int64, vp,
+                            c.c_double, vp, c.c_double, vp, vp, vp]),
         "bc2n_grad_list": (vp, [i, vp, vp, vp, vp]),
         "bc2n_adam_list": (vp, [i] + [vp] * 10),
         "bc2n_list_free": (i, [vp]),

@@ -9,8 +9,11 @@
 #include "heads.h"
 #include "designstep.h"
 #include "confidence.h"
+#include "headnorm.h"
 #include "logprobs.h"
 #include "optim.h"
+#include "packattn.h"
+#include "sample.h"
 
 #include <cmath>
 #include <cstdio>
@@ -1286,6 +1289,369 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
     a.d_logp = d_logp;
     a.d_entropy = d_entropy;
     logprobs_grad(own_stream(stream), a, work);
+  });
+}
+
+namespace {
+// A [tokens][heads][width] operand and the bytes that it takes.
+struct Span {
+  intptr_t p;
+  int64_t st, row, total;  // bytes: token stride, of one token's heads, of all
+  bool by_token;           // a token's heads lie before the next token's
+};
+Span span_of(const HeadView& v, int64_t tokens, int heads, int width, int64_t es) {
+  Span s;
+  s.p = reinterpret_cast<intptr_t>(v.p);
+  s.st = v.st * es;
+  s.row = ((heads - 1) * v.sh + width) * es;
+  s.total = (tokens - 1) * s.st + s.row;
+  s.by_token = tokens == 1 || s.st >= s.row;
+  return s;
+}
+// no element in both: ranges apart, or slices of the same tokens
+bool apart(const Span& a, const Span& b) {
+  if (b.p >= a.p + a.total || a.p >= b.p + b.total) return true;
+  if (!a.by_token || !b.by_token || a.st != b.st) return false;
+  const int64_t at = ((b.p - a.p) % a.st + a.st) % a.st;
+  return at >= a.row && at + b.row <= a.st;
+}
+struct Heads {
+  HeadView v;
+  int64_t tokens;
+  int heads, width;
+  int64_t es;
+  const char* what;
+  bool empty() const { return tokens == 0 || heads == 0; }
+  Span span() const { return span_of(v, tokens, heads, width, es); }
+};
+void refuse_unless(bool ok, const char* what, const char* msg) {
+  if (!ok) throw std::invalid_argument(std::string(what) + msg);
+}
+Heads heads_of(const char* what, const void* p, int64_t st, int64_t sh, int64_t tokens, int heads,
+               int width, int dtype, int align, bool written) {
+  Heads h;
+  h.v.p = p;
+  h.v.st = st;
+  h.v.sh = sh;
+  h.tokens = tokens;
+  h.heads = heads;
+  h.width = width;
+  h.es = dtype == BC2N_F32 ? 4 : 2;
+  h.what = what;
+  if (h.empty()) return h;
+  refuse_unless(p, what, ": null operand");
+  aligned(p, align, what);
+  refuse_unless(st >= 0 && sh >= 0, what, ": negative stride");
+  refuse_unless((st * h.es) % align == 0 || tokens == 1, what, ": strides have to keep the alignment");
+  refuse_unless((sh * h.es) % align == 0 || heads == 1, what, ": strides have to keep the alignment");
+  refuse_unless(st < (int64_t(1) << 40) && sh < (int64_t(1) << 40), what, ": stride too large");
+  if (written) {
+    const bool by_token = (heads == 1 || sh >= width) && (tokens == 1 || st >= (heads - 1) * sh + width);
+    const bool by_head = (tokens == 1 || st >= width) && (heads == 1 || sh >= (tokens - 1) * st + width);
+    refuse_unless(by_token || by_head, what, ": elements overlap");
+  }
+  return h;
+}
+// every written operand apart from all others, but those that may be the same
+void all_apart(const std::vector<Heads>& written, const std::vector<Heads>& read, bool in_place) {
+  for (size_t i = 0; i < written.size(); ++i) {
+    const Heads& w = written[i];
+    if (w.empty()) continue;
+    for (size_t j = 0; j < written.size() + read.size(); ++j) {
+      const Heads& o = j < written.size() ? written[j] : read[j - written.size()];
+      if (o.empty() || j == i) continue;
+      const bool same = in_place && j >= written.size() && o.v.p == w.v.p && o.heads == w.heads &&
+                        (o.v.st == w.v.st || o.tokens == 1) && (o.v.sh == w.v.sh || o.heads == 1);
+      if (!same && !apart(w.span(), o.span()))
+        throw std::invalid_argument(std::string(w.what) + " overlaps " + o.what);
+    }
+  }
+}
+
+HeadNorm headnorm_operands(int dtype, int64_t tokens, int heads, int kv_heads, int width, int rotated,
+                           int interleaved, const void* positions, int position_bits,
+                           const float* freq, const void* q_weight, const void* k_weight,
+                           int weight_dtype, float eps) {
+  need(known_type(dtype), "headnorm: bad dtype");
+  need(weight_dtype == BC2N_F32 || weight_dtype == dtype,
+       "headnorm: weights are f32 or of the operands' type");
+  need(tokens >= 0 && tokens < (int64_t(1) << 26), "headnorm: bad number of tokens");
+  need(heads >= 0 && kv_heads >= 0 && heads + kv_heads > 0 && heads <= 65536 && kv_heads <= 65536,
+       "headnorm: bad number of heads");
+  need(width >= 2 && width % 2 == 0, "headnorm: the width has to be even");
+  need(rotated >= 0 && rotated <= width && rotated % 2 == 0,
+       "headnorm: the rotated elements are an even number up to the width");
+  need(headnorm_vector(dtype, width, rotated, interleaved) > 0,
+       "headnorm: no layout for this width (64 vectors of a pair's elements at most)");
+  need(tokens == 0 || rotated == 0 || (positions && freq), "headnorm: null positions or frequencies");
+  need(position_bits == 32 || position_bits == 64, "headnorm: positions are i32 or i64");
+  need(heads == 0 || q_weight, "headnorm: null q_weight");
+  need(kv_heads == 0 || k_weight, "headnorm: null k_weight");
+  need(eps >= 0 && std::isfinite(eps), "headnorm: bad eps");
+  if (positions) aligned(positions, position_bits / 8, "positions");
+  if (freq) aligned(freq, 4, "frequencies");
+  for (const void* w : {q_weight, k_weight})
+    if (w) aligned(w, weight_dtype == BC2N_F32 ? 4 : 2, "weight");
+  HeadNorm a;
+  a.dtype = dtype;
+  a.weight_dtype = weight_dtype;
+  a.tokens = tokens;
+  a.heads[0] = heads;
+  a.heads[1] = kv_heads;
+  a.width = width;
+  a.rotated = rotated;
+  a.interleaved = interleaved != 0;
+  a.pos = positions;
+  a.pos64 = position_bits == 64;
+  a.freq = freq;
+  a.weight[0] = q_weight;
+  a.weight[1] = k_weight;
+  a.eps = eps;
+  return a;
+}
+
+PackedAttn attention_operands(int dtype, int causal, int sequences, int64_t q_tokens, int64_t k_tokens,
+                              int heads, int kv_heads, int width, float scale,
+                              const int32_t* q_offsets, const int32_t* k_offsets,
+                              const int32_t* q_lengths, const int32_t* k_lengths) {
+  need(dtype == BC2N_F16 || dtype == BC2N_BF16, "attention: f16 or bf16");
+  need(sequences >= 0 && sequences <= (1 << 24), "attention: bad number of sequences");
+  need(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536,
+       "attention: the heads have to be a multiple of the keys' heads");
+  need(width > 0 && width % 8 == 0 && width <= PA_MAX_WIDTH,
+       "attention: the width has to be a multiple of 8 up to 128");
+  const int64_t G = heads / kv_heads, most = (int64_t(1) << 31) - 1024;
+  need(q_tokens >= 0 && k_tokens >= 0 && q_tokens * G < most && k_tokens * G < most,
+       "attention: bad number of tokens");
+  need(scale > 0 && std::isfinite(scale), "attention: the scale has to be positive");
+  need(q_offsets && k_offsets, "attention: null offsets");
+  for (const void* p : {q_offsets, k_offsets, q_lengths, k_lengths})
+    if (p) aligned(p, 4, "offsets");
+  PackedAttn a;
+  a.dtype = dtype;
+  a.causal = causal != 0;
+  a.sequences = sequences;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.width = width;
+  a.q_tokens = q_tokens;
+  a.k_tokens = k_tokens;
+  a.scale = scale;
+  a.q_off = q_offsets;
+  a.k_off = k_offsets;
+  a.q_len = q_lengths;
+  a.k_len = k_lengths;
+  return a;
+}
+// 64 tokens of all heads of a group within 2 GiB: the copies' offsets have 32 bits
+void near_enough(const Heads& h, int group) {
+  if (h.empty()) return;
+  refuse_unless(66 * h.v.st + (group + 1) * h.v.sh + h.width < (int64_t(1) << 30), h.what,
+                ": stride too large");
+}
+}  // namespace
+
+int bc2n_headnorm_fwd(void* stream, int dtype, int64_t tokens, int heads, int kv_heads, int width,
+                      int rotated, int interleaved, const void* q, int64_t q_st, int64_t q_sh,
+                      const void* k, int64_t k_st, int64_t k_sh, const void* positions,
+                      int position_bits, const float* freq, const void* q_weight,
+                      const void* k_weight, int weight_dtype, float eps, void* q_out, int64_t qo_st,
+                      int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh) {
+  return guarded([&] {
+    HeadNorm a = headnorm_operands(dtype, tokens, heads, kv_heads, width, rotated, interleaved, positions,
+                                   position_bits, freq, q_weight, k_weight, weight_dtype, eps);
+    const int es = dtype == BC2N_F32 ? 4 : 2;
+    auto view = [&](const char* what, const void* p, int64_t st, int64_t sh, int n, bool w) {
+      return heads_of(what, p, st, sh, tokens, n, width, dtype, es, w);
+    };
+    const Heads x[2] = {view("q", q, q_st, q_sh, heads, false), view("k", k, k_st, k_sh, kv_heads, false)};
+    const Heads y[2] = {view("q_out", q_out, qo_st, qo_sh, heads, true),
+                        view("k_out", k_out, ko_st, ko_sh, kv_heads, true)};
+    all_apart({y[0], y[1]}, {x[0], x[1]}, true);
+    for (int i = 0; i < 2; ++i) {
+      a.x[i] = x[i].v;
+      a.out[i] = y[i].v;
+    }
+    headnorm_fwd(own_stream(stream), a);
+  });
+}
+
+size_t bc2n_headnorm_work_bytes(int64_t tokens, int width) {
+  return tokens > 0 && width > 0 ? headnorm_work_bytes(tokens, width) : 0;
+}
+
+int bc2n_headnorm_bwd(void* stream, int dtype, int64_t tokens, int heads, int kv_heads, int width,
+                      int rotated, int interleaved, const void* d_q, int64_t dq_st, int64_t dq_sh,
+                      const void* d_k, int64_t dk_st, int64_t dk_sh, const void* q, int64_t q_st,
+                      int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* positions,
+                      int position_bits, const float* freq, const void* q_weight,
+                      const void* k_weight, int weight_dtype, float eps, void* q_grad, int64_t qg_st,
+                      int64_t qg_sh, void* k_grad, int64_t kg_st, int64_t kg_sh, float* d_q_weight,
+                      float* d_k_weight, void* work) {
+  return guarded([&] {
+    HeadNorm a = headnorm_operands(dtype, tokens, heads, kv_heads, width, rotated, interleaved, positions,
+                                   position_bits, freq, q_weight, k_weight, weight_dtype, eps);
+    const int es = dtype == BC2N_F32 ? 4 : 2;
+    auto view = [&](const char* what, const void* p, int64_t st, int64_t sh, int n, bool w) {
+      return heads_of(what, p, st, sh, tokens, n, width, dtype, es, w);
+    };
+    const Heads x[2] = {view("q", q, q_st, q_sh, heads, false), view("k", k, k_st, k_sh, kv_heads, false)};
+    const Heads d[2] = {view("d_q", d_q, dq_st, dq_sh, heads, false),
+                        view("d_k", d_k, dk_st, dk_sh, kv_heads, false)};
+    const Heads y[2] = {view("q_grad", q_grad, qg_st, qg_sh, heads, true),
+                        view("k_grad", k_grad, kg_st, kg_sh, kv_heads, true)};
+    all_apart({y[0], y[1]}, {x[0], x[1], d[0], d[1]}, true);
+    need(tokens == 0 || work, "headnorm: null work");
+    aligned(work, 16, "work");
+    for (int i = 0; i < 2; ++i) {
+      a.x[i] = x[i].v;
+      a.d[i] = d[i].v;
+      a.out[i] = y[i].v;
+    }
+    a.d_weight[0] = heads ? d_q_weight : nullptr;
+    a.d_weight[1] = kv_heads ? d_k_weight : nullptr;
+    headnorm_bwd(own_stream(stream), a, work);
+  });
+}
+
+size_t bc2n_attention_fwd_work_bytes(int dtype, int causal, int sequences, int64_t q_tokens,
+                                     int64_t k_tokens, int heads, int kv_heads, int width) {
+  size_t n = 0;
+  guarded([&] {
+    const int32_t none = 0;
+    n = packattn_fwd_work_bytes(attention_operands(dtype, causal, sequences, q_tokens, k_tokens, heads,
+                                                   kv_heads, width, 1.f, &none, &none, nullptr, nullptr));
+  });
+  return n;
+}
+size_t bc2n_attention_bwd_work_bytes(int dtype, int causal, int sequences, int64_t q_tokens,
+                                     int64_t k_tokens, int heads, int kv_heads, int width) {
+  size_t n = 0;
+  guarded([&] {
+    const int32_t none = 0;
+    n = packattn_bwd_work_bytes(attention_operands(dtype, causal, sequences, q_tokens, k_tokens, heads,
+                                                   kv_heads, width, 1.f, &none, &none, nullptr, nullptr));
+  });
+  return n;
+}
+
+int bc2n_attention_fwd(void* stream, int dtype, int causal, int sequences, int64_t q_tokens,
+                       int64_t k_tokens, int heads, int kv_heads, int width, float scale,
+                       const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* q_lengths,
+                       const int32_t* k_lengths, const void* q, int64_t q_st, int64_t q_sh,
+                       const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                       int64_t v_sh, int fill, void* out, int64_t o_st, int64_t o_sh, float* lse,
+                       void* work) {
+  return guarded([&] {
+    PackedAttn a = attention_operands(dtype, causal, sequences, q_tokens, k_tokens, heads, kv_heads, width,
+                                      scale, q_offsets, k_offsets, q_lengths, k_lengths);
+    const Heads hq = heads_of("q", q, q_st, q_sh, q_tokens, heads, width, dtype, 16, false);
+    const Heads hk = heads_of("k", k, k_st, k_sh, k_tokens, kv_heads, width, dtype, 16, false);
+    const Heads hv = heads_of("v", v, v_st, v_sh, k_tokens, kv_heads, width, dtype, 16, false);
+    const Heads ho = heads_of("out", out, o_st, o_sh, q_tokens, heads, width, dtype, 16, true);
+    for (const Heads* h : {&hk, &hv}) {
+      near_enough(*h, 1);
+      refuse_unless(h->tokens <= 1 || h->v.st >= width, h->what, ": tokens overlap");
+    }
+    all_apart({ho}, {hq, hk, hv}, false);
+    need(q_tokens == 0 || lse, "attention: null lse");
+    aligned(lse, 4, "lse");
+    need(work || packattn_fwd_work_bytes(a) == 0, "attention: null work");
+    aligned(work, 16, "work");
+    a.fill = fill != 0;
+    a.q = hq.v;
+    a.k = hk.v;
+    a.v = hv.v;
+    a.o = ho.v;
+    a.lse = lse;
+    packattn_fwd(own_stream(stream), a, work);
+  });
+}
+
+int bc2n_attention_bwd(void* stream, int dtype, int causal, int sequences, int64_t q_tokens,
+                       int64_t k_tokens, int heads, int kv_heads, int width, float scale,
+                       const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* q_lengths,
+                       const int32_t* k_lengths, const void* d_out, int64_t do_st, int64_t do_sh,
+                       const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                       int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const void* out,
+                       int64_t o_st, int64_t o_sh, const float* lse, int fill, void* d_q, int64_t dq_st,
+                       int64_t dq_sh, void* d_k, int64_t dk_st, int64_t dk_sh, void* d_v, int64_t dv_st,
+                       int64_t dv_sh, void* work) {
+  return guarded([&] {
+    PackedAttn a = attention_operands(dtype, causal, sequences, q_tokens, k_tokens, heads, kv_heads, width,
+                                      scale, q_offsets, k_offsets, q_lengths, k_lengths);
+    auto rows = [&](const char* what, const void* p, int64_t st, int64_t sh, bool w) {
+      return heads_of(what, p, st, sh, q_tokens, heads, width, dtype, 16, w);
+    };
+    auto keys = [&](const char* what, const void* p, int64_t st, int64_t sh, bool w) {
+      return heads_of(what, p, st, sh, k_tokens, kv_heads, width, dtype, 16, w);
+    };
+    const Heads hq = rows("q", q, q_st, q_sh, false), hg = rows("d_out", d_out, do_st, do_sh, false);
+    const Heads ho = rows("out", out, o_st, o_sh, false), hdq = rows("d_q", d_q, dq_st, dq_sh, true);
+    const Heads hk = keys("k", k, k_st, k_sh, false), hv = keys("v", v, v_st, v_sh, false);
+    const Heads hdk = keys("d_k", d_k, dk_st, dk_sh, true), hdv = keys("d_v", d_v, dv_st, dv_sh, true);
+    for (const Heads* h : {&hk, &hv}) {
+      near_enough(*h, 1);
+      refuse_unless(h->tokens <= 1 || h->v.st >= width, h->what, ": tokens overlap");
+    }
+    for (const Heads* h : {&hq, &hg}) near_enough(*h, heads / kv_heads);
+    all_apart({hdq, hdk, hdv}, {hq, hk, hv, ho, hg}, false);
+    need(q_tokens == 0 || lse, "attention: null lse");
+    aligned(lse, 4, "lse");
+    need(work || packattn_bwd_work_bytes(a) == 0, "attention: null work");
+    aligned(work, 16, "work");
+    a.fill = fill != 0;
+    a.q = hq.v;
+    a.k = hk.v;
+    a.v = hv.v;
+    a.o = ho.v;
+    a.lse = const_cast<float*>(lse);
+    a.d_o = hg.v;
+    a.dq = hdq.v;
+    a.dk = hdk.v;
+    a.dv = hdv.v;
+    packattn_bwd(own_stream(stream), a, work);
+  });
+}
+
+int bc2n_sample(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows, int classes,
+                const float* uniforms, double temperature, const float* temperatures, int64_t top_k,
+                const int32_t* top_ks, double top_p, const float* top_ps, double min_p,
+                const float* min_ps, int32_t* index, float* logp) {
+  return guarded([&] {
+    need(known_type(dtype), "sample: bad dtype");
+    need(rows >= 0 && rows < (int64_t(1) << 31), "sample: bad number of rows");
+    need(classes > 0 && classes <= (1 << 28), "sample: bad number of classes");
+    need(rows <= 1 || ld >= classes, "sample: the row stride is below the number of classes");
+    need(rows == 0 || (logits && uniforms), "null operand");
+    need(rows == 0 || index, "null output");
+    need(temperatures || (temperature >= 0 && std::isfinite(temperature)),
+         "sample: the temperature has to be finite and not negative");
+    need(top_ks || top_k >= 0, "sample: top_k must not be negative");
+    need(top_ps || !std::isnan(top_p), "sample: top_p is NaN");
+    need(min_ps || !std::isnan(min_p), "sample: min_p is NaN");
+    aligned(logits, dtype == BC2N_F32 ? 4 : 2, "logits");
+    for (const void* p : {(const void*)uniforms, (const void*)temperatures, (const void*)top_ks,
+                          (const void*)top_ps, (const void*)min_ps, (const void*)index, (const void*)logp})
+      aligned(p, 4, "sample operand");
+    Sample a;
+    a.dtype = dtype;
+    a.x = logits;
+    a.ld = ld;
+    a.rows = rows;
+    a.V = classes;
+    a.u = uniforms;
+    a.temperature.v = temperature;
+    a.temperature.row = temperatures;
+    a.top_p.v = top_p;
+    a.top_p.row = top_ps;
+    a.min_p.v = min_p;
+    a.min_p.row = min_ps;
+    a.top_k = top_k;
+    a.top_k_row = top_ks;
+    a.index = index;
+    a.logp = logp;
+    sample(own_stream(stream), a);
   });
 }
 

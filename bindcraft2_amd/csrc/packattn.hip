@@ -1,0 +1,881 @@
+// Attention of packed sequences: sequence b has queries q_off[b] ..
+// q_off[b+1] - 1 and keys k_off[b] .. of two buffers of tokens, G = heads /
+// kv_heads query heads share a head of keys and values, and
+//
+//   S = scale q k^T over the keys that a query sees, P = softmax(S), o = P v,
+//   lse = log sum e^S;  D = sum_d (do o),  dS = P (do v^T - D),
+//   dv = P^T do,  dq = scale dS k,  dk = scale dS^T q  (summed over the group).
+//
+// A causal query i of m sees keys j <= i + n - m.  A row that sees none has
+// o = 0, lse = -inf and no gradient.
+//
+// The G heads of a group are rows of one problem, row r = i G + g, so that
+// they share every key tile that is staged and a few queries still fill a
+// tile.  All products are v_mfma_f32_32x32x16, arranged so that a result is
+// the next product's operand as it lies in the registers:
+//
+//   forward, dq:  S^T[key][row] = K Q^T, a lane owns one row: row maxima and
+//                 sums are a lane's own but for its other half's (lane ^ 32),
+//                 and rescaling o^T[d][row] += V^T P^T is one factor a lane
+//   dk, dv:       S[row][key] = Q K^T, a lane owns one key:
+//                 dv^T[d][key] += do^T P,  dk^T[d][key] += Q^T dS
+//
+// The result of a product holds rows 8 (r/4) + 4 (l/32) + r%4 in register r of
+// lane l; as the operand of the next one those are its contraction's slots, and
+// the other operand, a column of the row-major tile in LDS, is read in the same
+// order with two ds_read_b64_tr_b16.
+//
+// Tiles are copied global -> LDS directly through buffer descriptors whose
+// bounds turn what lies past a sequence or past the width into zeros.  A copy
+// fills LDS in lane order, so the source address carries the swizzle (fswz)
+// that keeps both the 16-byte row reads and the transposed reads off each
+// other's banks.
+#include "packattn.h"
+
+#include "common.h"
+#include "runtime.h"
+#include "vec.h"
+
+#include "../../include/bc2n.h"
+
+#include <algorithm>
+#include <numeric>
+
+namespace bc2n {
+
+namespace {
+
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef const __attribute__((address_space(3))) f32x4 lds_f32x4;
+
+constexpr int NT = 256, WAVES = 4;
+constexpr int BN = 64;  // keys of a staged tile (rows of one in the dk, dv kernel)
+constexpr float NEG_INF = -__builtin_inff();
+
+template <class T>
+struct Half;
+template <>
+struct Half<h16> {
+  typedef h16 V2 __attribute__((ext_vector_type(2)));
+  // Probabilities are kept 2^SHIFT times as large, within binary16's range
+  // beside a reference that lags the maximum by at most LAG: small ones stay
+  // normal numbers.
+  static constexpr float SHIFT = 7.f;
+  static constexpr bool SCALED = true;  // dS needs a scale (below)
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a),
+                                                  __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Half<bf16> {
+  typedef bf16 V2 __attribute__((ext_vector_type(2)));
+  static constexpr float SHIFT = 0.f;
+  static constexpr bool SCALED = false;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+// The running reference of a row's exponents is raised only where the maximum
+// has passed it by this much (log2): the products hold what lies between.
+constexpr float LAG = 8.f;
+
+// two f32 rounded to nearest even, in one register
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, typename Half<T>::V2));
+}
+// registers 8 s .. 8 s + 7 of a product as the operand of the next one
+template <class T>
+__device__ __forceinline__ u32x4 pack8(const f32x16& v, int s) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = pack2<T>(v[8 * s + 2 * i], v[8 * s + 2 * i + 1]);
+  return r;
+}
+
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// v of lane l ^ 32
+__device__ __forceinline__ float other_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v),
+                                                  __builtin_bit_cast(int, v), false, false);
+  return fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1]));
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v),
+                                                  __builtin_bit_cast(int, v), false, false);
+  return __builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)v) |
+                   (uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32);
+}
+
+// ---------------------------------------------------------------- sequences
+struct Seq {
+  int64_t q0, k0;  // first tokens
+  int lq, lk;      // its queries and keys
+  int have;        // tokens of the searched side that are its own, in it or not
+};
+
+// First token of entry s of `off`: 0, off[0], ..., off[B], n -- the tokens before the
+// first sequence and behind the last are sequences without queries or keys.
+// Offsets past the tokens are cut to them.
+__device__ __forceinline__ int start_of(const int32_t* off, int s, int B, int64_t n) {
+  return s == 0 ? 0 : (int)min((int64_t)max(off[min(s, B + 1) - 1], 0), n);
+}
+
+// Tile x of the rows of all sequences, `unit` rows a token and `tile` rows a
+// tile: sequence s's tiles take the numbers from floor(start * unit / tile) + s
+// on, which leaves each of them enough.  Sets s, returns the tile's index in it
+// (past its last one, and with offsets that fall below 0, for no tile).
+__device__ __forceinline__ int64_t find_tile(const int32_t* off, int B, int64_t n, int unit, int tile,
+                                             int64_t x, int& s) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, count = B + 2;
+  auto first = [&](int e) { return (int64_t)start_of(off, e, B, n) * unit / tile + e; };
+  while (count > 1) {  // 64 entries at a time
+    const int step = (count + 63) / 64, e = lo + lane * step;
+    const bool below = lane * step < count && first(min(e, B + 1)) <= x;
+    const int passed = max(__popcll(__ballot(below)) - 1, 0) * step;
+    lo += passed;
+    count = min(step, count - passed);
+  }
+  s = uniform(lo);
+  return uniform64(x - first(s));
+}
+
+__device__ __forceinline__ Seq sequence(const PackedAttn& a, int s, bool keys) {
+  const int B = a.sequences;
+  Seq r = {};
+  const int32_t* off = keys ? a.k_off : a.q_off;
+  const int64_t n = keys ? a.k_tokens : a.q_tokens;
+  const int from = start_of(off, s, B, n);
+  const int to = s == B + 1 ? (int)n : start_of(off, s + 1, B, n);
+  r.have = max(to - from, 0);
+  (keys ? r.k0 : r.q0) = from;
+  if (s == 0 || s == B + 1) return r;
+  const int other = start_of(keys ? a.q_off : a.k_off, s, B, keys ? a.q_tokens : a.k_tokens);
+  const int end = start_of(keys ? a.q_off : a.k_off, s + 1, B, keys ? a.q_tokens : a.k_tokens);
+  (keys ? r.q0 : r.k0) = other;
+  int lq = keys ? max(end - other, 0) : r.have, lk = keys ? r.have : max(end - other, 0);
+  if (a.q_len) lq = min(lq, max(a.q_len[s - 1], 0));
+  if (a.k_len) lk = min(lk, max(a.k_len[s - 1], 0));
+  r.lq = lq;
+  r.lk = lk;
+  r.q0 = uniform64(r.q0);
+  r.k0 = uniform64(r.k0);
+  r.lq = uniform(r.lq);
+  r.lk = uniform(r.lk);
+  r.have = uniform(r.have);
+  return r;
+}
+
+// Workgroups of `tiles` tiles for each head of keys: XCD b % 8 takes heads of
+// one class mod gcd(kv_heads, 8), so that the tiles which read one head's keys
+// and values share an L2; within it tiles run from the last (LAST: causal rows
+// with the most keys) or from the first.
+struct Place {
+  int head;
+  int64_t tile;  // < 0: none
+};
+__host__ __device__ inline int head_classes(int kv_heads) {
+  return kv_heads % 8 == 0 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
+}
+template <bool LAST>
+__device__ __forceinline__ Place place(int kv_heads, int64_t tiles) {
+  const int g = head_classes(kv_heads), share = NUM_XCD / g;
+  const int64_t per = (tiles + share - 1) / share;
+  const int64_t b = blockIdx.x, x = b % NUM_XCD, j = b / NUM_XCD;
+  Place r;
+  r.head = (int)(x % g + g * (j / per));
+  r.tile = (j % per) * share + x / g;
+  if (r.tile >= tiles) r.tile = -1;
+  else if (LAST) r.tile = tiles - 1 - r.tile;
+  return r;
+}
+unsigned place_grid(int kv_heads, int64_t tiles) {
+  const int g = head_classes(kv_heads), share = NUM_XCD / g;
+  const int64_t grid = NUM_XCD * (int64_t)(kv_heads / g) * ((tiles + share - 1) / share);
+  if (grid >= int64_t(1) << 24) throw std::invalid_argument("attention: too many tiles for one call");
+  return (unsigned)grid;
+}
+
+// ------------------------------------------------------------- tiles in LDS
+// 16-byte chunk c of row r of a [rows][DP] tile lies at chunk c ^ fswz(r).
+// A row read takes one chunk of 16 rows at a time and a transposed read 64
+// bytes of 4 rows: over all 64 banks in both, whatever DP.
+template <int DP>
+__device__ __forceinline__ int fswz(int r) {
+  if (DP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  if (DP == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  return (r >> 2) & 3;
+}
+
+__device__ __forceinline__ unsigned lds_addr(const void* p) {
+  return (unsigned)(size_t)((const __attribute__((address_space(3))) unsigned char*)p);
+}
+
+// 1 KB global -> LDS, 16 bytes a lane; zeros where the offset is past the
+// descriptor's bounds.
+__device__ __forceinline__ void copy16(unsigned voff, u32x4 rsrc, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff),
+               "s"(rsrc), "s"(lds)
+               : "memory", "m0");
+}
+__device__ __forceinline__ u32x4 descriptor(const void* p, unsigned bytes) {
+  const uint64_t b = (uint64_t)uniform64((int64_t)(uintptr_t)p);
+  return u32x4{(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, (uint32_t)uniform((int)bytes), 0x00027000u};
+}
+constexpr unsigned NOWHERE = 0x80000000u;  // past every descriptor's bounds
+
+// all of a wave's copies and LDS reads done, and every wave here
+__device__ __forceinline__ void wait_all_and_sync() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// A wave's copies of a [BN][DP] tile by 4 waves: piece w + 4 i.
+template <int DP>
+struct TileCopy {
+  static constexpr int PIECES = BN * DP * 2 / 1024, PER = PIECES / WAVES;
+  static constexpr int CPR = DP / 8;  // chunks a row
+  // row and element of lane's chunk of piece i
+  static __device__ __forceinline__ int row(int i, int wave, int lane) {
+    return ((wave + WAVES * i) * 64 + lane) / CPR;
+  }
+  static __device__ __forceinline__ int elem(int i, int wave, int lane) {
+    return (lane % CPR ^ fswz<DP>(row(i, wave, lane))) * 8;
+  }
+  static __device__ __forceinline__ unsigned dst(int i, int wave) { return (wave + WAVES * i) * 1024; }
+};
+
+// rows r0 + l%32, elements 16 ks + 8 (l/32) ..: operand of a contraction over
+// the width.  base: the tile's LDS address
+template <int DP>
+__device__ __forceinline__ u32x4 row_operand(unsigned base, int r0, int ks, int lane) {
+  const int r = lane & 31, c = (2 * ks + (lane >> 5)) ^ fswz<DP>(r);
+  return *(lds_u32x4*)(base + (r0 + r) * (DP * 2) + c * 16);
+}
+// column 32 db + l%32, rows r0 + {4 h .. 4 h + 3, 8 + 4 h ..}, h = l/32: operand
+// of a contraction over the rows
+template <int DP>
+__device__ __forceinline__ u32x4 column_operand(unsigned base, int r0, int db, int lane) {
+  const int m = lane & 15, c = 4 * db + 2 * ((lane >> 4) & 1) + ((m & 3) >> 1);
+  u32x4 v;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int r = 8 * x + 4 * (lane >> 5) + (m >> 2);
+    const unsigned p = base + (r0 + r) * (DP * 2) + (c ^ fswz<DP>(r)) * 16 + (m & 1) * 8;
+    const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+    v[2 * x] = t[0];
+    v[2 * x + 1] = t[1];
+  }
+  return v;
+}
+
+// 8 elements from element e of a head's row, zeros past the width
+template <class T>
+__device__ __forceinline__ u32x4 load8(const T* row, int e, int width) {
+  return e < width ? *global_ptr<const u32x4>(row + e) : u32x4{0, 0, 0, 0};
+}
+
+// Writes v[d][column] of a lane's column to `row` (16-bit, factor f): the halves
+// of the wave swap so that a lane holds 8 elements side by side.
+template <class T, int DB>
+__device__ __forceinline__ void store_columns(const f32x16 (&v)[DB], float f, T* row, int width,
+                                              int lane) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x = pack2<T>(v[db][8 * p + 2 * j] * f, v[db][8 * p + 2 * j + 1] * f);
+        const uint32_t y = pack2<T>(v[db][8 * p + 4 + 2 * j] * f, v[db][8 * p + 4 + 2 * j + 1] * f);
+        const auto s = __builtin_amdgcn_permlane32_swap((int)x, (int)y, false, false);
+        w[j] = s[0];
+        w[2 + j] = s[1];
+      }
+      const int e = 32 * db + 16 * p + 8 * (lane >> 5);
+      if (row && e < width) *global_ptr<u32x4>(row + e) = w;
+    }
+  }
+}
+
+// A wave's 32 rows of a problem's G heads: a lane's own.
+struct Row {
+  int i, g;     // token in the sequence, head in the group
+  int last;     // last key it sees, -1: none
+  bool stored;  // in or (fill) behind its sequence
+};
+__device__ __forceinline__ Row row_of(const PackedAttn& a, const Seq& s, int r, int G) {
+  const int have = a.fill ? s.have : s.lq;
+  Row o;
+  const int i = r / G;
+  o.stored = i < have;
+  o.i = o.stored ? i : max(have - 1, 0);
+  o.g = r - i * G;
+  o.last = -1;
+  if (o.i < s.lq && o.stored) o.last = a.causal ? min(o.i + s.lk - s.lq, s.lk - 1) : s.lk - 1;
+  return o;
+}
+
+template <class T>
+__device__ __forceinline__ T* row_ptr(const HeadView& v, int64_t token, int head) {
+  return (T*)v.p + token * v.st + (int64_t)head * v.sh;
+}
+
+// Largest (or smallest) over the lanes of a wave
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) v = max(v, __shfl_xor(v, m, 64));
+  return uniform(v);
+}
+__device__ __forceinline__ int wave_min(int v) { return -wave_max(-v); }
+
+// Copies of key tile at key k0 (its keys past lk zeros).
+template <class T, int DP>
+struct KeyTiles {
+  typedef TileCopy<DP> C;
+  unsigned ko[C::PER], vo[C::PER];  // a lane's offsets
+  const T *k, *v;
+  int64_t kst, vst;
+  int width, lk, wave;
+  __device__ __forceinline__ void init(const PackedAttn& a, const Seq& s, int head, int wave_, int lane) {
+    wave = wave_;
+    width = a.width;
+    lk = s.lk;
+    kst = a.k.st;
+    vst = a.v.st;
+    k = row_ptr<const T>(a.k, s.k0, head);
+    v = row_ptr<const T>(a.v, s.k0, head);
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) {
+      const int r = C::row(i, wave, lane), e = C::elem(i, wave, lane);
+      ko[i] = e < width ? (unsigned)(r * kst + e) * 2 : NOWHERE;
+      vo[i] = e < width ? (unsigned)(r * vst + e) * 2 : NOWHERE;
+    }
+  }
+  __device__ __forceinline__ void issue(int k0, unsigned lds) const {
+    const int rows = min(BN, lk - k0);
+    const u32x4 kd = descriptor(k + k0 * kst, (unsigned)((rows - 1) * kst + width) * 2);
+    const u32x4 vd = descriptor(v + k0 * vst, (unsigned)((rows - 1) * vst + width) * 2);
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) copy16(ko[i], kd, lds + C::dst(i, wave));
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) copy16(vo[i], vd, lds + BN * DP * 2 + C::dst(i, wave));
+  }
+};
+
+// ------------------------------------------------------------------ forward
+// Workgroup = 128 rows of one sequence and head of keys, 4 waves x 32 rows;
+// keys in tiles of 64, two buffers, one barrier a tile.
+template <class T, int DP>
+__global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64_t tiles) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  constexpr int BM = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
+  const Place at = place<true>(a.kv_heads, tiles);
+  if (at.tile < 0) return;
+  const int G = a.heads / a.kv_heads;
+  int s;
+  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, at.tile, s);
+  const Seq seq = sequence(a, s, false);
+  const int rows = (a.fill ? seq.have : seq.lq) * G;
+  if (t < 0 || t * BM >= rows) return;
+  const int r0 = (int)t * BM;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const Row row = row_of(a, seq, r0 + 32 * wave + (lane & 31), G);
+  const int head = at.head * G + row.g;
+  const int64_t token = seq.q0 + row.i;
+  const int most = wave_max(row.last), least = wave_min(row.last);
+  // the last row of the workgroup sees the most keys
+  const Row end = row_of(a, seq, min(r0 + BM, rows) - 1, G);
+  int far = uniform(end.last);
+  if (a.fill && seq.lq < seq.have) far = seq.lk - 1;  // rows behind the queries see none
+  const int nk = far < 0 ? 0 : far / BN + 1;
+
+  u32x4 q[KS];
+  const T* qrow = row_ptr<const T>(a.q, token, head);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
+  const float c = a.scale * LOG2E;
+  f32x16 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+  float ref = NEG_INF, mc = 0.f, sum = 0.f;  // reference of the exponents, times c
+  const unsigned lds0 = lds_addr(smem);
+  KeyTiles<T, DP> tile;
+  tile.init(a, seq, at.head, wave, lane);
+  if (nk > 0) tile.issue(0, lds0);
+
+  for (int kt = 0; kt < nk; ++kt) {
+    const unsigned kb0 = lds0 + (kt & 1) * 2 * TILE, vb0 = kb0 + TILE;
+    const int k0 = kt * BN;
+    wait_all_and_sync();
+    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + (~kt & 1) * 2 * TILE);
+    if (k0 > most) continue;
+    f32x16 p[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      p[b] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        p[b] = Half<T>::mma(row_operand<DP>(kb0, 32 * b, ks, lane), q[ks], p[b]);
+    }
+    if (k0 + BN - 1 > least) {
+      const int last = row.last - k0 - 4 * h;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + 8 * (i / 4) + i % 4 > last) p[b][i] = NEG_INF;
+    }
+    float m = p[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, p[b][i]);
+    m = other_half_max(m);
+    // NaN scores leave m and end in the sum
+    if (__any(m * c > ref * c + LAG || (ref == NEG_INF && m > NEG_INF))) {
+      const float to = fmaxf(ref, m), f = ref == NEG_INF ? 0.f : exp2_f((ref - to) * c);
+      ref = to;
+      mc = ref == NEG_INF ? 0.f : ref * c;
+      sum *= f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] *= f;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[b][i] = exp2_f(fmaf(p[b][i], c, Half<T>::SHIFT - mc));
+        sum += p[b][i];
+      }
+#pragma unroll
+    for (int kg = 0; kg < 4; ++kg) {
+      const u32x4 w = pack8<T>(p[kg / 2], kg & 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        o[db] = Half<T>::mma(column_operand<DP>(vb0, 16 * kg, db, lane), w, o[db]);
+    }
+  }
+  sum = other_half_sum(sum);
+  const bool none = sum == 0.f;
+  store_columns<T, DB>(o, none ? 0.f : 1.f / sum,
+                       row.stored ? row_ptr<T>(a.o, token, head) : nullptr, a.width, lane);
+  if (row.stored && h == 0)
+    a.lse[(int64_t)head * a.q_tokens + token] =
+        none ? NEG_INF : (mc - Half<T>::SHIFT + log2f(sum)) * LN2;
+}
+
+// ----------------------------------------------------------------- backward
+// In binary16 a dS of many keys falls below the normal numbers, so it is made
+// 2^e times as large, e from the largest norms of a row of do and of v, which
+// bound it: |dS| <= 2 |do| |v|.  maxima [blocks][2]: partial maxima of the
+// squares, of queries' blocks and of keys'.
+template <class T>
+__global__ __launch_bounds__(NT) void packattn_norms_kernel(PackedAttn a, int64_t q_tiles, int64_t k_tiles,
+                                                            float* maxima) {
+  __shared__ float best[WAVES];
+  constexpr int TOK = 64;
+  float top[2] = {0.f, 0.f};
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int chunks = (a.width + 7) / 8;
+  for (int64_t x = blockIdx.x; x < q_tiles + k_tiles; x += gridDim.x) {
+    const bool keys = x >= q_tiles;
+    int s;
+    const int64_t t = find_tile(keys ? a.k_off : a.q_off, a.sequences, keys ? a.k_tokens : a.q_tokens, 1,
+                            TOK, keys ? x - q_tiles : x, s);
+    const Seq seq = sequence(a, s, keys);
+    const int heads = keys ? a.kv_heads : a.heads;
+    const int n = t < 0 ? 0 : (int)min((int64_t)TOK, (keys ? seq.lk : seq.lq) - t * TOK) * heads;
+    float m = 0.f;
+    for (int r = threadIdx.x; r < n; r += NT) {
+      const int64_t token = (keys ? seq.k0 : seq.q0) + t * TOK + r / heads;
+      const T* row = row_ptr<const T>(keys ? a.v : a.d_o, token, r % heads);
+      float sq = 0.f;
+      for (int c = 0; c < chunks; ++c) {
+        float e[8];
+        Vec<T>::unpack(load8(row, 8 * c, a.width), e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq = fmaf(e[i], e[i], sq);
+      }
+      m = fmaxf(m, sq);
+    }
+    top[0] = keys ? top[0] : fmaxf(top[0], m);
+    top[1] = keys ? fmaxf(top[1], m) : top[1];
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float m = group_max<64>(top[k]);
+    if (lane == 0) best[wave] = m;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      maxima[2 * blockIdx.x + k] = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+    __syncthreads();
+  }
+}
+constexpr int NORM_BLOCKS = 256;
+
+// the scale of dS from the partial maxima: a power of two, dS below 2^14
+__device__ __forceinline__ float ds_scale(const float* maxima, int blocks) {
+  const int lane = threadIdx.x & 63;
+  float d = 0.f, v = 0.f;
+  for (int i = lane; i < blocks; i += 64) {
+    d = fmaxf(d, maxima[2 * i]);
+    v = fmaxf(v, maxima[2 * i + 1]);
+  }
+  const float b = sqrtf(group_max<64>(d)) * sqrtf(group_max<64>(v));  // |dS| <= 2 b
+  if (!(b > 0.f && b < 3e38f)) return 1.f;
+  return ldexpf(1.f, max(-100, min(100, 12 - (int)ceilf(log2f(b)))));
+}
+
+// dq, and D = sum (do o) of every row for the other kernel.
+template <class T, int DP>
+__global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_t tiles, float* delta,
+                                                            const float* maxima, int blocks) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  constexpr int BM = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
+  const Place at = place<true>(a.kv_heads, tiles);
+  if (at.tile < 0) return;
+  const int G = a.heads / a.kv_heads;
+  int s;
+  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, at.tile, s);
+  const Seq seq = sequence(a, s, false);
+  const int rows = (a.fill ? seq.have : seq.lq) * G;
+  if (t < 0 || t * BM >= rows) return;
+  const int r0 = (int)t * BM;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const Row row = row_of(a, seq, r0 + 32 * wave + (lane & 31), G);
+  const int head = at.head * G + row.g;
+  const int64_t token = seq.q0 + row.i, at_row = (int64_t)head * a.q_tokens + token;
+  const int most = wave_max(row.last), least = wave_min(row.last);
+  const Row end = row_of(a, seq, min(r0 + BM, rows) - 1, G);
+  int far = uniform(end.last);
+  if (a.fill && seq.lq < seq.have) far = seq.lk - 1;
+  const int nk = far < 0 ? 0 : far / BN + 1;
+  const float ds = Half<T>::SCALED ? ds_scale(maxima, blocks) : 1.f;
+
+  u32x4 q[KS], g[KS];
+  const T* qrow = row_ptr<const T>(a.q, token, head);
+  const T* grow = row_ptr<const T>(a.d_o, token, head);
+  const T* orow = row_ptr<const T>(a.o, token, head);
+  float D = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
+    g[ks] = load8(grow, 16 * ks + 8 * h, a.width);
+    float x[8], y[8];
+    Vec<T>::unpack(g[ks], x);
+    Vec<T>::unpack(load8(orow, 16 * ks + 8 * h, a.width), y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) D = fmaf(x[i], y[i], D);
+  }
+  D = other_half_sum(D);
+  float lse = a.lse[at_row] * LOG2E;
+  if (lse == NEG_INF) lse = -NEG_INF;  // a row without a key: P = 0
+  if (row.stored && row.i < seq.lq && h == 0) delta[at_row] = D;
+  const float c = a.scale * LOG2E;
+  f32x16 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+  const unsigned lds0 = lds_addr(smem);
+  // what was loaded above is here before the first copy is issued
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  KeyTiles<T, DP> tile;
+  tile.init(a, seq, at.head, wave, lane);
+  if (nk > 0) tile.issue(0, lds0);
+
+  for (int kt = 0; kt < nk; ++kt) {
+    const unsigned kb0 = lds0 + (kt & 1) * 2 * TILE, vb0 = kb0 + TILE;
+    const int k0 = kt * BN;
+    wait_all_and_sync();
+    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + (~kt & 1) * 2 * TILE);
+    if (k0 > most) continue;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 p = {}, d = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(row_operand<DP>(kb0, 32 * b, ks, lane), q[ks], p);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(row_operand<DP>(vb0, 32 * b, ks, lane), g[ks], d);
+      const bool cut = k0 + 32 * b + 31 > least;
+      const int last = row.last - k0 - 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        d[i] = exp2_f(fmaf(p[i], c, -lse)) * (d[i] - D);
+        if (Half<T>::SCALED) d[i] *= ds;
+      }
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + 8 * (i / 4) + i % 4 > last) d[i] = 0.f;
+      }
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg) {
+        const u32x4 w = pack8<T>(d, kg);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          o[db] = Half<T>::mma(column_operand<DP>(kb0, 32 * b + 16 * kg, db, lane), w, o[db]);
+      }
+    }
+  }
+  if (row.i >= seq.lq) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+  }
+  store_columns<T, DB>(o, a.scale / ds, row.stored ? row_ptr<T>(a.dq, token, head) : nullptr, a.width, lane);
+}
+
+// dk, dv: workgroup = 128 keys of one sequence and head, 4 waves x 32 keys,
+// over the rows of all the group's heads in tiles of 64.
+template <class T, int DP>
+__global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, const float* delta,
+                                                          const float* maxima, int blocks) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  typedef TileCopy<DP> C;
+  constexpr int BK = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
+  const Place at = place<false>(a.kv_heads, tiles);
+  if (at.tile < 0) return;
+  const int G = a.heads / a.kv_heads;
+  int s;
+  const int64_t t = find_tile(a.k_off, a.sequences, a.k_tokens, 1, BK, at.tile, s);
+  const Seq seq = sequence(a, s, true);
+  const int have = a.fill ? seq.have : seq.lk;
+  if (t < 0 || t * BK >= have) return;
+  const int j0 = (int)t * BK;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const int j = j0 + 32 * wave + (lane & 31);  // a lane's key
+  const bool stored = j < have, live = j < seq.lk;
+  const int64_t token = seq.k0 + min(j, have - 1);
+  const int lag = seq.lk - seq.lq;  // query i sees keys up to i + lag
+  // the first row that sees a key of the workgroup; without keys there is none
+  const int rows = j0 < seq.lk ? seq.lq * G : 0;
+  const int from = a.causal ? max(j0 - lag, 0) * G / BN * BN : 0;
+  const float ds = Half<T>::SCALED ? ds_scale(maxima, blocks) : 1.f;
+  // P is made 2^SHIFT times as large in binary16
+  constexpr float SHIFT = 2 * Half<T>::SHIFT;
+
+  u32x4 k[KS], v[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    k[ks] = live ? load8(row_ptr<const T>(a.k, token, at.head), 16 * ks + 8 * h, a.width) : u32x4{0, 0, 0, 0};
+    v[ks] = live ? load8(row_ptr<const T>(a.v, token, at.head), 16 * ks + 8 * h, a.width) : u32x4{0, 0, 0, 0};
+  }
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
+  const float c = a.scale * LOG2E;
+
+  // Two buffers of Q, do tiles and of lse, D and the last key of their rows.
+  constexpr int BUF = 2 * TILE + 3 * BN * 4;
+  const unsigned lds0 = lds_addr(smem);
+  auto stats = [&](int buf) { return reinterpret_cast<float*>(smem + buf * BUF + 2 * TILE); };
+  // a lane's row of each piece
+  int pi[C::PER], pg[C::PER];
+#pragma unroll
+  for (int i = 0; i < C::PER; ++i) {
+    const int r = from + C::row(i, wave, lane);
+    pi[i] = r / G;
+    pg[i] = r - pi[i] * G;
+  }
+  const int di = BN / G, dg = BN % G;
+  float n_lse = 0.f, n_delta = 0.f;
+  int n_last = -1;
+  auto issue = [&](int r0, int buf) __attribute__((always_inline)) {
+    const int i0 = r0 / G;
+    const u32x4 qd = descriptor(row_ptr<const T>(a.q, seq.q0 + i0, at.head * G), 0x7fffffffu);
+    const u32x4 gd = descriptor(row_ptr<const T>(a.d_o, seq.q0 + i0, at.head * G), 0x7fffffffu);
+    n_lse = -NEG_INF;
+    n_delta = 0.f;
+    n_last = -1;
+    if (threadIdx.x < BN) {
+      const int r = r0 + threadIdx.x, i = r / G;
+      if (r < rows) {
+        const int64_t p = (int64_t)(at.head * G + r - i * G) * a.q_tokens + seq.q0 + i;
+        n_lse = a.lse[p] * LOG2E;
+        n_delta = delta[p];
+        n_last = a.causal ? i + lag : seq.lk;
+      }
+    }
+    const unsigned lds = lds0 + buf * BUF;
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) {
+      const int e = C::elem(i, wave, lane);
+      const bool in = r0 + C::row(i, wave, lane) < rows && e < a.width;
+      const int64_t di64 = pi[i] - i0;
+      copy16(in ? (unsigned)(di64 * a.q.st + pg[i] * a.q.sh + e) * 2 : NOWHERE, qd, lds + C::dst(i, wave));
+      copy16(in ? (unsigned)(di64 * a.d_o.st + pg[i] * a.d_o.sh + e) * 2 : NOWHERE, gd,
+             lds + TILE + C::dst(i, wave));
+      pi[i] += di;
+      pg[i] += dg;
+      if (pg[i] >= G) {
+        pg[i] -= G;
+        ++pi[i];
+      }
+    }
+  };
+  auto keep = [&](int buf) {
+    if (threadIdx.x < BN) {
+      float* st = stats(buf);
+      st[threadIdx.x] = n_lse == NEG_INF ? -NEG_INF : n_lse;  // a row without a key: P = 0
+      st[BN + threadIdx.x] = n_delta;
+      reinterpret_cast<int*>(st)[2 * BN + threadIdx.x] = n_last;
+    }
+  };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (from < rows) {
+    issue(from, 0);
+    keep(0);
+  }
+  int buf = 0;
+  for (int r0 = from; r0 < rows; r0 += BN, buf ^= 1) {
+    wait_all_and_sync();
+    if (r0 + BN < rows) issue(r0 + BN, buf ^ 1);
+    const unsigned qb = lds0 + buf * BUF, gb = qb + TILE, sb = qb + 2 * TILE;
+    // the first row of the tile sees the fewest keys
+    const bool cut = a.causal && r0 / G + lag < j0 + 32 * wave + 31;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 p = {}, d = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(row_operand<DP>(qb, 32 * b, ks, lane), k[ks], p);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(row_operand<DP>(gb, 32 * b, ks, lane), v[ks], d);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const unsigned at_row = sb + (32 * b + 8 * x + 4 * h) * 4;
+        const f32x4 lse = *(lds_f32x4*)at_row, D = *(lds_f32x4*)(at_row + BN * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[4 * x + i] = exp2_f(fmaf(p[4 * x + i], c, SHIFT - lse[i]));
+          d[4 * x + i] = p[4 * x + i] * (d[4 * x + i] - D[i]);
+        }
+        if (cut) {
+          const u32x4 last = *(lds_u32x4*)(at_row + 2 * BN * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j > (int)last[i]) p[4 * x + i] = d[4 * x + i] = 0.f;
+        }
+        if (Half<T>::SCALED) {
+          const float f = ds * (1.f / 16384.f);  // 2^-SHIFT
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[4 * x + i] *= f;
+        }
+      }
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg) {
+        const u32x4 wp = pack8<T>(p, kg), wd = pack8<T>(d, kg);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          dv[db] = Half<T>::mma(column_operand<DP>(gb, 32 * b + 16 * kg, db, lane), wp, dv[db]);
+          dk[db] = Half<T>::mma(column_operand<DP>(qb, 32 * b + 16 * kg, db, lane), wd, dk[db]);
+        }
+      }
+    }
+    if (r0 + BN < rows) keep(buf ^ 1);
+  }
+  if (!live) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
+  }
+  store_columns<T, DB>(dk, a.scale / ds, stored ? row_ptr<T>(a.dk, token, at.head) : nullptr, a.width, lane);
+  store_columns<T, DB>(dv, Half<T>::SCALED ? 1.f / 16384.f : 1.f,
+                       stored ? row_ptr<T>(a.dv, token, at.head) : nullptr, a.width, lane);
+}
+
+// ------------------------------------------------------------------ launches
+int64_t tiles_of(int64_t tokens, int unit, int tile, int sequences) {
+  return tokens * unit / tile + sequences + 2;
+}
+
+template <class F, class T>
+void by_width(const PackedAttn& a, T, F f) {
+  if (a.width <= 32) f(T(), std::integral_constant<int, 32>());
+  else if (a.width <= 64) f(T(), std::integral_constant<int, 64>());
+  else f(T(), std::integral_constant<int, 128>());
+}
+template <class F>
+void by_type(const PackedAttn& a, F f) {
+  if (a.dtype == BC2N_F16) by_width(a, h16(), f);
+  else by_width(a, bf16(), f);
+  hip_check(hipGetLastError(), "attention launch");
+}
+// more than 64 KB of LDS has to be asked for
+template <class K>
+void with_lds(K* kernel, size_t bytes) {
+  if (bytes > 64 * 1024)
+    hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+            "hipFuncSetAttribute");
+}
+
+}  // namespace
+
+size_t packattn_fwd_work_bytes(const PackedAttn&) { return 0; }
+
+size_t packattn_bwd_work_bytes(const PackedAttn& a) {
+  Sizer z;
+  z.take<float>((size_t)a.heads * a.q_tokens);
+  if (a.dtype == BC2N_F16) z.take<float>(2 * NORM_BLOCKS);
+  return z.off;
+}
+
+void packattn_fwd(hipStream_t st, const PackedAttn& a, void*) {
+  if (a.q_tokens == 0) return;
+  KTimed kt("attention.fwd", st);
+  by_type(a, [&](auto v, auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    const int64_t tiles = tiles_of(a.q_tokens, a.heads / a.kv_heads, 32 * WAVES, a.sequences);
+    auto* kernel = &packattn_fwd_kernel<decltype(v), DP>;
+    const size_t lds = 4 * BN * DP * 2;
+    with_lds(kernel, lds);
+    kernel<<<place_grid(a.kv_heads, tiles), NT, lds, st>>>(a, tiles);
+  });
+}
+
+void packattn_bwd(hipStream_t st, const PackedAttn& a, void* work) {
+  if (a.q_tokens == 0 && a.k_tokens == 0) return;
+  KTimed kt("attention.bwd", st);
+  Carver c(work);
+  float* delta = c.take<float>((size_t)a.heads * a.q_tokens);
+  float* maxima = a.dtype == BC2N_F16 ? c.take<float>(2 * NORM_BLOCKS) : nullptr;
+  by_type(a, [&](auto v, auto dp) {
+    typedef decltype(v) T;
+    constexpr int DP = decltype(dp)::value;
+    const int64_t q_tiles = tiles_of(a.q_tokens, a.heads / a.kv_heads, 32 * WAVES, a.sequences);
+    const int64_t k_tiles = tiles_of(a.k_tokens, 1, 32 * WAVES, a.sequences);
+    if (maxima)
+      packattn_norms_kernel<T><<<NORM_BLOCKS, NT, 0, st>>>(a, tiles_of(a.q_tokens, 1, 64, a.sequences),
+                                                          tiles_of(a.k_tokens, 1, 64, a.sequences), maxima);
+    if (a.q_tokens) {
+      auto* dq = &packattn_dq_kernel<T, DP>;
+      const size_t lds = 4 * BN * DP * 2;
+      with_lds(dq, lds);
+      dq<<<place_grid(a.kv_heads, q_tiles), NT, lds, st>>>(a, q_tiles, delta, maxima, NORM_BLOCKS);
+    }
+    if (a.k_tokens) {
+      auto* dkv = &packattn_dkv_kernel<T, DP>;
+      const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4);
+      with_lds(dkv, lds);
+      dkv<<<place_grid(a.kv_heads, k_tiles), NT, lds, st>>>(a, k_tiles, delta, maxima, NORM_BLOCKS);
+    }
+  });
+}
+
+}  // namespace bc2n

@@ -1,0 +1,565 @@
+// Drawing a class from each row of logits x[V] by a given uniform number u.
+// With m = max x and the classes ranked by x, ties to the lowest index:
+//
+//   e_j   = exp((x_j - m) / temperature)
+//   top-k  keeps the first k; top-p those whose forerunners hold less than
+//   top_p of what top-k kept; min-p those with e_j >= min_p; the first stays
+//   index = the first class, by index, at which the running sum of the kept
+//           e_j exceeds u times their whole sum
+//   logp  = log of its share of that sum
+//
+// The class hangs on which side of a border a sum lies, so nothing here may
+// depend on the order of a sum: e_j is held as a whole number of 2^-S (its
+// exponential in 64 bits), 2^S as large as a row's sum in 64 bits allows (2^44
+// for 131 k classes), and sums of those are exact in any order.  An e_j below
+// half of that counts as zero and can be left out of everything.
+//
+// A row is a workgroup's.  A rank or a share of the mass becomes a threshold on
+// (x, index) in one pass that counts the classes by their distance to the
+// maximum, in 2048 steps, and an exact ranking of the few in the step that the
+// border falls into; where ties or odd distributions leave many there, further
+// passes divide that step.  Exponentials in 64 bits cost twenty instructions
+// and are made only of classes still in play.
+#include "sample.h"
+
+#include "common.h"
+#include "runtime.h"
+#include "vec.h"
+
+#include "../../include/bc2n.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace bc2n {
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int BINS = 2048;
+constexpr int LIST = 256;  // classes ranked one against all
+constexpr float NEG_INF = -__builtin_inff();
+
+// bits of a mass: V of them fit 62 bits
+__host__ __device__ constexpr int mass_bits(int V) {
+  int b = 0;
+  while ((int64_t(1) << b) < V) ++b;
+  return 61 - b < 48 ? 61 - b : 48;
+}
+
+// 2^t for t <= 0 in units of 2^-S, in whole ones.  The series of e^(f log 2) for
+// |f| <= 1/2 ends at 4e-16.
+__device__ __forceinline__ u64 mass_of(double t, int S) {
+  if (!(t > -(double)(S + 2))) return 0;
+  const double n = rint(t), f = (t - n) * 0.69314718055994530942;
+  double p = 1.0 / 479001600.0;
+  p = fma(p, f, 1.0 / 39916800.0);
+  p = fma(p, f, 1.0 / 3628800.0);
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return (u64)(ldexp(p, (int)n + S) + 0.5);
+}
+
+// Larger for larger x; -0 as 0.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// Larger for a better rank; no two classes have the same.
+__device__ __forceinline__ u64 rank_key(float x, int j) {
+  return (u64)key_of(x) << 32 | (uint32_t)(~j);
+}
+
+struct Settings {
+  double inv;    // log2(e) / temperature
+  int64_t k;     // 0: all
+  double p;
+  double floor;  // log2 of min-p, at most 0
+  float u;
+  bool greedy, bad;
+};
+__device__ __forceinline__ Settings settings_of(const Sample& a, int64_t r) {
+  Settings s;
+  const double t = a.temperature.row ? (double)a.temperature.row[r] : a.temperature.v;
+  s.k = a.top_k_row ? (int64_t)a.top_k_row[r] : a.top_k;
+  if (s.k < 1 || s.k >= a.V) s.k = 0;
+  s.p = a.top_p.row ? (double)a.top_p.row[r] : a.top_p.v;
+  const double floor = a.min_p.row ? (double)a.min_p.row[r] : a.min_p.v;
+  s.floor = floor > 0 ? log2(fmin(floor, 1.0)) : (double)NEG_INF;
+  s.u = a.u[r];
+  s.bad = !(s.u == s.u) || !(fabs(t) < (double)-NEG_INF);
+  s.greedy = !(t > 0) || s.k == 1;
+  s.inv = fmin(1.4426950408889634 / t, 1e300);
+  return s;
+}
+// the least sum of forerunners that ends top-p: p of the mass, at least 1
+__device__ __forceinline__ u64 share_of(double p, u64 mass) {
+  const double x = ceil(fmax(p, 0.0) * (double)mass);
+  return x < 1.0 ? 1 : x >= (double)mass ? mass : (u64)x;
+}
+__device__ __forceinline__ u64 target_of(float u, u64 mass) {
+  const double x = fmax((double)u, 0.0) * (double)mass;
+  return x >= (double)mass ? mass - 1 : min((u64)x, mass - 1);
+}
+__device__ __forceinline__ void write(const Sample& a, int64_t r, int j, float logp) {
+  a.index[r] = j;
+  if (a.logp) a.logp[r] = logp;
+}
+// log of e^((x - m) / t) 2^S / mass; d = (x - m) inv in log 2
+__device__ __forceinline__ float log_share(double d, u64 mass, int S) {
+  return (float)((d - (log2((double)mass) - (double)S)) * 0.69314718055994530942);
+}
+
+// ---------------------------------------------------------------------------
+// Rows of at most W classes: a class a lane, W lanes a row.  Ranks and sums of
+// forerunners by comparing each class with all.
+template <class T, int W>
+__global__ __launch_bounds__(256) void sample_few_kernel(Sample a) {
+  const int lane = threadIdx.x & (W - 1);
+  const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / W;
+  if (r >= a.rows) return;  // whole groups
+  const int S = mass_bits(a.V);
+  const Settings s = settings_of(a, r);
+  const float x = lane < a.V ? (float)reinterpret_cast<const T*>(a.x)[r * a.ld + lane] : NEG_INF;
+  const u64 c = rank_key(x, lane);
+  const float m = group_max<W>(x);
+  const float nan = group_max<W>(x != x || x == -NEG_INF ? 1.f : 0.f);
+  if (nan != 0.f || m == NEG_INF || s.bad) {
+    if (lane == 0) write(a, r, -1, __builtin_nanf(""));
+    return;
+  }
+  const double d = ((double)x - (double)m) * s.inv;
+  u64 w = s.greedy ? 0 : mass_of(d, S);
+  auto sum = [&](u64 v) {
+#pragma unroll
+    for (int i = 1; i < W; i *= 2) v += __shfl_xor(v, i, W);
+    return v;
+  };
+  int rank = 0;
+  if (s.k || s.greedy) {
+    for (int j = 0; j < a.V; ++j) rank += __shfl(c, j, W) > c;
+    if (s.greedy) {
+      if (rank == 0) write(a, r, lane, 0.f);
+      return;
+    }
+    if (rank >= s.k) w = 0;
+  }
+  if (s.p < 1.0) {
+    const u64 end = share_of(s.p, sum(w));
+    u64 before = 0;
+    for (int j = 0; j < a.V; ++j) {
+      const u64 cj = __shfl(c, j, W), wj = __shfl(w, j, W);
+      before += cj > c ? wj : 0;
+    }
+    if (before >= end) w = 0;
+  }
+  if (d < s.floor) w = 0;
+  u64 run = w;
+#pragma unroll
+  for (int i = 1; i < W; i *= 2) {
+    const u64 v = __shfl_up(run, i, W);
+    if (lane >= i) run += v;
+  }
+  const u64 mass = __shfl(run, W - 1, W), t = target_of(s.u, mass);
+  if (w && run > t && run - w <= t) write(a, r, lane, log_share(d, mass, S));
+}
+
+// ---------------------------------------------------------------------------
+// A workgroup a row.
+template <int NT>
+struct Shared {
+  u64 mass[BINS];
+  uint32_t count[BINS];
+  u64 list_key[LIST];
+  u64 list_mass[LIST];
+  u64 wave_a[NT / 64], wave_b[NT / 64];
+  u64 out[4];
+  uint32_t n;
+};
+
+template <class F>
+__device__ __forceinline__ u64 wave_fold(u64 v, F f) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) v = f(v, (u64)__shfl_xor(v, i, 64));
+  return v;
+}
+// over the workgroup, the result in every thread
+template <int NT, class F>
+__device__ __forceinline__ u64 block_fold(u64 v, u64* waves, F f) {
+  v = wave_fold(v, f);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = waves[0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; ++i) v = f(v, waves[i]);
+  return v;
+}
+struct Sum {
+  __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+  __device__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
+};
+struct Min {
+  __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; }
+};
+template <int NT>
+__device__ __forceinline__ u64 block_scan(u64 v, u64* waves) {  // exclusive
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u64 run = v;
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) {
+    const u64 o = __shfl_up(run, i, 64);
+    if (lane >= i) run += o;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = run;
+  __syncthreads();
+  u64 before = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) before += i < wave ? waves[i] : 0;
+  return before + run - v;
+}
+
+// A row in tiles of consecutive classes, a vector a thread.
+template <class T, int NT>
+struct RowOf {
+  static constexpr int E = Vec<T>::N;
+  static constexpr int TILE = NT * E;
+  const T* x;
+  int V, tiles;
+
+  // classes past the row's end are -infinity
+  __device__ __forceinline__ u32x4 load(int i) const {
+    const int64_t j = (int64_t)i * TILE + threadIdx.x * E;
+    if (j + E <= V) return Vec<T>::load(x + j);
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = j + e < V ? (float)x[j + e] : NEG_INF;
+    return Vec<T>::pack(v);
+  }
+  __device__ __forceinline__ void init(const T* row, int V_) {
+    x = row;
+    V = V_;
+    tiles = (V + TILE - 1) / TILE;
+  }
+  template <class F>
+  __device__ __forceinline__ void tile(int i, F f) const {
+    float v[E];
+    Vec<T>::unpack(load(i), v);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f(v[e], i * TILE + (int)threadIdx.x * E + e);
+  }
+  // f(x, index) of a thread's classes
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) tile(i, f);
+  }
+};
+
+// What a row's kept classes have at least: rank key and distance.
+template <class T, int NT>
+struct Drawer {
+  Shared<NT>& sh;
+  const RowOf<T, NT>& row;
+  float m, range, steps;  // maximum, largest distance of a mass, steps a distance
+  double inv;
+  int S;
+
+  __device__ __forceinline__ double distance(float x) const { return ((double)x - (double)m) * inv; }
+  __device__ __forceinline__ u64 mass(float x) const { return mass_of(distance(x), S); }
+  // a class that can have a mass
+  __device__ __forceinline__ bool counts(float x) const { return m - x <= range; }
+  __device__ __forceinline__ int step_of(float x) const {
+    return (int)fminf((m - x) * steps, (float)(BINS - 1));
+  }
+
+  // The rank key of the last class whose forerunners, among the classes of
+  // rank keys >= least, weigh less than `end`: by number, or (MASS) by mass.
+  template <bool MASS>
+  __device__ u64 last_before(u64 end, u64 least) {
+    u64 lo = 0, hi = ~u64(0), before = 0;
+    int shift = -1;  // -1: steps of distance
+    for (;;) {
+      for (int i = threadIdx.x; i < BINS; i += NT) {
+        sh.count[i] = 0;
+        if (MASS) sh.mass[i] = 0;
+      }
+      if (threadIdx.x == 0) sh.n = 0;
+      __syncthreads();
+      auto bin_of = [&](float x, u64 c) {
+        return shift < 0 ? step_of(x) : (int)((hi - c) >> shift);
+      };
+      row.each([&](float x, int j) {
+        if (!counts(x)) return;
+        const u64 c = rank_key(x, j);
+        if (c < least || c < lo || c > hi) return;
+        const int b = bin_of(x, c);
+        atomicAdd(&sh.count[b], 1u);
+        if (MASS) atomicAdd(&sh.mass[b], mass(x));
+      });
+      __syncthreads();
+      // the last filled bin whose forerunners weigh less than the end
+      constexpr int PER = BINS / NT;
+      u64 w = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = threadIdx.x * PER + i;
+        w += MASS ? sh.mass[b] : sh.count[b];
+      }
+      u64 run = before + block_scan<NT>(w, sh.wave_a);
+      u64 best = 0;  // bin + 1
+      u64 best_run = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = threadIdx.x * PER + i;
+        if (sh.count[b] && run < end) {
+          best = b + 1;
+          best_run = run;
+        }
+        run += MASS ? sh.mass[b] : sh.count[b];
+      }
+      const u64 top = block_fold<NT>(best, sh.wave_b, Max());
+      if (best == top && best) sh.out[0] = best_run;
+      __syncthreads();
+      const int bin = (int)top - 1;
+      before = sh.out[0];
+      const uint32_t in_bin = sh.count[bin];
+      if (in_bin <= LIST) {
+        row.each([&](float x, int j) {
+          if (!counts(x)) return;
+          const u64 c = rank_key(x, j);
+          if (c < least || c < lo || c > hi || bin_of(x, c) != bin) return;
+          const uint32_t at = atomicAdd(&sh.n, 1u);
+          sh.list_key[at] = c;
+          sh.list_mass[at] = MASS ? mass(x) : 1;
+        });
+        __syncthreads();
+        u64 key = ~u64(0);
+        for (int i = threadIdx.x; i < (int)in_bin; i += NT) {
+          const u64 c = sh.list_key[i];
+          u64 f = before;
+          for (int k = 0; k < (int)in_bin; ++k) f += sh.list_key[k] > c ? sh.list_mass[k] : 0;
+          if (f < end) key = min(key, c);
+        }
+        return block_fold<NT>(key, sh.wave_a, Min());
+      }
+      // too many: their range of rank keys in 2048 parts
+      u64 a = ~u64(0), b = 0;
+      row.each([&](float x, int j) {
+        if (!counts(x)) return;
+        const u64 c = rank_key(x, j);
+        if (c < least || c < lo || c > hi || bin_of(x, c) != bin) return;
+        a = min(a, c);
+        b = max(b, c);
+      });
+      a = block_fold<NT>(a, sh.wave_a, Min());
+      b = block_fold<NT>(b, sh.wave_b, Max());
+      lo = a;
+      hi = b;
+      shift = 0;
+      while (((hi - lo) >> shift) >= BINS) ++shift;
+      __syncthreads();
+    }
+  }
+};
+
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
+  __shared__ Shared<NT> sh;
+  constexpr int WAVES = NT / 64;
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Settings s = settings_of(a, r);
+  RowOf<T, NT> row;
+  row.init(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
+  float hi = NEG_INF, lo = -NEG_INF;
+  bool nan = false;
+  row.each([&](float x, int) {
+    nan |= x != x;
+    hi = fmaxf(hi, x);
+    if (x != NEG_INF) lo = fminf(lo, x);
+  });
+  const u64 top = block_fold<NT>(nan ? ~u64(0) : (u64)key_of(hi), sh.wave_a, Max());
+  const u64 low = block_fold<NT>((u64)key_of(lo), sh.wave_b, Min());
+  auto value = [](u64 k) {
+    const uint32_t b = (uint32_t)k;
+    return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
+  };
+  const float m = value(top);
+  if (top == ~u64(0) || m == -NEG_INF || m == NEG_INF || s.bad) {
+    if (threadIdx.x == 0) write(a, r, -1, __builtin_nanf(""));
+    return;
+  }
+  if (s.greedy) {
+    u64 first = ~u64(0);
+    row.each([&](float x, int j) {
+      if (x == m) first = min(first, (u64)j);
+    });
+    first = block_fold<NT>(first, sh.wave_a, Min());
+    if (threadIdx.x == 0) write(a, r, (int)first, 0.f);
+    return;
+  }
+  Drawer<T, NT> d{sh, row, m, 0.f, 0.f, s.inv, mass_bits(a.V)};
+  // a little past the last distance with a mass; at least what a step of the
+  // maximum's own is
+  const double range = (d.S + 2) / s.inv * 1.0001;
+  d.range = (float)fmin(range, 3e38);
+  const float span = fminf(d.range, m - value(low));
+  d.steps = span > 0.f ? fminf((float)(BINS - 1) / span, 3e38f) : 0.f;
+
+  u64 least = 0;
+  if (s.k) least = d.template last_before<false>((u64)s.k, 0);
+  auto kept_mass = [&](float x, int j) -> u64 {
+    if (!d.counts(x) || rank_key(x, j) < least) return 0;
+    const double t = d.distance(x);
+    return t < s.floor ? 0 : mass_of(t, d.S);
+  };
+  if (s.p < 1.0) {
+    u64 mass = 0;
+    row.each([&](float x, int j) {
+      if (d.counts(x) && rank_key(x, j) >= least) mass += d.mass(x);
+    });
+    mass = block_fold<NT>(mass, sh.wave_a, Sum());
+    least = d.template last_before<true>(share_of(s.p, mass), least);
+  }
+
+  // the running sum: groups of tiles, then the tiles of one group, then the
+  // waves of one tile
+  int t0 = 0, t1 = row.tiles;
+  u64 before = 0, mass = 0, target = 0;
+  bool first = true;
+  for (;;) {
+    const int per = (t1 - t0 + BINS / WAVES - 1) / (BINS / WAVES);
+    __syncthreads();
+    for (int i = threadIdx.x; i < BINS; i += NT) sh.mass[i] = 0;
+    __syncthreads();
+    u64 sum = 0;
+    int at = t0;
+    auto put = [&](int tile) {  // the tiles before `tile` are summed
+      const u64 w = wave_fold(sum, Sum());
+      if (lane == 0) sh.mass[(at - t0) / per * WAVES + wave] += w;
+      sum = 0;
+      at = tile;
+    };
+#pragma unroll 1
+    for (int i = t0; i < t1; ++i) {
+      row.tile(i, [&](float x, int j) { sum += kept_mass(x, j); });
+      put(i + 1);
+    }
+    __syncthreads();
+    // `groups` of WAVES entries; entries within a group are in the classes'
+    // order where it is one tile
+    const int entries = ((t1 - t0 + per - 1) / per) * WAVES;
+    constexpr int PER = BINS / NT;
+    u64 w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) w += sh.mass[threadIdx.x * PER + i];
+    u64 run = before + block_scan<NT>(w, sh.wave_a);
+    if (first) {
+      mass = block_fold<NT>(w, sh.wave_b, Sum());
+      target = target_of(s.u, mass);
+      first = false;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = threadIdx.x * PER + i;
+      const u64 v = sh.mass[e];
+      if (e < entries && run <= target && run + v > target) {
+        sh.out[0] = e;
+        sh.out[1] = run;
+      }
+      run += v;
+    }
+    __syncthreads();
+    const int e = (int)sh.out[0], group = e / WAVES;
+    if (per == 1) {
+      before = sh.out[1];
+      t0 += group;
+      if (wave != e % WAVES) return;
+      break;
+    }
+    before = sh.out[1];
+    for (int i = group * WAVES; i < e; ++i) before -= sh.mass[i];
+    t0 += group * per;
+    t1 = min(t0 + per, t1);
+  }
+  // one wave's classes of tile t0
+  constexpr int E = RowOf<T, NT>::E;
+  float xs[E];
+  u64 ws[E], sum = 0;
+  row.tile(t0, [&](float x, int j) {
+    const int e = j - (t0 * RowOf<T, NT>::TILE + (int)threadIdx.x * E);
+    xs[e] = x;
+    ws[e] = kept_mass(x, j);
+    sum += ws[e];
+  });
+  u64 run = sum;
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) {
+    const u64 o = __shfl_up(run, i, 64);
+    if (lane >= i) run += o;
+  }
+  run += before - sum;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (run <= target && run + ws[e] > target)
+      write(a, r, t0 * RowOf<T, NT>::TILE + (int)threadIdx.x * E + e,
+            log_share(d.distance(xs[e]), mass, d.S));
+    run += ws[e];
+  }
+}
+
+template <class T, int NT>
+void row_go(hipStream_t st, const Sample& a) {
+  sample_row_kernel<T, NT><<<(unsigned)a.rows, NT, 0, st>>>(a);
+}
+template <class T>
+void go(hipStream_t st, const Sample& a) {
+  constexpr int E = Vec<T>::N;
+  if (a.V <= 64) {
+    const int W = a.V <= 16 ? 16 : a.V <= 32 ? 32 : 64;
+    const unsigned grid = (unsigned)((a.rows * W + 255) / 256);
+    if (W == 16) sample_few_kernel<T, 16><<<grid, 256, 0, st>>>(a);
+    else if (W == 32) sample_few_kernel<T, 32><<<grid, 256, 0, st>>>(a);
+    else sample_few_kernel<T, 64><<<grid, 256, 0, st>>>(a);
+  } else if (a.V <= 4 * 256 * E) row_go<T, 256>(st, a);
+  else row_go<T, 1024>(st, a);
+}
+
+}  // namespace
+
+void sample(hipStream_t st, const Sample& a) {
+  // a grid holds fewer than 2^32 threads
+  constexpr int64_t SLICE = int64_t(1) << 21;
+  for (int64_t r = 0; r < a.rows; r += SLICE) {
+    Sample b = a;
+    b.rows = std::min(SLICE, a.rows - r);
+    const int64_t w = a.dtype == BC2N_F32 ? 4 : 2;
+    b.x = (const char*)a.x + r * a.ld * w;
+    b.u += r;
+    b.index += r;
+    if (b.logp) b.logp += r;
+    if (b.top_k_row) b.top_k_row += r;
+    for (Setting* s : {&b.temperature, &b.top_p, &b.min_p})
+      if (s->row) s->row += r;
+    KTimed kt("sample", st);
+    if (a.dtype == BC2N_F32) go<float>(st, b);
+    else if (a.dtype == BC2N_F16) go<h16>(st, b);
+    else go<bf16>(st, b);
+    hip_check(hipGetLastError(), "sample launch");
+  }
+}
+
+}  // namespace bc2n

@@ -890,6 +890,233 @@ class LogProbs:
         return (logp, entropy), out
 
 
+def _heads(t, what, dtype=None, shape=None):
+    """(address, token stride, head stride) of [tokens, heads, width]."""
+    if t.dim() != 3 or (shape is not None and tuple(t.shape) != shape):
+        raise ValueError(f"{what}: expected {shape or '[tokens, heads, width]'}, got {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
+    _current(t, what)
+    st, sh, e = t.stride()
+    if e != 1 and t.shape[2] > 1:
+        raise ValueError(f"{what}: a head's elements must be contiguous")
+    return t.data_ptr(), st, sh
+
+
+def _vector(t, n, dtypes, what):
+    """The address of a contiguous [n] on the current device."""
+    if t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes:
+        raise ValueError(f"{what}: expected {', '.join(map(str, dtypes))} [{n}], got {t.dtype} {tuple(t.shape)}")
+    if not _current(t, what).is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous tensor")
+    return t.data_ptr()
+
+
+class HeadNormRotate:
+    """Root-mean-square norm of every head of queries and keys, and their
+    rotation by position in the same pass (bc2n_headnorm_*).
+
+    freq f32 [pairs]: a pair turns by position * freq; the first 2 * pairs
+    elements of a head rotate, as pairs (i, i + pairs) or, interleaved,
+    (2 i, 2 i + 1).  q [tokens, heads, width] and k [tokens, kv_heads, width] (or
+    None) f32, f16 or bf16, any token and head strides; positions i32 or i64
+    [tokens]; weights [width], f32 or of q's type."""
+
+    def __init__(self, freq, eps=1e-6, interleaved=False):
+        if freq.dtype != torch.float32 or freq.dim() != 1 or not freq.is_contiguous():
+            raise ValueError("freq: expected a contiguous float32 [pairs]")
+        if not 0 <= eps < float("inf"):
+            raise ValueError("eps must be finite and not negative")
+        self.freq, self.eps, self.interleaved = freq, float(eps), int(bool(interleaved))
+
+    def _operands(self, q, k, positions, q_weight, k_weight):
+        """(the calls' operands before the tensors of heads, those after them)"""
+        if q.dim() != 3 or q.dtype not in _DTYPES:
+            raise ValueError(f"q: expected float32, float16 or bfloat16 [tokens, heads, width], got {q.dtype} "
+                             f"{tuple(q.shape)}")
+        n, heads, width = q.shape
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"positions: expected int32 or int64, got {positions.dtype}")
+        pairs, wt = self.freq.shape[0], q_weight.dtype
+        at = _vector(positions, n, (positions.dtype,), "positions")
+        _current(self.freq, "freq")
+        qw, kw = _vector(q_weight, width, (torch.float32, q.dtype), "q_weight"), None
+        if k is not None:
+            kw = _vector(k_weight, width, (wt,), "k_weight")
+        return ((_DTYPES[q.dtype], n, heads, 0 if k is None else k.shape[1], width, 2 * pairs, self.interleaved),
+                (at, 64 if positions.dtype == torch.int64 else 32, self.freq.data_ptr(), qw, kw, _DTYPES[wt],
+                 self.eps))
+
+    @staticmethod
+    def _pair(q, k, like_q, like_k, what):
+        """The six operands of queries and keys, checked against the inputs."""
+        a = _heads(q, what[0], like_q.dtype, tuple(like_q.shape))
+        if like_k is None:
+            return (*a, None, 0, 0)
+        if like_k.dim() != 3 or like_k.shape[0] != like_q.shape[0] or like_k.shape[2] != like_q.shape[2]:
+            raise ValueError(f"k: expected [{like_q.shape[0]}, heads, {like_q.shape[2]}], got {tuple(like_k.shape)}")
+        return (*a, *_heads(k, what[1], like_q.dtype, tuple(like_k.shape)))
+
+    def forward(self, q, k, positions, q_weight, k_weight=None, out=None):
+        """-> (q, k) normed and rotated, in new tensors or in out = (q, k), which
+        may be the inputs; without k, k is None"""
+        first, last = self._operands(q, k, positions, q_weight, k_weight)
+        x = self._pair(q, k, q, k, ("q", "k"))
+        if out is None:
+            out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+                   None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        y = self._pair(*out, q, k, ("out", "out"))
+        check(lib().bc2n_headnorm_fwd(_stream(), *first, *x, *last, *y))
+        return tuple(out)
+
+    def backward(self, cts, q, k, positions, q_weight, k_weight=None, out=None):
+        """cts = (d_q, d_k), q and k the forward's inputs -> (d_q, d_k, d_q_weight,
+        d_k_weight), the first two in out = (d_q, d_k) where given, the weights'
+        f32"""
+        first, last = self._operands(q, k, positions, q_weight, k_weight)
+        x = self._pair(q, k, q, k, ("q", "k"))
+        d = self._pair(*cts, q, k, ("d_q", "d_k"))
+        if out is None:
+            out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+                   None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        y = self._pair(*out, q, k, ("out", "out"))
+        width, dev = q.shape[2], q.device
+        dw = torch.empty(2, width, dtype=torch.float32, device=dev)
+        work = torch.empty(lib().bc2n_headnorm_work_bytes(q.shape[0], width), dtype=torch.uint8, device=dev)
+        at = dw.data_ptr()
+        check(lib().bc2n_headnorm_bwd(_stream(), *first, *d, *x, *last, *y, at,
+                                      None if k is None else at + 4 * width, work.data_ptr()))
+        return (*out, dw[0], None if k is None else dw[1])
+
+
+class PackedAttention:
+    """Attention of sequences packed one after another, with grouped heads
+    (bc2n_attention_*).
+
+    q [q_tokens, heads, width], k and v [k_tokens, kv_heads, width] f16 or bf16, any
+    token and head strides that keep 16 bytes, width a multiple of 8 up to 128.
+    Sequence b's queries are the tokens q_offsets[b] .. q_offsets[b + 1] (i32
+    [sequences + 1] on the device), its keys likewise by k_offsets; of those the
+    first q_lengths[b] and k_lengths[b] where given (a cache of fixed capacity).
+    causal: query i of m sees keys 0 .. i + n - m of n.  Rows of the results that
+    belong to no sequence are zeros (lse -inf) in tensors that a call makes, and
+    left as they were in given ones."""
+
+    def __init__(self, causal=True, scale=None):
+        if scale is not None and not 0 < scale < float("inf"):
+            raise ValueError("scale must be positive and finite")
+        self.causal, self.scale = int(bool(causal)), scale
+
+    def _operands(self, q, k, v, q_offsets, k_offsets, k_lengths, q_lengths):
+        if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"q: expected float16 or bfloat16 [tokens, heads, width], got {q.dtype} "
+                             f"{tuple(q.shape)}")
+        n, heads, width = q.shape
+        if k.dim() != 3 or k.shape[2] != width or k.shape[1] == 0 or heads == 0 or heads % k.shape[1]:
+            raise ValueError(f"k: expected [tokens, a divisor of {heads}, {width}], got {tuple(k.shape)}")
+        x = _heads(q, "q") + _heads(k, "k", q.dtype) + _heads(v, "v", q.dtype, tuple(k.shape))
+        i32 = (torch.int32,)
+        count = q_offsets.shape[0] - 1 if q_offsets.dim() == 1 else -1
+        if count < 0:
+            raise ValueError("q_offsets: expected int32 [sequences + 1]")
+        offsets = [_vector(q_offsets, count + 1, i32, "q_offsets"),
+                   _vector(q_offsets if k_offsets is None else k_offsets, count + 1, i32, "k_offsets")]
+        lengths = [None if t is None else _vector(t, count, i32, what)
+                   for t, what in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths"))]
+        if k_offsets is None and k.shape[0] != n:
+            raise ValueError(f"k_offsets: needed, q has {n} tokens and k {k.shape[0]}")
+        sizes = (_DTYPES[q.dtype], self.causal, count, n, k.shape[0], heads, k.shape[1], width)
+        scale = width ** -0.5 if self.scale is None else self.scale
+        return sizes, (scale, *offsets, *lengths), x
+
+    def forward(self, q, k, v, q_offsets, k_offsets=None, k_lengths=None, q_lengths=None, out=None):
+        """-> (out like q, lse f32 [heads, q_tokens]), out in `out` where given.
+        Without k_offsets the keys are the queries' tokens."""
+        sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths)
+        fill = out is None
+        if fill:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o = _heads(out, "out", q.dtype, tuple(q.shape))
+        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
+        work = self._work(lib().bc2n_attention_fwd_work_bytes, sizes, q.device)
+        check(lib().bc2n_attention_fwd(_stream(), *sizes, *where, *x, int(fill), *o, lse.data_ptr(), _ptr(work)))
+        return out, lse
+
+    @staticmethod
+    def _work(size, sizes, device):
+        n = size(*sizes)
+        return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+    def backward(self, d_out, q, k, v, out, lse, q_offsets, k_offsets=None, k_lengths=None, q_lengths=None,
+                 grads=None):
+        """out and lse the forward's -> (d_q, d_k, d_v), in grads = (d_q, d_k, d_v)
+        where given"""
+        sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths)
+        shape = tuple(q.shape)
+        g, o = _heads(d_out, "d_out", q.dtype, shape), _heads(out, "out", q.dtype, shape)
+        _f32(lse, (shape[1], shape[0]), "lse")
+        if not _current(lse, "lse").is_contiguous():
+            raise ValueError("lse: expected a contiguous tensor")
+        fill = grads is None
+        if fill:
+            grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        d = ()
+        for t, like, what in zip(grads, (q, k, v), ("d_q", "d_k", "d_v")):
+            d += _heads(t, what, q.dtype, tuple(like.shape))
+        work = self._work(lib().bc2n_attention_bwd_work_bytes, sizes, q.device)
+        check(lib().bc2n_attention_bwd(_stream(), *sizes, *where, *g, *x, *o, lse.data_ptr(), int(fill), *d,
+                                       _ptr(work)))
+        return tuple(grads)
+
+
+class Sampler:
+    """A class a row of logits by given uniform numbers, from what temperature,
+    top-k, top-p and min-p leave (bc2n_sample).
+
+    Each setting is a number for all rows, or a contiguous tensor of the rows'
+    own on the device (f32; top_k i32).  top_k 0 and top_p 1 cut nothing; a
+    temperature of 0 takes the first class."""
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        self.settings = []
+        for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+            whole = name == "top_k"
+            if torch.is_tensor(v):
+                if v.dtype != (torch.int32 if whole else torch.float32):
+                    raise ValueError(f"{name}: expected {'int32' if whole else 'float32'}, got {v.dtype}")
+                self.settings.append((name, 0, v))
+                continue
+            v = int(v) if whole else float(v)
+            if not (0 <= v if name != "temperature" else 0 <= v < float("inf")):
+                raise ValueError(f"{name} must not be negative" + ("" if whole else ", infinite or NaN"))
+            self.settings.append((name, v, None))
+
+    def sample(self, logits, uniforms):
+        """logits [..., classes] f32, f16 or bf16, any row stride, uniforms f32 [...]
+        in [0, 1) -> (index i32 [...], logp f32 [...]): -1 and NaN for a row that
+        nothing can be drawn from"""
+        code, lead = _DTYPES.get(logits.dtype), logits.shape[:-1]
+        if code is None or not logits.shape or logits.shape[-1] == 0:
+            raise ValueError(f"logits: expected float32, float16 or bfloat16 [..., classes], got "
+                             f"{logits.dtype} {tuple(logits.shape)}")
+        x, ld = LogProbs._rows(logits, "logits")
+        _f32(uniforms, lead, "uniforms")
+        rows, own = uniforms.numel(), []
+        for name, v, t in self.settings:
+            at = None
+            if t is not None:
+                if t.numel() != rows:
+                    raise ValueError(f"{name}: expected a value for each of {rows} rows, got {t.numel()}")
+                at = LogProbs._given(t, name)
+            own += [v, at]
+        index = torch.empty(lead, dtype=torch.int32, device=logits.device)
+        logp = torch.empty(lead, dtype=torch.float32, device=logits.device)
+        check(lib().bc2n_sample(_stream(), code, x, ld, rows, logits.shape[-1],
+                                LogProbs._given(uniforms, "uniforms"), *own, index.data_ptr(),
+                                logp.data_ptr()))
+        return index, logp
+
+
 class _TensorList:
     """A list of the C ABI over tensors, which it keeps alive and takes to
     stay where they are: it holds their addresses, so what a call returns in a

@@ -658,6 +658,130 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
                        int64_t d_ld, void* work);
 
 /* ------------------------------------------------------------------------
+ * Norms of queries and keys for each head, with the rotation by position in
+ * the same pass, and their gradient (next to LayerNorm: what a sequence
+ * model's attention takes).  No reference counterpart.
+ * q [tokens][heads][width] and k [tokens][kv_heads][width] of BC2N_F32,
+ * BC2N_F16 or BC2N_BF16, each with a token stride and a head stride in
+ * elements (slices of one projection, or heads first), a head's elements
+ * contiguous; either may have 0 heads.  With x a head's row and w its weight
+ * [width] (BC2N_F32 or the operands' type):
+ *   y = x (mean x^2 + eps)^-1/2 w
+ * and the pairs of its first `rotated` elements -- (i, i + rotated / 2), or
+ * (2 i, 2 i + 1) where interleaved -- turn by positions[token] * freq[i]:
+ *   (a, b) -> (a cos t - b sin t, b cos t + a sin t).
+ * positions i32 or i64 (position_bits) [tokens], freq f32[rotated / 2]; the angle
+ * is taken in 64 bits.  Norms, rotation and sums are f32, results rounded
+ * once.  Widths: even; half of `rotated` and the rest are cut into vectors of
+ * one power of two of elements, 8 (f32: 4) at most, of which a head has 128
+ * at most: every width that is a multiple of 16 up to 1024 (f32: of 8, to
+ * 512) with a quarter, half or all of it rotated, every even one up to 128.
+ * Outputs may be their own inputs; they overlap nothing else.
+ * bwd: d_q, d_k cotangents of the outputs and q, k the inputs -> q_grad,
+ * k_grad of the operands' type (they may be those inputs or cotangents) and
+ * d_q_weight, d_k_weight f32 [width] (either may be NULL), summed over tokens
+ * and heads in one order; work is bc2n_headnorm_work_bytes() bytes, 16-byte
+ * aligned, for the time of the call.
+ * ---------------------------------------------------------------------- */
+int bc2n_headnorm_fwd(void* stream, int dtype, int64_t tokens, int heads, int kv_heads, int width,
+                      int rotated, int interleaved, const void* q, int64_t q_st, int64_t q_sh,
+                      const void* k, int64_t k_st, int64_t k_sh, const void* positions,
+                      int position_bits, const float* freq, const void* q_weight,
+                      const void* k_weight, int weight_dtype, float eps, void* q_out, int64_t qo_st,
+                      int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh);
+size_t bc2n_headnorm_work_bytes(int64_t tokens, int width);
+int bc2n_headnorm_bwd(void* stream, int dtype, int64_t tokens, int heads, int kv_heads, int width,
+                      int rotated, int interleaved, const void* d_q, int64_t dq_st, int64_t dq_sh,
+                      const void* d_k, int64_t dk_st, int64_t dk_sh, const void* q, int64_t q_st,
+                      int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* positions,
+                      int position_bits, const float* freq, const void* q_weight,
+                      const void* k_weight, int weight_dtype, float eps, void* q_grad, int64_t qg_st,
+                      int64_t qg_sh, void* k_grad, int64_t kg_st, int64_t kg_sh, float* d_q_weight,
+                      float* d_k_weight, void* work);
+
+/* ------------------------------------------------------------------------
+ * Attention of sequences packed one after another (chains, prompts, running
+ * sequences against their caches), and its gradient.  No reference
+ * counterpart: the trunk's attentions have one length and a pair bias.
+ * q [q_tokens][heads][width], k and v [k_tokens][kv_heads][width] of BC2N_F16
+ * or BC2N_BF16, strides as above; base addresses and strides keep 16 bytes.
+ * heads is a multiple of kv_heads, query head h reads head h / (heads /
+ * kv_heads) of k and v; width a multiple of 8 up to 128.  Sequence b of
+ * `sequences` has the queries from token q_offsets[b] to q_offsets[b + 1] and the
+ * keys from k_offsets[b] to k_offsets[b + 1] (i32 [sequences + 1] on the
+ * device, rising); with q_lengths or k_lengths (i32 [sequences], or NULL) only the
+ * first so many of them (a padded batch, a cache of fixed capacity).  The
+ * offsets are read on the device alone, and cut to the tokens that there are.
+ *   S = scale q k^T over the keys a query sees (all of its sequence's, or
+ *   causal: query i of m sees the keys 0 .. i + n - m of n), P = softmax S,
+ *   out = P v,  lse f32 [heads][q_tokens] = log sum e^S.
+ *   - A query that sees no key has out 0, lse -inf and no gradient.
+ *   - Tokens of no sequence (before the first, behind the last, past a
+ *     length) may hold anything.  Their rows of the results are zeros (lse
+ *     -inf) where `fill` is set and left as they were where it is not.
+ *   - A NaN or an infinity in a key reaches the rows that see it; in a value
+ *     of a causal sequence it may also reach rows up to 63 tokens before it, as
+ *     0 * NaN in a product of tiles.
+ * Products take the operands as they are, accumulate in f32 and round P and
+ * its cotangent to the operands' type; maxima, sums and lse are f32, added in an
+ * order that goes by the shapes and lengths alone.  In binary16 the
+ * cotangent of S is scaled by a power of two from the largest norms of d_out
+ * and v.
+ * work: bc2n_attention_*_work_bytes() bytes, 16-byte aligned, for the time of the
+ * call (NULL where that is 0).  bwd takes the forward's out and lse, and
+ * returns d_q, d_k and d_v (the group's sum), which overlap nothing.
+ * ---------------------------------------------------------------------- */
+size_t bc2n_attention_fwd_work_bytes(int dtype, int causal, int sequences, int64_t q_tokens,
+                                     int64_t k_tokens, int heads, int kv_heads, int width);
+size_t bc2n_attention_bwd_work_bytes(int dtype, int causal, int sequences, int64_t q_tokens,
+                                     int64_t k_tokens, int heads, int kv_heads, int width);
+int bc2n_attention_fwd(void* stream, int dtype, int causal, int sequences, int64_t q_tokens,
+                       int64_t k_tokens, int heads, int kv_heads, int width, float scale,
+                       const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* q_lengths,
+                       const int32_t* k_lengths, const void* q, int64_t q_st, int64_t q_sh,
+                       const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                       int64_t v_sh, int fill, void* out, int64_t o_st, int64_t o_sh, float* lse,
+                       void* work);
+int bc2n_attention_bwd(void* stream, int dtype, int causal, int sequences, int64_t q_tokens,
+                       int64_t k_tokens, int heads, int kv_heads, int width, float scale,
+                       const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* q_lengths,
+                       const int32_t* k_lengths, const void* d_out, int64_t do_st, int64_t do_sh,
+                       const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                       int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const void* out,
+                       int64_t o_st, int64_t o_sh, const float* lse, int fill, void* d_q, int64_t dq_st,
+                       int64_t dq_sh, void* d_k, int64_t dk_st, int64_t dk_sh, void* d_v, int64_t dv_st,
+                       int64_t dv_sh, void* work);
+
+/* ------------------------------------------------------------------------
+ * A class a row of logits by a given uniform number (next to the
+ * log-probabilities: acids for designed positions, the next token of running
+ * sequences).  No reference counterpart.
+ * logits [rows][classes] of BC2N_F32, BC2N_F16 or BC2N_BF16, row stride ld;
+ * uniforms f32 [rows] in [0, 1) (others are taken to the nearer end).  The
+ * settings are one value for all rows, or f32 (top_ks i32) [rows] on the device
+ * where the array is not NULL.  With m the row's maximum, classes ranked by
+ * logit, ties to the lowest index, and e = exp((x - m) / temperature):
+ *   top_k keeps the first top_k (below 1 or past the classes: all), top_p
+ *   (from 1 on: no cut) the classes whose forerunners hold less than top_p
+ *   of the sum of what top_k kept, min_p those of e >= min_p (at most 1); the
+ *   first class stays.
+ *   index = the first class by index at which the kept ones' running sum of
+ *   e exceeds uniform times their whole sum; logp (f32, or NULL) = log of its e
+ *   over that sum.
+ * A temperature of 0 (in an array: not positive) takes the first class, logp 0.
+ * Sums are exact in units of 2^-48 of the largest e (of 2^-44 at 131 072 classes:
+ * 2^-61 times the classes' next power of two), so that the choice does not hang
+ * on their order; an e below half a unit counts as 0.
+ *   - A logit of -inf is never drawn.  A row with a NaN or +inf logit, of
+ *     -inf alone, or with a NaN uniform or a NaN or infinite temperature has
+ *     index -1 and logp NaN.
+ * ---------------------------------------------------------------------- */
+int bc2n_sample(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows, int classes,
+                const float* uniforms, double temperature, const float* temperatures, int64_t top_k,
+                const int32_t* top_ks, double top_p, const float* top_ps, double min_p,
+                const float* min_ps, int32_t* index, float* logp);
+
+/* ------------------------------------------------------------------------
  * Lists of gradients (the designed logits' of several states, a model's
  * parameters'): global norm, clipping, and the Adam update that takes the
  * clipped gradients.  No reference counterpart (the reference leaves them to
