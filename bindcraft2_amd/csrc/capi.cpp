@@ -1416,7 +1416,7 @@ PackedAttn attention_operands(int dtype, int causal, int sequences, int64_t q_to
                               const int32_t* q_lengths, const int32_t* k_lengths) {
   need(dtype == BC2N_F16 || dtype == BC2N_BF16, "attention: f16 or bf16");
   need(sequences >= 0 && sequences <= (1 << 24), "attention: bad number of sequences");
-  need(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536,
+  need(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads < 65536,
        "attention: the heads have to be a multiple of the keys' heads");
   need(width > 0 && width % 8 == 0 && width <= PA_MAX_WIDTH,
        "attention: the width has to be a multiple of 8 up to 128");

@@ -266,28 +266,28 @@ __global__ __launch_bounds__(NT) void headnorm_bwd_kernel(HeadNorm p, int W, flo
   }
   __syncthreads();
   for (int e = threadIdx.x; e < 2 * D; e += NT) {
-    float s = 0.f;
+    double s = 0;
     for (int i = 0; i < WAVES * step; ++i) s += sums[i * 2 * D + e];
-    partial[(int64_t)blockIdx.x * 2 * D + e] = s;
+    partial[(int64_t)blockIdx.x * 2 * D + e] = (float)s;
   }
 }
 
 // d_weight from the workgroups' partial sums, in a fixed order: 16 columns a
 // workgroup, 16 threads a column.
 __global__ __launch_bounds__(NT) void headnorm_join_kernel(HeadNorm p, const float* partial, int parts) {
-  __shared__ float sums[16][17];
+  __shared__ double sums[16][17];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
   const int e = blockIdx.x * 16 + c, D = p.width;
-  float s = 0.f;
+  double s = 0;
   if (e < 2 * D)
     for (int i = r; i < parts; i += 16) s += partial[(int64_t)i * 2 * D + e];
   sums[r][c] = s;
   __syncthreads();
   if (r == 0 && e < 2 * D) {
-    s = 0.f;
+    s = 0;
     for (int i = 0; i < 16; ++i) s += sums[i][c];
     const int k = e >= D;
-    if (p.d_weight[k]) p.d_weight[k][e - k * D] = s;
+    if (p.d_weight[k]) p.d_weight[k][e - k * D] = (float)s;
   }
 }
 

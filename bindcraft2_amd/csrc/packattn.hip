@@ -240,24 +240,32 @@ __device__ __forceinline__ u32x4 descriptor(const void* p, unsigned bytes) {
 }
 constexpr unsigned NOWHERE = 0x80000000u;  // past every descriptor's bounds
 
+// a wave's copies done but the last N
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// all of a wave's LDS reads done: what they read may be written again
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // all of a wave's copies and LDS reads done, and every wave here
 __device__ __forceinline__ void wait_all_and_sync() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// A wave's copies of a [BN][DP] tile by 4 waves: piece w + 4 i.
-template <int DP>
+// A wave's copies of a [ROWS][DP] tile by W waves: piece w + W i.
+template <int DP, int ROWS, int W>
 struct TileCopy {
-  static constexpr int PIECES = BN * DP * 2 / 1024, PER = PIECES / WAVES;
+  static constexpr int PIECES = ROWS * DP * 2 / 1024, PER = PIECES / W;
   static constexpr int CPR = DP / 8;  // chunks a row
   // row and element of lane's chunk of piece i
   static __device__ __forceinline__ int row(int i, int wave, int lane) {
-    return ((wave + WAVES * i) * 64 + lane) / CPR;
+    return ((wave + W * i) * 64 + lane) / CPR;
   }
   static __device__ __forceinline__ int elem(int i, int wave, int lane) {
     return (lane % CPR ^ fswz<DP>(row(i, wave, lane))) * 8;
   }
-  static __device__ __forceinline__ unsigned dst(int i, int wave) { return (wave + WAVES * i) * 1024; }
+  static __device__ __forceinline__ unsigned dst(int i, int wave) { return (wave + W * i) * 1024; }
 };
 
 // rows r0 + l%32, elements 16 ks + 8 (l/32) ..: operand of a contraction over
@@ -345,10 +353,10 @@ __device__ __forceinline__ int wave_max(int v) {
 }
 __device__ __forceinline__ int wave_min(int v) { return -wave_max(-v); }
 
-// Copies of key tile at key k0 (its keys past lk zeros).
-template <class T, int DP>
+// Copies of ROWS keys and their values from key k0 on (past lk zeros), by W waves.
+template <class T, int DP, int ROWS, int W>
 struct KeyTiles {
-  typedef TileCopy<DP> C;
+  typedef TileCopy<DP, ROWS, W> C;
   unsigned ko[C::PER], vo[C::PER];  // a lane's offsets
   const T *k, *v;
   int64_t kst, vst;
@@ -369,17 +377,84 @@ struct KeyTiles {
     }
   }
   __device__ __forceinline__ void issue(int k0, unsigned lds) const {
-    const int rows = min(BN, lk - k0);
+    const int rows = min(ROWS, lk - k0);
     const u32x4 kd = descriptor(k + k0 * kst, (unsigned)((rows - 1) * kst + width) * 2);
     const u32x4 vd = descriptor(v + k0 * vst, (unsigned)((rows - 1) * vst + width) * 2);
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) copy16(ko[i], kd, lds + C::dst(i, wave));
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i) copy16(vo[i], vd, lds + BN * DP * 2 + C::dst(i, wave));
+    for (int i = 0; i < C::PER; ++i) copy16(vo[i], vd, lds + ROWS * DP * 2 + C::dst(i, wave));
   }
 };
 
 // ------------------------------------------------------------------ forward
+// A wave's 32 rows over tiles of 32 NB keys: outputs, sums and exponents'
+// references of a lane's row.
+template <class T, int DP, int NB>
+struct Online {
+  static constexpr int KS = DP / 16, DB = DP / 32;
+  f32x16 o[DB];
+  float ref, mc, sum;  // mc: ref times c; sum: of a lane's own keys
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+    ref = NEG_INF;
+    mc = sum = 0.f;
+  }
+  // last: the last key that the lane's row sees, from the tile's first and its
+  // lane half's; cut: whether some row sees less than the tile
+  __device__ __forceinline__ void tile(unsigned kb0, unsigned vb0, const u32x4 (&q)[KS], float c, int last,
+                                       bool cut, int lane) {
+    f32x16 p[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      p[b] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        p[b] = Half<T>::mma(row_operand<DP>(kb0, 32 * b, ks, lane), q[ks], p[b]);
+    }
+    if (cut) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + 8 * (i / 4) + i % 4 > last) p[b][i] = NEG_INF;
+    }
+    float m = p[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, p[b][i]);
+    m = other_half_max(m);
+    // NaN scores leave m and end in the sum
+    if (__any(m * c > ref * c + LAG || (ref == NEG_INF && m > NEG_INF))) {
+      const float to = fmaxf(ref, m), f = ref == NEG_INF ? 0.f : exp2_f((ref - to) * c);
+      ref = to;
+      mc = ref == NEG_INF ? 0.f : ref * c;
+      sum *= f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] *= f;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[b][i] = exp2_f(fmaf(p[b][i], c, Half<T>::SHIFT - mc));
+        sum += p[b][i];
+      }
+#pragma unroll
+    for (int kg = 0; kg < 2 * NB; ++kg) {
+      const u32x4 w = pack8<T>(p[kg / 2], kg & 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        o[db] = Half<T>::mma(column_operand<DP>(vb0, 16 * kg, db, lane), w, o[db]);
+    }
+  }
+};
+
 // Workgroup = 128 rows of one sequence and head of keys, 4 waves x 32 rows;
 // keys in tiles of 64, two buffers, one barrier a tile.
 template <class T, int DP>
@@ -411,12 +486,10 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
   const float c = a.scale * LOG2E;
-  f32x16 o[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db) o[db] = f32x16{};
-  float ref = NEG_INF, mc = 0.f, sum = 0.f;  // reference of the exponents, times c
+  Online<T, DP, 2> st;
+  st.init();
   const unsigned lds0 = lds_addr(smem);
-  KeyTiles<T, DP> tile;
+  KeyTiles<T, DP, BN, WAVES> tile;
   tile.init(a, seq, at.head, wave, lane);
   if (nk > 0) tile.issue(0, lds0);
 
@@ -426,61 +499,184 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
     wait_all_and_sync();
     if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + (~kt & 1) * 2 * TILE);
     if (k0 > most) continue;
-    f32x16 p[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      p[b] = f32x16{};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        p[b] = Half<T>::mma(row_operand<DP>(kb0, 32 * b, ks, lane), q[ks], p[b]);
-    }
-    if (k0 + BN - 1 > least) {
-      const int last = row.last - k0 - 4 * h;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (32 * b + 8 * (i / 4) + i % 4 > last) p[b][i] = NEG_INF;
-    }
-    float m = p[0][0];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) m = fmaxf(m, p[b][i]);
-    m = other_half_max(m);
-    // NaN scores leave m and end in the sum
-    if (__any(m * c > ref * c + LAG || (ref == NEG_INF && m > NEG_INF))) {
-      const float to = fmaxf(ref, m), f = ref == NEG_INF ? 0.f : exp2_f((ref - to) * c);
-      ref = to;
-      mc = ref == NEG_INF ? 0.f : ref * c;
-      sum *= f;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[db][i] *= f;
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[b][i] = exp2_f(fmaf(p[b][i], c, Half<T>::SHIFT - mc));
-        sum += p[b][i];
-      }
-#pragma unroll
-    for (int kg = 0; kg < 4; ++kg) {
-      const u32x4 w = pack8<T>(p[kg / 2], kg & 1);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-        o[db] = Half<T>::mma(column_operand<DP>(vb0, 16 * kg, db, lane), w, o[db]);
-    }
+    st.tile(kb0, vb0, q, c, row.last - k0 - 4 * h, k0 + BN - 1 > least, lane);
   }
-  sum = other_half_sum(sum);
+  const float sum = other_half_sum(st.sum);
   const bool none = sum == 0.f;
-  store_columns<T, DB>(o, none ? 0.f : 1.f / sum,
+  store_columns<T, DB>(st.o, none ? 0.f : 1.f / sum,
                        row.stored ? row_ptr<T>(a.o, token, head) : nullptr, a.width, lane);
   if (row.stored && h == 0)
     a.lse[(int64_t)head * a.q_tokens + token] =
-        none ? NEG_INF : (mc - Half<T>::SHIFT + log2f(sum)) * LN2;
+        none ? NEG_INF : (st.mc - Half<T>::SHIFT + log2f(sum)) * LN2;
+}
+
+// Few rows: workgroup = 32 rows of one sequence and head of keys and one of
+// `parts` stretches of the sequence's keys, of which each of its 4 waves takes
+// every fourth 32 in two buffers of its own, without a barrier.  The waves
+// join in LDS, the parts in packattn_join_kernel.
+struct Parts {
+  int n;
+  float* o;   // [part][heads][q_tokens][DP], times 1 / (sum of the part's exponents)
+  float2* ml; // [part][heads][q_tokens]: reference in log 2, sum (0: no key)
+};
+template <class T, int DP>
+__global__ __launch_bounds__(NT) void packattn_keys_kernel(PackedAttn a, int64_t tiles, Parts parts) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  constexpr int KN = 32, KS = DP / 16, DB = DP / 32, TILE = KN * DP * 2;
+  const Place at = place<true>(a.kv_heads, tiles);
+  if (at.tile < 0) return;
+  const int G = a.heads / a.kv_heads, part = blockIdx.y;
+  int s;
+  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, 32, at.tile, s);
+  const Seq seq = sequence(a, s, false);
+  const int rows = (a.fill ? seq.have : seq.lq) * G;
+  if (t < 0 || t * 32 >= rows) return;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const Row row = row_of(a, seq, (int)t * 32 + (lane & 31), G);
+  const int head = at.head * G + row.g;
+  const int64_t token = seq.q0 + row.i, at_row = (int64_t)head * a.q_tokens + token;
+  const int most = wave_max(row.last), least = wave_min(row.last);
+  const int blocks = (most + KN) / KN;  // of the keys that a row sees
+  const int per = (blocks + parts.n * WAVES - 1) / (parts.n * WAVES) * WAVES;
+  const int b0 = part * per, b1 = min(b0 + per, blocks);
+  const int64_t at_part = (int64_t)part * a.heads * a.q_tokens + at_row;
+  if (parts.n > 1 && b0 >= b1) {
+    if (wave == 0 && h == 0 && row.stored) parts.ml[at_part] = make_float2(0.f, 0.f);
+    return;
+  }
+  u32x4 q[KS];
+  const T* qrow = row_ptr<const T>(a.q, token, head);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
+  const float c = a.scale * LOG2E;
+  Online<T, DP, 1> st;
+  st.init();
+  const unsigned lds0 = lds_addr(smem) + wave * 4 * TILE;
+  wait_copies<0>();  // q: what follows counts copies alone
+  KeyTiles<T, DP, KN, 1> tile;
+  tile.init(a, seq, at.head, 0, lane);
+  int b = b0 + wave, buf = 0;
+  if (b < b1) tile.issue(b * KN, lds0);
+  for (; b < b1; b += WAVES, buf ^= 1) {
+    wait_reads();
+    if (b + WAVES < b1) {
+      tile.issue((b + WAVES) * KN, lds0 + (buf ^ 1) * 2 * TILE);
+      wait_copies<2 * decltype(tile)::C::PER>();
+    } else {
+      wait_copies<0>();
+    }
+    const unsigned kb0 = lds0 + buf * 2 * TILE;
+    st.tile(kb0, kb0 + TILE, q, c, row.last - b * KN - 4 * h, b * KN + KN - 1 > least, lane);
+  }
+  // the four waves' sums of a row, relative to the largest reference
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(smem);          // [wave][32 rows][DP + 4]
+  float2* sml = reinterpret_cast<float2*>(so + WAVES * 32 * (DP + 4));  // [wave][32]
+  const float sum = other_half_sum(st.sum);
+  if (h == 0) sml[wave * 32 + lane] = make_float2(st.mc, sum);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* p = so + (wave * 32 + (lane & 31)) * (DP + 4) + 32 * db + 8 * i + 4 * h;
+      *reinterpret_cast<float4*>(p) =
+          make_float4(st.o[db][4 * i], st.o[db][4 * i + 1], st.o[db][4 * i + 2], st.o[db][4 * i + 3]);
+    }
+  __syncthreads();
+  // 8 threads a row
+  const int r = threadIdx.x / 8;
+  const Row mine = row_of(a, seq, (int)t * 32 + r, G);
+  const int my_head = at.head * G + mine.g;
+  const int64_t my_token = seq.q0 + mine.i, my_row = (int64_t)my_head * a.q_tokens + my_token;
+  float top = NEG_INF, all = 0.f, f[WAVES];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const float2 v = sml[w * 32 + r];
+    if (!(v.y == 0.f)) top = fmaxf(top, v.x);
+  }
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const float2 v = sml[w * 32 + r];
+    f[w] = v.y == 0.f ? 0.f : exp2_f(v.x - top);
+    all += v.y * f[w];
+  }
+  const bool none = all == 0.f;
+  const float inv = none ? 0.f : 1.f / all;
+  if (!mine.stored) return;
+  for (int e = (threadIdx.x & 7) * 8; e < a.width; e += 64) {
+    float v[8] = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = fmaf(so[(w * 32 + r) * (DP + 4) + e + i], f[w], v[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    if (parts.n == 1) {
+      Vec<T>::store(row_ptr<T>(a.o, my_token, my_head) + e, Vec<T>::pack(v));
+    } else {
+      float4* p = reinterpret_cast<float4*>(parts.o + ((int64_t)part * a.heads * a.q_tokens + my_row) * DP + e);
+      p[0] = make_float4(v[0], v[1], v[2], v[3]);
+      p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  }
+  if ((threadIdx.x & 7) == 0) {
+    if (parts.n == 1) a.lse[my_row] = none ? NEG_INF : (top - Half<T>::SHIFT + log2f(all)) * LN2;
+    else parts.ml[(int64_t)part * a.heads * a.q_tokens + my_row] = make_float2(none ? 0.f : top, all);
+  }
+}
+
+// The parts of a row: workgroup = one row; wave w takes parts w, w + 4 ..,
+// lanes the width.
+template <class T, int DP>
+__global__ __launch_bounds__(NT) void packattn_join_kernel(PackedAttn a, int64_t tiles, Parts parts) {
+  __shared__ float so[WAVES][DP];
+  __shared__ float sl[WAVES];
+  const int G = a.heads / a.kv_heads, at_head = blockIdx.z;
+  int s;
+  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, 32, blockIdx.x, s);
+  const Seq seq = sequence(a, s, false);
+  const int rows = (a.fill ? seq.have : seq.lq) * G;
+  const int64_t r = t * 32 + blockIdx.y;
+  if (t < 0 || r >= rows) return;
+  const Row row = row_of(a, seq, (int)r, G);
+  const int head = at_head * G + row.g;
+  const int64_t token = seq.q0 + row.i, at_row = (int64_t)head * a.q_tokens + token;
+  const int64_t stride = (int64_t)a.heads * a.q_tokens;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float top = NEG_INF;
+  for (int p = lane; p < parts.n; p += 64) {
+    const float2 v = parts.ml[p * stride + at_row];
+    if (!(v.y == 0.f)) top = fmaxf(top, v.x);
+  }
+  top = group_max<64>(top);
+  constexpr int PL = DP < 64 ? 1 : DP / 64;  // elements a lane
+  float v[PL] = {}, all = 0.f;
+  const bool in = lane * PL < DP;
+#pragma unroll 4
+  for (int p = wave; p < parts.n; p += WAVES) {
+    const float2 m = parts.ml[p * stride + at_row];
+    if (m.y == 0.f) continue;
+    const float f = m.y * exp2_f(m.x - top);
+    all += f;
+    if (in && lane * PL < a.width) {
+      float x[PL];
+      Few<float, PL>::template load<false>(parts.o + (p * stride + at_row) * DP + lane * PL, x);
+#pragma unroll
+      for (int i = 0; i < PL; ++i) v[i] = fmaf(x[i], f, v[i]);
+    }
+  }
+  if (in) {
+#pragma unroll
+    for (int i = 0; i < PL; ++i) so[wave][lane * PL + i] = v[i];
+  }
+  if (lane == 0) sl[wave] = all;
+  __syncthreads();
+  all = sl[0] + sl[1] + sl[2] + sl[3];
+  const bool none = all == 0.f;
+  const float inv = none ? 0.f : 1.f / all;
+  const int e = threadIdx.x;
+  if (e < a.width) row_ptr<T>(a.o, token, head)[e] = (T)((so[0][e] + so[1][e] + so[2][e] + so[3][e]) * inv);
+  if (e == 0) a.lse[at_row] = none ? NEG_INF : (top - Half<T>::SHIFT + log2f(all)) * LN2;
 }
 
 // ----------------------------------------------------------------- backward
@@ -597,7 +793,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   const unsigned lds0 = lds_addr(smem);
   // what was loaded above is here before the first copy is issued
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  KeyTiles<T, DP> tile;
+  KeyTiles<T, DP, BN, WAVES> tile;
   tile.init(a, seq, at.head, wave, lane);
   if (nk > 0) tile.issue(0, lds0);
 
@@ -648,7 +844,7 @@ template <class T, int DP>
 __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, const float* delta,
                                                           const float* maxima, int blocks) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  typedef TileCopy<DP> C;
+  typedef TileCopy<DP, BN, WAVES> C;
   constexpr int BK = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
   const Place at = place<false>(a.kv_heads, tiles);
   if (at.tile < 0) return;
@@ -827,7 +1023,44 @@ void with_lds(K* kernel, size_t bytes) {
 
 }  // namespace
 
-size_t packattn_fwd_work_bytes(const PackedAttn&) { return 0; }
+namespace {
+
+// Stretches of the keys for the few-rows kernel, 0 where the other one runs.
+int parts_of(const PackedAttn& a) {
+  const int64_t G = a.heads / a.kv_heads, rows = a.q_tokens * G, cus = device_cus();
+  const int64_t full = std::max((rows + 127) / 128, std::min<int64_t>(a.sequences, a.q_tokens)) * a.kv_heads;
+  const int64_t few = std::max((rows + 31) / 32, std::min<int64_t>(a.sequences, a.q_tokens)) * a.kv_heads;
+  if (few == 0) return 0;  // no rows
+  const bool single = rows <= 32 * (int64_t)a.sequences;  // 32 rows a sequence and fewer
+  if (!single && full >= cus) return 0;
+  const int64_t keys = a.k_tokens / std::max(a.sequences, 1);  // of a sequence on average
+  const int64_t most = std::max<int64_t>(1, keys / 256);
+  return (int)std::min(std::min<int64_t>(most, 256), std::max<int64_t>(1, (4 * cus + few - 1) / few));
+}
+Parts carve(const PackedAttn& a, int n, Carver* c, size_t* bytes) {
+  const int DP = a.width <= 32 ? 32 : a.width <= 64 ? 64 : 128;
+  const size_t rows = (size_t)n * a.heads * a.q_tokens;
+  Parts p = {n, nullptr, nullptr};
+  if (n <= 1) return p;
+  if (c) {
+    p.o = c->take<float>(rows * DP);
+    p.ml = c->take<float2>(rows);
+  } else {
+    Sizer z;
+    z.take<float>(rows * DP);
+    z.take<float2>(rows);
+    *bytes = z.off;
+  }
+  return p;
+}
+
+}  // namespace
+
+size_t packattn_fwd_work_bytes(const PackedAttn& a) {
+  size_t n = 0;
+  carve(a, parts_of(a), nullptr, &n);
+  return n;
+}
 
 size_t packattn_bwd_work_bytes(const PackedAttn& a) {
   Sizer z;
@@ -836,16 +1069,32 @@ size_t packattn_bwd_work_bytes(const PackedAttn& a) {
   return z.off;
 }
 
-void packattn_fwd(hipStream_t st, const PackedAttn& a, void*) {
+void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
   if (a.q_tokens == 0) return;
   KTimed kt("attention.fwd", st);
+  const int64_t G = a.heads / a.kv_heads;
+  const int n = parts_of(a);
+  Carver c(work);
+  const Parts parts = carve(a, n, &c, nullptr);
   by_type(a, [&](auto v, auto dp) {
+    typedef decltype(v) T;
     constexpr int DP = decltype(dp)::value;
-    const int64_t tiles = tiles_of(a.q_tokens, a.heads / a.kv_heads, 32 * WAVES, a.sequences);
-    auto* kernel = &packattn_fwd_kernel<decltype(v), DP>;
-    const size_t lds = 4 * BN * DP * 2;
+    if (n == 0) {
+      const int64_t tiles = tiles_of(a.q_tokens, G, 32 * WAVES, a.sequences);
+      auto* kernel = &packattn_fwd_kernel<T, DP>;
+      const size_t lds = 4 * BN * DP * 2;
+      with_lds(kernel, lds);
+      kernel<<<place_grid(a.kv_heads, tiles), NT, lds, st>>>(a, tiles);
+      return;
+    }
+    const int64_t tiles = tiles_of(a.q_tokens, G, 32, a.sequences);
+    auto* kernel = &packattn_keys_kernel<T, DP>;
+    const size_t copies = WAVES * 4 * 32 * DP * 2, join = WAVES * 32 * ((DP + 4) * 4 + 8);
+    const size_t lds = std::max(copies, join);
     with_lds(kernel, lds);
-    kernel<<<place_grid(a.kv_heads, tiles), NT, lds, st>>>(a, tiles);
+    kernel<<<dim3(place_grid(a.kv_heads, tiles), n), NT, lds, st>>>(a, tiles, parts);
+    if (n > 1)
+      packattn_join_kernel<T, DP><<<dim3((unsigned)tiles, 32, a.kv_heads), NT, 0, st>>>(a, tiles, parts);
   });
 }
 
