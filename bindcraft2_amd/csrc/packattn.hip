@@ -156,6 +156,7 @@ __device__ __forceinline__ int64_t find_tile(const int32_t* off, int B, int64_t 
   return uniform64(x - first(s));
 }
 
+// entry s: a sequence, or the tokens outside all
 __device__ __forceinline__ Seq sequence(const PackedAttn& a, int s, bool keys) {
   const int B = a.sequences;
   Seq r = {};
@@ -174,11 +175,20 @@ __device__ __forceinline__ Seq sequence(const PackedAttn& a, int s, bool keys) {
   if (a.k_len) lk = min(lk, max(a.k_len[s - 1], 0));
   r.lq = lq;
   r.lk = lk;
-  r.q0 = uniform64(r.q0);
-  r.k0 = uniform64(r.k0);
-  r.lq = uniform(r.lq);
-  r.lk = uniform(r.lk);
-  r.have = uniform(r.have);
+  return r;
+}
+
+__device__ __forceinline__ int64_t lane64(int64_t v, int lane) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32);
+}
+__device__ __forceinline__ Seq lane_seq(const Seq& s, int lane) {
+  Seq r;
+  r.q0 = lane64(s.q0, lane);
+  r.k0 = lane64(s.k0, lane);
+  r.lq = __builtin_amdgcn_readlane(s.lq, lane);
+  r.lk = __builtin_amdgcn_readlane(s.lk, lane);
+  r.have = __builtin_amdgcn_readlane(s.have, lane);
   return r;
 }
 
@@ -376,14 +386,21 @@ struct KeyTiles {
       vo[i] = e < width ? (unsigned)(r * vst + e) * 2 : NOWHERE;
     }
   }
-  __device__ __forceinline__ void issue(int k0, unsigned lds) const {
+  __device__ __forceinline__ void keys(int k0, unsigned lds) const {
     const int rows = min(ROWS, lk - k0);
-    const u32x4 kd = descriptor(k + k0 * kst, (unsigned)((rows - 1) * kst + width) * 2);
-    const u32x4 vd = descriptor(v + k0 * vst, (unsigned)((rows - 1) * vst + width) * 2);
+    const u32x4 d = descriptor(k + k0 * kst, (unsigned)((rows - 1) * kst + width) * 2);
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i) copy16(ko[i], kd, lds + C::dst(i, wave));
+    for (int i = 0; i < C::PER; ++i) copy16(ko[i], d, lds + C::dst(i, wave));
+  }
+  __device__ __forceinline__ void values(int k0, unsigned lds) const {
+    const int rows = min(ROWS, lk - k0);
+    const u32x4 d = descriptor(v + k0 * vst, (unsigned)((rows - 1) * vst + width) * 2);
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i) copy16(vo[i], vd, lds + ROWS * DP * 2 + C::dst(i, wave));
+    for (int i = 0; i < C::PER; ++i) copy16(vo[i], d, lds + C::dst(i, wave));
+  }
+  __device__ __forceinline__ void issue(int k0, unsigned lds) const {
+    keys(k0, lds);
+    values(k0, lds + ROWS * DP * 2);
   }
 };
 
@@ -402,11 +419,8 @@ struct Online {
     ref = NEG_INF;
     mc = sum = 0.f;
   }
-  // last: the last key that the lane's row sees, from the tile's first and its
-  // lane half's; cut: whether some row sees less than the tile
-  __device__ __forceinline__ void tile(unsigned kb0, unsigned vb0, const u32x4 (&q)[KS], float c, int last,
-                                       bool cut, int lane) {
-    f32x16 p[NB];
+  // S^T of a tile whose keys lie at kb0
+  static __device__ __forceinline__ void scores(f32x16 (&p)[NB], unsigned kb0, const u32x4 (&q)[KS], int lane) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       p[b] = f32x16{};
@@ -414,6 +428,11 @@ struct Online {
       for (int ks = 0; ks < KS; ++ks)
         p[b] = Half<T>::mma(row_operand<DP>(kb0, 32 * b, ks, lane), q[ks], p[b]);
     }
+  }
+  // their exponents in place.  last: the last key that the lane's row sees, from
+  // the tile's first and its lane half's; cut: whether some row sees less than
+  // the tile
+  __device__ __forceinline__ void weights(f32x16 (&p)[NB], float c, int last, bool cut) {
     if (cut) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -445,6 +464,9 @@ struct Online {
         p[b][i] = exp2_f(fmaf(p[b][i], c, Half<T>::SHIFT - mc));
         sum += p[b][i];
       }
+  }
+  // o^T += V^T P^T, the values at vb0
+  __device__ __forceinline__ void values(const f32x16 (&p)[NB], unsigned vb0, int lane) {
 #pragma unroll
     for (int kg = 0; kg < 2 * NB; ++kg) {
       const u32x4 w = pack8<T>(p[kg / 2], kg & 1);
@@ -466,7 +488,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
   const int G = a.heads / a.kv_heads;
   int s;
   const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, at.tile, s);
-  const Seq seq = sequence(a, s, false);
+  const Seq seq = lane_seq(sequence(a, s, false), 0);
   const int rows = (a.fill ? seq.have : seq.lq) * G;
   if (t < 0 || t * BM >= rows) return;
   const int r0 = (int)t * BM;
@@ -499,7 +521,10 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
     wait_all_and_sync();
     if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + (~kt & 1) * 2 * TILE);
     if (k0 > most) continue;
-    st.tile(kb0, vb0, q, c, row.last - k0 - 4 * h, k0 + BN - 1 > least, lane);
+    f32x16 p[2];
+    st.scores(p, kb0, q, lane);
+    st.weights(p, c, row.last - k0 - 4 * h, k0 + BN - 1 > least);
+    st.values(p, vb0, lane);
   }
   const float sum = other_half_sum(st.sum);
   const bool none = sum == 0.f;
@@ -510,173 +535,337 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
         none ? NEG_INF : (st.mc - Half<T>::SHIFT + log2f(sum)) * LN2;
 }
 
-// Few rows: workgroup = 32 rows of one sequence and head of keys and one of
-// `parts` stretches of the sequence's keys, of which each of its 4 waves takes
-// every fourth 32 in two buffers of its own, without a barrier.  The waves
-// join in LDS, the parts in packattn_join_kernel.
-struct Parts {
-  int n;
-  float* o;   // [part][heads][q_tokens][DP], times 1 / (sum of the part's exponents)
-  float2* ml; // [part][heads][q_tokens]: reference in log 2, sum (0: no key)
+// Few rows (single tokens against caches, short chains): a workgroup takes 32
+// rows of one sequence and head of keys with a stretch of the sequence's keys, in
+// blocks of 32 or 64.
+//
+// W = 1, long caches: a wave by itself is a workgroup.  What bounds it is the
+// keys and values read once, so every stretch has to be as long as the others,
+// whatever the sequences' lengths, and the card full of copies in flight: each
+// wave adds up all sequences' blocks, which gives the length of a stretch for
+// `goal` equal ones a head, and finds its own among them.  A wave has one
+// buffer of keys and one of values, and refills each as soon as it is read, so
+// that nearly all of the LDS is in flight nearly all of the time.  Rows of more
+// than one stretch go to packattn_join_kernel through memory.
+// W = 4, few keys: all of a sequence's by one workgroup, every fourth block a
+// wave, joined in LDS: no second launch.
+struct Split {
+  float* o;    // [slot][32 rows][DP], sums of exponents times values
+  float2* ml;  // [slot][32]: reference in log 2, sum of exponents
 };
-template <class T, int DP>
-__global__ __launch_bounds__(NT) void packattn_keys_kernel(PackedAttn a, int64_t tiles, Parts parts) {
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  constexpr int KN = 32, KS = DP / 16, DB = DP / 32, TILE = KN * DP * 2;
-  const Place at = place<true>(a.kv_heads, tiles);
-  if (at.tile < 0) return;
-  const int G = a.heads / a.kv_heads, part = blockIdx.y;
-  int s;
-  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, 32, at.tile, s);
-  const Seq seq = sequence(a, s, false);
-  const int rows = (a.fill ? seq.have : seq.lq) * G;
-  if (t < 0 || t * 32 >= rows) return;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
-  const Row row = row_of(a, seq, (int)t * 32 + (lane & 31), G);
-  const int head = at.head * G + row.g;
-  const int64_t token = seq.q0 + row.i, at_row = (int64_t)head * a.q_tokens + token;
-  const int most = wave_max(row.last), least = wave_min(row.last);
-  const int blocks = (most + KN) / KN;  // of the keys that a row sees
-  const int per = (blocks + parts.n * WAVES - 1) / (parts.n * WAVES) * WAVES;
-  const int b0 = part * per, b1 = min(b0 + per, blocks);
-  const int64_t at_part = (int64_t)part * a.heads * a.q_tokens + at_row;
-  if (parts.n > 1 && b0 >= b1) {
-    if (wave == 0 && h == 0 && row.stored) parts.ml[at_part] = make_float2(0.f, 0.f);
-    return;
-  }
-  u32x4 q[KS];
-  const T* qrow = row_ptr<const T>(a.q, token, head);
+// keys of a block: 16 KB of keys and values at the widths 64 and 128
+__host__ __device__ constexpr int block_keys(int DP) { return DP == 128 ? 32 : 64; }
+constexpr int SHORTEST = 256;  // keys of a stretch at least
+
+struct Item {
+  Seq seq;
+  int tile;         // of 32 rows
+  int part, parts;  // stretch, of how many
+  int64_t slot;     // of the tile's first stretch (parts > 1)
+  int per;          // blocks of a stretch
+};
+// An entry (sequence, or the tokens outside) as one lane sees it.
+struct Entry {
+  Seq seq;
+  int tiles, blocks;
+};
+template <int KN>
+__device__ __forceinline__ Entry entry_of(const PackedAttn& a, int e, int G) {
+  Entry r = {};
+  if (e >= a.sequences + 2) return r;
+  r.seq = sequence(a, e, false);
+  r.tiles = (int)(((int64_t)(a.fill ? r.seq.have : r.seq.lq) * G + 31) / 32);
+  r.blocks = r.seq.lq > 0 ? (r.seq.lk + KN - 1) / KN : 0;
+  return r;
+}
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
+  for (int i = 1; i < 64; i *= 2) v += __shfl_xor(v, i, 64);
+  return v;
+}
+// what the lanes before this one have
+__device__ __forceinline__ int64_t wave_before(int64_t v, int lane) {
+  int64_t run = v;
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) {
+    const int64_t o = __shfl_up(run, i, 64);
+    if (lane >= i) run += o;
+  }
+  return run - v;
+}
+// The wave's view of all sequences: what the first 64 HELD entries come to stays
+// in its lanes, more are read again at each search.
+template <int KN>
+struct Stretches {
+  static constexpr int HELD = 4;
+  int tiles[HELD], blocks[HELD];  // of entry 64 i + lane
+  int per, G, lane, entries;
+
+  __device__ __forceinline__ void init(const PackedAttn& a, int G_, int64_t goal) {
+    G = G_;
+    lane = threadIdx.x & 63;
+    entries = a.sequences + 2;
+    int64_t work = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      const Entry x = entry_of<KN>(a, 64 * i + lane, G);
+      tiles[i] = x.tiles;
+      blocks[i] = x.blocks;
+      work += (int64_t)x.tiles * x.blocks;
+      all += x.tiles;
+    }
+    for (int e = 64 * HELD + lane; e - lane < entries; e += 64) {
+      const Entry x = entry_of<KN>(a, e, G);
+      work += (int64_t)x.tiles * x.blocks;
+      all += x.tiles;
+    }
+    work = wave_sum64(work);
+    all = wave_sum64(all);
+    // every tile may end in a short stretch: with those too one round of waves
+    // (64 sequences of 11 .. 8192 keys, 8 heads of 128: 70.5 -> 60 us)
+    if (all < goal / 2) goal -= all;
+    per = uniform((int)max((int64_t)(SHORTEST / KN), (work + goal - 1) / goal));
+  }
+  // Item x of all (SPLIT: tile x of those with more stretches than one);
+  // false past the last.
+  template <bool SPLIT>
+  __device__ __forceinline__ bool find(const PackedAttn& a, int64_t x, Item& r) const {
+    int64_t slots = 0;
+    auto look = [&](int e0, int tiles_, int blocks_) {
+      const int parts = max(1, (blocks_ + per - 1) / per);
+      const int64_t n = SPLIT ? (parts > 1 ? tiles_ : 0) : (int64_t)tiles_ * parts;
+      const int64_t before = wave_before(n, lane), s = parts > 1 ? (int64_t)tiles_ * parts : 0;
+      const unsigned long long at = __ballot(before <= x && x < before + n);
+      if (at) {
+        const int l = uniform(__ffsll(at) - 1);
+        const int64_t y = x - lane64(before, l);
+        r.seq = lane_seq(sequence(a, e0 + l, false), 0);
+        r.parts = __builtin_amdgcn_readlane(parts, l);
+        r.tile = (int)(SPLIT ? y : y / r.parts);
+        r.part = (int)(SPLIT ? 0 : y % r.parts);
+        r.slot = slots + lane64(wave_before(s, lane), l) + (int64_t)r.tile * r.parts;
+        r.per = per;
+        return true;
+      }
+      x -= wave_sum64(n);
+      slots += wave_sum64(s);
+      return false;
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (64 * i < entries && look(64 * i, tiles[i], blocks[i])) return true;
+    for (int e0 = 64 * HELD; e0 < entries; e0 += 64) {
+      const Entry m = entry_of<KN>(a, e0 + lane, G);
+      if (look(e0, m.tiles, m.blocks)) return true;
+    }
+    return false;
+  }
+};
+
+template <class T, int DP, int W>
+__global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, int64_t goal, Split split) {
+  constexpr int KN = block_keys(DP), KS = DP / 16, DB = DP / 32, TILE = KN * DP * 2, LD = DP + 4;
+  constexpr int JOIN = W > 1 ? W * 32 * (LD * 4 + 8) : 0;
+  constexpr int LDS = W * 2 * TILE > JOIN ? W * 2 * TILE : JOIN;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[LDS];
+  const int G = a.heads / a.kv_heads, lane = threadIdx.x & 63, h = lane >> 5;
+  const int wave = W > 1 ? uniform(threadIdx.x >> 6) : 0;
+  Stretches<KN> all;
+  all.init(a, G, goal);
+  const unsigned kb = lds_addr(smem) + wave * 2 * TILE, vb = kb + TILE;
   const float c = a.scale * LOG2E;
-  Online<T, DP, 1> st;
-  st.init();
-  const unsigned lds0 = lds_addr(smem) + wave * 4 * TILE;
-  wait_copies<0>();  // q: what follows counts copies alone
-  KeyTiles<T, DP, KN, 1> tile;
-  tile.init(a, seq, at.head, 0, lane);
-  int b = b0 + wave, buf = 0;
-  if (b < b1) tile.issue(b * KN, lds0);
-  for (; b < b1; b += WAVES, buf ^= 1) {
+  typedef KeyTiles<T, DP, KN, 1> Tiles;
+  Item it;
+  for (int64_t x = blockIdx.x; all.template find<false>(a, x / a.kv_heads, it); x += gridDim.x) {
+    const int kv = (int)(x % a.kv_heads);
+    const Seq& seq = it.seq;
+    const Row row = row_of(a, seq, it.tile * 32 + (lane & 31), G);
+    const int head = kv * G + row.g;
+    const int64_t token = seq.q0 + row.i;
+    const int most = wave_max(row.last), least = wave_min(row.last);
+    const int b0 = it.part * it.per, b1 = min(b0 + it.per, (most + KN) / KN);
+    u32x4 q[KS];
+    const T* qrow = row_ptr<const T>(a.q, token, head);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
+    Online<T, DP, KN / 32> st;
+    st.init();
+    Tiles tile;
+    tile.init(a, seq, kv, 0, lane);
     wait_reads();
-    if (b + WAVES < b1) {
-      tile.issue((b + WAVES) * KN, lds0 + (buf ^ 1) * 2 * TILE);
-      wait_copies<2 * decltype(tile)::C::PER>();
-    } else {
-      wait_copies<0>();
+    wait_copies<0>();  // q: what follows counts copies alone
+    int b = b0 + wave;
+    if (b < b1) {
+      tile.keys(b * KN, kb);
+      tile.values(b * KN, vb);
     }
-    const unsigned kb0 = lds0 + buf * 2 * TILE;
-    st.tile(kb0, kb0 + TILE, q, c, row.last - b * KN - 4 * h, b * KN + KN - 1 > least, lane);
-  }
-  // the four waves' sums of a row, relative to the largest reference
-  __syncthreads();
-  float* so = reinterpret_cast<float*>(smem);          // [wave][32 rows][DP + 4]
-  float2* sml = reinterpret_cast<float2*>(so + WAVES * 32 * (DP + 4));  // [wave][32]
-  const float sum = other_half_sum(st.sum);
-  if (h == 0) sml[wave * 32 + lane] = make_float2(st.mc, sum);
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float* p = so + (wave * 32 + (lane & 31)) * (DP + 4) + 32 * db + 8 * i + 4 * h;
-      *reinterpret_cast<float4*>(p) =
-          make_float4(st.o[db][4 * i], st.o[db][4 * i + 1], st.o[db][4 * i + 2], st.o[db][4 * i + 3]);
+    for (; b < b1; b += W) {
+      const bool more = b + W < b1;
+      wait_copies<Tiles::C::PER>();  // the keys are here, the values on their way
+      f32x16 p[KN / 32];
+      st.scores(p, kb, q, lane);
+      wait_reads();
+      if (more) tile.keys((b + W) * KN, kb);
+      st.weights(p, c, row.last - b * KN - 4 * h, b * KN + KN - 1 > least);
+      if (more) wait_copies<Tiles::C::PER>();
+      else wait_copies<0>();
+      st.values(p, vb, lane);
+      wait_reads();
+      if (more) tile.values((b + W) * KN, vb);
     }
-  __syncthreads();
-  // 8 threads a row
-  const int r = threadIdx.x / 8;
-  const Row mine = row_of(a, seq, (int)t * 32 + r, G);
-  const int my_head = at.head * G + mine.g;
-  const int64_t my_token = seq.q0 + mine.i, my_row = (int64_t)my_head * a.q_tokens + my_token;
-  float top = NEG_INF, all = 0.f, f[WAVES];
+    const float sum = other_half_sum(st.sum);
+    if constexpr (W > 1) {
+      // the waves' sums of a row, relative to the largest reference
+      __syncthreads();
+      float* so = reinterpret_cast<float*>(smem);                 // [wave][32 rows][LD]
+      float2* sml = reinterpret_cast<float2*>(so + W * 32 * LD);  // [wave][32]
+      if (h == 0) sml[wave * 32 + lane] = make_float2(st.mc, sum);
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const float2 v = sml[w * 32 + r];
-    if (!(v.y == 0.f)) top = fmaxf(top, v.x);
-  }
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const float2 v = sml[w * 32 + r];
-    f[w] = v.y == 0.f ? 0.f : exp2_f(v.x - top);
-    all += v.y * f[w];
-  }
-  const bool none = all == 0.f;
-  const float inv = none ? 0.f : 1.f / all;
-  if (!mine.stored) return;
-  for (int e = (threadIdx.x & 7) * 8; e < a.width; e += 64) {
-    float v[8] = {};
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(so + (wave * 32 + (lane & 31)) * LD + 32 * db + 8 * i + 4 * h) =
+              make_float4(st.o[db][4 * i], st.o[db][4 * i + 1], st.o[db][4 * i + 2], st.o[db][4 * i + 3]);
+      __syncthreads();
+      constexpr int PER_ROW = 2 * W;  // threads a row
+      const int r = threadIdx.x / PER_ROW, part = threadIdx.x % PER_ROW;
+      const Row mine = row_of(a, seq, it.tile * 32 + r, G);
+      const int my_head = kv * G + mine.g;
+      const int64_t my_token = seq.q0 + mine.i;
+      float top = NEG_INF, l = 0.f, f[W];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w)
+      for (int w = 0; w < W; ++w) {
+        const float2 v = sml[w * 32 + r];
+        if (!(v.y == 0.f)) top = fmaxf(top, v.x);
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf(so[(w * 32 + r) * (DP + 4) + e + i], f[w], v[i]);
+      for (int w = 0; w < W; ++w) {
+        const float2 v = sml[w * 32 + r];
+        f[w] = v.y == 0.f ? 0.f : exp2_f(v.x - top);
+        l += v.y * f[w];
+      }
+      const bool none = l == 0.f;
+      const float inv = none ? 0.f : 1.f / l;
+      if (mine.stored) {
+        for (int e = part * 8; e < a.width; e += PER_ROW * 8) {
+          float v[8] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inv;
-    if (parts.n == 1) {
-      Vec<T>::store(row_ptr<T>(a.o, my_token, my_head) + e, Vec<T>::pack(v));
-    } else {
-      float4* p = reinterpret_cast<float4*>(parts.o + ((int64_t)part * a.heads * a.q_tokens + my_row) * DP + e);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
+          for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(so[(w * 32 + r) * LD + e + i], f[w], v[i]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= inv;
+          Vec<T>::store(row_ptr<T>(a.o, my_token, my_head) + e, Vec<T>::pack(v));
+        }
+        if (part == 0)
+          a.lse[(int64_t)my_head * a.q_tokens + my_token] =
+              none ? NEG_INF : (top - Half<T>::SHIFT + log2f(l)) * LN2;
+      }
+      __syncthreads();
+    } else if (it.parts == 1) {
+      const bool none = sum == 0.f;
+      store_columns<T, DB>(st.o, none ? 0.f : 1.f / sum,
+                           row.stored ? row_ptr<T>(a.o, token, head) : nullptr, a.width, lane);
+      if (row.stored && h == 0)
+        a.lse[(int64_t)head * a.q_tokens + token] =
+            none ? NEG_INF : (st.mc - Half<T>::SHIFT + log2f(sum)) * LN2;
+    } else if (row.stored) {
+      const int64_t at = ((it.slot + it.part) * a.kv_heads + kv) * 32 + (lane & 31);
+      if (h == 0) split.ml[at] = make_float2(st.mc, sum);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(split.o + at * DP + 32 * db + 8 * i + 4 * h) =
+              make_float4(st.o[db][4 * i], st.o[db][4 * i + 1], st.o[db][4 * i + 2], st.o[db][4 * i + 3]);
     }
-  }
-  if ((threadIdx.x & 7) == 0) {
-    if (parts.n == 1) a.lse[my_row] = none ? NEG_INF : (top - Half<T>::SHIFT + log2f(all)) * LN2;
-    else parts.ml[(int64_t)part * a.heads * a.q_tokens + my_row] = make_float2(none ? 0.f : top, all);
   }
 }
 
-// The parts of a row: workgroup = one row; wave w takes parts w, w + 4 ..,
-// lanes the width.
-template <class T, int DP>
-__global__ __launch_bounds__(NT) void packattn_join_kernel(PackedAttn a, int64_t tiles, Parts parts) {
-  __shared__ float so[WAVES][DP];
-  __shared__ float sl[WAVES];
-  const int G = a.heads / a.kv_heads, at_head = blockIdx.z;
-  int s;
-  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, 32, blockIdx.x, s);
-  const Seq seq = sequence(a, s, false);
-  const int rows = (a.fill ? seq.have : seq.lq) * G;
-  const int64_t r = t * 32 + blockIdx.y;
-  if (t < 0 || r >= rows) return;
-  const Row row = row_of(a, seq, (int)r, G);
-  const int head = at_head * G + row.g;
-  const int64_t token = seq.q0 + row.i, at_row = (int64_t)head * a.q_tokens + token;
-  const int64_t stride = (int64_t)a.heads * a.q_tokens;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float top = NEG_INF;
-  for (int p = lane; p < parts.n; p += 64) {
-    const float2 v = parts.ml[p * stride + at_row];
-    if (!(v.y == 0.f)) top = fmaxf(top, v.x);
-  }
-  top = group_max<64>(top);
-  constexpr int PL = DP < 64 ? 1 : DP / 64;  // elements a lane
-  float v[PL] = {}, all = 0.f;
-  const bool in = lane * PL < DP;
-#pragma unroll 4
-  for (int p = wave; p < parts.n; p += WAVES) {
-    const float2 m = parts.ml[p * stride + at_row];
-    if (m.y == 0.f) continue;
-    const float f = m.y * exp2_f(m.x - top);
-    all += f;
-    if (in && lane * PL < a.width) {
-      float x[PL];
-      Few<float, PL>::template load<false>(parts.o + (p * stride + at_row) * DP + lane * PL, x);
+// The stretches of rows, RW waves a row: DP / 4 lanes a stretch, each lane group
+// with a reference of its own.
+template <class T, int DP, int RW>
+__global__ __launch_bounds__(RW > 1 ? 64 * RW : NT) void packattn_join_kernel(PackedAttn a, int64_t goal, Split split) {
+  constexpr int KN = block_keys(DP), LP = DP / 4, ROWS = RW > 1 ? 1 : WAVES, GROUPS = 64 * RW / LP;
+  __shared__ float so[ROWS][RW][DP];
+  __shared__ float2 sml[ROWS][RW];
+  const int G = a.heads / a.kv_heads;
+  Stretches<KN> all;
+  all.init(a, G, goal);
+  const int mine = threadIdx.x / (64 * RW), t = threadIdx.x % (64 * RW);
+  const int group = t / LP, e = t % LP * 4;
+  Item it;
+  for (int64_t x = blockIdx.x; all.template find<true>(a, x / a.kv_heads, it); x += gridDim.x) {
+    const int kv = (int)(x % a.kv_heads);
+    for (int r0 = blockIdx.y * ROWS; r0 < 32; r0 += gridDim.y * ROWS) {
+      if (!row_of(a, it.seq, it.tile * 32 + r0, G).stored) break;
+      const int r = r0 + mine;
+      const Row row = row_of(a, it.seq, it.tile * 32 + r, G);
+      const int64_t stride = (int64_t)a.kv_heads * 32, at = (it.slot * a.kv_heads + kv) * 32 + r;
+      float top = NEG_INF, sum = 0.f;
+      f32x4 v = {};
+      auto add = [&](float2 m, f32x4 o) __attribute__((always_inline)) {
+        const float to = fmaxf(top, m.x), f = top == NEG_INF ? 0.f : exp2_f(top - to);
+        const float g = exp2_f(m.x - to);
+        top = to;
+        sum = fmaf(sum, f, m.y * g);
 #pragma unroll
-      for (int i = 0; i < PL; ++i) v[i] = fmaf(x[i], f, v[i]);
+        for (int k = 0; k < 4; ++k) v[k] = fmaf(v[k], f, o[k] * g);
+      };
+      for (int p = group; p < it.parts && row.stored; p += 4 * GROUPS) {
+        float2 m[4];
+        f32x4 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // in flight together
+          const int64_t s = at + min(p + i * GROUPS, it.parts - 1) * stride;
+          m[i] = split.ml[s];
+          o[i] = *reinterpret_cast<const f32x4*>(split.o + s * DP + e);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (p + i * GROUPS >= it.parts || m[i].y == 0.f) continue;
+          add(m[i], o[i]);
+        }
+      }
+      // the lane groups of a wave, then the waves
+#pragma unroll
+      for (int i = LP; i < 64; i *= 2) {
+        f32x4 o;
+        const float2 m = make_float2(__shfl_xor(top, i, 64), __shfl_xor(sum, i, 64));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = __shfl_xor(v[k], i, 64);
+        if (!(m.y == 0.f)) add(m, o);
+      }
+      if constexpr (RW > 1) {
+        __syncthreads();
+        if (t % 64 < LP) *reinterpret_cast<float4*>(&so[mine][t / 64][e]) = make_float4(v[0], v[1], v[2], v[3]);
+        if (t % 64 == 0) sml[mine][t / 64] = make_float2(top, sum);
+        __syncthreads();
+        top = NEG_INF;
+        sum = 0.f;
+        v = f32x4{};
+        if (t < LP) {
+#pragma unroll 4
+          for (int i = 0; i < RW; ++i) {
+            const float2 m = sml[mine][i];
+            const float4 o = *reinterpret_cast<const float4*>(&so[mine][i][e]);
+            if (!(m.y == 0.f)) add(m, f32x4{o.x, o.y, o.z, o.w});
+          }
+        }
+      }
+      if (t < LP && row.stored) {
+        const bool none = sum == 0.f;
+        const float inv = none ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] *= inv;
+        const float w[4] = {v[0], v[1], v[2], v[3]};
+        if (e < a.width) Few<T, 4>::template store<false>(row_ptr<T>(a.o, it.seq.q0 + row.i, kv * G + row.g) + e, w);
+        if (t == 0)
+          a.lse[(int64_t)(kv * G + row.g) * a.q_tokens + it.seq.q0 + row.i] =
+              none ? NEG_INF : (top - Half<T>::SHIFT + log2f(sum)) * LN2;
+      }
     }
   }
-  if (in) {
-#pragma unroll
-    for (int i = 0; i < PL; ++i) so[wave][lane * PL + i] = v[i];
-  }
-  if (lane == 0) sl[wave] = all;
-  __syncthreads();
-  all = sl[0] + sl[1] + sl[2] + sl[3];
-  const bool none = all == 0.f;
-  const float inv = none ? 0.f : 1.f / all;
-  const int e = threadIdx.x;
-  if (e < a.width) row_ptr<T>(a.o, token, head)[e] = (T)((so[0][e] + so[1][e] + so[2][e] + so[3][e]) * inv);
-  if (e == 0) a.lse[at_row] = none ? NEG_INF : (top - Half<T>::SHIFT + log2f(all)) * LN2;
 }
 
 // ----------------------------------------------------------------- backward
@@ -752,7 +941,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   const int G = a.heads / a.kv_heads;
   int s;
   const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, at.tile, s);
-  const Seq seq = sequence(a, s, false);
+  const Seq seq = lane_seq(sequence(a, s, false), 0);
   const int rows = (a.fill ? seq.have : seq.lq) * G;
   if (t < 0 || t * BM >= rows) return;
   const int r0 = (int)t * BM;
@@ -851,7 +1040,7 @@ __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t 
   const int G = a.heads / a.kv_heads;
   int s;
   const int64_t t = find_tile(a.k_off, a.sequences, a.k_tokens, 1, BK, at.tile, s);
-  const Seq seq = sequence(a, s, true);
+  const Seq seq = lane_seq(sequence(a, s, true), 0);
   const int have = a.fill ? seq.have : seq.lk;
   if (t < 0 || t * BK >= have) return;
   const int j0 = (int)t * BK;
@@ -1025,40 +1214,40 @@ void with_lds(K* kernel, size_t bytes) {
 
 namespace {
 
-// Stretches of the keys for the few-rows kernel, 0 where the other one runs.
-int parts_of(const PackedAttn& a) {
-  const int64_t G = a.heads / a.kv_heads, rows = a.q_tokens * G, cus = device_cus();
-  const int64_t full = std::max((rows + 127) / 128, std::min<int64_t>(a.sequences, a.q_tokens)) * a.kv_heads;
-  const int64_t few = std::max((rows + 31) / 32, std::min<int64_t>(a.sequences, a.q_tokens)) * a.kv_heads;
-  if (few == 0) return 0;  // no rows
-  const bool single = rows <= 32 * (int64_t)a.sequences;  // 32 rows a sequence and fewer
-  if (!single && full >= cus) return 0;
-  const int64_t keys = a.k_tokens / std::max(a.sequences, 1);  // of a sequence on average
-  const int64_t most = std::max<int64_t>(1, keys / 256);
-  return (int)std::min(std::min<int64_t>(most, 256), std::max<int64_t>(1, (4 * cus + few - 1) / few));
+int padded(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : 128; }
+
+// Whether the rows go to the few-rows kernel: where a sequence has 32 rows or
+// fewer, or 128-row workgroups would leave compute units idle.
+bool few_rows(const PackedAttn& a) {
+  const int64_t rows = a.q_tokens * (a.heads / a.kv_heads);
+  const int64_t live = std::min<int64_t>(a.sequences, a.q_tokens);
+  return rows <= 32 * live || std::max((rows + 127) / 128, live) * a.kv_heads < device_cus();
 }
-Parts carve(const PackedAttn& a, int n, Carver* c, size_t* bytes) {
-  const int DP = a.width <= 32 ? 32 : a.width <= 64 ? 64 : 128;
-  const size_t rows = (size_t)n * a.heads * a.q_tokens;
-  Parts p = {n, nullptr, nullptr};
-  if (n <= 1) return p;
-  if (c) {
-    p.o = c->take<float>(rows * DP);
-    p.ml = c->take<float2>(rows);
-  } else {
-    Sizer z;
-    z.take<float>(rows * DP);
-    z.take<float2>(rows);
-    *bytes = z.off;
-  }
-  return p;
+// Waves of it that the card holds, by their registers.
+int64_t few_grid(const PackedAttn&) { return (int64_t)device_cus() * 8; }
+// Stretches of a head of keys that fill it once.  A sequence with more than
+// one has more blocks than a stretch, so all of those have at most twice as many.
+int64_t few_goal(const PackedAttn& a) { return std::max<int64_t>(1, few_grid(a) / a.kv_heads); }
+Split carve_split(const PackedAttn& a, char* p, size_t* bytes) {
+  const size_t rows = (size_t)2 * few_goal(a) * a.kv_heads * 32;
+  Split s;
+  Sizer z;
+  s.o = reinterpret_cast<float*>(p);
+  z.take<float>(rows * padded(a.width));
+  s.ml = reinterpret_cast<float2*>(p + z.off);
+  z.take<float2>(rows);
+  *bytes = z.off;
+  return s;
 }
+// Up to so many keys of all sequences one workgroup takes any sequence's.
+constexpr int64_t UNSPLIT = 4096;
+bool may_split(const PackedAttn& a) { return a.q_tokens > 0 && few_rows(a) && a.k_tokens > UNSPLIT; }
 
 }  // namespace
 
 size_t packattn_fwd_work_bytes(const PackedAttn& a) {
   size_t n = 0;
-  carve(a, parts_of(a), nullptr, &n);
+  if (may_split(a)) carve_split(a, nullptr, &n);
   return n;
 }
 
@@ -1073,13 +1262,10 @@ void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
   if (a.q_tokens == 0) return;
   KTimed kt("attention.fwd", st);
   const int64_t G = a.heads / a.kv_heads;
-  const int n = parts_of(a);
-  Carver c(work);
-  const Parts parts = carve(a, n, &c, nullptr);
   by_type(a, [&](auto v, auto dp) {
     typedef decltype(v) T;
     constexpr int DP = decltype(dp)::value;
-    if (n == 0) {
+    if (!few_rows(a)) {
       const int64_t tiles = tiles_of(a.q_tokens, G, 32 * WAVES, a.sequences);
       auto* kernel = &packattn_fwd_kernel<T, DP>;
       const size_t lds = 4 * BN * DP * 2;
@@ -1088,13 +1274,25 @@ void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
       return;
     }
     const int64_t tiles = tiles_of(a.q_tokens, G, 32, a.sequences);
-    auto* kernel = &packattn_keys_kernel<T, DP>;
-    const size_t copies = WAVES * 4 * 32 * DP * 2, join = WAVES * 32 * ((DP + 4) * 4 + 8);
-    const size_t lds = std::max(copies, join);
-    with_lds(kernel, lds);
-    kernel<<<dim3(place_grid(a.kv_heads, tiles), n), NT, lds, st>>>(a, tiles, parts);
-    if (n > 1)
-      packattn_join_kernel<T, DP><<<dim3((unsigned)tiles, 32, a.kv_heads), NT, 0, st>>>(a, tiles, parts);
+    if (!may_split(a)) {
+      const int64_t items = std::min(tiles * a.kv_heads, 4 * (int64_t)device_cus());
+      packattn_keys_kernel<T, DP, 4><<<(unsigned)items, 256, 0, st>>>(a, 1, Split{});
+      return;
+    }
+    size_t bytes = 0;
+    const Split split = carve_split(a, reinterpret_cast<char*>(work), &bytes);
+    const int64_t goal = few_goal(a);
+    // items: a tile's first stretch each, and the further ones
+    const int64_t items = (tiles + goal) * a.kv_heads;
+    packattn_keys_kernel<T, DP, 1><<<(unsigned)std::min(items, few_grid(a)), 64, 0, st>>>(a, goal, split);
+    // a row's share of the waves, and of the stretches, were all sequences alike
+    const int64_t rows = a.q_tokens * G, live = std::max<int64_t>(1, std::min<int64_t>(a.sequences, a.q_tokens));
+    const int64_t x = std::min(live + rows / 32, goal) * a.kv_heads;
+    const int64_t y = std::min<int64_t>(32, (rows + live - 1) / live);
+    if (goal >= 32 * live)
+      packattn_join_kernel<T, DP, 16><<<dim3((unsigned)x, (unsigned)y), 1024, 0, st>>>(a, goal, split);
+    else
+      packattn_join_kernel<T, DP, 1><<<dim3((unsigned)x, (unsigned)(y + 3) / 4), NT, 0, st>>>(a, goal, split);
   });
 }
 
