@@ -29,6 +29,7 @@ FLAGS = [
 # every MFMA result: MFMA writing VGPRs directly saves the AGPR->VGPR moves.
 EXTRA = {
     "flash.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "packattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

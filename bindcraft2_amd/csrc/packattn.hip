@@ -278,29 +278,45 @@ struct TileCopy {
   static __device__ __forceinline__ unsigned dst(int i, int wave) { return (wave + W * i) * 1024; }
 };
 
-// rows r0 + l%32, elements 16 ks + 8 (l/32) ..: operand of a contraction over
-// the width.  base: the tile's LDS address
+// A lane's LDS addresses of the operands in a [rows][DP] tile at address 0; a tile
+// and the rows in it are constants beside them, which the reads take as offsets.
 template <int DP>
-__device__ __forceinline__ u32x4 row_operand(unsigned base, int r0, int ks, int lane) {
-  const int r = lane & 31, c = (2 * ks + (lane >> 5)) ^ fswz<DP>(r);
-  return *(lds_u32x4*)(base + (r0 + r) * (DP * 2) + c * 16);
-}
-// column 32 db + l%32, rows r0 + {4 h .. 4 h + 3, 8 + 4 h ..}, h = l/32: operand
-// of a contraction over the rows
-template <int DP>
-__device__ __forceinline__ u32x4 column_operand(unsigned base, int r0, int db, int lane) {
-  const int m = lane & 15, c = 4 * db + 2 * ((lane >> 4) & 1) + ((m & 3) >> 1);
-  u32x4 v;
+struct Operands {
+  unsigned row_[DP / 16], column_[DP / 32][2];
+  __device__ __forceinline__ void init(unsigned base, int lane) {
+    const int r = lane & 31, m = lane & 15;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int r = 8 * x + 4 * (lane >> 5) + (m >> 2);
-    const unsigned p = base + (r0 + r) * (DP * 2) + (c ^ fswz<DP>(r)) * 16 + (m & 1) * 8;
-    const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
-    v[2 * x] = t[0];
-    v[2 * x + 1] = t[1];
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      row_[ks] = base + r * (DP * 2) + (((2 * ks + (lane >> 5)) ^ fswz<DP>(r)) * 16);
+      asm volatile("" : "+v"(row_[ks]));  // made once, not at each use
+    }
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int q = 8 * x + 4 * (lane >> 5) + (m >> 2);
+        const int c = 4 * db + 2 * ((lane >> 4) & 1) + ((m & 3) >> 1);
+        column_[db][x] = base + q * (DP * 2) + ((c ^ fswz<DP>(q)) * 16) + (m & 1) * 8;
+        asm volatile("" : "+v"(column_[db][x]));
+      }
   }
-  return v;
-}
+  // rows r0 + l%32, elements 16 ks + 8 (l/32) ..: of a contraction over the width;
+  // at: r0 times the row's bytes, and the tile
+  __device__ __forceinline__ u32x4 row(unsigned at, int ks) const { return *(lds_u32x4*)(row_[ks] + at); }
+  // column 32 db + l%32, rows r0 + {4 h .. 4 h + 3, 8 + 4 h ..}, h = l/32: of a
+  // contraction over the rows
+  __device__ __forceinline__ u32x4 column(unsigned at, int db) const {
+    u32x4 v;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const u32x2 t = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(column_[db][x] + at)));
+      v[2 * x] = t[0];
+      v[2 * x + 1] = t[1];
+    }
+    return v;
+  }
+};
 
 // 8 elements from element e of a head's row, zeros past the width
 template <class T>
@@ -419,14 +435,15 @@ struct Online {
     ref = NEG_INF;
     mc = sum = 0.f;
   }
-  // S^T of a tile whose keys lie at kb0
-  static __device__ __forceinline__ void scores(f32x16 (&p)[NB], unsigned kb0, const u32x4 (&q)[KS], int lane) {
+  // S^T of a tile whose keys lie at `at`
+  static __device__ __forceinline__ void scores(f32x16 (&p)[NB], const Operands<DP>& x, unsigned at,
+                                                const u32x4 (&q)[KS]) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       p[b] = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        p[b] = Half<T>::mma(row_operand<DP>(kb0, 32 * b, ks, lane), q[ks], p[b]);
+        p[b] = Half<T>::mma(x.row(at + 32 * b * DP * 2, ks), q[ks], p[b]);
     }
   }
   // their exponents in place.  last: the last key that the lane's row sees, from
@@ -465,14 +482,14 @@ struct Online {
         sum += p[b][i];
       }
   }
-  // o^T += V^T P^T, the values at vb0
-  __device__ __forceinline__ void values(const f32x16 (&p)[NB], unsigned vb0, int lane) {
+  // o^T += V^T P^T, the values at `at`
+  __device__ __forceinline__ void values(const f32x16 (&p)[NB], const Operands<DP>& x, unsigned at) {
 #pragma unroll
     for (int kg = 0; kg < 2 * NB; ++kg) {
       const u32x4 w = pack8<T>(p[kg / 2], kg & 1);
 #pragma unroll
       for (int db = 0; db < DB; ++db)
-        o[db] = Half<T>::mma(column_operand<DP>(vb0, 16 * kg, db, lane), w, o[db]);
+        o[db] = Half<T>::mma(x.column(at + 16 * kg * DP * 2, db), w, o[db]);
     }
   }
 };
@@ -515,16 +532,21 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
   tile.init(a, seq, at.head, wave, lane);
   if (nk > 0) tile.issue(0, lds0);
 
-  for (int kt = 0; kt < nk; ++kt) {
-    const unsigned kb0 = lds0 + (kt & 1) * 2 * TILE, vb0 = kb0 + TILE;
+  Operands<DP> x;
+  x.init(lds0, lane);
+  auto step = [&](int kt, unsigned here, unsigned next) __attribute__((always_inline)) {
     const int k0 = kt * BN;
     wait_all_and_sync();
-    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + (~kt & 1) * 2 * TILE);
-    if (k0 > most) continue;
+    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + next);
+    if (k0 > most) return;
     f32x16 p[2];
-    st.scores(p, kb0, q, lane);
+    st.scores(p, x, here, q);
     st.weights(p, c, row.last - k0 - 4 * h, k0 + BN - 1 > least);
-    st.values(p, vb0, lane);
+    st.values(p, x, here + TILE);
+  };
+  for (int kt = 0; kt < nk; kt += 2) {  // the two buffers at constant places
+    step(kt, 0, 2 * TILE);
+    if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
   }
   const float sum = other_half_sum(st.sum);
   const bool none = sum == 0.f;
@@ -673,6 +695,8 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
   Stretches<KN> all;
   all.init(a, G, goal);
   const unsigned kb = lds_addr(smem) + wave * 2 * TILE, vb = kb + TILE;
+  Operands<DP> ops;
+  ops.init(kb, lane);
   const float c = a.scale * LOG2E;
   typedef KeyTiles<T, DP, KN, 1> Tiles;
   Item it;
@@ -703,13 +727,13 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
       const bool more = b + W < b1;
       wait_copies<Tiles::C::PER>();  // the keys are here, the values on their way
       f32x16 p[KN / 32];
-      st.scores(p, kb, q, lane);
+      st.scores(p, ops, 0, q);
       wait_reads();
       if (more) tile.keys((b + W) * KN, kb);
       st.weights(p, c, row.last - b * KN - 4 * h, b * KN + KN - 1 > least);
       if (more) wait_copies<Tiles::C::PER>();
       else wait_copies<0>();
-      st.values(p, vb, lane);
+      st.values(p, ops, TILE);
       wait_reads();
       if (more) tile.values((b + W) * KN, vb);
     }
@@ -986,19 +1010,21 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   tile.init(a, seq, at.head, wave, lane);
   if (nk > 0) tile.issue(0, lds0);
 
-  for (int kt = 0; kt < nk; ++kt) {
-    const unsigned kb0 = lds0 + (kt & 1) * 2 * TILE, vb0 = kb0 + TILE;
+  Operands<DP> x;
+  x.init(lds0, lane);
+  auto step = [&](int kt, unsigned here, unsigned next) __attribute__((always_inline)) {
     const int k0 = kt * BN;
     wait_all_and_sync();
-    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + (~kt & 1) * 2 * TILE);
-    if (k0 > most) continue;
+    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + next);
+    if (k0 > most) return;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      const unsigned kb = here + 32 * b * DP * 2, vb = kb + TILE;
       f32x16 p = {}, d = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(row_operand<DP>(kb0, 32 * b, ks, lane), q[ks], p);
+      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(x.row(kb, ks), q[ks], p);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(row_operand<DP>(vb0, 32 * b, ks, lane), g[ks], d);
+      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(x.row(vb, ks), g[ks], d);
       const bool cut = k0 + 32 * b + 31 > least;
       const int last = row.last - k0 - 4 * h;
 #pragma unroll
@@ -1015,10 +1041,13 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
       for (int kg = 0; kg < 2; ++kg) {
         const u32x4 w = pack8<T>(d, kg);
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-          o[db] = Half<T>::mma(column_operand<DP>(kb0, 32 * b + 16 * kg, db, lane), w, o[db]);
+        for (int db = 0; db < DB; ++db) o[db] = Half<T>::mma(x.column(kb + 16 * kg * DP * 2, db), w, o[db]);
       }
     }
+  };
+  for (int kt = 0; kt < nk; kt += 2) {
+    step(kt, 0, 2 * TILE);
+    if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
   }
   if (row.i >= seq.lq) {
 #pragma unroll
@@ -1128,20 +1157,23 @@ __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t 
     issue(from, 0);
     keep(0);
   }
-  int buf = 0;
-  for (int r0 = from; r0 < rows; r0 += BN, buf ^= 1) {
+  Operands<DP> ops;
+  ops.init(lds0, lane);
+  auto step = [&](int r0, auto buf_) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buf_)::value;
     wait_all_and_sync();
     if (r0 + BN < rows) issue(r0 + BN, buf ^ 1);
-    const unsigned qb = lds0 + buf * BUF, gb = qb + TILE, sb = qb + 2 * TILE;
+    const unsigned sb = lds0 + buf * BUF + 2 * TILE;
     // the first row of the tile sees the fewest keys
     const bool cut = a.causal && r0 / G + lag < j0 + 32 * wave + 31;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      const unsigned qb = buf * BUF + 32 * b * DP * 2, gb = qb + TILE;
       f32x16 p = {}, d = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(row_operand<DP>(qb, 32 * b, ks, lane), k[ks], p);
+      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(ops.row(qb, ks), k[ks], p);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(row_operand<DP>(gb, 32 * b, ks, lane), v[ks], d);
+      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(ops.row(gb, ks), v[ks], d);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const unsigned at_row = sb + (32 * b + 8 * x + 4 * h) * 4;
@@ -1168,12 +1200,16 @@ __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t 
         const u32x4 wp = pack8<T>(p, kg), wd = pack8<T>(d, kg);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          dv[db] = Half<T>::mma(column_operand<DP>(gb, 32 * b + 16 * kg, db, lane), wp, dv[db]);
-          dk[db] = Half<T>::mma(column_operand<DP>(qb, 32 * b + 16 * kg, db, lane), wd, dk[db]);
+          dv[db] = Half<T>::mma(ops.column(gb + 16 * kg * DP * 2, db), wp, dv[db]);
+          dk[db] = Half<T>::mma(ops.column(qb + 16 * kg * DP * 2, db), wd, dk[db]);
         }
       }
     }
     if (r0 + BN < rows) keep(buf ^ 1);
+  };
+  for (int r0 = from; r0 < rows; r0 += 2 * BN) {
+    step(r0, std::integral_constant<int, 0>());
+    if (r0 + BN < rows) step(r0 + BN, std::integral_constant<int, 1>());
   }
   if (!live) {
 #pragma unroll
