@@ -39,7 +39,7 @@
 #include "../../include/bc2n.h"
 
 #include <algorithm>
-#include <numeric>
+#include <type_traits>
 
 namespace bc2n {
 
@@ -194,8 +194,7 @@ __device__ __forceinline__ Seq lane_seq(const Seq& s, int lane) {
 
 // Workgroups of `tiles` tiles for each head of keys: XCD b % 8 takes heads of
 // one class mod gcd(kv_heads, 8), so that the tiles which read one head's keys
-// and values share an L2; within it tiles run from the last (LAST: causal rows
-// with the most keys) or from the first.
+// and values share an L2.
 struct Place {
   int head;
   int64_t tile;  // < 0: none
@@ -203,7 +202,6 @@ struct Place {
 __host__ __device__ inline int head_classes(int kv_heads) {
   return kv_heads % 8 == 0 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
 }
-template <bool LAST>
 __device__ __forceinline__ Place place(int kv_heads, int64_t tiles) {
   const int g = head_classes(kv_heads), share = NUM_XCD / g;
   const int64_t per = (tiles + share - 1) / share;
@@ -212,7 +210,6 @@ __device__ __forceinline__ Place place(int kv_heads, int64_t tiles) {
   r.head = (int)(x % g + g * (j / per));
   r.tile = (j % per) * share + x / g;
   if (r.tile >= tiles) r.tile = -1;
-  else if (LAST) r.tile = tiles - 1 - r.tile;
   return r;
 }
 unsigned place_grid(int kv_heads, int64_t tiles) {
@@ -220,6 +217,74 @@ unsigned place_grid(int kv_heads, int64_t tiles) {
   const int64_t grid = NUM_XCD * (int64_t)(kv_heads / g) * ((tiles + share - 1) / share);
   if (grid >= int64_t(1) << 24) throw std::invalid_argument("attention: too many tiles for one call");
   return (unsigned)grid;
+}
+
+// over a wave, by DPP within 16 lanes: what a search waits for is its latency
+template <class F>
+__device__ __forceinline__ int wave_fold(int v, F f) {
+  auto step = [&](auto ctrl) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  step(std::integral_constant<int, DPP_QUAD_1032>());
+  step(std::integral_constant<int, DPP_QUAD_2301>());
+  step(std::integral_constant<int, DPP_ROW_HALF_MIRROR>());
+  step(std::integral_constant<int, DPP_ROW_MIRROR>());
+  return f(f(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+           f(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+__device__ __forceinline__ int wave_add(int v) {
+  return wave_fold(v, [](int a, int b) { return a + b; });
+}
+
+// Tile x of 128 keys of all sequences, those with the most rows to see them first:
+// a launch's workgroups are a few times what runs at once, and a long causal
+// sequence's first tiles begun late would run alone at its end (packed prompts of
+// 140 .. 3435 tokens: dk and dv 672 -> 579 us; the rows' tiles, whose sequences
+// share an L2's keys in their own order, lost 2% by it).  A tile's weight falls
+// by the same step in all sequences, so the x-th heaviest of all is found by
+// bisecting the weight, every lane counting its sequence's tiles above it.
+// Whole sequences, and more than 64 entries, are taken in their order.
+__device__ __forceinline__ bool find_work(const PackedAttn& a, int64_t x, int& s, int64_t& t) {
+  const int lane = threadIdx.x & 63, entries = a.sequences + 2;
+  if (!a.causal || entries > 64) {
+    t = find_tile(a.k_off, a.sequences, a.k_tokens, 1, 128, x, s);
+    return t >= 0;
+  }
+  int n = 0, top = 0;  // a lane's sequence: tiles, weight of the heaviest
+  if (lane < entries) {
+    const Seq q = sequence(a, lane, true);
+    n = ((a.fill ? q.have : q.lk) + 127) / 128;
+    top = q.lk;
+  }
+  auto above = [&](int v) -> int {
+    const int64_t d = (int64_t)top - v;
+    return d <= 0 ? 0 : (int)min((int64_t)n, (d + 127) >> 7);
+  };
+  if (x >= wave_add(n)) return false;
+  int hi = wave_fold(top, [](int a, int b) { return max(a, b); });
+  // all tiles weigh more than lo; none more than hi
+  int lo = wave_fold(top - n * 128, [](int a, int b) { return min(a, b); }) - 1;
+  while (hi - lo > 1) {
+    const int v = (int)(((int64_t)hi + lo) >> 1);
+    if (wave_add(above(v)) > x) lo = v;
+    else hi = v;
+  }
+  // tile x weighs hi: the x - (those above) -th of that weight
+  int k = above(hi), rest = (int)x;
+  const int same = above(hi - 1) - k;
+  int before = same;
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) {
+    const int o = __shfl_up(before, i, 64);
+    if (lane >= i) before += o;
+  }
+  before -= same;
+  rest -= wave_add(k);
+  const unsigned long long at = __ballot(before <= rest && rest < before + same);
+  if (!at) return false;
+  s = uniform(__ffsll(at) - 1);
+  t = __builtin_amdgcn_readlane(k, s) + rest - __builtin_amdgcn_readlane(before, s);
+  return true;
 }
 
 // ------------------------------------------------------------- tiles in LDS
@@ -266,7 +331,9 @@ __device__ __forceinline__ void wait_all_and_sync() {
 // A wave's copies of a [ROWS][DP] tile by W waves: piece w + W i.
 template <int DP, int ROWS, int W>
 struct TileCopy {
-  static constexpr int PIECES = ROWS * DP * 2 / 1024, PER = PIECES / W;
+  static constexpr int PIECES = ROWS * DP * 2 / 1024, PER = (PIECES + W - 1) / W;
+  // waves past the pieces have none
+  static __device__ __forceinline__ bool any(int i, int wave) { return PIECES % W == 0 || wave + W * i < PIECES; }
   static constexpr int CPR = DP / 8;  // chunks a row
   // row and element of lane's chunk of piece i
   static __device__ __forceinline__ int row(int i, int wave, int lane) {
@@ -402,6 +469,7 @@ struct KeyTiles {
       vo[i] = e < width ? (unsigned)(r * vst + e) * 2 : NOWHERE;
     }
   }
+  static_assert(C::PIECES % W == 0, "every wave has as many pieces");
   __device__ __forceinline__ void keys(int k0, unsigned lds) const {
     const int rows = min(ROWS, lk - k0);
     const u32x4 d = descriptor(k + k0 * kst, (unsigned)((rows - 1) * kst + width) * 2);
@@ -500,11 +568,12 @@ template <class T, int DP>
 __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64_t tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   constexpr int BM = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
-  const Place at = place<true>(a.kv_heads, tiles);
+  const Place at = place(a.kv_heads, tiles);
   if (at.tile < 0) return;
   const int G = a.heads / a.kv_heads;
   int s;
-  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, at.tile, s);
+  // from the last tile: a causal sequence's last rows see the most keys
+  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, tiles - 1 - at.tile, s);
   const Seq seq = lane_seq(sequence(a, s, false), 0);
   const int rows = (a.fill ? seq.have : seq.lq) * G;
   if (t < 0 || t * BM >= rows) return;
@@ -960,11 +1029,12 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
                                                             const float* maxima, int blocks) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   constexpr int BM = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
-  const Place at = place<true>(a.kv_heads, tiles);
+  const Place at = place(a.kv_heads, tiles);
   if (at.tile < 0) return;
   const int G = a.heads / a.kv_heads;
   int s;
-  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, at.tile, s);
+  // from the last tile: a causal sequence's last rows see the most keys
+  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, tiles - 1 - at.tile, s);
   const Seq seq = lane_seq(sequence(a, s, false), 0);
   const int rows = (a.fill ? seq.have : seq.lq) * G;
   if (t < 0 || t * BM >= rows) return;
@@ -1056,25 +1126,35 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   store_columns<T, DB>(o, a.scale / ds, row.stored ? row_ptr<T>(a.dq, token, head) : nullptr, a.width, lane);
 }
 
-// dk, dv: workgroup = 128 keys of one sequence and head, 4 waves x 32 keys,
-// over the rows of all the group's heads in tiles of 64.
+// dk, dv: workgroup = 128 keys of one sequence and head over the rows of all the
+// group's heads in tiles of 64; wave w has the keys 32 (w % 4) .. and the half
+// w / 4 of every tile's rows, and the halves are added in LDS at the end.
+//
+// dk and dv take half of a wave's registers, so two waves a SIMD, without which
+// the matrix cores wait for each exponential, leave room for the values' operands
+// beside them and not for the keys': those are read from LDS, in operand order.
 template <class T, int DP>
-__global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, const float* delta,
-                                                          const float* maxima, int blocks) {
+__global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, const float* delta,
+                                                                 const float* maxima, int blocks) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  typedef TileCopy<DP, BN, WAVES> C;
+  typedef TileCopy<DP, BN, 2 * WAVES> C;
   constexpr int BK = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
-  const Place at = place<false>(a.kv_heads, tiles);
+  const Place at = place(a.kv_heads, tiles);
   if (at.tile < 0) return;
   const int G = a.heads / a.kv_heads;
   int s;
-  const int64_t t = find_tile(a.k_off, a.sequences, a.k_tokens, 1, BK, at.tile, s);
+  int64_t t;
+  if (!find_work(a, at.tile, s, t)) return;
   const Seq seq = lane_seq(sequence(a, s, true), 0);
   const int have = a.fill ? seq.have : seq.lk;
-  if (t < 0 || t * BK >= have) return;
+  if (t * BK >= have) return;
   const int j0 = (int)t * BK;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
-  const int j = j0 + 32 * wave + (lane & 31);  // a lane's key
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
+  const int group = wave & 3, half = wave >> 2;
+  // one wave of a SIMD ahead of the other: its exponentials beside their products
+  if (half) __builtin_amdgcn_s_setprio(0);
+  else __builtin_amdgcn_s_setprio(1);
+  const int j = j0 + 32 * group + (lane & 31);  // a lane's key
   const bool stored = j < have, live = j < seq.lk;
   const int64_t token = seq.k0 + min(j, have - 1);
   const int lag = seq.lk - seq.lq;  // query i sees keys up to i + lag
@@ -1085,20 +1165,24 @@ __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t 
   // P is made 2^SHIFT times as large in binary16
   constexpr float SHIFT = 2 * Half<T>::SHIFT;
 
-  u32x4 k[KS], v[KS];
+  // the buffers (Q, do, and lse, D and the last key of their rows), then K
+  constexpr int BUF = 2 * TILE + 3 * BN * 4;
+  const unsigned lds0 = lds_addr(smem);
+  u32x4 v[KS];
+  const unsigned kop = lds0 + 2 * BUF + group * (KS * 1024) + lane * 16;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    k[ks] = live ? load8(row_ptr<const T>(a.k, token, at.head), 16 * ks + 8 * h, a.width) : u32x4{0, 0, 0, 0};
-    v[ks] = live ? load8(row_ptr<const T>(a.v, token, at.head), 16 * ks + 8 * h, a.width) : u32x4{0, 0, 0, 0};
+    const u32x4 none = {0, 0, 0, 0};
+    v[ks] = live ? load8(row_ptr<const T>(a.v, token, at.head), 16 * ks + 8 * h, a.width) : none;
+    if (half == ks % 2)
+      *(__attribute__((address_space(3))) u32x4*)(kop + ks * 1024) =
+          live ? load8(row_ptr<const T>(a.k, token, at.head), 16 * ks + 8 * h, a.width) : none;
   }
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
   const float c = a.scale * LOG2E;
 
-  // Two buffers of Q, do tiles and of lse, D and the last key of their rows.
-  constexpr int BUF = 2 * TILE + 3 * BN * 4;
-  const unsigned lds0 = lds_addr(smem);
   auto stats = [&](int buf) { return reinterpret_cast<float*>(smem + buf * BUF + 2 * TILE); };
   // a lane's row of each piece
   int pi[C::PER], pg[C::PER];
@@ -1130,6 +1214,7 @@ __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t 
     const unsigned lds = lds0 + buf * BUF;
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) {
+      if (!C::any(i, wave)) continue;
       const int e = C::elem(i, wave, lane);
       const bool in = r0 + C::row(i, wave, lane) < rows && e < a.width;
       const int64_t di64 = pi[i] - i0;
@@ -1158,25 +1243,26 @@ __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t 
     keep(0);
   }
   Operands<DP> ops;
-  ops.init(lds0, lane);
+  ops.init(lds0 + half * (32 * DP * 2), lane);
   auto step = [&](int r0, auto buf_) __attribute__((always_inline)) {
     constexpr int buf = decltype(buf_)::value;
     wait_all_and_sync();
     if (r0 + BN < rows) issue(r0 + BN, buf ^ 1);
-    const unsigned sb = lds0 + buf * BUF + 2 * TILE;
-    // the first row of the tile sees the fewest keys
-    const bool cut = a.causal && r0 / G + lag < j0 + 32 * wave + 31;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const unsigned qb = buf * BUF + 32 * b * DP * 2, gb = qb + TILE;
+    const int mine = r0 + 32 * half;  // the wave's rows of the tile
+    // its last row sees the most keys, its first the fewest
+    const bool any = mine < rows && (!a.causal || (mine + 31) / G + lag >= j0 + 32 * group);
+    if (any) {
+      const unsigned sb = lds0 + buf * BUF + 2 * TILE + 128 * half;
+      const bool cut = a.causal && mine / G + lag < j0 + 32 * group + 31;
+      constexpr unsigned qb = buf * BUF, gb = qb + TILE;
       f32x16 p = {}, d = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(ops.row(qb, ks), k[ks], p);
+      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(ops.row(qb, ks), *(lds_u32x4*)(kop + ks * 1024), p);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(ops.row(gb, ks), v[ks], d);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const unsigned at_row = sb + (32 * b + 8 * x + 4 * h) * 4;
+        const unsigned at_row = sb + (8 * x + 4 * h) * 4;
         const f32x4 lse = *(lds_f32x4*)at_row, D = *(lds_f32x4*)(at_row + BN * 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1211,10 +1297,27 @@ __global__ __launch_bounds__(NT) void packattn_dkv_kernel(PackedAttn a, int64_t 
     step(r0, std::integral_constant<int, 0>());
     if (r0 + BN < rows) step(r0 + BN, std::integral_constant<int, 1>());
   }
-  if (!live) {
+  // the second half's sums to the first: dk, then dv, in [group][element][lane]
+  float* sums = reinterpret_cast<float*>(smem) + group * (DB * 16 * 64) + lane;
+  auto join = [&](f32x16 (&x)[DB]) __attribute__((always_inline)) {
+    __syncthreads();
+    if (half) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
-  }
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(db * 16 + i) * 64] = x[db][i];
+    }
+    __syncthreads();
+    if (!half) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[db][i] = live ? x[db][i] + sums[(db * 16 + i) * 64] : 0.f;
+    }
+  };
+  join(dk);
+  join(dv);
+  if (half) return;
   store_columns<T, DB>(dk, a.scale / ds, stored ? row_ptr<T>(a.dk, token, at.head) : nullptr, a.width, lane);
   store_columns<T, DB>(dv, Half<T>::SCALED ? 1.f / 16384.f : 1.f,
                        stored ? row_ptr<T>(a.dv, token, at.head) : nullptr, a.width, lane);
@@ -1354,9 +1457,9 @@ void packattn_bwd(hipStream_t st, const PackedAttn& a, void* work) {
     }
     if (a.k_tokens) {
       auto* dkv = &packattn_dkv_kernel<T, DP>;
-      const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4);
+      const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4) + 32 * WAVES * DP * 2;
       with_lds(dkv, lds);
-      dkv<<<place_grid(a.kv_heads, k_tiles), NT, lds, st>>>(a, k_tiles, delta, maxima, NORM_BLOCKS);
+      dkv<<<place_grid(a.kv_heads, k_tiles), 2 * NT, lds, st>>>(a, k_tiles, delta, maxima, NORM_BLOCKS);
     }
   });
 }
