@@ -287,6 +287,15 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, int64_t x, int& s
   return true;
 }
 
+// The order of the instructions around the products: left to itself the compiler
+// reads an operand, waits for it and multiplies, which leaves the matrix cores
+// idle for each read's latency.  next<M, N>: N instructions of kind M come next.
+enum Kind { VALU = 0x2, MFMA = 0x8, LDS_READ = 0x100 };
+template <int M, int N>
+__device__ __forceinline__ void next() {
+  if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(M, N, 0);
+}
+
 // ------------------------------------------------------------- tiles in LDS
 // 16-byte chunk c of row r of a [rows][DP] tile lies at chunk c ^ fswz(r).
 // A row read takes one chunk of 16 rows at a time and a transposed read 64
@@ -446,45 +455,56 @@ __device__ __forceinline__ int wave_max(int v) {
 }
 __device__ __forceinline__ int wave_min(int v) { return -wave_max(-v); }
 
-// Copies of ROWS keys and their values from key k0 on (past lk zeros), by W waves.
+// Copies of ROWS keys and of their values (zeros past the sequence), by W waves, from
+// key k0 on and every `step` keys.
 template <class T, int DP, int ROWS, int W>
 struct KeyTiles {
   typedef TileCopy<DP, ROWS, W> C;
+  static_assert(C::PIECES % W == 0, "every wave has as many pieces");
   unsigned ko[C::PER], vo[C::PER];  // a lane's offsets
-  const T *k, *v;
-  int64_t kst, vst;
-  int width, lk, wave;
-  __device__ __forceinline__ void init(const PackedAttn& a, const Seq& s, int head, int wave_, int lane) {
+  // the next ones' address, what is left of the sequence from there, and a step, in bytes
+  uint64_t k, v;
+  int64_t k_left, v_left, k_step, v_step;
+  int wave;
+  __device__ __forceinline__ void init(const PackedAttn& a, const Seq& s, int head, int k0, int step, int wave_,
+                                       int lane) {
     wave = wave_;
-    width = a.width;
-    lk = s.lk;
-    kst = a.k.st;
-    vst = a.v.st;
-    k = row_ptr<const T>(a.k, s.k0, head);
-    v = row_ptr<const T>(a.v, s.k0, head);
+    const int64_t kst = a.k.st, vst = a.v.st;
+    k = uniform64((int64_t)(uintptr_t)row_ptr<const T>(a.k, s.k0 + k0, head));
+    v = uniform64((int64_t)(uintptr_t)row_ptr<const T>(a.v, s.k0 + k0, head));
+    k_left = uniform64(((int64_t)(s.lk - k0 - 1) * kst + a.width) * 2);
+    v_left = uniform64(((int64_t)(s.lk - k0 - 1) * vst + a.width) * 2);
+    k_step = uniform64(step * kst * 2);
+    v_step = uniform64(step * vst * 2);
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) {
       const int r = C::row(i, wave, lane), e = C::elem(i, wave, lane);
-      ko[i] = e < width ? (unsigned)(r * kst + e) * 2 : NOWHERE;
-      vo[i] = e < width ? (unsigned)(r * vst + e) * 2 : NOWHERE;
+      ko[i] = e < a.width ? (unsigned)(r * kst + e) * 2 : NOWHERE;
+      vo[i] = e < a.width ? (unsigned)(r * vst + e) * 2 : NOWHERE;
     }
   }
-  static_assert(C::PIECES % W == 0, "every wave has as many pieces");
-  __device__ __forceinline__ void keys(int k0, unsigned lds) const {
-    const int rows = min(ROWS, lk - k0);
-    const u32x4 d = descriptor(k + k0 * kst, (unsigned)((rows - 1) * kst + width) * 2);
+  // a descriptor's bounds have 32 bits, and a tile's offsets 30
+  static __device__ __forceinline__ u32x4 here(uint64_t p, int64_t left) {
+    const uint32_t bytes = (uint64_t)left >> 31 ? 0x7fffffffu : (uint32_t)left;
+    return u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, bytes, 0x00027000u};
+  }
+  __device__ __forceinline__ void keys(unsigned lds) {
+    const u32x4 d = here(k, k_left);
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) copy16(ko[i], d, lds + C::dst(i, wave));
+    k += k_step;
+    k_left -= k_step;
   }
-  __device__ __forceinline__ void values(int k0, unsigned lds) const {
-    const int rows = min(ROWS, lk - k0);
-    const u32x4 d = descriptor(v + k0 * vst, (unsigned)((rows - 1) * vst + width) * 2);
+  __device__ __forceinline__ void values(unsigned lds) {
+    const u32x4 d = here(v, v_left);
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) copy16(vo[i], d, lds + C::dst(i, wave));
+    v += v_step;
+    v_left -= v_step;
   }
-  __device__ __forceinline__ void issue(int k0, unsigned lds) const {
-    keys(k0, lds);
-    values(k0, lds + ROWS * DP * 2);
+  __device__ __forceinline__ void both(unsigned lds) {
+    keys(lds);
+    values(lds + ROWS * DP * 2);
   }
 };
 
@@ -506,15 +526,23 @@ struct Online {
   // S^T of a tile whose keys lie at `at`
   static __device__ __forceinline__ void scores(f32x16 (&p)[NB], const Operands<DP>& x, unsigned at,
                                                 const u32x4 (&q)[KS]) {
+    constexpr int N = NB * KS, AHEAD = N < 8 ? N : 8;  // reads ahead of their products
+    u32x4 f[N];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      p[b] = f32x16{};
+    for (int i = 0; i < N; ++i) f[i] = x.row(at + 32 * (i % NB) * DP * 2, i / NB);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        p[b] = Half<T>::mma(x.row(at + 32 * b * DP * 2, ks), q[ks], p[b]);
+    for (int b = 0; b < NB; ++b) p[b] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i % NB] = Half<T>::mma(f[i], q[i / NB], p[i % NB]);
+    next<LDS_READ, AHEAD>();
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+      next<MFMA, 1>();
+      next<LDS_READ, 1>();
     }
+    next<MFMA, AHEAD>();
   }
-  // their exponents in place.  last: the last key that the lane's row sees, from
+  // the reference of their exponents.  last: the last key that the lane's row sees, from
   // the tile's first and its lane half's; cut: whether some row sees less than
   // the tile
   __device__ __forceinline__ void weights(f32x16 (&p)[NB], float c, int last, bool cut) {
@@ -542,23 +570,41 @@ struct Online {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[db][i] *= f;
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[b][i] = exp2_f(fmaf(p[b][i], c, Half<T>::SHIFT - mc));
-        sum += p[b][i];
-      }
   }
-  // o^T += V^T P^T, the values at `at`
-  __device__ __forceinline__ void values(const f32x16 (&p)[NB], const Operands<DP>& x, unsigned at) {
+  // exponents, and o^T += V^T P^T, the values at `at`: 16 keys' exponents beside the
+  // products of the 16 before
+  __device__ __forceinline__ void values(f32x16 (&p)[NB], float c, const Operands<DP>& x, unsigned at) {
+    constexpr int N = 2 * NB;
+    u32x4 v[N][DB];
 #pragma unroll
-    for (int kg = 0; kg < 2 * NB; ++kg) {
-      const u32x4 w = pack8<T>(p[kg / 2], kg & 1);
+    for (int g = 0; g < N; ++g)
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-        o[db] = Half<T>::mma(x.column(at + 16 * kg * DP * 2, db), w, o[db]);
+      for (int db = 0; db < DB; ++db) v[g][db] = x.column(at + 16 * g * DP * 2, db);
+    const float shift = Half<T>::SHIFT - mc;
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      f32x16& e = p[g / 2];
+#pragma unroll
+      for (int i = 8 * (g & 1); i < 8 * (g & 1) + 8; ++i) {
+        e[i] = exp2_f(fmaf(e[i], c, shift));
+        sum += e[i];
+      }
+      const u32x4 w = pack8<T>(e, g & 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = Half<T>::mma(v[g][db], w, o[db]);
     }
+    next<LDS_READ, 2 * DB>();
+    next<VALU, 28>();
+#pragma unroll
+    for (int g = 1; g < N; ++g) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        next<MFMA, 1>();
+        next<LDS_READ, 2>();
+        next<VALU, 28 / DB>();
+      }
+    }
+    next<MFMA, DB>();
   }
 };
 
@@ -598,20 +644,20 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
   st.init();
   const unsigned lds0 = lds_addr(smem);
   KeyTiles<T, DP, BN, WAVES> tile;
-  tile.init(a, seq, at.head, wave, lane);
-  if (nk > 0) tile.issue(0, lds0);
+  tile.init(a, seq, at.head, 0, BN, wave, lane);
+  if (nk > 0) tile.both(lds0);
 
   Operands<DP> x;
   x.init(lds0, lane);
   auto step = [&](int kt, unsigned here, unsigned next) __attribute__((always_inline)) {
     const int k0 = kt * BN;
     wait_all_and_sync();
-    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + next);
+    if (kt + 1 < nk) tile.both(lds0 + next);
     if (k0 > most) return;
     f32x16 p[2];
     st.scores(p, x, here, q);
     st.weights(p, c, row.last - k0 - 4 * h, k0 + BN - 1 > least);
-    st.values(p, x, here + TILE);
+    st.values(p, c, x, here + TILE);
   };
   for (int kt = 0; kt < nk; kt += 2) {  // the two buffers at constant places
     step(kt, 0, 2 * TILE);
@@ -732,8 +778,8 @@ struct Stretches {
         const int64_t y = x - lane64(before, l);
         r.seq = lane_seq(sequence(a, e0 + l, false), 0);
         r.parts = __builtin_amdgcn_readlane(parts, l);
-        r.tile = (int)(SPLIT ? y : y / r.parts);
-        r.part = (int)(SPLIT ? 0 : y % r.parts);
+        r.tile = uniform((int)(SPLIT ? y : y / r.parts));
+        r.part = SPLIT ? 0 : uniform((int)(y % r.parts));
         r.slot = slots + lane64(wave_before(s, lane), l) + (int64_t)r.tile * r.parts;
         r.per = per;
         return true;
@@ -770,7 +816,7 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
   typedef KeyTiles<T, DP, KN, 1> Tiles;
   Item it;
   for (int64_t x = blockIdx.x; all.template find<false>(a, x / a.kv_heads, it); x += gridDim.x) {
-    const int kv = (int)(x % a.kv_heads);
+    const int kv = uniform((int)(x % a.kv_heads));
     const Seq& seq = it.seq;
     const Row row = row_of(a, seq, it.tile * 32 + (lane & 31), G);
     const int head = kv * G + row.g;
@@ -784,27 +830,24 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
     Online<T, DP, KN / 32> st;
     st.init();
     Tiles tile;
-    tile.init(a, seq, kv, 0, lane);
     wait_reads();
     wait_copies<0>();  // q: what follows counts copies alone
     int b = b0 + wave;
-    if (b < b1) {
-      tile.keys(b * KN, kb);
-      tile.values(b * KN, vb);
-    }
+    tile.init(a, seq, kv, b * KN, W * KN, 0, lane);
+    if (b < b1) tile.both(kb);
     for (; b < b1; b += W) {
       const bool more = b + W < b1;
       wait_copies<Tiles::C::PER>();  // the keys are here, the values on their way
       f32x16 p[KN / 32];
       st.scores(p, ops, 0, q);
       wait_reads();
-      if (more) tile.keys((b + W) * KN, kb);
+      if (more) tile.keys(kb);
       st.weights(p, c, row.last - b * KN - 4 * h, b * KN + KN - 1 > least);
       if (more) wait_copies<Tiles::C::PER>();
       else wait_copies<0>();
-      st.values(p, ops, TILE);
+      st.values(p, c, ops, TILE);
       wait_reads();
-      if (more) tile.values((b + W) * KN, vb);
+      if (more) tile.values(vb);
     }
     const float sum = other_half_sum(st.sum);
     if constexpr (W > 1) {
@@ -889,7 +932,7 @@ __global__ __launch_bounds__(RW > 1 ? 64 * RW : NT) void packattn_join_kernel(Pa
   const int group = t / LP, e = t % LP * 4;
   Item it;
   for (int64_t x = blockIdx.x; all.template find<true>(a, x / a.kv_heads, it); x += gridDim.x) {
-    const int kv = (int)(x % a.kv_heads);
+    const int kv = uniform((int)(x % a.kv_heads));
     for (int r0 = blockIdx.y * ROWS; r0 < 32; r0 += gridDim.y * ROWS) {
       if (!row_of(a, it.seq, it.tile * 32 + r0, G).stored) break;
       const int r = r0 + mine;
@@ -1077,15 +1120,15 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   // what was loaded above is here before the first copy is issued
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   KeyTiles<T, DP, BN, WAVES> tile;
-  tile.init(a, seq, at.head, wave, lane);
-  if (nk > 0) tile.issue(0, lds0);
+  tile.init(a, seq, at.head, 0, BN, wave, lane);
+  if (nk > 0) tile.both(lds0);
 
   Operands<DP> x;
   x.init(lds0, lane);
   auto step = [&](int kt, unsigned here, unsigned next) __attribute__((always_inline)) {
     const int k0 = kt * BN;
     wait_all_and_sync();
-    if (kt + 1 < nk) tile.issue(k0 + BN, lds0 + next);
+    if (kt + 1 < nk) tile.both(lds0 + next);
     if (k0 > most) return;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -1151,9 +1194,6 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   const int j0 = (int)t * BK;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int group = wave & 3, half = wave >> 2;
-  // one wave of a SIMD ahead of the other: its exponentials beside their products
-  if (half) __builtin_amdgcn_s_setprio(0);
-  else __builtin_amdgcn_s_setprio(1);
   const int j = j0 + 32 * group + (lane & 31);  // a lane's key
   const bool stored = j < have, live = j < seq.lk;
   const int64_t token = seq.k0 + min(j, have - 1);
