@@ -289,10 +289,10 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, int64_t x, int& s
 
 // The order of the instructions around the products: left to itself the compiler
 // reads an operand, waits for it and multiplies, which leaves the matrix cores
-// idle for each read's latency.  next<M, N>: N instructions of kind M come next.
+// idle for each read's latency.  order<M, N>: N instructions of kind M come next.
 enum Kind { VALU = 0x2, MFMA = 0x8, LDS_READ = 0x100 };
 template <int M, int N>
-__device__ __forceinline__ void next() {
+__device__ __forceinline__ void order() {
   if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(M, N, 0);
 }
 
@@ -318,9 +318,8 @@ __device__ __forceinline__ void copy16(unsigned voff, u32x4 rsrc, unsigned lds) 
                "s"(rsrc), "s"(lds)
                : "memory", "m0");
 }
-__device__ __forceinline__ u32x4 descriptor(const void* p, unsigned bytes) {
-  const uint64_t b = (uint64_t)uniform64((int64_t)(uintptr_t)p);
-  return u32x4{(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, (uint32_t)uniform((int)bytes), 0x00027000u};
+__device__ __forceinline__ u32x4 descriptor(uint64_t p) {
+  return u32x4{(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)) & 0xffffu, 0x7fffffffu, 0x00027000u};
 }
 constexpr unsigned NOWHERE = 0x80000000u;  // past every descriptor's bounds
 
@@ -534,13 +533,13 @@ struct Online {
     for (int b = 0; b < NB; ++b) p[b] = f32x16{};
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i % NB] = Half<T>::mma(f[i], q[i / NB], p[i % NB]);
-    next<LDS_READ, AHEAD>();
+    order<LDS_READ, AHEAD>();
 #pragma unroll
     for (int i = 0; i < N - AHEAD; ++i) {
-      next<MFMA, 1>();
-      next<LDS_READ, 1>();
+      order<MFMA, 1>();
+      order<LDS_READ, 1>();
     }
-    next<MFMA, AHEAD>();
+    order<MFMA, AHEAD>();
   }
   // the reference of their exponents.  last: the last key that the lane's row sees, from
   // the tile's first and its lane half's; cut: whether some row sees less than
@@ -593,18 +592,18 @@ struct Online {
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = Half<T>::mma(v[g][db], w, o[db]);
     }
-    next<LDS_READ, 2 * DB>();
-    next<VALU, 28>();
+    order<LDS_READ, 2 * DB>();
+    order<VALU, 28>();
 #pragma unroll
     for (int g = 1; g < N; ++g) {
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        next<MFMA, 1>();
-        next<LDS_READ, 2>();
-        next<VALU, 28 / DB>();
+        order<MFMA, 1>();
+        order<LDS_READ, 2>();
+        order<VALU, 28 / DB>();
       }
     }
-    next<MFMA, DB>();
+    order<MFMA, DB>();
   }
 };
 
@@ -1134,28 +1133,58 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
     for (int b = 0; b < 2; ++b) {
       const unsigned kb = here + 32 * b * DP * 2, vb = kb + TILE;
       f32x16 p = {}, d = {};
+      {
+        u32x4 f[2 * KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(x.row(kb, ks), q[ks], p);
+        for (int i = 0; i < 2 * KS; ++i) f[i] = x.row(i & 1 ? vb : kb, i / 2);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(x.row(vb, ks), g[ks], d);
-      const bool cut = k0 + 32 * b + 31 > least;
-      const int last = row.last - k0 - 4 * h;
+        for (int ks = 0; ks < KS; ++ks) {
+          p = Half<T>::mma(f[2 * ks], q[ks], p);
+          d = Half<T>::mma(f[2 * ks + 1], g[ks], d);
+        }
+        constexpr int AHEAD = KS < 4 ? 2 * KS : 8;
+        order<LDS_READ, AHEAD>();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        d[i] = exp2_f(fmaf(p[i], c, -lse)) * (d[i] - D);
-        if (Half<T>::SCALED) d[i] *= ds;
+        for (int i = 0; i < 2 * KS - AHEAD; ++i) {
+          order<MFMA, 1>();
+          order<LDS_READ, 1>();
+        }
+        order<MFMA, AHEAD>();
       }
-      if (cut) {
+      const int last = row.last - k0 - 4 * h;
+      if (k0 + 32 * b + 31 > least) {  // a dP of NaN in a masked place stays there
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * b + 8 * (i / 4) + i % 4 > last) d[i] = 0.f;
+          if (32 * b + 8 * (i / 4) + i % 4 > last) {
+            p[i] = NEG_INF;
+            d[i] = 0.f;
+          }
       }
+      u32x4 f[2][DB];
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) f[kg][db] = x.column(kb + 16 * kg * DP * 2, db);
 #pragma unroll
       for (int kg = 0; kg < 2; ++kg) {
+#pragma unroll
+        for (int i = 8 * kg; i < 8 * kg + 8; ++i) {
+          d[i] = exp2_f(fmaf(p[i], c, -lse)) * (d[i] - D);
+          if (Half<T>::SCALED) d[i] *= ds;
+        }
         const u32x4 w = pack8<T>(d, kg);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = Half<T>::mma(x.column(kb + 16 * kg * DP * 2, db), w, o[db]);
+        for (int db = 0; db < DB; ++db) o[db] = Half<T>::mma(f[kg][db], w, o[db]);
       }
+      order<LDS_READ, 2 * DB>();
+      order<VALU, 36>();
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        order<MFMA, 1>();
+        order<LDS_READ, 2>();
+        order<VALU, 36 / DB>();
+      }
+      order<MFMA, DB>();
     }
   };
   for (int kt = 0; kt < nk; kt += 2) {
@@ -1174,8 +1203,8 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
 // w / 4 of every tile's rows, and the halves are added in LDS at the end.
 //
 // dk and dv take half of a wave's registers, so two waves a SIMD, without which
-// the matrix cores wait for each exponential, leave room for the values' operands
-// beside them and not for the keys': those are read from LDS, in operand order.
+// the matrix cores wait for each exponential, leave no room for the keys' and
+// values' operands beside them: those are read from LDS, in operand order.
 template <class T, int DP>
 __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, const float* delta,
                                                                  const float* maxima, int blocks) {
@@ -1205,18 +1234,16 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   // P is made 2^SHIFT times as large in binary16
   constexpr float SHIFT = 2 * Half<T>::SHIFT;
 
-  // the buffers (Q, do, and lse, D and the last key of their rows), then K
-  constexpr int BUF = 2 * TILE + 3 * BN * 4;
+  // the buffers (Q, do, and lse, D and the last key of their rows), then K, V
+  constexpr int BUF = 2 * TILE + 3 * BN * 4, OPERANDS = KS * 1024;
   const unsigned lds0 = lds_addr(smem);
-  u32x4 v[KS];
-  const unsigned kop = lds0 + 2 * BUF + group * (KS * 1024) + lane * 16;
+  const unsigned kop = lds0 + 2 * BUF + group * (2 * OPERANDS) + lane * 16;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     const u32x4 none = {0, 0, 0, 0};
-    v[ks] = live ? load8(row_ptr<const T>(a.v, token, at.head), 16 * ks + 8 * h, a.width) : none;
-    if (half == ks % 2)
-      *(__attribute__((address_space(3))) u32x4*)(kop + ks * 1024) =
-          live ? load8(row_ptr<const T>(a.k, token, at.head), 16 * ks + 8 * h, a.width) : none;
+    const HeadView& kv = half ? a.v : a.k;
+    *(__attribute__((address_space(3))) u32x4*)(kop + half * OPERANDS + ks * 1024) =
+        live ? load8(row_ptr<const T>(kv, token, at.head), 16 * ks + 8 * h, a.width) : none;
   }
   f32x16 dk[DB], dv[DB];
 #pragma unroll
@@ -1224,57 +1251,73 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   const float c = a.scale * LOG2E;
 
   auto stats = [&](int buf) { return reinterpret_cast<float*>(smem + buf * BUF + 2 * TILE); };
-  // a lane's row of each piece
-  int pi[C::PER], pg[C::PER];
+  // Where 64 rows are whole tokens, the next tile's lie as this one's, so many
+  // tokens on; elsewhere each tile divides its rows anew.
+  const bool even = BN % G == 0;
+  const int tokens = BN / G;
+  auto offset = [&](const HeadView& v, int r, int i0, int i) {
+    const int token_ = r / G, e = C::elem(i, wave, lane);
+    return e < a.width ? (unsigned)((token_ - i0) * v.st + (r - token_ * G) * v.sh + e) * 2 : NOWHERE;
+  };
+  unsigned qo[C::PER], go[C::PER];
+  const int i_from = from / G;
 #pragma unroll
   for (int i = 0; i < C::PER; ++i) {
     const int r = from + C::row(i, wave, lane);
-    pi[i] = r / G;
-    pg[i] = r - pi[i] * G;
+    qo[i] = offset(a.q, r, i_from, i);
+    go[i] = offset(a.d_o, r, i_from, i);
   }
-  const int di = BN / G, dg = BN % G;
+  uint64_t qp = uniform64((int64_t)(uintptr_t)row_ptr<const T>(a.q, seq.q0 + i_from, at.head * G));
+  uint64_t gp = uniform64((int64_t)(uintptr_t)row_ptr<const T>(a.d_o, seq.q0 + i_from, at.head * G));
+  const int64_t q_step = uniform64(tokens * a.q.st * 2), g_step = uniform64(tokens * a.d_o.st * 2);
+  // the row whose lse, D and last key a thread of the first wave fetches
+  int my_i = (from + (int)threadIdx.x) / G, my_g = from + (int)threadIdx.x - my_i * G;
   float n_lse = 0.f, n_delta = 0.f;
   int n_last = -1;
   auto issue = [&](int r0, int buf) __attribute__((always_inline)) {
-    const int i0 = r0 / G;
-    const u32x4 qd = descriptor(row_ptr<const T>(a.q, seq.q0 + i0, at.head * G), 0x7fffffffu);
-    const u32x4 gd = descriptor(row_ptr<const T>(a.d_o, seq.q0 + i0, at.head * G), 0x7fffffffu);
-    n_lse = -NEG_INF;
-    n_delta = 0.f;
-    n_last = -1;
-    if (threadIdx.x < BN) {
-      const int r = r0 + threadIdx.x, i = r / G;
-      if (r < rows) {
-        const int64_t p = (int64_t)(at.head * G + r - i * G) * a.q_tokens + seq.q0 + i;
+    if (!even) {
+      const int i0 = r0 / G;
+      qp = uniform64((int64_t)(uintptr_t)row_ptr<const T>(a.q, seq.q0 + i0, at.head * G));
+      gp = uniform64((int64_t)(uintptr_t)row_ptr<const T>(a.d_o, seq.q0 + i0, at.head * G));
+#pragma unroll
+      for (int i = 0; i < C::PER; ++i) {
+        const int r = r0 + C::row(i, wave, lane);
+        qo[i] = offset(a.q, r, i0, i);
+        go[i] = offset(a.d_o, r, i0, i);
+      }
+      my_i = (r0 + (int)threadIdx.x) / G;
+      my_g = r0 + (int)threadIdx.x - my_i * G;
+    }
+    if (wave == 0) {
+      n_lse = -NEG_INF;
+      n_delta = 0.f;
+      n_last = -1;
+      if (r0 + lane < rows) {
+        const int64_t p = (int64_t)(at.head * G + my_g) * a.q_tokens + seq.q0 + my_i;
         n_lse = a.lse[p] * LOG2E;
         n_delta = delta[p];
-        n_last = a.causal ? i + lag : seq.lk;
+        n_last = a.causal ? my_i + lag : seq.lk;
       }
     }
     const unsigned lds = lds0 + buf * BUF;
+    const u32x4 qd = descriptor(qp), gd = descriptor(gp);
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) {
       if (!C::any(i, wave)) continue;
-      const int e = C::elem(i, wave, lane);
-      const bool in = r0 + C::row(i, wave, lane) < rows && e < a.width;
-      const int64_t di64 = pi[i] - i0;
-      copy16(in ? (unsigned)(di64 * a.q.st + pg[i] * a.q.sh + e) * 2 : NOWHERE, qd, lds + C::dst(i, wave));
-      copy16(in ? (unsigned)(di64 * a.d_o.st + pg[i] * a.d_o.sh + e) * 2 : NOWHERE, gd,
-             lds + TILE + C::dst(i, wave));
-      pi[i] += di;
-      pg[i] += dg;
-      if (pg[i] >= G) {
-        pg[i] -= G;
-        ++pi[i];
-      }
+      const bool in = r0 + C::row(i, wave, lane) < rows;
+      copy16(in ? qo[i] : NOWHERE, qd, lds + C::dst(i, wave));
+      copy16(in ? go[i] : NOWHERE, gd, lds + TILE + C::dst(i, wave));
     }
+    qp += q_step;
+    gp += g_step;
+    my_i += tokens;
   };
   auto keep = [&](int buf) {
-    if (threadIdx.x < BN) {
+    if (wave == 0) {
       float* st = stats(buf);
-      st[threadIdx.x] = n_lse == NEG_INF ? -NEG_INF : n_lse;  // a row without a key: P = 0
-      st[BN + threadIdx.x] = n_delta;
-      reinterpret_cast<int*>(st)[2 * BN + threadIdx.x] = n_last;
+      st[lane] = n_lse == NEG_INF ? -NEG_INF : n_lse;  // a row without a key: P = 0
+      st[BN + lane] = n_delta;
+      reinterpret_cast<int*>(st)[2 * BN + lane] = n_last;
     }
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1296,40 +1339,87 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
       const bool cut = a.causal && mine / G + lag < j0 + 32 * group + 31;
       constexpr unsigned qb = buf * BUF, gb = qb + TILE;
       f32x16 p = {}, d = {};
+      {
+        u32x4 f[4 * KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) p = Half<T>::mma(ops.row(qb, ks), *(lds_u32x4*)(kop + ks * 1024), p);
+        for (int ks = 0; ks < KS; ++ks) {
+          f[4 * ks] = ops.row(qb, ks);
+          f[4 * ks + 1] = *(lds_u32x4*)(kop + ks * 1024);
+          f[4 * ks + 2] = ops.row(gb, ks);
+          f[4 * ks + 3] = *(lds_u32x4*)(kop + OPERANDS + ks * 1024);
+        }
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) d = Half<T>::mma(ops.row(gb, ks), v[ks], d);
+        for (int ks = 0; ks < KS; ++ks) {
+          p = Half<T>::mma(f[4 * ks], f[4 * ks + 1], p);
+          d = Half<T>::mma(f[4 * ks + 2], f[4 * ks + 3], d);
+        }
+        constexpr int AHEAD = 2;  // steps of the width
+        order<LDS_READ, 4 * AHEAD>();
+#pragma unroll
+        for (int i = 0; i < KS - AHEAD; ++i) {
+          order<MFMA, 1>();
+          order<LDS_READ, 2>();
+          order<MFMA, 1>();
+          order<LDS_READ, 2>();
+        }
+        order<MFMA, 2 * AHEAD>();
+      }
+      f32x4 lse[4], D[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const unsigned at_row = sb + (8 * x + 4 * h) * 4;
-        const f32x4 lse = *(lds_f32x4*)at_row, D = *(lds_f32x4*)(at_row + BN * 4);
+        lse[x] = *(lds_f32x4*)at_row;
+        D[x] = *(lds_f32x4*)(at_row + BN * 4);
+      }
+      if (cut) {  // a dP of NaN in a masked place stays there
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[4 * x + i] = exp2_f(fmaf(p[4 * x + i], c, SHIFT - lse[i]));
-          d[4 * x + i] = p[4 * x + i] * (d[4 * x + i] - D[i]);
-        }
-        if (cut) {
-          const u32x4 last = *(lds_u32x4*)(at_row + 2 * BN * 4);
+        for (int x = 0; x < 4; ++x) {
+          const u32x4 last = *(lds_u32x4*)(sb + (8 * x + 4 * h) * 4 + 2 * BN * 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (j > (int)last[i]) p[4 * x + i] = d[4 * x + i] = 0.f;
-        }
-        if (Half<T>::SCALED) {
-          const float f = ds * (1.f / 16384.f);  // 2^-SHIFT
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[4 * x + i] *= f;
+            if (j > (int)last[i]) {
+              p[4 * x + i] = NEG_INF;
+              d[4 * x + i] = 0.f;
+            }
         }
       }
+      u32x4 fg[2][DB], fq[2][DB];
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          fg[kg][db] = ops.column(gb + 16 * kg * DP * 2, db);
+          fq[kg][db] = ops.column(qb + 16 * kg * DP * 2, db);
+        }
 #pragma unroll
       for (int kg = 0; kg < 2; ++kg) {
+#pragma unroll
+        for (int i = 8 * kg; i < 8 * kg + 8; ++i) {
+          p[i] = exp2_f(fmaf(p[i], c, SHIFT - lse[i / 4][i % 4]));
+          d[i] = p[i] * (d[i] - D[i / 4][i % 4]);
+          if (Half<T>::SCALED) d[i] *= ds * (1.f / 16384.f);  // 2^-SHIFT
+        }
         const u32x4 wp = pack8<T>(p, kg), wd = pack8<T>(d, kg);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          dv[db] = Half<T>::mma(ops.column(gb + 16 * kg * DP * 2, db), wp, dv[db]);
-          dk[db] = Half<T>::mma(ops.column(qb + 16 * kg * DP * 2, db), wd, dk[db]);
+          dv[db] = Half<T>::mma(fg[kg][db], wp, dv[db]);
+          dk[db] = Half<T>::mma(fq[kg][db], wd, dk[db]);
         }
       }
+      order<LDS_READ, 4>();
+      order<VALU, 48>();
+#pragma unroll
+      for (int i = 0; i < 2 * DB; ++i) {
+        order<LDS_READ, 2>();
+        order<MFMA, 1>();
+        order<VALU, 48 / (2 * DB)>();
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * DB - 2; ++i) {
+        order<LDS_READ, 2>();
+        order<MFMA, 1>();
+      }
+      order<MFMA, 2>();
     }
     if (r0 + BN < rows) keep(buf ^ 1);
   };
@@ -1497,7 +1587,7 @@ void packattn_bwd(hipStream_t st, const PackedAttn& a, void* work) {
     }
     if (a.k_tokens) {
       auto* dkv = &packattn_dkv_kernel<T, DP>;
-      const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4) + 32 * WAVES * DP * 2;
+      const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4) + 2 * 32 * WAVES * DP * 2;
       with_lds(dkv, lds);
       dkv<<<place_grid(a.kv_heads, k_tiles), 2 * NT, lds, st>>>(a, k_tiles, delta, maxima, NORM_BLOCKS);
     }
