@@ -175,22 +175,57 @@ __global__ __launch_bounds__(256) void sample_few_kernel(Sample a) {
 
 // ---------------------------------------------------------------------------
 // A workgroup a row.
+constexpr int CANDIDATES = 1024;
 template <int NT>
 struct Shared {
   u64 mass[BINS];
   uint32_t count[BINS];
   u64 list_key[LIST];
   u64 list_mass[LIST];
+  float x[CANDIDATES];
+  int j[CANDIDATES];
   u64 wave_a[NT / 64], wave_b[NT / 64];
   u64 out[4];
-  uint32_t n;
+  uint32_t n, found;
 };
 
+// DPP moves: what a fold or a scan waits for is its latency, a tenth of a shuffle's.
+constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp64(u64 v, u64 none) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp((int)(none >> 32), (int)(v >> 32), CTRL, ROWS, 0xF, false);
+  return (u64)hi << 32 | lo;
+}
+struct Sum {
+  static constexpr u64 NONE = 0;
+  __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+  static constexpr u64 NONE = 0;
+  __device__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
+};
+struct Min {
+  static constexpr u64 NONE = ~u64(0);
+  __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; }
+};
+// of the lanes up to this one
+template <class F>
+__device__ __forceinline__ u64 wave_scan(u64 v, F f) {
+  v = f(v, dpp64<ROW_SHR + 1, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_SHR + 2, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_SHR + 4, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_SHR + 8, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_BCAST15, 0xA>(v, F::NONE));
+  return f(v, dpp64<ROW_BCAST31, 0xC>(v, F::NONE));
+}
+__device__ __forceinline__ u64 lane_value(u64 v, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
 template <class F>
 __device__ __forceinline__ u64 wave_fold(u64 v, F f) {
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) v = f(v, (u64)__shfl_xor(v, i, 64));
-  return v;
+  return lane_value(wave_scan(v, f), 63);
 }
 // over the workgroup, the result in every thread
 template <int NT, class F>
@@ -204,24 +239,10 @@ __device__ __forceinline__ u64 block_fold(u64 v, u64* waves, F f) {
   for (int i = 1; i < NT / 64; ++i) v = f(v, waves[i]);
   return v;
 }
-struct Sum {
-  __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
-};
-struct Max {
-  __device__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
-};
-struct Min {
-  __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; }
-};
 template <int NT>
 __device__ __forceinline__ u64 block_scan(u64 v, u64* waves) {  // exclusive
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 run = v;
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) {
-    const u64 o = __shfl_up(run, i, 64);
-    if (lane >= i) run += o;
-  }
+  const u64 run = wave_scan(v, Sum());
   __syncthreads();
   if (lane == 63) waves[wave] = run;
   __syncthreads();
@@ -231,48 +252,76 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* waves) {  // exclusive
   return before + run - v;
 }
 
-// A row in tiles of consecutive classes, a vector a thread.
-template <class T, int NT>
+// A row: NV vectors a thread held in registers, for passes of a few instructions a
+// class, or (NV = 0) read at each of those; and for the passes with exponentials
+// a class at a time, whose loads are the least of it.
+template <class T, int NT, int NV>
 struct RowOf {
   static constexpr int E = Vec<T>::N;
-  static constexpr int TILE = NT * E;
   const T* x;
-  int V, tiles;
+  int V;
+  u32x4 held[NV ? NV : 1];
 
-  // classes past the row's end are -infinity
-  __device__ __forceinline__ u32x4 load(int i) const {
-    const int64_t j = (int64_t)i * TILE + threadIdx.x * E;
-    if (j + E <= V) return Vec<T>::load(x + j);
+  // A vector that would pass the row's end is read ending there, so that all of a
+  // thread's are in flight together, and its classes that another thread has
+  // are -infinity.
+  __device__ __forceinline__ int first(int i) const { return min((i * NT + (int)threadIdx.x) * E, V - E); }
+  __device__ __forceinline__ u32x4 alone(u32x4 raw, int i) const {
+    if ((int64_t)(i + 1) * NT * E <= V) return raw;  // the same for all threads
     float v[E];
+    Vec<T>::unpack(raw, v);
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = j + e < V ? (float)x[j + e] : NEG_INF;
+    for (int e = 0; e < E; ++e) v[e] = first(i) + e < (i * NT + (int)threadIdx.x) * E ? NEG_INF : v[e];
     return Vec<T>::pack(v);
   }
   __device__ __forceinline__ void init(const T* row, int V_) {
     x = row;
     V = V_;
-    tiles = (V + TILE - 1) / TILE;
-  }
-  template <class F>
-  __device__ __forceinline__ void tile(int i, F f) const {
-    float v[E];
-    Vec<T>::unpack(load(i), v);
 #pragma unroll
-    for (int e = 0; e < E; ++e) f(v[e], i * TILE + (int)threadIdx.x * E + e);
+    for (int i = 0; i < NV; ++i) held[i] = Vec<T>::load(x + first(i));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) held[i] = alone(held[i], i);
   }
   // f(x, index) of a thread's classes
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-#pragma unroll 1
-    for (int i = 0; i < tiles; ++i) tile(i, f);
+#pragma unroll 2
+    for (int j = threadIdx.x; j < V; j += NT) f((float)x[j], j);
+  }
+  // f(classes' values, index of the first) of a thread's vectors
+  template <class F>
+  __device__ __forceinline__ void vectors(F f) const {
+    float v[E];
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        Vec<T>::unpack(held[i], v);
+        f(v, first(i));
+      }
+    } else {
+      const int n = (V + NT * E - 1) / (NT * E);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        Vec<T>::unpack(alone(Vec<T>::load(x + first(i)), i), v);
+        f(v, first(i));
+      }
+    }
+  }
+};
+// The classes that a row's draw is among, where they are few: in LDS, in no order.
+template <int NT>
+struct Candidates {
+  Shared<NT>& sh;
+  int n;
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = threadIdx.x; i < n; i += NT) f(sh.x[i], sh.j[i]);
   }
 };
 
-// What a row's kept classes have at least: rank key and distance.
-template <class T, int NT>
+template <int NT>
 struct Drawer {
   Shared<NT>& sh;
-  const RowOf<T, NT>& row;
   float m, range, steps;  // maximum, largest distance of a mass, steps a distance
   double inv;
   int S;
@@ -284,24 +333,53 @@ struct Drawer {
   __device__ __forceinline__ int step_of(float x) const {
     return (int)fminf((m - x) * steps, (float)(BINS - 1));
   }
-
-  // The rank key of the last class whose forerunners, among the classes of
-  // rank keys >= least, weigh less than `end`: by number, or (MASS) by mass.
+  __device__ __forceinline__ void clear(bool masses) {
+    for (int i = threadIdx.x; i < BINS; i += NT) {
+      sh.count[i] = 0;
+      if (masses) sh.mass[i] = 0;
+    }
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+  }
+  // The last filled step whose forerunners, `before` and the steps before it,
+  // weigh less than the end; `before` becomes what those weigh.
   template <bool MASS>
-  __device__ u64 last_before(u64 end, u64 least) {
+  __device__ int last_step(u64 end, u64& before) {
+    constexpr int PER = BINS / NT;
+    u64 w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = threadIdx.x * PER + i;
+      w += MASS ? sh.mass[b] : sh.count[b];
+    }
+    u64 run = before + block_scan<NT>(w, sh.wave_a);
+    u64 best = 0, best_run = 0;  // step + 1
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = threadIdx.x * PER + i;
+      if (sh.count[b] && run < end) {
+        best = b + 1;
+        best_run = run;
+      }
+      run += MASS ? sh.mass[b] : sh.count[b];
+    }
+    const u64 top = block_fold<NT>(best, sh.wave_b, Max());
+    if (best == top && best) sh.out[0] = best_run;
+    __syncthreads();
+    before = sh.out[0];
+    return (int)top - 1;
+  }
+
+  // The rank key of the last class of `from` whose forerunners, among those of
+  // rank keys >= least, weigh less than `end`: by number, or (MASS) by mass.
+  template <bool MASS, class S_>
+  __device__ u64 last_before(const S_& from, u64 end, u64 least) {
     u64 lo = 0, hi = ~u64(0), before = 0;
     int shift = -1;  // -1: steps of distance
     for (;;) {
-      for (int i = threadIdx.x; i < BINS; i += NT) {
-        sh.count[i] = 0;
-        if (MASS) sh.mass[i] = 0;
-      }
-      if (threadIdx.x == 0) sh.n = 0;
-      __syncthreads();
-      auto bin_of = [&](float x, u64 c) {
-        return shift < 0 ? step_of(x) : (int)((hi - c) >> shift);
-      };
-      row.each([&](float x, int j) {
+      clear(MASS);
+      auto bin_of = [&](float x, u64 c) { return shift < 0 ? step_of(x) : (int)((hi - c) >> shift); };
+      from.each([&](float x, int j) {
         if (!counts(x)) return;
         const u64 c = rank_key(x, j);
         if (c < least || c < lo || c > hi) return;
@@ -310,34 +388,10 @@ struct Drawer {
         if (MASS) atomicAdd(&sh.mass[b], mass(x));
       });
       __syncthreads();
-      // the last filled bin whose forerunners weigh less than the end
-      constexpr int PER = BINS / NT;
-      u64 w = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int b = threadIdx.x * PER + i;
-        w += MASS ? sh.mass[b] : sh.count[b];
-      }
-      u64 run = before + block_scan<NT>(w, sh.wave_a);
-      u64 best = 0;  // bin + 1
-      u64 best_run = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int b = threadIdx.x * PER + i;
-        if (sh.count[b] && run < end) {
-          best = b + 1;
-          best_run = run;
-        }
-        run += MASS ? sh.mass[b] : sh.count[b];
-      }
-      const u64 top = block_fold<NT>(best, sh.wave_b, Max());
-      if (best == top && best) sh.out[0] = best_run;
-      __syncthreads();
-      const int bin = (int)top - 1;
-      before = sh.out[0];
+      const int bin = last_step<MASS>(end, before);
       const uint32_t in_bin = sh.count[bin];
       if (in_bin <= LIST) {
-        row.each([&](float x, int j) {
+        from.each([&](float x, int j) {
           if (!counts(x)) return;
           const u64 c = rank_key(x, j);
           if (c < least || c < lo || c > hi || bin_of(x, c) != bin) return;
@@ -357,7 +411,7 @@ struct Drawer {
       }
       // too many: their range of rank keys in 2048 parts
       u64 a = ~u64(0), b = 0;
-      row.each([&](float x, int j) {
+      from.each([&](float x, int j) {
         if (!counts(x)) return;
         const u64 c = rank_key(x, j);
         if (c < least || c < lo || c > hi || bin_of(x, c) != bin) return;
@@ -373,71 +427,203 @@ struct Drawer {
       __syncthreads();
     }
   }
+
+  // The first CANDIDATES of the classes that are at least `low` to LDS; how many
+  // there are.
+  template <class R>
+  __device__ int collect(const R& row, float low) {
+    row.vectors([&](const float (&v)[R::E], int j) {
+      float top = v[0];
+#pragma unroll
+      for (int e = 1; e < R::E; ++e) top = fmaxf(top, v[e]);
+      if (top < low) return;
+#pragma unroll
+      for (int e = 0; e < R::E; ++e) {
+        if (v[e] >= low) {
+          const uint32_t at = atomicAdd(&sh.found, 1u);
+          if (at < CANDIDATES) {
+            sh.x[at] = v[e];
+            sh.j[at] = j + e;
+          }
+        }
+      }
+    });
+    __syncthreads();
+    return (int)sh.found;
+  }
+  // a value that no class of the steps up to `step` is below
+  __device__ __forceinline__ float lowest(int step) const {
+    if (step >= BINS - 1) return m - range;
+    const float d = (float)(step + 1) / steps;  // of the next step's first, but for rounding
+    return m - fminf(d * 1.0001f, range) - 1e-6f * fabsf(m);
+  }
+
+  // The same as cut and draw, of at most 64 candidates by one wave: ranks and sums
+  // of forerunners by comparing each with all.
+  template <class ST>
+  __device__ void draw_few(const Sample& a, int64_t r, int n, const ST& s, u64 whole) {
+    const int lane = threadIdx.x;
+    const float x = lane < n ? sh.x[lane] : NEG_INF;
+    const int j = lane < n ? sh.j[lane] : 0x7fffffff;
+    const u64 c = lane < n ? rank_key(x, j) : 0;
+    const double t = distance(x);
+    u64 w = lane < n && counts(x) ? mass_of(t, S) : 0;
+    if (s.k) {
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += lane_value(c, i) > c;
+      if (rank >= s.k) w = 0;
+    }
+    if (s.p < 1.0) {
+      if (s.k) whole = wave_fold(w, Sum());
+      const u64 end = share_of(s.p, whole);
+      u64 before = 0;
+      for (int i = 0; i < n; ++i) before += lane_value(c, i) > c ? lane_value(w, i) : 0;
+      if (before >= end) w = 0;
+    }
+    if (t < s.floor) w = 0;
+    const u64 mass = wave_fold(w, Sum()), target = target_of(s.u, mass);
+    u64 before = 0;
+    for (int i = 0; i < n; ++i) before += __builtin_amdgcn_readlane(j, i) < j ? lane_value(w, i) : 0;
+    if (w && before <= target && before + w > target) write(a, r, j, log_share(t, mass, S));
+  }
+
+  // The class of `from` at which the kept masses' running sum by index passes u of
+  // the whole: written.  bits: of an index.
+  template <class KEPT>
+  __device__ void draw(const Sample& a, int64_t r, const Candidates<NT>& from, float u, int bits, KEPT kept) {
+    clear(true);
+    const int shift = max(bits - 11, 0);  // 2048 runs of indexes
+    u64 mine = 0;
+    from.each([&](float x, int j) {
+      const u64 w = kept(x, j);
+      mine += w;
+      if (w) {
+        atomicAdd(&sh.mass[j >> shift], w);
+        atomicAdd(&sh.count[j >> shift], 1u);
+      }
+    });
+    const u64 whole = block_fold<NT>(mine, sh.wave_b, Sum()), target = target_of(u, whole);
+    // the last run whose forerunners weigh at most the target
+    u64 before = 0;
+    const int run = last_step<true>(target + 1, before);
+    from.each([&](float x, int j) {
+      if (j >> shift != run) return;
+      const u64 w = kept(x, j);
+      u64 f = before;
+      if (sh.count[run] > 1 && w)
+        for (int i = 0; i < from.n; ++i)
+          if (sh.j[i] < j && sh.j[i] >> shift == run) f += kept(sh.x[i], sh.j[i]);
+      if (w && f <= target && f + w > target) write(a, r, j, log_share(distance(x), whole, S));
+    });
+  }
 };
 
-template <class T, int NT>
+template <class T, int NT, int NV>
 __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   __shared__ Shared<NT> sh;
   constexpr int WAVES = NT / 64;
   const int64_t r = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Settings s = settings_of(a, r);
-  RowOf<T, NT> row;
+  RowOf<T, NT, NV> row;
   row.init(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
-  float hi = NEG_INF, lo = -NEG_INF;
+  const Settings s = settings_of(a, r);
+  if (threadIdx.x == 0) sh.found = 0;
+  float hi = NEG_INF;
   bool nan = false;
-  row.each([&](float x, int) {
-    nan |= x != x;
-    hi = fmaxf(hi, x);
-    if (x != NEG_INF) lo = fminf(lo, x);
+  typedef RowOf<T, NT, NV> R;
+  row.vectors([&](const float (&v)[R::E], int) {
+#pragma unroll
+    for (int e = 0; e < R::E; ++e) {
+      nan |= v[e] != v[e];
+      hi = fmaxf(hi, v[e]);
+    }
   });
   const u64 top = block_fold<NT>(nan ? ~u64(0) : (u64)key_of(hi), sh.wave_a, Max());
-  const u64 low = block_fold<NT>((u64)key_of(lo), sh.wave_b, Min());
-  auto value = [](u64 k) {
-    const uint32_t b = (uint32_t)k;
-    return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
-  };
-  const float m = value(top);
+  const uint32_t bits = (uint32_t)top;
+  const float m = __builtin_bit_cast(float, bits & 0x80000000u ? bits & 0x7fffffffu : ~bits);
   if (top == ~u64(0) || m == -NEG_INF || m == NEG_INF || s.bad) {
     if (threadIdx.x == 0) write(a, r, -1, __builtin_nanf(""));
     return;
   }
   if (s.greedy) {
     u64 first = ~u64(0);
-    row.each([&](float x, int j) {
-      if (x == m) first = min(first, (u64)j);
+    row.vectors([&](const float (&v)[R::E], int j) {
+#pragma unroll
+      for (int e = 0; e < R::E; ++e)
+        if (v[e] == m) first = min(first, (u64)(j + e));
     });
-    first = block_fold<NT>(first, sh.wave_a, Min());
+    first = block_fold<NT>(first, sh.wave_b, Min());
     if (threadIdx.x == 0) write(a, r, (int)first, 0.f);
     return;
   }
-  Drawer<T, NT> d{sh, row, m, 0.f, 0.f, s.inv, mass_bits(a.V)};
-  // a little past the last distance with a mass; at least what a step of the
-  // maximum's own is
-  const double range = (d.S + 2) / s.inv * 1.0001;
-  d.range = (float)fmin(range, 3e38);
-  const float span = fminf(d.range, m - value(low));
-  d.steps = span > 0.f ? fminf((float)(BINS - 1) / span, 3e38f) : 0.f;
+  Drawer<NT> d{sh, m, 0.f, 0.f, s.inv, mass_bits(a.V)};
+  // a little past the last distance with a mass
+  d.range = (float)fmin((d.S + 2) / s.inv * 1.0001, 3e38);
+  d.steps = fminf((float)(BINS - 1) / d.range, 3e38f);
 
-  u64 least = 0;
-  if (s.k) least = d.template last_before<false>((u64)s.k, 0);
+  u64 least = 0, whole = 0;
+  // The candidates: with top-k, what is within the step that holds the k-th of the
+  // threads' own maxima, which is at least the k-th class; with top-p alone, what
+  // is within the step in which the mass passes it.
+  int n = CANDIDATES + 1;
+  const bool by_k = s.k && s.k <= NT / 2 && s.k <= CANDIDATES / 2;
+  if (by_k || (!s.k && s.p < 1.0)) {
+    d.clear(!by_k);
+    if (by_k) {
+      if (d.counts(hi)) atomicAdd(&sh.count[d.step_of(hi)], 1u);
+    } else {
+      row.each([&](float x, int) {
+        if (!d.counts(x)) return;
+        const u64 w = d.mass(x);
+        whole += w;
+        const int b = d.step_of(x);
+        atomicAdd(&sh.count[b], 1u);
+        atomicAdd(&sh.mass[b], w);
+      });
+      whole = block_fold<NT>(whole, sh.wave_a, Sum());
+    }
+    __syncthreads();
+    u64 before = 0;
+    int step = by_k ? d.template last_step<false>((u64)s.k, before)
+                    : d.template last_step<true>(share_of(s.p, whole), before);
+    // fewer than k threads with a class that counts: all that count
+    if (by_k && before + sh.count[step] < (u64)s.k) step = BINS - 1;
+    n = d.collect(row, d.lowest(step));
+  }
   auto kept_mass = [&](float x, int j) -> u64 {
     if (!d.counts(x) || rank_key(x, j) < least) return 0;
     const double t = d.distance(x);
     return t < s.floor ? 0 : mass_of(t, d.S);
   };
-  if (s.p < 1.0) {
-    u64 mass = 0;
-    row.each([&](float x, int j) {
-      if (d.counts(x) && rank_key(x, j) >= least) mass += d.mass(x);
-    });
-    mass = block_fold<NT>(mass, sh.wave_a, Sum());
-    least = d.template last_before<true>(share_of(s.p, mass), least);
+  auto cut = [&](const auto& from) {
+    if (s.k) least = d.template last_before<false>(from, (u64)s.k, 0);
+    if (s.p < 1.0) {
+      if (s.k) {
+        from.each([&](float x, int j) {
+          if (d.counts(x) && rank_key(x, j) >= least) whole += d.mass(x);
+        });
+        whole = block_fold<NT>(whole, sh.wave_a, Sum());
+      }
+      least = d.template last_before<true>(from, share_of(s.p, whole), least);
+    }
+  };
+  if (n <= 64) {
+    if (wave == 0) d.draw_few(a, r, n, s, whole);
+    return;
   }
+  if (n <= CANDIDATES) {
+    const Candidates<NT> few{sh, n};
+    cut(few);
+    int index_bits = 0;
+    while ((int64_t(1) << index_bits) < a.V) ++index_bits;
+    d.draw(a, r, few, s.u, index_bits, kept_mass);
+    return;
+  }
+  cut(row);
 
-  // the running sum: groups of tiles, then the tiles of one group, then the
-  // waves of one tile
-  int t0 = 0, t1 = row.tiles;
+  // the running sum over the whole row in tiles of NT classes: groups of tiles,
+  // then the tiles of one group, then the waves of one tile
+  int t0 = 0, t1 = (a.V + NT - 1) / NT;
   u64 before = 0, mass = 0, target = 0;
   bool first = true;
   for (;;) {
@@ -445,22 +631,14 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += NT) sh.mass[i] = 0;
     __syncthreads();
-    u64 sum = 0;
-    int at = t0;
-    auto put = [&](int tile) {  // the tiles before `tile` are summed
-      const u64 w = wave_fold(sum, Sum());
-      if (lane == 0) sh.mass[(at - t0) / per * WAVES + wave] += w;
-      sum = 0;
-      at = tile;
-    };
-#pragma unroll 1
+#pragma unroll 2
     for (int i = t0; i < t1; ++i) {
-      row.tile(i, [&](float x, int j) { sum += kept_mass(x, j); });
-      put(i + 1);
+      const int j = i * NT + (int)threadIdx.x;
+      const u64 sum = wave_fold(j < a.V ? kept_mass((float)row.x[j], j) : 0, Sum());
+      if (lane == 0) sh.mass[(i - t0) / per * WAVES + wave] += sum;
     }
     __syncthreads();
-    // `groups` of WAVES entries; entries within a group are in the classes'
-    // order where it is one tile
+    // entries within a group are in the classes' order where it is one tile
     const int entries = ((t1 - t0 + per - 1) / per) * WAVES;
     constexpr int PER = BINS / NT;
     u64 w = 0;
@@ -484,46 +662,33 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     }
     __syncthreads();
     const int e = (int)sh.out[0], group = e / WAVES;
+    before = sh.out[1];
     if (per == 1) {
-      before = sh.out[1];
       t0 += group;
       if (wave != e % WAVES) return;
       break;
     }
-    before = sh.out[1];
     for (int i = group * WAVES; i < e; ++i) before -= sh.mass[i];
     t0 += group * per;
     t1 = min(t0 + per, t1);
   }
   // one wave's classes of tile t0
-  constexpr int E = RowOf<T, NT>::E;
-  float xs[E];
-  u64 ws[E], sum = 0;
-  row.tile(t0, [&](float x, int j) {
-    const int e = j - (t0 * RowOf<T, NT>::TILE + (int)threadIdx.x * E);
-    xs[e] = x;
-    ws[e] = kept_mass(x, j);
-    sum += ws[e];
-  });
-  u64 run = sum;
+  const int j = t0 * NT + (int)threadIdx.x;
+  const float x = j < a.V ? (float)row.x[j] : NEG_INF;
+  const u64 own = j < a.V ? kept_mass(x, j) : 0;
+  u64 run = own;
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) {
     const u64 o = __shfl_up(run, i, 64);
     if (lane >= i) run += o;
   }
-  run += before - sum;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (run <= target && run + ws[e] > target)
-      write(a, r, t0 * RowOf<T, NT>::TILE + (int)threadIdx.x * E + e,
-            log_share(d.distance(xs[e]), mass, d.S));
-    run += ws[e];
-  }
+  run += before;
+  if (run > target && run - own <= target) write(a, r, j, log_share(d.distance(x), mass, d.S));
 }
 
-template <class T, int NT>
+template <class T, int NT, int NV>
 void row_go(hipStream_t st, const Sample& a) {
-  sample_row_kernel<T, NT><<<(unsigned)a.rows, NT, 0, st>>>(a);
+  sample_row_kernel<T, NT, NV><<<(unsigned)a.rows, NT, 0, st>>>(a);
 }
 template <class T>
 void go(hipStream_t st, const Sample& a) {
@@ -534,8 +699,11 @@ void go(hipStream_t st, const Sample& a) {
     if (W == 16) sample_few_kernel<T, 16><<<grid, 256, 0, st>>>(a);
     else if (W == 32) sample_few_kernel<T, 32><<<grid, 256, 0, st>>>(a);
     else sample_few_kernel<T, 64><<<grid, 256, 0, st>>>(a);
-  } else if (a.V <= 4 * 256 * E) row_go<T, 256>(st, a);
-  else row_go<T, 1024>(st, a);
+  } else if (a.V <= 256 * E) row_go<T, 256, 1>(st, a);
+  else if (a.V <= 4 * 256 * E) row_go<T, 256, 4>(st, a);
+  else if (a.V <= 4 * 1024 * E) row_go<T, 1024, 4>(st, a);
+  else if (a.V <= 16 * 1024 * E) row_go<T, 1024, 16>(st, a);
+  else row_go<T, 1024, 0>(st, a);
 }
 
 }  // namespace
