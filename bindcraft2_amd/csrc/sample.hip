@@ -252,60 +252,49 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* waves) {  // exclusive
   return before + run - v;
 }
 
-// A row: NV vectors a thread held in registers, for passes of a few instructions a
-// class, or (NV = 0) read at each of those; and for the passes with exponentials
-// a class at a time, whose loads are the least of it.
-template <class T, int NT, int NV>
+// A row, read at each pass: out of the caches after the first.  (Held in registers
+// it needs so many for the vectors' places that they spill: 64 rows of 131 k
+// bfloat16 67 us against 25.)  Passes of a few instructions a class take vectors;
+// those with exponentials take a class at a time, their loads are the least of it.
+template <class T, int NT>
 struct RowOf {
   static constexpr int E = Vec<T>::N;
   const T* x;
   int V;
-  u32x4 held[NV ? NV : 1];
 
-  // A vector that would pass the row's end is read ending there, so that all of a
-  // thread's are in flight together, and its classes that another thread has
-  // are -infinity.
-  __device__ __forceinline__ int first(int i) const { return min((i * NT + (int)threadIdx.x) * E, V - E); }
-  __device__ __forceinline__ u32x4 alone(u32x4 raw, int i) const {
-    if ((int64_t)(i + 1) * NT * E <= V) return raw;  // the same for all threads
-    float v[E];
-    Vec<T>::unpack(raw, v);
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = first(i) + e < (i * NT + (int)threadIdx.x) * E ? NEG_INF : v[e];
-    return Vec<T>::pack(v);
-  }
-  __device__ __forceinline__ void init(const T* row, int V_) {
-    x = row;
-    V = V_;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) held[i] = Vec<T>::load(x + first(i));
-#pragma unroll
-    for (int i = 0; i < NV; ++i) held[i] = alone(held[i], i);
-  }
   // f(x, index) of a thread's classes
   template <class F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll 2
     for (int j = threadIdx.x; j < V; j += NT) f((float)x[j], j);
   }
-  // f(classes' values, index of the first) of a thread's vectors
+  // f(classes' values, index of the first, number of the vector) of a thread's
+  // vectors.  One that would pass the row's end is read ending there, and its
+  // classes that another thread has are -infinity.
   template <class F>
   __device__ __forceinline__ void vectors(F f) const {
-    float v[E];
-    if constexpr (NV > 0) {
+    constexpr int AT_ONCE = 4;
+    const int n = (V + NT * E - 1) / (NT * E);
+    auto first = [&](int i) { return min((i * NT + (int)threadIdx.x) * E, V - E); };
+    auto one = [&](u32x4 raw, int i, int u) __attribute__((always_inline)) {
+      float v[E];
+      Vec<T>::unpack(raw, v);
+      const int j = first(i), own = (i * NT + (int)threadIdx.x) * E;
+      if ((int64_t)(i + 1) * NT * E > V) {  // the same for all threads
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        Vec<T>::unpack(held[i], v);
-        f(v, first(i));
+        for (int e = 0; e < E; ++e) v[e] = j + e < own ? NEG_INF : v[e];
       }
-    } else {
-      const int n = (V + NT * E - 1) / (NT * E);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        Vec<T>::unpack(alone(Vec<T>::load(x + first(i)), i), v);
-        f(v, first(i));
-      }
+      f(v, j, u);
+    };
+    int i = 0;
+    for (; i + AT_ONCE <= n; i += AT_ONCE) {
+      u32x4 raw[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) raw[u] = Vec<T>::load(x + first(i + u));
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) one(raw[u], i + u, u);
     }
+    for (; i < n; ++i) one(Vec<T>::load(x + first(i)), i, 0);
   }
 };
 // The classes that a row's draw is among, where they are few: in LDS, in no order.
@@ -432,7 +421,7 @@ struct Drawer {
   // there are.
   template <class R>
   __device__ int collect(const R& row, float low) {
-    row.vectors([&](const float (&v)[R::E], int j) {
+    row.vectors([&](const float (&v)[R::E], int j, int) {
       float top = v[0];
 #pragma unroll
       for (int e = 1; e < R::E; ++e) top = fmaxf(top, v[e]);
@@ -458,32 +447,41 @@ struct Drawer {
     return m - fminf(d * 1.0001f, range) - 1e-6f * fabsf(m);
   }
 
-  // The same as cut and draw, of at most 64 candidates by one wave: ranks and sums
-  // of forerunners by comparing each with all.
+  // The same as cut and draw, of at most 64 candidates by one wave: ranks by value and
+  // by index from comparing each with all, sums of forerunners by scans in
+  // their orders.
   template <class ST>
   __device__ void draw_few(const Sample& a, int64_t r, int n, const ST& s, u64 whole) {
     const int lane = threadIdx.x;
     const float x = lane < n ? sh.x[lane] : NEG_INF;
     const int j = lane < n ? sh.j[lane] : 0x7fffffff;
-    const u64 c = lane < n ? rank_key(x, j) : 0;
+    const uint32_t key = lane < n ? key_of(x) : 0;
     const double t = distance(x);
     u64 w = lane < n && counts(x) ? mass_of(t, S) : 0;
-    if (s.k) {
-      int rank = 0;
-      for (int i = 0; i < n; ++i) rank += lane_value(c, i) > c;
-      if (rank >= s.k) w = 0;
+    int rank = 0, place = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+      const int before = __builtin_amdgcn_readlane(j, i) < j;
+      place += before;
+      rank += k > key || (k == key && before);
     }
+    if (s.k && rank >= s.k) w = 0;
+    auto forerunners = [&](u64 v, int at) {  // by the order that `at` numbers
+      if (lane < n) sh.list_mass[at] = v;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const u64 mine = lane < n ? sh.list_mass[lane] : 0, run = wave_scan(mine, Sum()) - mine;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (lane < n) sh.list_key[lane] = run;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      return lane < n ? sh.list_key[at] : 0;
+    };
     if (s.p < 1.0) {
       if (s.k) whole = wave_fold(w, Sum());
-      const u64 end = share_of(s.p, whole);
-      u64 before = 0;
-      for (int i = 0; i < n; ++i) before += lane_value(c, i) > c ? lane_value(w, i) : 0;
-      if (before >= end) w = 0;
+      if (forerunners(w, rank) >= share_of(s.p, whole)) w = 0;
     }
     if (t < s.floor) w = 0;
-    const u64 mass = wave_fold(w, Sum()), target = target_of(s.u, mass);
-    u64 before = 0;
-    for (int i = 0; i < n; ++i) before += __builtin_amdgcn_readlane(j, i) < j ? lane_value(w, i) : 0;
+    const u64 mass = wave_fold(w, Sum()), target = target_of(s.u, mass), before = forerunners(w, place);
     if (w && before <= target && before + w > target) write(a, r, j, log_share(t, mass, S));
   }
 
@@ -518,26 +516,27 @@ struct Drawer {
   }
 };
 
-template <class T, int NT, int NV>
+template <class T, int NT>
 __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   __shared__ Shared<NT> sh;
   constexpr int WAVES = NT / 64;
   const int64_t r = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  RowOf<T, NT, NV> row;
-  row.init(reinterpret_cast<const T*>(a.x) + r * a.ld, a.V);
+  typedef RowOf<T, NT> R;
+  const R row{reinterpret_cast<const T*>(a.x) + r * a.ld, a.V};
   const Settings s = settings_of(a, r);
   if (threadIdx.x == 0) sh.found = 0;
-  float hi = NEG_INF;
+  // maxima of four parts of a thread's vectors
+  float part[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
   bool nan = false;
-  typedef RowOf<T, NT, NV> R;
-  row.vectors([&](const float (&v)[R::E], int) {
+  row.vectors([&](const float (&v)[R::E], int, int u) {
 #pragma unroll
     for (int e = 0; e < R::E; ++e) {
       nan |= v[e] != v[e];
-      hi = fmaxf(hi, v[e]);
+      part[u] = fmaxf(part[u], v[e]);
     }
   });
+  const float hi = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
   const u64 top = block_fold<NT>(nan ? ~u64(0) : (u64)key_of(hi), sh.wave_a, Max());
   const uint32_t bits = (uint32_t)top;
   const float m = __builtin_bit_cast(float, bits & 0x80000000u ? bits & 0x7fffffffu : ~bits);
@@ -547,7 +546,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   }
   if (s.greedy) {
     u64 first = ~u64(0);
-    row.vectors([&](const float (&v)[R::E], int j) {
+    row.vectors([&](const float (&v)[R::E], int j, int) {
 #pragma unroll
       for (int e = 0; e < R::E; ++e)
         if (v[e] == m) first = min(first, (u64)(j + e));
@@ -562,32 +561,45 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   d.steps = fminf((float)(BINS - 1) / d.range, 3e38f);
 
   u64 least = 0, whole = 0;
-  // The candidates: with top-k, what is within the step that holds the k-th of the
-  // threads' own maxima, which is at least the k-th class; with top-p alone, what
-  // is within the step in which the mass passes it.
+  // The candidates: with top-k, what is at least the k-th of the maxima of the
+  // threads' parts, but for a coarse step, which the k-th class is; with top-p
+  // alone, what is within the step in which the mass passes it.
   int n = CANDIDATES + 1;
-  const bool by_k = s.k && s.k <= NT / 2 && s.k <= CANDIDATES / 2;
-  if (by_k || (!s.k && s.p < 1.0)) {
-    d.clear(!by_k);
-    if (by_k) {
-      if (d.counts(hi)) atomicAdd(&sh.count[d.step_of(hi)], 1u);
-    } else {
-      row.each([&](float x, int) {
-        if (!d.counts(x)) return;
-        const u64 w = d.mass(x);
-        whole += w;
-        const int b = d.step_of(x);
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd(&sh.mass[b], w);
-      });
-      whole = block_fold<NT>(whole, sh.wave_a, Sum());
-    }
+  const bool by_k = s.k && s.k <= 2 * NT && s.k <= CANDIDATES / 2;
+  if (by_k) {
+    constexpr int COARSE = 4, BINS_K = BINS / COARSE, PER = BINS_K / 64;
+    for (int i = threadIdx.x; i < BINS_K; i += NT) sh.count[i] = 0;
     __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (d.counts(part[u])) atomicAdd(&sh.count[d.step_of(part[u]) / COARSE], 1u);
+    __syncthreads();
+    // each wave for itself
+    uint32_t own = 0, c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) own += c[i] = sh.count[lane * PER + i];
+    u64 run = wave_scan((u64)own, Sum()) - own;
+    int step = BINS_K;  // fewer than k parts that count: all classes that do
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (run < (u64)s.k && run + c[i] >= (u64)s.k) step = lane * PER + i;
+      run += c[i];
+    }
+    step = (int)wave_fold((u64)step, Min());
+    n = d.collect(row, d.lowest(min(step * COARSE + COARSE - 1, BINS - 1)));
+  } else if (!s.k && s.p < 1.0) {
+    d.clear(true);
+    row.each([&](float x, int) {
+      if (!d.counts(x)) return;
+      const u64 w = d.mass(x);
+      whole += w;
+      const int b = d.step_of(x);
+      atomicAdd(&sh.count[b], 1u);
+      atomicAdd(&sh.mass[b], w);
+    });
+    whole = block_fold<NT>(whole, sh.wave_a, Sum());
     u64 before = 0;
-    int step = by_k ? d.template last_step<false>((u64)s.k, before)
-                    : d.template last_step<true>(share_of(s.p, whole), before);
-    // fewer than k threads with a class that counts: all that count
-    if (by_k && before + sh.count[step] < (u64)s.k) step = BINS - 1;
+    const int step = d.template last_step<true>(share_of(s.p, whole), before);
     n = d.collect(row, d.lowest(step));
   }
   auto kept_mass = [&](float x, int j) -> u64 {
@@ -686,9 +698,9 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   if (run > target && run - own <= target) write(a, r, j, log_share(d.distance(x), mass, d.S));
 }
 
-template <class T, int NT, int NV>
+template <class T, int NT>
 void row_go(hipStream_t st, const Sample& a) {
-  sample_row_kernel<T, NT, NV><<<(unsigned)a.rows, NT, 0, st>>>(a);
+  sample_row_kernel<T, NT><<<(unsigned)a.rows, NT, 0, st>>>(a);
 }
 template <class T>
 void go(hipStream_t st, const Sample& a) {
@@ -699,11 +711,9 @@ void go(hipStream_t st, const Sample& a) {
     if (W == 16) sample_few_kernel<T, 16><<<grid, 256, 0, st>>>(a);
     else if (W == 32) sample_few_kernel<T, 32><<<grid, 256, 0, st>>>(a);
     else sample_few_kernel<T, 64><<<grid, 256, 0, st>>>(a);
-  } else if (a.V <= 256 * E) row_go<T, 256, 1>(st, a);
-  else if (a.V <= 4 * 256 * E) row_go<T, 256, 4>(st, a);
-  else if (a.V <= 4 * 1024 * E) row_go<T, 1024, 4>(st, a);
-  else if (a.V <= 16 * 1024 * E) row_go<T, 1024, 16>(st, a);
-  else row_go<T, 1024, 0>(st, a);
+  } else if (a.V <= 16 * 256 * E) row_go<T, 256>(st, a);
+  else if (a.rows > device_cus()) row_go<T, 512>(st, a);
+  else row_go<T, 1024>(st, a);
 }
 
 }  // namespace
