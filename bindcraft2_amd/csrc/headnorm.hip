@@ -85,22 +85,44 @@ __device__ __forceinline__ Unit unit_of(const HeadNorm& p, int u) {
 }
 
 // cos and sin of position * freq.  The product is taken in 64 bits (exact for
-// positions below 2^29; one of 10^6 would lose a tenth of a radian in 32) and cut
-// to half a turn there; the rest is good to 2^-25 of one.
+// positions below 2^29; one of 10^6 would lose a tenth of a radian in 32), in
+// turns, and whole turns leave there; the rest is good to 2^-26 of one.  Then
+// quarters of a turn, and the series of both for an eighth at most, which end
+// below 2^-29 (a library call for both, with its own reductions, takes twice the
+// instructions).
 template <int N>
 struct Turn {
+  double f[N];  // a lane's frequencies in turns; 0 where it does not rotate
   float c[N], s[N];
-  __device__ __forceinline__ void make(const HeadNorm& p, const Unit& u, int64_t t) {
-    const double pos = p.pos64 ? (double)reinterpret_cast<const int64_t*>(p.pos)[t]
-                               : (double)reinterpret_cast<const int32_t*>(p.pos)[t];
+  __device__ __forceinline__ void init(const HeadNorm& p, const Unit& u) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      f[i] = i < u.turned ? (double)p.freq[u.pair + i] * 0.15915494309189535 : 0.0;
+  }
+  __device__ __forceinline__ double position(const HeadNorm& p, int64_t t) const {
+    if (!p.pos) return 0.0;
+    return p.pos64 ? (double)reinterpret_cast<const int64_t*>(p.pos)[t]
+                   : (double)reinterpret_cast<const int32_t*>(p.pos)[t];
+  }
+  __device__ __forceinline__ void make(double pos) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      c[i] = 1.f;
-      s[i] = 0.f;
-      if (i < u.turned) {
-        const double half_turns = pos * (double)p.freq[u.pair + i] * 0.31830988618379067;
-        sincospif((float)(half_turns - 2.0 * rint(0.5 * half_turns)), &s[i], &c[i]);
-      }
+      const double turns = pos * f[i];
+      const float t = (float)(turns - rint(turns)), q = rintf(4.f * t), r = fmaf(4.f, t, -q), z = r * r;
+      // of r quarters: powers of pi / 2 over factorials
+      float sn = fmaf(z, 1.6044118e-4f, -4.6817541e-3f);
+      sn = fmaf(z, sn, 7.9692626e-2f);
+      sn = fmaf(z, sn, -6.4596410e-1f);
+      sn = r * fmaf(z, sn, 1.5707963e0f);
+      float cs = fmaf(z, -2.5202042e-5f, 9.1926028e-4f);
+      cs = fmaf(z, cs, -2.0863481e-2f);
+      cs = fmaf(z, cs, 2.5366951e-1f);
+      cs = fmaf(z, cs, -1.2337005e0f);
+      cs = fmaf(z, cs, 1.f);
+      const int k = (int)q;
+      const float a = k & 1 ? cs : sn, b = k & 1 ? sn : cs;
+      s[i] = k & 2 ? -a : a;
+      c[i] = (k + 1) & 2 ? -b : b;
     }
   }
 };
@@ -130,65 +152,82 @@ __device__ __forceinline__ void rotate(const Turn<N>& t, bool interleaved, float
 }
 
 template <int N>
-__device__ __forceinline__ void load_weight(const HeadNorm& p, int which, const Unit& u, float* a,
-                                            float* b) {
+__device__ __forceinline__ void load_weight(const HeadNorm& p, int which, const Unit& u, float (&a)[N],
+                                            float (&b)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e[2] = {u.a + i, u.b + i};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float v = 0.f;
-      if (u.live) {
-        if (p.weight_dtype == BC2N_F32) v = reinterpret_cast<const float*>(p.weight[which])[e[j]];
-        else if (p.weight_dtype == BC2N_F16) v = (float)reinterpret_cast<const h16*>(p.weight[which])[e[j]];
-        else v = (float)reinterpret_cast<const bf16*>(p.weight[which])[e[j]];
-      }
-      (j ? b : a)[i] = v;
-    }
-  }
+  for (int i = 0; i < N; ++i) a[i] = b[i] = 0.f;
+  if (!u.live || !p.heads[which]) return;
+  auto load = [&](auto type) {
+    typedef decltype(type) T;
+    Few<T, N>::template load<false>(reinterpret_cast<const T*>(p.weight[which]) + u.a, a);
+    Few<T, N>::template load<false>(reinterpret_cast<const T*>(p.weight[which]) + u.b, b);
+  };
+  if (p.weight_dtype == BC2N_F32) load(float());
+  else if (p.weight_dtype == BC2N_F16) load(h16());
+  else load(bf16());
 }
 
-// A wave: one token and `per` rounds of 64 / W heads from the blockIdx.y-th
-// share of them, queries first, then keys.
+// Waves walk the tokens; each takes `per` rounds of 64 / W heads of a token, the
+// blockIdx.y-th share of them, first the queries' `q_rounds`, then the keys'.  The
+// first round's loads are issued ahead of the angles, each other's ahead of the
+// work before it.
 template <class T, int N>
-__global__ __launch_bounds__(NT) void headnorm_fwd_kernel(HeadNorm p, int W, int per) {
+__global__ __launch_bounds__(NT) void headnorm_fwd_kernel(HeadNorm p, int W, int q_rounds, int rounds, int per) {
   const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
-  if (t >= p.tokens) return;
   const Unit u = unit_of<N>(p, lane & (W - 1));
+  const int step = 64 / W, mine = lane / W;
+  const int r0 = blockIdx.y * per, r1 = min(rounds, r0 + per);
   Turn<N> turn;
-  turn.make(p, u, t);
-  const int step = 64 / W, all = p.heads[0] + p.heads[1];
-  const int h0 = blockIdx.y * per * step + lane / W, h1 = min(all, (int)(blockIdx.y + 1) * per * step);
+  turn.init(p, u);
   const float inv = 1.f / (float)p.width;
   float wa[2][N], wb[2][N];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (p.heads[k]) load_weight<N>(p, k, u, wa[k], wb[k]);
-  }
-  for (int h = h0; h < h1; h += step) {
-    const int k = h >= p.heads[0];
-    const int g = k ? h - p.heads[0] : h;
-    float a[N] = {}, b[N] = {};
-    const T* x = at<const T>(k ? p.x[1] : p.x[0], t, g);
-    if (u.live) {
-      Few<T, N>::template load<false>(x + u.a, a);
-      Few<T, N>::template load<false>(x + u.b, b);
-    }
-    float s = 0.f;
+  for (int k = 0; k < 2; ++k) load_weight<N>(p, k, u, wa[k], wb[k]);
+  for (int64_t t = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6); t < p.tokens;
+       t += (int64_t)gridDim.x * WAVES) {
+    float na[N] = {}, nb[N] = {};
+    // the head of a lane in round r, the same tensor for all lanes
+    auto fetch = [&](int r) __attribute__((always_inline)) {
+      if (r >= r1) return;
+      auto from = [&](const HeadView& v, int h, int heads) __attribute__((always_inline)) {
+        if (h >= heads || !u.live) return;
+        const T* x = at<const T>(v, t, h);
+        Few<T, N>::template load<false>(x + u.a, na);
+        Few<T, N>::template load<false>(x + u.b, nb);
+      };
+      if (r < q_rounds) from(p.x[0], r * step + mine, p.heads[0]);
+      else from(p.x[1], (r - q_rounds) * step + mine, p.heads[1]);
+    };
+    auto round = [&](int r, const HeadView& v, int h, int heads, const float (&wa)[N], const float (&wb)[N])
+                     __attribute__((always_inline)) {
+      float a[N], b[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(a[i], a[i], fmaf(b[i], b[i], s));
-    const float r = rsqrtf(fmaf(sum_lanes(s, W), inv, p.eps));
+      for (int i = 0; i < N; ++i) {
+        a[i] = na[i];
+        b[i] = nb[i];
+      }
+      fetch(r + 1);
+      float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      a[i] = a[i] * r * (k ? wa[1][i] : wa[0][i]);
-      b[i] = b[i] * r * (k ? wb[1][i] : wb[0][i]);
-    }
-    rotate<N, false>(turn, p.interleaved, a, b);
-    if (u.live) {
-      T* y = at<T>(k ? p.out[1] : p.out[0], t, g);
-      Few<T, N>::template store<false>(y + u.a, a);
-      Few<T, N>::template store<false>(y + u.b, b);
+      for (int i = 0; i < N; ++i) s = fmaf(a[i], a[i], fmaf(b[i], b[i], s));
+      const float scale = rsqrtf(fmaf(sum_lanes(s, W), inv, p.eps));
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        a[i] = a[i] * scale * wa[i];
+        b[i] = b[i] * scale * wb[i];
+      }
+      rotate<N, false>(turn, p.interleaved, a, b);
+      if (h < heads && u.live) {
+        T* y = at<T>(v, t, h);
+        Few<T, N>::template store<false>(y + u.a, a);
+        Few<T, N>::template store<false>(y + u.b, b);
+      }
+    };
+    fetch(r0);
+    turn.make(turn.position(p, t));
+    for (int r = r0; r < r1; ++r) {
+      if (r < q_rounds) round(r, p.out[0], r * step + mine, p.heads[0], wa[0], wb[0]);
+      else round(r, p.out[1], (r - q_rounds) * step + mine, p.heads[1], wa[1], wb[1]);
     }
   }
 }
@@ -205,12 +244,11 @@ __global__ __launch_bounds__(NT) void headnorm_bwd_kernel(HeadNorm p, int W, flo
   float da[2][N] = {}, db[2][N] = {};
   float wa[2][N], wb[2][N];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (p.heads[k]) load_weight<N>(p, k, u, wa[k], wb[k]);
-  }
+  for (int k = 0; k < 2; ++k) load_weight<N>(p, k, u, wa[k], wb[k]);
+  Turn<N> turn;
+  turn.init(p, u);
   for (int64_t t = (int64_t)blockIdx.x * WAVES + wave; t < p.tokens; t += (int64_t)gridDim.x * WAVES) {
-    Turn<N> turn;
-    turn.make(p, u, t);
+    turn.make(turn.position(p, t));
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       for (int h = lane / W; h < p.heads[k]; h += step) {
@@ -272,22 +310,25 @@ __global__ __launch_bounds__(NT) void headnorm_bwd_kernel(HeadNorm p, int W, flo
   }
 }
 
-// d_weight from the workgroups' partial sums, in a fixed order: 16 columns a
-// workgroup, 16 threads a column.
+// d_weight from the workgroups' partial sums, in a fixed order: 4 columns a
+// workgroup, 64 threads a column.
 __global__ __launch_bounds__(NT) void headnorm_join_kernel(HeadNorm p, const float* partial, int parts) {
-  __shared__ double sums[16][17];
-  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
-  const int e = blockIdx.x * 16 + c, D = p.width;
+  __shared__ double sums[4][65];
+  const int c = threadIdx.x & 3, r = threadIdx.x >> 2;
+  const int e = blockIdx.x * 4 + c, D = p.width;
   double s = 0;
-  if (e < 2 * D)
-    for (int i = r; i < parts; i += 16) s += partial[(int64_t)i * 2 * D + e];
-  sums[r][c] = s;
+  if (e < 2 * D) {
+#pragma unroll 8
+    for (int i = r; i < parts; i += 64) s += partial[(int64_t)i * 2 * D + e];
+  }
+  sums[c][r] = s;
   __syncthreads();
-  if (r == 0 && e < 2 * D) {
+  if (threadIdx.x < 4 && blockIdx.x * 4 + threadIdx.x < 2 * D) {
+    const int col = blockIdx.x * 4 + threadIdx.x;
     s = 0;
-    for (int i = 0; i < 16; ++i) s += sums[i][c];
-    const int k = e >= D;
-    if (p.d_weight[k]) p.d_weight[k][e - k * D] = (float)s;
+    for (int i = 0; i < 64; ++i) s += sums[threadIdx.x][i];
+    const int k = col >= D;
+    if (p.d_weight[k]) p.d_weight[k][col - k * D] = (float)s;
   }
 }
 
@@ -339,12 +380,15 @@ void headnorm_fwd(hipStream_t st, const HeadNorm& a) {
   if (a.tokens == 0) return;
   KTimed kt("headnorm.fwd", st);
   by_type(a, [&](auto v, auto n) {
-    const int W = lanes(a, n), rounds = (a.heads[0] + a.heads[1] + 64 / W - 1) / (64 / W);
+    const int W = lanes(a, n), step = 64 / W;
+    const int q_rounds = (a.heads[0] + step - 1) / step, rounds = q_rounds + (a.heads[1] + step - 1) / step;
     // All heads by one wave make the angles once; few tokens spread their heads.
     int per = rounds;
     while (per > 1 && a.tokens * ((rounds + per - 1) / per) < 8 * (int64_t)device_cus()) per = (per + 1) / 2;
-    const dim3 grid((unsigned)((a.tokens + WAVES - 1) / WAVES), (rounds + per - 1) / per);
-    headnorm_fwd_kernel<decltype(v), n><<<grid, NT, 0, st>>>(a, W, per);
+    // eight workgroups a CU, what its registers hold twice over
+    const int64_t blocks = std::min<int64_t>((a.tokens + WAVES - 1) / WAVES, 8 * (int64_t)device_cus());
+    const dim3 grid((unsigned)blocks, (rounds + per - 1) / per);
+    headnorm_fwd_kernel<decltype(v), n><<<grid, NT, 0, st>>>(a, W, q_rounds, rounds, per);
   });
 }
 
@@ -357,7 +401,7 @@ void headnorm_bwd(hipStream_t st, const HeadNorm& a, void* work) {
     const size_t lds = (size_t)WAVES * (64 / W) * 2 * D * 4;
     headnorm_bwd_kernel<decltype(v), n><<<blocks, NT, lds, st>>>(a, W, partial);
   });
-  headnorm_join_kernel<<<(2 * D + 15) / 16, NT, 0, st>>>(a, partial, a.tokens ? blocks : 0);
+  headnorm_join_kernel<<<(2 * D + 3) / 4, NT, 0, st>>>(a, partial, a.tokens ? blocks : 0);
   hip_check(hipGetLastError(), "headnorm launch");
 }
 

@@ -361,21 +361,25 @@ struct Drawer {
 
   // The rank key of the last class of `from` whose forerunners, among those of
   // rank keys >= least, weigh less than `end`: by number, or (MASS) by mass.
+  // filled: the first pass's counts and masses are there.
   template <bool MASS, class S_>
-  __device__ u64 last_before(const S_& from, u64 end, u64 least) {
+  __device__ u64 last_before(const S_& from, u64 end, u64 least, bool filled = false) {
     u64 lo = 0, hi = ~u64(0), before = 0;
     int shift = -1;  // -1: steps of distance
     for (;;) {
-      clear(MASS);
+      if (!filled) clear(MASS);
       auto bin_of = [&](float x, u64 c) { return shift < 0 ? step_of(x) : (int)((hi - c) >> shift); };
-      from.each([&](float x, int j) {
-        if (!counts(x)) return;
-        const u64 c = rank_key(x, j);
-        if (c < least || c < lo || c > hi) return;
-        const int b = bin_of(x, c);
-        atomicAdd(&sh.count[b], 1u);
-        if (MASS) atomicAdd(&sh.mass[b], mass(x));
-      });
+      if (!filled) {
+        from.each([&](float x, int j) {
+          if (!counts(x)) return;
+          const u64 c = rank_key(x, j);
+          if (c < least || c < lo || c > hi) return;
+          const int b = bin_of(x, c);
+          atomicAdd(&sh.count[b], 1u);
+          if (MASS) atomicAdd(&sh.mass[b], mass(x));
+        });
+      }
+      filled = false;
       __syncthreads();
       const int bin = last_step<MASS>(end, before);
       const uint32_t in_bin = sh.count[bin];
@@ -607,7 +611,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     const double t = d.distance(x);
     return t < s.floor ? 0 : mass_of(t, d.S);
   };
-  auto cut = [&](const auto& from) {
+  auto cut = [&](const auto& from, bool filled) {
     if (s.k) least = d.template last_before<false>(from, (u64)s.k, 0);
     if (s.p < 1.0) {
       if (s.k) {
@@ -616,7 +620,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
         });
         whole = block_fold<NT>(whole, sh.wave_a, Sum());
       }
-      least = d.template last_before<true>(from, share_of(s.p, whole), least);
+      least = d.template last_before<true>(from, share_of(s.p, whole), least, filled);
     }
   };
   if (n <= 64) {
@@ -625,17 +629,18 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   }
   if (n <= CANDIDATES) {
     const Candidates<NT> few{sh, n};
-    cut(few);
+    cut(few, false);
     int index_bits = 0;
     while ((int64_t(1) << index_bits) < a.V) ++index_bits;
     d.draw(a, r, few, s.u, index_bits, kept_mass);
     return;
   }
-  cut(row);
+  cut(row, !by_k && !s.k);
 
-  // the running sum over the whole row in tiles of NT classes: groups of tiles,
-  // then the tiles of one group, then the waves of one tile
-  int t0 = 0, t1 = (a.V + NT - 1) / NT;
+  // the running sum over the whole row in tiles of OWN classes a thread: groups of
+  // tiles, then the tiles of one group, then the waves of one tile
+  constexpr int OWN = 8, TILE = OWN * NT;
+  int t0 = 0, t1 = (a.V + TILE - 1) / TILE;
   u64 before = 0, mass = 0, target = 0;
   bool first = true;
   for (;;) {
@@ -643,10 +648,12 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += NT) sh.mass[i] = 0;
     __syncthreads();
-#pragma unroll 2
     for (int i = t0; i < t1; ++i) {
-      const int j = i * NT + (int)threadIdx.x;
-      const u64 sum = wave_fold(j < a.V ? kept_mass((float)row.x[j], j) : 0, Sum());
+      const int j0 = i * TILE + (int)threadIdx.x * OWN;
+      u64 sum = 0;
+#pragma unroll 2
+      for (int j = j0; j < min(j0 + OWN, a.V); ++j) sum += kept_mass((float)row.x[j], j);
+      sum = wave_fold(sum, Sum());
       if (lane == 0) sh.mass[(i - t0) / per * WAVES + wave] += sum;
     }
     __syncthreads();
@@ -685,17 +692,17 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     t1 = min(t0 + per, t1);
   }
   // one wave's classes of tile t0
-  const int j = t0 * NT + (int)threadIdx.x;
-  const float x = j < a.V ? (float)row.x[j] : NEG_INF;
-  const u64 own = j < a.V ? kept_mass(x, j) : 0;
-  u64 run = own;
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) {
-    const u64 o = __shfl_up(run, i, 64);
-    if (lane >= i) run += o;
+  const int j0 = t0 * TILE + (int)threadIdx.x * OWN;
+  u64 own = 0;
+  for (int j = j0; j < min(j0 + OWN, a.V); ++j) own += kept_mass((float)row.x[j], j);
+  u64 run = before + wave_scan(own, Sum()) - own;
+  if (run > target || run + own <= target) return;
+  for (int j = j0; j < min(j0 + OWN, a.V); ++j) {  // one thread's
+    const float x = (float)row.x[j];
+    const u64 w = kept_mass(x, j);
+    if (run <= target && run + w > target) write(a, r, j, log_share(d.distance(x), mass, d.S));
+    run += w;
   }
-  run += before;
-  if (run > target && run - own <= target) write(a, r, j, log_share(d.distance(x), mass, d.S));
 }
 
 template <class T, int NT>
