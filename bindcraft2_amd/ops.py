@@ -892,8 +892,9 @@ class LogProbs:
 
 def _heads(t, what, dtype=None, shape=None):
     """(address, token stride, head stride) of [tokens, heads, width]."""
-    if t.dim() != 3 or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError(f"{what}: expected {shape or '[tokens, heads, width]'}, got {tuple(t.shape)}")
+    if t.dim() != 3 or (shape is not None and t.shape != shape):
+        want = "[tokens, heads, width]" if shape is None else tuple(shape)
+        raise ValueError(f"{what}: expected {want}, got {tuple(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
     _current(t, what)
@@ -901,6 +902,12 @@ def _heads(t, what, dtype=None, shape=None):
     if e != 1 and t.shape[2] > 1:
         raise ValueError(f"{what}: a head's elements must be contiguous")
     return t.data_ptr(), st, sh
+
+
+def _new_heads(t):
+    """A new contiguous tensor like t, and its (address, token stride, head stride)."""
+    out = torch.empty_like(t, memory_format=torch.contiguous_format)
+    return out, (out.data_ptr(), t.shape[1] * t.shape[2], t.shape[2])
 
 
 def _vector(t, n, dtypes, what):
@@ -942,6 +949,8 @@ class HeadNormRotate:
         _current(self.freq, "freq")
         qw, kw = _vector(q_weight, width, (torch.float32, q.dtype), "q_weight"), None
         if k is not None:
+            if k.dim() != 3 or k.shape[0] != n or k.shape[2] != width:
+                raise ValueError(f"k: expected [{n}, heads, {width}], got {tuple(k.shape)}")
             kw = _vector(k_weight, width, (wt,), "k_weight")
         return ((_DTYPES[q.dtype], n, heads, 0 if k is None else k.shape[1], width, 2 * pairs, self.interleaved),
                 (at, 64 if positions.dtype == torch.int64 else 32, self.freq.data_ptr(), qw, kw, _DTYPES[wt],
@@ -950,24 +959,27 @@ class HeadNormRotate:
     @staticmethod
     def _pair(q, k, like_q, like_k, what):
         """The six operands of queries and keys, checked against the inputs."""
-        a = _heads(q, what[0], like_q.dtype, tuple(like_q.shape))
+        a = _heads(q, what[0], like_q.dtype, like_q.shape)
         if like_k is None:
             return (*a, None, 0, 0)
-        if like_k.dim() != 3 or like_k.shape[0] != like_q.shape[0] or like_k.shape[2] != like_q.shape[2]:
-            raise ValueError(f"k: expected [{like_q.shape[0]}, heads, {like_q.shape[2]}], got {tuple(like_k.shape)}")
-        return (*a, *_heads(k, what[1], like_q.dtype, tuple(like_k.shape)))
+        return a + _heads(k, what[1], like_q.dtype, like_k.shape)
+
+    def _results(self, out, q, k):
+        """(results, the calls' six operands of them)"""
+        if out is not None:
+            return tuple(out), self._pair(*out, q, k, ("out", "out"))
+        a, x = _new_heads(q)
+        b, y = (None, (None, 0, 0)) if k is None else _new_heads(k)
+        return (a, b), x + y
 
     def forward(self, q, k, positions, q_weight, k_weight=None, out=None):
         """-> (q, k) normed and rotated, in new tensors or in out = (q, k), which
         may be the inputs; without k, k is None"""
         first, last = self._operands(q, k, positions, q_weight, k_weight)
         x = self._pair(q, k, q, k, ("q", "k"))
-        if out is None:
-            out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-                   None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
-        y = self._pair(*out, q, k, ("out", "out"))
+        out, y = self._results(out, q, k)
         check(lib().bc2n_headnorm_fwd(_stream(), *first, *x, *last, *y))
-        return tuple(out)
+        return out
 
     def backward(self, cts, q, k, positions, q_weight, k_weight=None, out=None):
         """cts = (d_q, d_k), q and k the forward's inputs -> (d_q, d_k, d_q_weight,
@@ -976,10 +988,7 @@ class HeadNormRotate:
         first, last = self._operands(q, k, positions, q_weight, k_weight)
         x = self._pair(q, k, q, k, ("q", "k"))
         d = self._pair(*cts, q, k, ("d_q", "d_k"))
-        if out is None:
-            out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-                   None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
-        y = self._pair(*out, q, k, ("out", "out"))
+        out, y = self._results(out, q, k)
         width, dev = q.shape[2], q.device
         dw = torch.empty(2, width, dtype=torch.float32, device=dev)
         work = torch.empty(lib().bc2n_headnorm_work_bytes(q.shape[0], width), dtype=torch.uint8, device=dev)
@@ -1014,7 +1023,7 @@ class PackedAttention:
         n, heads, width = q.shape
         if k.dim() != 3 or k.shape[2] != width or k.shape[1] == 0 or heads == 0 or heads % k.shape[1]:
             raise ValueError(f"k: expected [tokens, a divisor of {heads}, {width}], got {tuple(k.shape)}")
-        x = _heads(q, "q") + _heads(k, "k", q.dtype) + _heads(v, "v", q.dtype, tuple(k.shape))
+        x = _heads(q, "q") + _heads(k, "k", q.dtype) + _heads(v, "v", q.dtype, k.shape)
         i32 = (torch.int32,)
         count = q_offsets.shape[0] - 1 if q_offsets.dim() == 1 else -1
         if count < 0:
@@ -1035,8 +1044,9 @@ class PackedAttention:
         sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths)
         fill = out is None
         if fill:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        o = _heads(out, "out", q.dtype, tuple(q.shape))
+            out, o = _new_heads(q)
+        else:
+            o = _heads(out, "out", q.dtype, q.shape)
         lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
         work = self._work(lib().bc2n_attention_fwd_work_bytes, sizes, q.device)
         check(lib().bc2n_attention_fwd(_stream(), *sizes, *where, *x, int(fill), *o, lse.data_ptr(), _ptr(work)))
@@ -1052,20 +1062,20 @@ class PackedAttention:
         """out and lse the forward's -> (d_q, d_k, d_v), in grads = (d_q, d_k, d_v)
         where given"""
         sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths)
-        shape = tuple(q.shape)
+        shape = q.shape
         g, o = _heads(d_out, "d_out", q.dtype, shape), _heads(out, "out", q.dtype, shape)
         _f32(lse, (shape[1], shape[0]), "lse")
         if not _current(lse, "lse").is_contiguous():
             raise ValueError("lse: expected a contiguous tensor")
         fill = grads is None
         if fill:
-            grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        d = ()
-        for t, like, what in zip(grads, (q, k, v), ("d_q", "d_k", "d_v")):
-            d += _heads(t, what, q.dtype, tuple(like.shape))
+            grads, d = zip(*map(_new_heads, (q, k, v)))
+        else:
+            d = [_heads(t, what, q.dtype, like.shape)
+                 for t, like, what in zip(grads, (q, k, v), ("d_q", "d_k", "d_v"))]
         work = self._work(lib().bc2n_attention_bwd_work_bytes, sizes, q.device)
-        check(lib().bc2n_attention_bwd(_stream(), *sizes, *where, *g, *x, *o, lse.data_ptr(), int(fill), *d,
-                                       _ptr(work)))
+        check(lib().bc2n_attention_bwd(_stream(), *sizes, *where, *g, *x, *o, lse.data_ptr(), int(fill), *d[0],
+                                       *d[1], *d[2], _ptr(work)))
         return tuple(grads)
 
 
