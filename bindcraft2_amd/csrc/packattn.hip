@@ -1353,7 +1353,7 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
           p = Half<T>::mma(f[4 * ks], f[4 * ks + 1], p);
           d = Half<T>::mma(f[4 * ks + 2], f[4 * ks + 3], d);
         }
-        constexpr int AHEAD = 2;  // steps of the width
+        constexpr int AHEAD = 1;  // steps of the width
         order<LDS_READ, 4 * AHEAD>();
 #pragma unroll
         for (int i = 0; i < KS - AHEAD; ++i) {

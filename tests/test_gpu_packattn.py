@@ -122,6 +122,73 @@ def test_no_tokens_and_no_sequences(cuda):
     Problem([], 2, 1, 64, spare=70).verify()
 
 
+WIDE = [(300, 300), (0, 7), (130, 130), (70, 200), (90, 30), (3, 0)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [16, 40, 64, 72, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_that_fill_the_card(cuda, causal, d, dtype):
+    """128-row workgroups: with as many heads as here, from a few hundred tokens."""
+    print(f"rows {d} {dtype} {causal}", flush=True)
+    Problem(WIDE, 64, 64, d, TYPES[dtype], causal, d).verify()
+    Problem(WIDE[:4], 192, 64, d, TYPES[dtype], causal, d).verify()
+
+
+def test_rows_that_fill_the_card_padded(cuda):
+    lengths = [(200, 200), (0, 0), (64, 40), (17, 40), (0, 30), (12, 0), (300, 301)]
+    for fill in (True, False):
+        p = Problem(lengths, 64, 64, 32, torch.bfloat16, True, q_cap=300, k_cap=301, spare=150)
+        if fill:
+            p.verify()
+            continue
+        out = torch.full_like(p.q, 7.0)
+        _, lse = p.op.forward(p.q, p.k, p.v, *p.where(), out=out)
+        grads = tuple(torch.full_like(t, 7.0) for t in (p.q, p.k, p.v))
+        p.op.backward(p.d_out, p.q, p.k, p.v, out, lse, *p.where(), grads=grads)
+        p.verify(dict(zip(("out", "d_q", "d_k", "d_v"), (out, *grads))), rest=7.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,d", [(8, 1, 64), (2, 2, 128), (12, 3, 32), (64, 64, 16), (40, 1, 24), (1, 1, 104)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_long_caches(cuda, causal, heads, kv, d, dtype):
+    """Keys in stretches over workgroups, joined: few and many of them a row."""
+    print(f"caches {heads} {kv} {d} {dtype} {causal}", flush=True)
+    Problem([(1, 20000)], heads, kv, d, TYPES[dtype], causal, 1).verify()
+    Problem([(1, 5000), (3, 70), (0, 9), (2, 0), (1, 1), (5, 4097), (1, 300)], heads, kv, d, TYPES[dtype], causal,
+            2).verify()
+
+
+def test_long_caches_of_fixed_capacity(cuda):
+    lengths = [(1, n) for n in (1, 0, 700, 2048, 31, 33, 257, 2047)]
+    p = Problem(lengths, 8, 2, 64, torch.bfloat16, True, k_cap=2048, spare=40)
+    p.verify()
+    out = torch.full_like(p.q, 7.0)
+    p.op.forward(p.q, p.k, p.v, *p.where(), out=out)
+    p.verify({"out": out}, rest=7.0)
+
+
+@pytest.mark.parametrize("count", [61, 62, 63, 200, 300, 1000])
+def test_many_caches(cuda, count):
+    """One query each: held in a wave's lanes to 256 entries, read again beyond."""
+    g = torch.Generator().manual_seed(count)
+    lengths = [(1, n) for n in torch.randint(0, 90000 // count, (count,), generator=g).tolist()]
+    p = Problem(lengths, 4, 2, 32, torch.float16, True)
+    out, lse = p.op.forward(p.q, p.k, p.v, *p.where())
+    assert not out.isnan().any()
+    for b in sorted({0, 1, 60, count // 2, count - 2, count - 1}):
+        i, j, n = b, int(p.ko[b]), lengths[b][1]
+        want = R.attention(p.q[i:i + 1], p.k[j:j + n], p.v[j:j + n], True, 32 ** -0.5)
+        R.check(f"out of sequence {b}", out[i:i + 1], *want["out"])
+        R.check(f"lse of sequence {b}", lse[:, i:i + 1], *want["lse"])
+
+
+def test_a_wide_row_among_caches(cuda):
+    """More than 32 rows in a sequence beside single tokens."""
+    Problem([(1, 3000), (50, 3000), (1, 10), (1, 1)], 8, 2, 64, torch.bfloat16, True).verify()
+
+
 @pytest.mark.parametrize("count", [63, 64, 65, 300, 5000])
 def test_many_sequences(cuda, count):
     """Searched 64 at a time: one, two and three levels of them."""
@@ -295,18 +362,14 @@ def test_differences(cuda):
     """The gradient formulas against differences of the 64-bit definition."""
     p = Problem([(5, 9)], 4, 2, 16, torch.float16)
     got = p.run()
-    loss = lambda q, k, v: (R.attention(q, k, v, True, 0.25)["out"][0] * p.d_out.double()).sum()  # noqa: E731
     x, h = [t.double() for t in (p.q, p.k, p.v)], 1e-4
-
-    class Wide(torch.Tensor):
-        pass
-    # the definition reads the type for its tolerances alone: give it f32 views of the values
+    # the definition reads the type for its tolerances alone, and f32 holds the steps
     loss32 = lambda xs: (R.attention(*[t.float() for t in xs], True, 0.25)["out"][0] * p.d_out.double()).sum()  # noqa: E731
     for i, name in enumerate(("d_q", "d_k", "d_v")):
         for at in [(0, 0, 0), (3, 1, 7), (4, 0, 15)]:
             up, down = [t.clone() for t in x], [t.clone() for t in x]
-            up[i][at] = torch.tensor(up[i][at] + h).float().double()
-            down[i][at] = torch.tensor(down[i][at] - h).float().double()
+            up[i][at] = (up[i][at] + h).float().double()
+            down[i][at] = (down[i][at] - h).float().double()
             slope = (loss32(up) - loss32(down)) / (up[i][at] - down[i][at])
             # binary16's roundings of P, dS, out and the result: 4 half steps of the
             # terms' size, and h^2
