@@ -423,6 +423,18 @@ __device__ __forceinline__ void store_columns(const f32x16 (&v)[DB], float f, T*
   }
 }
 
+// The same unrounded, to `row` of f32 of DP elements.
+template <int DB>
+__device__ __forceinline__ void store_sums(const f32x16 (&v)[DB], float f, float* row, int lane) {
+  if (!row) return;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<float4*>(row + 32 * db + 8 * i + 4 * (lane >> 5)) =
+          make_float4(v[db][4 * i] * f, v[db][4 * i + 1] * f, v[db][4 * i + 2] * f, v[db][4 * i + 3] * f);
+}
+
 // A wave's 32 rows of a problem's G heads: a lane's own.
 struct Row {
   int i, g;     // token in the sequence, head in the group
@@ -1065,10 +1077,20 @@ __device__ __forceinline__ float ds_scale(const float* maxima, int blocks) {
   return ldexpf(1.f, max(-100, min(100, 12 - (int)ceilf(log2f(b)))));
 }
 
+// What the gradient's two kernels share.  Where one has fewer workgroups than the
+// card takes, each sequence's keys (of dq) or rows (of dk, dv) are cut into
+// parts, whose sums packattn_sum_kernel adds in their order.
+struct Back {
+  float* delta;         // [heads][q_tokens]
+  const float* maxima;  // binary16: [NORM_BLOCKS][2]
+  int q_parts, k_parts;
+  float* dq;            // [part][q_tokens][heads][DP]
+  float *dk, *dv;       // [part][k_tokens][kv_heads][DP]
+};
+
 // dq, and D = sum (do o) of every row for the other kernel.
 template <class T, int DP>
-__global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_t tiles, float* delta,
-                                                            const float* maxima, int blocks) {
+__global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_t tiles, Back back) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   constexpr int BM = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
   const Place at = place(a.kv_heads, tiles);
@@ -1089,8 +1111,9 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   const Row end = row_of(a, seq, min(r0 + BM, rows) - 1, G);
   int far = uniform(end.last);
   if (a.fill && seq.lq < seq.have) far = seq.lk - 1;
-  const int nk = far < 0 ? 0 : far / BN + 1;
-  const float ds = Half<T>::SCALED ? ds_scale(maxima, blocks) : 1.f;
+  const int every = far < 0 ? 0 : far / BN + 1, per = (every + back.q_parts - 1) / back.q_parts;
+  const int part = blockIdx.y, kt0 = part * per, nk = min(every, kt0 + per);
+  const float ds = Half<T>::SCALED ? ds_scale(back.maxima, NORM_BLOCKS) : 1.f;
 
   u32x4 q[KS], g[KS];
   const T* qrow = row_ptr<const T>(a.q, token, head);
@@ -1110,7 +1133,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   D = other_half_sum(D);
   float lse = a.lse[at_row] * LOG2E;
   if (lse == NEG_INF) lse = -NEG_INF;  // a row without a key: P = 0
-  if (row.stored && row.i < seq.lq && h == 0) delta[at_row] = D;
+  if (row.stored && row.i < seq.lq && h == 0 && part == 0) back.delta[at_row] = D;
   const float c = a.scale * LOG2E;
   f32x16 o[DB];
 #pragma unroll
@@ -1119,8 +1142,8 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   // what was loaded above is here before the first copy is issued
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   KeyTiles<T, DP, BN, WAVES> tile;
-  tile.init(a, seq, at.head, 0, BN, wave, lane);
-  if (nk > 0) tile.both(lds0);
+  tile.init(a, seq, at.head, kt0 * BN, BN, wave, lane);
+  if (kt0 < nk) tile.both(lds0);
 
   Operands<DP> x;
   x.init(lds0, lane);
@@ -1187,7 +1210,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
       order<MFMA, DB>();
     }
   };
-  for (int kt = 0; kt < nk; kt += 2) {
+  for (int kt = kt0; kt < nk; kt += 2) {
     step(kt, 0, 2 * TILE);
     if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
   }
@@ -1195,7 +1218,13 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16{};
   }
-  store_columns<T, DB>(o, a.scale / ds, row.stored ? row_ptr<T>(a.dq, token, head) : nullptr, a.width, lane);
+  const float f = a.scale / ds;
+  if (back.q_parts == 1) {
+    store_columns<T, DB>(o, f, row.stored ? row_ptr<T>(a.dq, token, head) : nullptr, a.width, lane);
+  } else {
+    const int64_t at_sum = ((part * a.q_tokens + token) * a.heads + head) * DP;
+    store_sums<DB>(o, f, row.stored ? back.dq + at_sum : nullptr, lane);
+  }
 }
 
 // dk, dv: workgroup = 128 keys of one sequence and head over the rows of all the
@@ -1206,8 +1235,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
 // the matrix cores wait for each exponential, leave no room for the keys' and
 // values' operands beside them: those are read from LDS, in operand order.
 template <class T, int DP>
-__global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, const float* delta,
-                                                                 const float* maxima, int blocks) {
+__global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, Back back) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef TileCopy<DP, BN, 2 * WAVES> C;
   constexpr int BK = 32 * WAVES, KS = DP / 16, DB = DP / 32, TILE = BN * DP * 2;
@@ -1228,9 +1256,11 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   const int64_t token = seq.k0 + min(j, have - 1);
   const int lag = seq.lk - seq.lq;  // query i sees keys up to i + lag
   // the first row that sees a key of the workgroup; without keys there is none
-  const int rows = j0 < seq.lk ? seq.lq * G : 0;
-  const int from = a.causal ? max(j0 - lag, 0) * G / BN * BN : 0;
-  const float ds = Half<T>::SCALED ? ds_scale(maxima, blocks) : 1.f;
+  const int all = j0 < seq.lk ? seq.lq * G : 0;
+  const int first = a.causal ? min(max(j0 - lag, 0) * G / BN * BN, all) : 0;
+  const int per = ((all - first + BN - 1) / BN + back.k_parts - 1) / back.k_parts * BN;
+  const int part = blockIdx.y, from = min(first + part * per, all), rows = min(all, from + per);
+  const float ds = Half<T>::SCALED ? ds_scale(back.maxima, NORM_BLOCKS) : 1.f;
   // P is made 2^SHIFT times as large in binary16
   constexpr float SHIFT = 2 * Half<T>::SHIFT;
 
@@ -1295,7 +1325,7 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
       if (r0 + lane < rows) {
         const int64_t p = (int64_t)(at.head * G + my_g) * a.q_tokens + seq.q0 + my_i;
         n_lse = a.lse[p] * LOG2E;
-        n_delta = delta[p];
+        n_delta = back.delta[p];
         n_last = a.causal ? my_i + lag : seq.lk;
       }
     }
@@ -1448,9 +1478,49 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   join(dk);
   join(dv);
   if (half) return;
-  store_columns<T, DB>(dk, a.scale / ds, stored ? row_ptr<T>(a.dk, token, at.head) : nullptr, a.width, lane);
-  store_columns<T, DB>(dv, Half<T>::SCALED ? 1.f / 16384.f : 1.f,
-                       stored ? row_ptr<T>(a.dv, token, at.head) : nullptr, a.width, lane);
+  const float fk = a.scale / ds, fv = Half<T>::SCALED ? 1.f / 16384.f : 1.f;
+  if (back.k_parts == 1) {
+    store_columns<T, DB>(dk, fk, stored ? row_ptr<T>(a.dk, token, at.head) : nullptr, a.width, lane);
+    store_columns<T, DB>(dv, fv, stored ? row_ptr<T>(a.dv, token, at.head) : nullptr, a.width, lane);
+  } else {
+    const int64_t at_sum = ((part * a.k_tokens + token) * a.kv_heads + at.head) * DP;
+    store_sums<DB>(dk, fk, stored ? back.dk + at_sum : nullptr, lane);
+    store_sums<DB>(dv, fv, stored ? back.dv + at_sum : nullptr, lane);
+  }
+}
+
+// The parts' sums of 32 tokens of one sequence: blockIdx.y 0 of dq, 1 of dk, 2 of dv.
+template <class T, int DP>
+__global__ __launch_bounds__(NT) void packattn_sum_kernel(PackedAttn a, Back back) {
+  const bool keys = blockIdx.y > 0;
+  const int parts = keys ? back.k_parts : back.q_parts;
+  if (parts == 1) return;
+  const int64_t n = keys ? a.k_tokens : a.q_tokens;
+  int s;
+  const int64_t t = find_tile(keys ? a.k_off : a.q_off, a.sequences, n, 1, 32, blockIdx.x, s);
+  const Seq seq = lane_seq(sequence(a, s, keys), 0);
+  const int have = a.fill ? seq.have : keys ? seq.lk : seq.lq, heads = keys ? a.kv_heads : a.heads;
+  if (t < 0 || t * 32 >= have) return;
+  const int count = (int)min((int64_t)32, have - t * 32);
+  const int64_t token0 = (keys ? seq.k0 : seq.q0) + t * 32, stride = n * heads * DP;
+  const float* sums = blockIdx.y == 0 ? back.dq : blockIdx.y == 1 ? back.dk : back.dv;
+  const HeadView& out = blockIdx.y == 0 ? a.dq : blockIdx.y == 1 ? a.dk : a.dv;
+  for (int i = threadIdx.x; i < count * heads * (DP / 4); i += NT) {
+    const int e = i % (DP / 4) * 4, row = i / (DP / 4);
+    if (e >= a.width) continue;
+    const int64_t token = token0 + row / heads;
+    const float* p = sums + (token0 * heads + row) * DP + e;
+    float v[4] = {};
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(p + k * stride);
+      v[0] += x.x;
+      v[1] += x.y;
+      v[2] += x.z;
+      v[3] += x.w;
+    }
+    Few<T, 4>::template store<false>(row_ptr<T>(out, token, row % heads) + e, v);
+  }
 }
 
 // ------------------------------------------------------------------ launches
@@ -1520,11 +1590,41 @@ size_t packattn_fwd_work_bytes(const PackedAttn& a) {
   return n;
 }
 
-size_t packattn_bwd_work_bytes(const PackedAttn& a) {
+namespace {
+
+// Parts of the sequences in the gradient's kernels: as many as the card takes
+// workgroups beside each other, of four tiles at least.
+Back carve_back(const PackedAttn& a, char* base, size_t* bytes) {
+  const int64_t G = a.heads / a.kv_heads, cus = device_cus(), DP = padded(a.width);
+  const int64_t live = std::max<int64_t>(1, std::min<int64_t>(a.sequences, std::min(a.q_tokens, a.k_tokens)));
+  auto parts = [&](int64_t items, int64_t tiles, int64_t room) {
+    const int64_t groups = std::max(live, (items + 127) / 128) * a.kv_heads;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({room / groups, tiles / live / 4, 64}));
+  };
+  Back b = {};
+  b.q_parts = parts(a.q_tokens * G, a.k_tokens / BN, 2 * cus);
+  b.k_parts = parts(a.k_tokens, a.q_tokens * G / BN, cus);
   Sizer z;
-  z.take<float>((size_t)a.heads * a.q_tokens);
-  if (a.dtype == BC2N_F16) z.take<float>(2 * NORM_BLOCKS);
-  return z.off;
+  auto take = [&](int64_t n) {
+    float* p = reinterpret_cast<float*>(base + z.off);
+    z.take<float>((size_t)n);
+    return p;
+  };
+  b.delta = take(a.heads * a.q_tokens);
+  b.maxima = take(a.dtype == BC2N_F16 ? 2 * NORM_BLOCKS : 0);
+  b.dq = take(b.q_parts > 1 ? b.q_parts * a.q_tokens * a.heads * DP : 0);
+  b.dk = take(b.k_parts > 1 ? b.k_parts * a.k_tokens * a.kv_heads * DP : 0);
+  b.dv = take(b.k_parts > 1 ? b.k_parts * a.k_tokens * a.kv_heads * DP : 0);
+  *bytes = z.off;
+  return b;
+}
+
+}  // namespace
+
+size_t packattn_bwd_work_bytes(const PackedAttn& a) {
+  size_t n = 0;
+  carve_back(a, nullptr, &n);
+  return n;
 }
 
 void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
@@ -1568,28 +1668,32 @@ void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
 void packattn_bwd(hipStream_t st, const PackedAttn& a, void* work) {
   if (a.q_tokens == 0 && a.k_tokens == 0) return;
   KTimed kt("attention.bwd", st);
-  Carver c(work);
-  float* delta = c.take<float>((size_t)a.heads * a.q_tokens);
-  float* maxima = a.dtype == BC2N_F16 ? c.take<float>(2 * NORM_BLOCKS) : nullptr;
+  size_t bytes = 0;
+  const Back back = carve_back(a, reinterpret_cast<char*>(work), &bytes);
   by_type(a, [&](auto v, auto dp) {
     typedef decltype(v) T;
     constexpr int DP = decltype(dp)::value;
     const int64_t q_tiles = tiles_of(a.q_tokens, a.heads / a.kv_heads, 32 * WAVES, a.sequences);
     const int64_t k_tiles = tiles_of(a.k_tokens, 1, 32 * WAVES, a.sequences);
-    if (maxima)
+    if (a.dtype == BC2N_F16)
       packattn_norms_kernel<T><<<NORM_BLOCKS, NT, 0, st>>>(a, tiles_of(a.q_tokens, 1, 64, a.sequences),
-                                                          tiles_of(a.k_tokens, 1, 64, a.sequences), maxima);
+                                                          tiles_of(a.k_tokens, 1, 64, a.sequences),
+                                                          const_cast<float*>(back.maxima));
     if (a.q_tokens) {
       auto* dq = &packattn_dq_kernel<T, DP>;
       const size_t lds = 4 * BN * DP * 2;
       with_lds(dq, lds);
-      dq<<<place_grid(a.kv_heads, q_tiles), NT, lds, st>>>(a, q_tiles, delta, maxima, NORM_BLOCKS);
+      dq<<<dim3(place_grid(a.kv_heads, q_tiles), back.q_parts), NT, lds, st>>>(a, q_tiles, back);
     }
     if (a.k_tokens) {
       auto* dkv = &packattn_dkv_kernel<T, DP>;
       const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4) + 2 * 32 * WAVES * DP * 2;
       with_lds(dkv, lds);
-      dkv<<<place_grid(a.kv_heads, k_tiles), 2 * NT, lds, st>>>(a, k_tiles, delta, maxima, NORM_BLOCKS);
+      dkv<<<dim3(place_grid(a.kv_heads, k_tiles), back.k_parts), 2 * NT, lds, st>>>(a, k_tiles, back);
+    }
+    if (back.q_parts > 1 || back.k_parts > 1) {
+      const int64_t most = std::max(tiles_of(a.q_tokens, 1, 32, a.sequences), tiles_of(a.k_tokens, 1, 32, a.sequences));
+      packattn_sum_kernel<T, DP><<<dim3((unsigned)most, 3), NT, 0, st>>>(a, back);
     }
   });
 }
