@@ -1489,7 +1489,8 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   }
 }
 
-// The parts' sums of 32 tokens of one sequence: blockIdx.y 0 of dq, 1 of dk, 2 of dv.
+constexpr int SUM_TOKENS = 4;  // of a workgroup
+// The parts' sums of a few tokens of one sequence: blockIdx.y 0 of dq, 1 of dk, 2 of dv.
 template <class T, int DP>
 __global__ __launch_bounds__(NT) void packattn_sum_kernel(PackedAttn a, Back back) {
   const bool keys = blockIdx.y > 0;
@@ -1497,12 +1498,12 @@ __global__ __launch_bounds__(NT) void packattn_sum_kernel(PackedAttn a, Back bac
   if (parts == 1) return;
   const int64_t n = keys ? a.k_tokens : a.q_tokens;
   int s;
-  const int64_t t = find_tile(keys ? a.k_off : a.q_off, a.sequences, n, 1, 32, blockIdx.x, s);
+  const int64_t t = find_tile(keys ? a.k_off : a.q_off, a.sequences, n, 1, SUM_TOKENS, blockIdx.x, s);
   const Seq seq = lane_seq(sequence(a, s, keys), 0);
   const int have = a.fill ? seq.have : keys ? seq.lk : seq.lq, heads = keys ? a.kv_heads : a.heads;
-  if (t < 0 || t * 32 >= have) return;
-  const int count = (int)min((int64_t)32, have - t * 32);
-  const int64_t token0 = (keys ? seq.k0 : seq.q0) + t * 32, stride = n * heads * DP;
+  if (t < 0 || t * SUM_TOKENS >= have) return;
+  const int count = (int)min((int64_t)SUM_TOKENS, have - t * SUM_TOKENS);
+  const int64_t token0 = (keys ? seq.k0 : seq.q0) + t * SUM_TOKENS, stride = n * heads * DP;
   const float* sums = blockIdx.y == 0 ? back.dq : blockIdx.y == 1 ? back.dk : back.dv;
   const HeadView& out = blockIdx.y == 0 ? a.dq : blockIdx.y == 1 ? a.dk : a.dv;
   for (int i = threadIdx.x; i < count * heads * (DP / 4); i += NT) {
@@ -1511,7 +1512,7 @@ __global__ __launch_bounds__(NT) void packattn_sum_kernel(PackedAttn a, Back bac
     const int64_t token = token0 + row / heads;
     const float* p = sums + (token0 * heads + row) * DP + e;
     float v[4] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < parts; ++k) {
       const float4 x = *reinterpret_cast<const float4*>(p + k * stride);
       v[0] += x.x;
@@ -1592,18 +1593,20 @@ size_t packattn_fwd_work_bytes(const PackedAttn& a) {
 
 namespace {
 
-// Parts of the sequences in the gradient's kernels: as many as the card takes
-// workgroups beside each other, of four tiles at least.
+// Parts of the sequences in the gradient's kernels: as many as make one round of
+// workgroups, two a compute unit for dq and one for dk and dv, and no shorter than
+// what a part costs by itself: 4 tiles of keys, 8 of rows (two sequences of 1262
+// keys, 8 heads over one: 19 parts of 5 tiles 48 us, 9 of 10 34).
 Back carve_back(const PackedAttn& a, char* base, size_t* bytes) {
   const int64_t G = a.heads / a.kv_heads, cus = device_cus(), DP = padded(a.width);
   const int64_t live = std::max<int64_t>(1, std::min<int64_t>(a.sequences, std::min(a.q_tokens, a.k_tokens)));
-  auto parts = [&](int64_t items, int64_t tiles, int64_t room) {
-    const int64_t groups = std::max(live, (items + 127) / 128) * a.kv_heads;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({room / groups, tiles / live / 4, 64}));
+  auto parts = [&](int64_t room, int64_t items, int64_t tiles, int64_t shortest) {
+    const int64_t blocks = std::max(live, (items + 127) / 128) * a.kv_heads;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({room / blocks, tiles / live / shortest, 64}));
   };
   Back b = {};
-  b.q_parts = parts(a.q_tokens * G, a.k_tokens / BN, 2 * cus);
-  b.k_parts = parts(a.k_tokens, a.q_tokens * G / BN, cus);
+  b.q_parts = parts(2 * cus, a.q_tokens * G, a.k_tokens / BN, 4);
+  b.k_parts = parts(cus, a.k_tokens, a.q_tokens * G / BN, 8);
   Sizer z;
   auto take = [&](int64_t n) {
     float* p = reinterpret_cast<float*>(base + z.off);
@@ -1692,7 +1695,8 @@ void packattn_bwd(hipStream_t st, const PackedAttn& a, void* work) {
       dkv<<<dim3(place_grid(a.kv_heads, k_tiles), back.k_parts), 2 * NT, lds, st>>>(a, k_tiles, back);
     }
     if (back.q_parts > 1 || back.k_parts > 1) {
-      const int64_t most = std::max(tiles_of(a.q_tokens, 1, 32, a.sequences), tiles_of(a.k_tokens, 1, 32, a.sequences));
+      const int64_t most = std::max(tiles_of(a.q_tokens, 1, SUM_TOKENS, a.sequences),
+                                    tiles_of(a.k_tokens, 1, SUM_TOKENS, a.sequences));
       packattn_sum_kernel<T, DP><<<dim3((unsigned)most, 3), NT, 0, st>>>(a, back);
     }
   });
