@@ -1088,6 +1088,7 @@ struct Back {
   float *dk, *dv;       // [part][k_tokens][kv_heads][DP]
 };
 
+constexpr int FEW_KEYS = 256;
 // dq, and D = sum (do o) of every row for the other kernel.
 template <class T, int DP>
 __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_t tiles, Back back) {
@@ -1133,7 +1134,6 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   D = other_half_sum(D);
   float lse = a.lse[at_row] * LOG2E;
   if (lse == NEG_INF) lse = -NEG_INF;  // a row without a key: P = 0
-  if (row.stored && row.i < seq.lq && h == 0 && part == 0) back.delta[at_row] = D;
   const float c = a.scale * LOG2E;
   f32x16 o[DB];
 #pragma unroll
@@ -1142,11 +1142,40 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   // what was loaded above is here before the first copy is issued
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   KeyTiles<T, DP, BN, WAVES> tile;
-  tile.init(a, seq, at.head, kt0 * BN, BN, wave, lane);
-  if (kt0 < nk) tile.both(lds0);
-
   Operands<DP> x;
   x.init(lds0, lane);
+  // Rows of few keys: out, an average of few values, is as large as each of them,
+  // and its rounding would weigh as much in dS as that of dS itself.  Their D is
+  // taken from the keys, sum P dP (224 keys, binary16: dq 1.56 times as far off
+  // as its own rounding with the rounded out, 1.46 so).
+  if (back.q_parts == 1 && nk <= FEW_KEYS / BN) {
+    tile.init(a, seq, at.head, 0, BN, wave, lane);
+    float sum = 0.f;
+    for (int kt = 0; kt < nk; ++kt) {
+      if (kt == 0) tile.both(lds0);
+      const unsigned here = (kt & 1) * 2 * TILE;
+      wait_all_and_sync();
+      if (kt + 1 < nk) tile.both(lds0 + (~kt & 1) * 2 * TILE);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        f32x16 p = {}, d = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          p = Half<T>::mma(x.row(here + 32 * b * DP * 2, ks), q[ks], p);
+          d = Half<T>::mma(x.row(here + 32 * b * DP * 2 + TILE, ks), g[ks], d);
+        }
+        const int last = row.last - kt * BN - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + 8 * (i / 4) + i % 4 <= last) sum = fmaf(exp2_f(fmaf(p[i], c, -lse)), d[i], sum);
+      }
+    }
+    D = other_half_sum(sum);
+    wait_all_and_sync();
+  }
+  if (row.stored && row.i < seq.lq && h == 0 && part == 0) back.delta[at_row] = D;
+  tile.init(a, seq, at.head, kt0 * BN, BN, wave, lane);
+  if (kt0 < nk) tile.both(lds0);
   auto step = [&](int kt, unsigned here, unsigned next) __attribute__((always_inline)) {
     const int k0 = kt * BN;
     wait_all_and_sync();
