@@ -119,6 +119,44 @@ __device__ __forceinline__ float log_share(double d, u64 mass, int S) {
   return (float)((d - (log2((double)mass) - (double)S)) * 0.69314718055994530942);
 }
 
+// DPP moves: what a fold or a scan waits for is its latency, a tenth of a shuffle's.
+constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp64(u64 v, u64 none) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp((int)(none >> 32), (int)(v >> 32), CTRL, ROWS, 0xF, false);
+  return (u64)hi << 32 | lo;
+}
+struct Sum {
+  static constexpr u64 NONE = 0;
+  __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+  static constexpr u64 NONE = 0;
+  __device__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
+};
+struct Min {
+  static constexpr u64 NONE = ~u64(0);
+  __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; }
+};
+// of the lanes up to this one
+template <class F>
+__device__ __forceinline__ u64 wave_scan(u64 v, F f) {
+  v = f(v, dpp64<ROW_SHR + 1, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_SHR + 2, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_SHR + 4, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_SHR + 8, 0xF>(v, F::NONE));
+  v = f(v, dpp64<ROW_BCAST15, 0xA>(v, F::NONE));
+  return f(v, dpp64<ROW_BCAST31, 0xC>(v, F::NONE));
+}
+__device__ __forceinline__ u64 lane_value(u64 v, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+template <class F>
+__device__ __forceinline__ u64 wave_fold(u64 v, F f) {
+  return lane_value(wave_scan(v, f), 63);
+}
 // ---------------------------------------------------------------------------
 // Rows of at most W classes: a class a lane, W lanes a row.  Ranks and sums of
 // forerunners by comparing each class with all.
@@ -174,6 +212,161 @@ __global__ __launch_bounds__(256) void sample_few_kernel(Sample a) {
 }
 
 // ---------------------------------------------------------------------------
+// Rows of at most 64 R classes: a wave a row, R consecutive classes a lane in its
+// registers.  A cut is a threshold on x found by halving: the sum of what is above
+// a value, all lanes', against the cut's end, until one class is left between.
+template <class T, int R>
+struct WaveRow {
+  float x[R];
+  uint32_t key[R];  // 0: not in play
+  u64 w[R];
+  int lane, j0;
+
+  template <bool MASS>
+  __device__ __forceinline__ u64 above(uint32_t v) const {
+    if constexpr (MASS) {
+      u64 sum = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) sum += key[i] > v ? w[i] : 0;
+      return wave_fold(sum, Sum());
+    } else {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] > v));
+      return (u64)n;
+    }
+  }
+  __device__ __forceinline__ int between(uint32_t lo, uint32_t hi) const {  // in (lo, hi]
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] > lo && key[i] <= hi));
+    return n;
+  }
+  // Takes out of play the classes whose forerunners weigh `end` or more, by number
+  // or (MASS) by mass; low: a value below all that count.
+  template <bool MASS>
+  __device__ __forceinline__ void cut(u64 end, float m, float low) {
+    // above hi all stay, up to lo none
+    uint32_t hi = key_of(m), lo = key_of(low) - 1;
+    if (above<MASS>(lo) <= (MASS ? end - 1 : end)) lo = 0;  // all stay, the last in any case
+    float a = low, b = m;
+    for (int turn = 0; lo && hi - lo > 1; ++turn) {
+      // halves of the values first, which logits are spread over, then of the keys
+      uint32_t mid = lo + (hi - lo) / 2;
+      if (turn < 16) {
+        const uint32_t v = key_of(0.5f * a + 0.5f * b);
+        if (v > lo && v < hi) mid = v;
+      }
+      const bool stays = above<MASS>(mid) < end;
+      if (stays) hi = mid;
+      else lo = mid;
+      const uint32_t bits = mid & 0x80000000u ? mid & 0x7fffffffu : ~mid;
+      (stays ? b : a) = __builtin_bit_cast(float, bits);
+      if (between(lo, hi) <= 1) {
+        hi = lo;  // one class, whose forerunners are those above: it stays
+        break;
+      }
+    }
+    if (!lo) return;
+    if (hi == lo) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (key[i] <= lo) key[i] = 0;
+      return;
+    }
+    // classes of one value, hi: the first of them by index
+    const u64 before = above<MASS>(hi);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) mine += key[i] == hi;
+    u64 rank = wave_scan((u64)mine, Sum()) - mine;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const bool tie = key[i] == hi;
+      if (key[i] < hi || (tie && before + rank * (MASS ? w[i] : 1) >= end)) key[i] = 0;
+      rank += tie;
+    }
+  }
+};
+
+template <class T, int R>
+__global__ __launch_bounds__(256) void sample_wave_kernel(Sample a) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= a.rows) return;
+  const int S = mass_bits(a.V);
+  WaveRow<T, R> row;
+  row.lane = threadIdx.x & 63;
+  row.j0 = row.lane * R;
+  const T* x = reinterpret_cast<const T*>(a.x) + r * a.ld;
+#pragma unroll
+  for (int i = 0; i < R; ++i) row.x[i] = NEG_INF;
+  if (row.j0 + R <= a.V) {
+    constexpr int N = R < 16 / (int)sizeof(T) ? R : 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < R; i += N) Few<T, N>::template load<false>(x + row.j0 + i, row.x + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (row.j0 + i < a.V) row.x[i] = (float)x[row.j0 + i];
+  }
+  const Settings s = settings_of(a, r);
+  float m = NEG_INF;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    nan |= row.x[i] != row.x[i];
+    m = fmaxf(m, row.x[i]);
+  }
+  m = group_max<64>(m);
+  if (__any(nan) || m == -NEG_INF || m == NEG_INF || s.bad) {
+    if (row.lane == 0) write(a, r, -1, __builtin_nanf(""));
+    return;
+  }
+  if (s.greedy) {
+    int first = 0x7fffffff;
+#pragma unroll
+    for (int i = R - 1; i >= 0; --i)
+      if (row.x[i] == m) first = row.j0 + i;
+    first = (int)wave_fold((u64)first, Min());
+    if (row.lane == 0) write(a, r, first, 0.f);
+    return;
+  }
+  // a value a little below the last with a mass
+  const float low = fmaxf(m - (float)fmin((S + 2) / s.inv * 1.0001, 3e38), -3e38f);
+  u64 mine = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool counts = row.x[i] >= low;
+    const double t = ((double)row.x[i] - (double)m) * s.inv;
+    row.key[i] = counts ? key_of(row.x[i]) : 0;
+    row.w[i] = counts ? mass_of(t, S) : 0;
+  }
+  if (s.k) row.template cut<false>((u64)s.k, m, low);
+  if (s.p < 1.0) {
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) mine += row.key[i] ? row.w[i] : 0;
+    row.template cut<true>(share_of(s.p, wave_fold(mine, Sum())), m, low);
+  }
+  mine = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const double t = ((double)row.x[i] - (double)m) * s.inv;
+    if (!row.key[i] || t < s.floor) row.w[i] = 0;
+    mine += row.w[i];
+  }
+  const u64 run = wave_scan(mine, Sum()), mass = lane_value(run, 63), target = target_of(s.u, mass);
+  u64 before = run - mine;
+  if (before > target || run <= target) return;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {  // one lane's
+    if (before <= target && before + row.w[i] > target)
+      write(a, r, row.j0 + i, log_share(((double)row.x[i] - (double)m) * s.inv, mass, S));
+    before += row.w[i];
+  }
+}
+
+// ---------------------------------------------------------------------------
 // A workgroup a row.
 constexpr int CANDIDATES = 1024;
 template <int NT>
@@ -189,44 +382,6 @@ struct Shared {
   uint32_t n, found;
 };
 
-// DPP moves: what a fold or a scan waits for is its latency, a tenth of a shuffle's.
-constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
-template <int CTRL, int ROWS>
-__device__ __forceinline__ u64 dpp64(u64 v, u64 none) {
-  const uint32_t lo = __builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xF, false);
-  const uint32_t hi = __builtin_amdgcn_update_dpp((int)(none >> 32), (int)(v >> 32), CTRL, ROWS, 0xF, false);
-  return (u64)hi << 32 | lo;
-}
-struct Sum {
-  static constexpr u64 NONE = 0;
-  __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
-};
-struct Max {
-  static constexpr u64 NONE = 0;
-  __device__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
-};
-struct Min {
-  static constexpr u64 NONE = ~u64(0);
-  __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; }
-};
-// of the lanes up to this one
-template <class F>
-__device__ __forceinline__ u64 wave_scan(u64 v, F f) {
-  v = f(v, dpp64<ROW_SHR + 1, 0xF>(v, F::NONE));
-  v = f(v, dpp64<ROW_SHR + 2, 0xF>(v, F::NONE));
-  v = f(v, dpp64<ROW_SHR + 4, 0xF>(v, F::NONE));
-  v = f(v, dpp64<ROW_SHR + 8, 0xF>(v, F::NONE));
-  v = f(v, dpp64<ROW_BCAST15, 0xA>(v, F::NONE));
-  return f(v, dpp64<ROW_BCAST31, 0xC>(v, F::NONE));
-}
-__device__ __forceinline__ u64 lane_value(u64 v, int lane) {
-  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
-}
-template <class F>
-__device__ __forceinline__ u64 wave_fold(u64 v, F f) {
-  return lane_value(wave_scan(v, f), 63);
-}
 // over the workgroup, the result in every thread
 template <int NT, class F>
 __device__ __forceinline__ u64 block_fold(u64 v, u64* waves, F f) {
@@ -235,7 +390,7 @@ __device__ __forceinline__ u64 block_fold(u64 v, u64* waves, F f) {
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
   __syncthreads();
   v = waves[0];
-#pragma unroll
+#pragma unroll 4
   for (int i = 1; i < NT / 64; ++i) v = f(v, waves[i]);
   return v;
 }
@@ -247,7 +402,7 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* waves) {  // exclusive
   if (lane == 63) waves[wave] = run;
   __syncthreads();
   u64 before = 0;
-#pragma unroll
+#pragma unroll 4
   for (int i = 0; i < NT / 64; ++i) before += i < wave ? waves[i] : 0;
   return before + run - v;
 }
@@ -265,7 +420,7 @@ struct RowOf {
   // f(x, index) of a thread's classes
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-#pragma unroll 2
+#pragma unroll 1
     for (int j = threadIdx.x; j < V; j += NT) f((float)x[j], j);
   }
   // f(classes' values, index of the first, number of the vector) of a thread's
@@ -359,30 +514,41 @@ struct Drawer {
     return (int)top - 1;
   }
 
+  // Counts and (masses) masses of the classes of `from` in steps of distance, those
+  // of rank keys >= least.
+  template <class S_>
+  __device__ void fill(const S_& from, bool masses, u64 least) {
+    clear(masses);
+    from.each([&](float x, int j) {
+      if (!counts(x) || rank_key(x, j) < least) return;
+      const int b = step_of(x);
+      atomicAdd(&sh.count[b], 1u);
+      if (masses) atomicAdd(&sh.mass[b], mass(x));
+    });
+    __syncthreads();
+  }
+  // The weight of all steps.
+  __device__ u64 filled_mass(int steps_) {
+    u64 w = 0;
+    for (int b = threadIdx.x; b < steps_; b += NT) w += sh.mass[b];
+    return block_fold<NT>(w, sh.wave_b, Sum());
+  }
+
   // The rank key of the last class of `from` whose forerunners, among those of
-  // rank keys >= least, weigh less than `end`: by number, or (MASS) by mass.
-  // filled: the first pass's counts and masses are there.
+  // rank keys >= least, weigh less than `end`: by number, or (MASS) by mass.  The
+  // steps have to be filled, with those at least; `kept`, where given, gets the
+  // mass of the classes up to that one, if the steps' masses are filled and tell
+  // it, and false is left in `intact` where the steps were filled anew.
   template <bool MASS, class S_>
-  __device__ u64 last_before(const S_& from, u64 end, u64 least, bool filled = false) {
+  __device__ u64 last_before(const S_& from, u64 end, u64 least, bool& intact, u64* kept = nullptr) {
     u64 lo = 0, hi = ~u64(0), before = 0;
     int shift = -1;  // -1: steps of distance
     for (;;) {
-      if (!filled) clear(MASS);
       auto bin_of = [&](float x, u64 c) { return shift < 0 ? step_of(x) : (int)((hi - c) >> shift); };
-      if (!filled) {
-        from.each([&](float x, int j) {
-          if (!counts(x)) return;
-          const u64 c = rank_key(x, j);
-          if (c < least || c < lo || c > hi) return;
-          const int b = bin_of(x, c);
-          atomicAdd(&sh.count[b], 1u);
-          if (MASS) atomicAdd(&sh.mass[b], mass(x));
-        });
-      }
-      filled = false;
-      __syncthreads();
       const int bin = last_step<MASS>(end, before);
+      if (threadIdx.x == 0) sh.n = 0;
       const uint32_t in_bin = sh.count[bin];
+      __syncthreads();
       if (in_bin <= LIST) {
         from.each([&](float x, int j) {
           if (!counts(x)) return;
@@ -390,17 +556,24 @@ struct Drawer {
           if (c < least || c < lo || c > hi || bin_of(x, c) != bin) return;
           const uint32_t at = atomicAdd(&sh.n, 1u);
           sh.list_key[at] = c;
-          sh.list_mass[at] = MASS ? mass(x) : 1;
+          sh.list_mass[at] = MASS || kept ? mass(x) : 1;
         });
         __syncthreads();
+        const int n = (int)sh.n;
         u64 key = ~u64(0);
-        for (int i = threadIdx.x; i < (int)in_bin; i += NT) {
+        for (int i = threadIdx.x; i < n; i += NT) {
           const u64 c = sh.list_key[i];
           u64 f = before;
-          for (int k = 0; k < (int)in_bin; ++k) f += sh.list_key[k] > c ? sh.list_mass[k] : 0;
+          for (int k = 0; k < n; ++k) f += sh.list_key[k] > c ? (MASS ? sh.list_mass[k] : 1) : 0;
           if (f < end) key = min(key, c);
         }
-        return block_fold<NT>(key, sh.wave_a, Min());
+        key = block_fold<NT>(key, sh.wave_a, Min());
+        if (kept && intact) {
+          u64 w = 0;
+          for (int i = threadIdx.x; i < n; i += NT) w += sh.list_key[i] >= key ? sh.list_mass[i] : 0;
+          *kept = filled_mass(bin) + block_fold<NT>(w, sh.wave_a, Sum());
+        }
+        return key;
       }
       // too many: their range of rank keys in 2048 parts
       u64 a = ~u64(0), b = 0;
@@ -417,6 +590,16 @@ struct Drawer {
       hi = b;
       shift = 0;
       while (((hi - lo) >> shift) >= BINS) ++shift;
+      intact = false;
+      clear(MASS);
+      from.each([&](float x, int j) {
+        if (!counts(x)) return;
+        const u64 c = rank_key(x, j);
+        if (c < least || c < lo || c > hi) return;
+        const int b_ = bin_of(x, c);
+        atomicAdd(&sh.count[b_], 1u);
+        if (MASS) atomicAdd(&sh.mass[b_], mass(x));
+      });
       __syncthreads();
     }
   }
@@ -592,16 +775,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     step = (int)wave_fold((u64)step, Min());
     n = d.collect(row, d.lowest(min(step * COARSE + COARSE - 1, BINS - 1)));
   } else if (!s.k && s.p < 1.0) {
-    d.clear(true);
-    row.each([&](float x, int) {
-      if (!d.counts(x)) return;
-      const u64 w = d.mass(x);
-      whole += w;
-      const int b = d.step_of(x);
-      atomicAdd(&sh.count[b], 1u);
-      atomicAdd(&sh.mass[b], w);
-    });
-    whole = block_fold<NT>(whole, sh.wave_a, Sum());
+    d.fill(row, true, 0);
+    whole = d.filled_mass(BINS);
     u64 before = 0;
     const int step = d.template last_step<true>(share_of(s.p, whole), before);
     n = d.collect(row, d.lowest(step));
@@ -611,17 +786,23 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     const double t = d.distance(x);
     return t < s.floor ? 0 : mass_of(t, d.S);
   };
+  // The cuts, each by the steps that the one before has left where they tell it.
   auto cut = [&](const auto& from, bool filled) {
-    if (s.k) least = d.template last_before<false>(from, (u64)s.k, 0);
-    if (s.p < 1.0) {
-      if (s.k) {
-        from.each([&](float x, int j) {
-          if (d.counts(x) && rank_key(x, j) >= least) whole += d.mass(x);
-        });
-        whole = block_fold<NT>(whole, sh.wave_a, Sum());
+    const bool by_mass = s.p < 1.0;
+    bool intact = true;
+    if (s.k) {
+      d.fill(from, by_mass, 0);
+      least = d.template last_before<false>(from, (u64)s.k, 0, intact, by_mass ? &whole : nullptr);
+      if (by_mass && !intact) {
+        d.fill(from, true, least);
+        whole = d.filled_mass(BINS);
+        intact = true;
       }
-      least = d.template last_before<true>(from, share_of(s.p, whole), least, filled);
+    } else if (by_mass && !filled) {
+      d.fill(from, true, 0);
     }
+    // steps beyond the k-th class weigh nothing here: what is before them is the whole
+    if (by_mass) least = d.template last_before<true>(from, share_of(s.p, whole), least, intact);
   };
   if (n <= 64) {
     if (wave == 0) d.draw_few(a, r, n, s, whole);
@@ -635,7 +816,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     d.draw(a, r, few, s.u, index_bits, kept_mass);
     return;
   }
-  cut(row, !by_k && !s.k);
+  cut(row, !s.k && s.p < 1.0);
 
   // the running sum over the whole row in tiles of OWN classes a thread: groups of
   // tiles, then the tiles of one group, then the waves of one tile
@@ -718,6 +899,12 @@ void go(hipStream_t st, const Sample& a) {
     if (W == 16) sample_few_kernel<T, 16><<<grid, 256, 0, st>>>(a);
     else if (W == 32) sample_few_kernel<T, 32><<<grid, 256, 0, st>>>(a);
     else sample_few_kernel<T, 64><<<grid, 256, 0, st>>>(a);
+  } else if (a.V <= 1024) {
+    const unsigned grid = (unsigned)((a.rows + 3) / 4);
+    if (a.V <= 128) sample_wave_kernel<T, 2><<<grid, 256, 0, st>>>(a);
+    else if (a.V <= 256) sample_wave_kernel<T, 4><<<grid, 256, 0, st>>>(a);
+    else if (a.V <= 512) sample_wave_kernel<T, 8><<<grid, 256, 0, st>>>(a);
+    else sample_wave_kernel<T, 16><<<grid, 256, 0, st>>>(a);
   } else if (a.V <= 16 * 256 * E) row_go<T, 256>(st, a);
   else if (a.rows > device_cus()) row_go<T, 512>(st, a);
   else row_go<T, 1024>(st, a);
