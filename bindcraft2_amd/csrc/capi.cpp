@@ -1339,12 +1339,15 @@ Heads heads_of(const char* what, const void* p, int64_t st, int64_t sh, int64_t 
   h.es = dtype == BC2N_F32 ? 4 : 2;
   h.what = what;
   if (h.empty()) return h;
+  if (tokens == 1) h.v.st = st = width;  // no call steps by these
+  if (heads == 1) h.v.sh = sh = width;
   refuse_unless(p, what, ": null operand");
   aligned(p, align, what);
   refuse_unless(st >= 0 && sh >= 0, what, ": negative stride");
-  refuse_unless((st * h.es) % align == 0 || tokens == 1, what, ": strides have to keep the alignment");
-  refuse_unless((sh * h.es) % align == 0 || heads == 1, what, ": strides have to keep the alignment");
   refuse_unless(st < (int64_t(1) << 40) && sh < (int64_t(1) << 40), what, ": stride too large");
+  refuse_unless((st * h.es) % align == 0 && (sh * h.es) % align == 0, what,
+                ": strides have to keep the alignment");
+  refuse_unless((tokens - 1) * (double)st + (heads - 1) * (double)sh < 0x1p56, what, ": stride too large");
   if (written) {
     const bool by_token = (heads == 1 || sh >= width) && (tokens == 1 || st >= (heads - 1) * sh + width);
     const bool by_head = (tokens == 1 || st >= width) && (heads == 1 || sh >= (tokens - 1) * st + width);
@@ -1352,7 +1355,8 @@ Heads heads_of(const char* what, const void* p, int64_t st, int64_t sh, int64_t 
   }
   return h;
 }
-// every written operand apart from all others, but those that may be the same
+// every written operand apart from all others, but (in_place) for the one that is
+// read in the same place of each as many
 void all_apart(const std::vector<Heads>& written, const std::vector<Heads>& read, bool in_place) {
   for (size_t i = 0; i < written.size(); ++i) {
     const Heads& w = written[i];
@@ -1360,7 +1364,7 @@ void all_apart(const std::vector<Heads>& written, const std::vector<Heads>& read
     for (size_t j = 0; j < written.size() + read.size(); ++j) {
       const Heads& o = j < written.size() ? written[j] : read[j - written.size()];
       if (o.empty() || j == i) continue;
-      const bool same = in_place && j >= written.size() && o.v.p == w.v.p && o.heads == w.heads &&
+      const bool same = in_place && j >= written.size() && j % written.size() == i && o.v.p == w.v.p && o.heads == w.heads &&
                         (o.v.st == w.v.st || o.tokens == 1) && (o.v.sh == w.v.sh || o.heads == 1);
       if (!same && !apart(w.span(), o.span()))
         throw std::invalid_argument(std::string(w.what) + " overlaps " + o.what);
@@ -1420,7 +1424,7 @@ PackedAttn attention_operands(int dtype, int causal, int sequences, int64_t q_to
        "attention: the heads have to be a multiple of the keys' heads");
   need(width > 0 && width % 8 == 0 && width <= PA_MAX_WIDTH,
        "attention: the width has to be a multiple of 8 up to 128");
-  const int64_t G = heads / kv_heads, most = (int64_t(1) << 31) - 1024;
+  const int64_t G = heads / kv_heads, most = (int64_t(1) << 31) - (1 << 14);
   need(q_tokens >= 0 && k_tokens >= 0 && q_tokens * G < most && k_tokens * G < most,
        "attention: bad number of tokens");
   need(scale > 0 && std::isfinite(scale), "attention: the scale has to be positive");
@@ -1508,8 +1512,8 @@ int bc2n_headnorm_bwd(void* stream, int dtype, int64_t tokens, int heads, int kv
       a.d[i] = d[i].v;
       a.out[i] = y[i].v;
     }
-    a.d_weight[0] = heads ? d_q_weight : nullptr;
-    a.d_weight[1] = kv_heads ? d_k_weight : nullptr;
+    a.d_weight[0] = d_q_weight;
+    a.d_weight[1] = d_k_weight;
     headnorm_bwd(own_stream(stream), a, work);
   });
 }

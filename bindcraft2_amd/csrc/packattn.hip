@@ -215,7 +215,8 @@ __device__ __forceinline__ Place place(int kv_heads, int64_t tiles) {
 unsigned place_grid(int kv_heads, int64_t tiles) {
   const int g = head_classes(kv_heads), share = NUM_XCD / g;
   const int64_t grid = NUM_XCD * (int64_t)(kv_heads / g) * ((tiles + share - 1) / share);
-  if (grid >= int64_t(1) << 24) throw std::invalid_argument("attention: too many tiles for one call");
+  // 512 threads each: a launch has fewer than 2^32
+  if (grid >= int64_t(1) << 23) throw std::invalid_argument("attention: too many tiles for one call");
   return (unsigned)grid;
 }
 
@@ -770,7 +771,7 @@ struct Stretches {
     work = wave_sum64(work);
     all = wave_sum64(all);
     // every tile may end in a short stretch: with those too one round of waves
-    // (64 sequences of 11 .. 8192 keys, 8 heads of 128: 70.5 -> 60 us)
+    // (64 sequences of 11 .. 8192 keys, 8 heads of 128: 70.5 -> 62 us)
     if (all < goal / 2) goal -= all;
     per = uniform((int)max((int64_t)(SHORTEST / KN), (work + goal - 1) / goal));
   }
@@ -1173,6 +1174,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
     D = other_half_sum(sum);
     wait_all_and_sync();
   }
+  if (row.last < 0) D = 0.f;  // no gradient, whatever do holds
   if (row.stored && row.i < seq.lq && h == 0 && part == 0) back.delta[at_row] = D;
   tile.init(a, seq, at.head, kt0 * BN, BN, wave, lane);
   if (kt0 < nk) tile.both(lds0);
@@ -1243,7 +1245,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
     step(kt, 0, 2 * TILE);
     if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
   }
-  if (row.i >= seq.lq) {
+  if (row.last < 0) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16{};
   }
@@ -1287,6 +1289,7 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   // the first row that sees a key of the workgroup; without keys there is none
   const int all = j0 < seq.lk ? seq.lq * G : 0;
   const int first = a.causal ? min(max(j0 - lag, 0) * G / BN * BN, all) : 0;
+  const int sees = a.causal ? max(-lag, 0) * G : 0;  // rows before see no key: taken as zeros
   const int per = ((all - first + BN - 1) / BN + back.k_parts - 1) / back.k_parts * BN;
   const int part = blockIdx.y, from = min(first + part * per, all), rows = min(all, from + per);
   const float ds = Half<T>::SCALED ? ds_scale(back.maxima, NORM_BLOCKS) : 1.f;
@@ -1363,7 +1366,8 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) {
       if (!C::any(i, wave)) continue;
-      const bool in = r0 + C::row(i, wave, lane) < rows;
+      const int r = r0 + C::row(i, wave, lane);
+      const bool in = r >= sees && r < rows;
       copy16(in ? qo[i] : NOWHERE, qd, lds + C::dst(i, wave));
       copy16(in ? go[i] : NOWHERE, gd, lds + TILE + C::dst(i, wave));
     }

@@ -892,6 +892,8 @@ class LogProbs:
 
 def _heads(t, what, dtype=None, shape=None):
     """(address, token stride, head stride) of [tokens, heads, width]."""
+    if t is None:
+        raise ValueError(f"{what}: missing")
     if t.dim() != 3 or (shape is not None and t.shape != shape):
         want = "[tokens, heads, width]" if shape is None else tuple(shape)
         raise ValueError(f"{what}: expected {want}, got {tuple(t.shape)}")
@@ -912,6 +914,8 @@ def _new_heads(t):
 
 def _vector(t, n, dtypes, what):
     """The address of a contiguous [n] on the current device."""
+    if t is None:
+        raise ValueError(f"{what}: missing")
     if t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes:
         raise ValueError(f"{what}: expected {', '.join(map(str, dtypes))} [{n}], got {t.dtype} {tuple(t.shape)}")
     if not _current(t, what).is_contiguous():
@@ -1047,7 +1051,11 @@ class PackedAttention:
             out, o = _new_heads(q)
         else:
             o = _heads(out, "out", q.dtype, q.shape)
-        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
+        shape = (q.shape[1], q.shape[0])
+        if fill:
+            lse = torch.empty(shape, dtype=torch.float32, device=q.device)
+        else:
+            lse = torch.full(shape, float("-inf"), device=q.device)
         work = self._work(lib().bc2n_attention_fwd_work_bytes, sizes, q.device)
         check(lib().bc2n_attention_fwd(_stream(), *sizes, *where, *x, int(fill), *o, lse.data_ptr(), _ptr(work)))
         return out, lse
@@ -1096,7 +1104,7 @@ class Sampler:
                     raise ValueError(f"{name}: expected {'int32' if whole else 'float32'}, got {v.dtype}")
                 self.settings.append((name, 0, v))
                 continue
-            v = int(v) if whole else float(v)
+            v = min(int(v), 1 << 31) if whole else float(v)
             if not (0 <= v if name != "temperature" else 0 <= v < float("inf")):
                 raise ValueError(f"{name} must not be negative" + ("" if whole else ", infinite or NaN"))
             self.settings.append((name, v, None))

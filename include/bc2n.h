@@ -663,8 +663,8 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
  * model's attention takes).  No reference counterpart.
  * q [tokens][heads][width] and k [tokens][kv_heads][width] of BC2N_F32,
  * BC2N_F16 or BC2N_BF16, each with a token stride and a head stride in
- * elements (slices of one projection, or heads first), a head's elements
- * contiguous; either may have 0 heads.  With x a head's row and w its weight
+ * elements (slices of one projection, or heads first; of one token or one head
+ * any), a head's elements contiguous; either may have 0 heads.  With x a head's row and w its weight
  * [width] (BC2N_F32 or the operands' type):
  *   y = x (mean x^2 + eps)^-1/2 w
  * and the pairs of its first `rotated` elements -- (i, i + rotated / 2), or
@@ -674,11 +674,11 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
  * is taken in 64 bits.  Norms, rotation and sums are f32, results rounded
  * once.  Widths: even; half of `rotated` and the rest are cut into vectors of
  * one power of two of elements, 8 (f32: 4) at most, of which a head has 128
- * at most: every width that is a multiple of 16 up to 1024 (f32: of 8, to
- * 512) with a quarter, half or all of it rotated, every even one up to 128.
- * Outputs may be their own inputs; they overlap nothing else.
+ * at most: every even width up to 128; beyond, multiples of 16 up to 1024 (f32:
+ * of 8, to 512) with all of them rotated, of 64 (f32: 32) with a half or a
+ * quarter too.  Either output may be its own input; they overlap nothing else.
  * bwd: d_q, d_k cotangents of the outputs and q, k the inputs -> q_grad,
- * k_grad of the operands' type (they may be those inputs or cotangents) and
+ * k_grad of the operands' type (each may be its own input or cotangent) and
  * d_q_weight, d_k_weight f32 [width] (either may be NULL), summed over tokens
  * and heads in one order; work is bc2n_headnorm_work_bytes() bytes, 16-byte
  * aligned, for the time of the call.
@@ -711,17 +711,22 @@ int bc2n_headnorm_bwd(void* stream, int dtype, int64_t tokens, int heads, int kv
  * keys from k_offsets[b] to k_offsets[b + 1] (i32 [sequences + 1] on the
  * device, rising); with q_lengths or k_lengths (i32 [sequences], or NULL) only the
  * first so many of them (a padded batch, a cache of fixed capacity).  The
- * offsets are read on the device alone, and cut to the tokens that there are.
+ * offsets are read on the device alone, and cut to the tokens that there are;
+ * where they fall, or cross each other, the results are unspecified.  Tiles of
+ * 128 rows, one more a sequence, times kv_heads stay below 2^23, and tokens
+ * times the heads of a group below 2^31 - 2^14.
  *   S = scale q k^T over the keys a query sees (all of its sequence's, or
  *   causal: query i of m sees the keys 0 .. i + n - m of n), P = softmax S,
  *   out = P v,  lse f32 [heads][q_tokens] = log sum e^S.
- *   - A query that sees no key has out 0, lse -inf and no gradient.
+ *   - A query that sees no key has out 0, lse -inf and no gradient, whatever it
+ *     and its cotangent hold.
  *   - Tokens of no sequence (before the first, behind the last, past a
  *     length) may hold anything.  Their rows of the results are zeros (lse
  *     -inf) where `fill` is set and left as they were where it is not.
  *   - A NaN or an infinity in a key reaches the rows that see it; in a value
  *     of a causal sequence it may also reach rows up to 63 tokens before it, as
- *     0 * NaN in a product of tiles.
+ *     0 * NaN in a product of tiles, and so may one in a key, a query or a
+ *     cotangent reach gradients up to 127 tokens from those it belongs to.
  * Products take the operands as they are, accumulate in f32 and round P and
  * its cotangent to the operands' type; maxima, sums and lse are f32, added in an
  * order that goes by the shapes and lengths alone.  In binary16 the
@@ -775,6 +780,7 @@ int bc2n_attention_bwd(void* stream, int dtype, int causal, int sequences, int64
  *   - A logit of -inf is never drawn.  A row with a NaN or +inf logit, of
  *     -inf alone, or with a NaN uniform or a NaN or infinite temperature has
  *     index -1 and logp NaN.
+ * index and logp overlap nothing that is read.
  * ---------------------------------------------------------------------- */
 int bc2n_sample(void* stream, int dtype, const void* logits, int64_t ld, int64_t rows, int classes,
                 const float* uniforms, double temperature, const float* temperatures, int64_t top_k,
