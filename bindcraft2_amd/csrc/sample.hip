@@ -14,12 +14,22 @@
 // for 131 k classes), and sums of those are exact in any order.  An e_j below
 // half of that counts as zero and can be left out of everything.
 //
-// A row is a workgroup's.  A rank or a share of the mass becomes a threshold on
-// (x, index) in one pass that counts the classes by their distance to the
-// maximum, in 2048 steps, and an exact ranking of the few in the step that the
-// border falls into; where ties or odd distributions leave many there, further
-// passes divide that step.  Exponentials in 64 bits cost twenty instructions
-// and are made only of classes still in play.
+// Rows of up to 64 classes take a lane a class, up to 1024 a wave a row, with the
+// row in registers; longer ones a workgroup a row.  Read once they are bound by
+// memory (1021 rows of 50 k f32: 41 us, 64 of them), so their one pass leaves the
+// maxima of short runs: what a cut can keep lies in the runs whose maxima reach
+// it, and those alone are read again.  The few classes of them (1024 at most) are put
+// in buckets by value and by index, compared with their own buckets, and drawn
+// from by sums in both orders.
+//
+// Where more stay, a rank or a share of the mass becomes a threshold on (x, index)
+// in one pass that counts the classes by their distance to the maximum, in 2048
+// steps, and an exact ranking of the few in the step that the border falls into;
+// where ties or odd distributions leave many there, further passes divide that
+// step.  Exponentials in 64 bits cost twenty instructions and are made only of
+// classes still in play; the passes that need them of all classes are bound by
+// them (64 rows of 131 k bfloat16: nothing cut 86 us, top-p of 0.9 191, top-k of
+// 50 19).
 #include "sample.h"
 
 #include "common.h"
@@ -30,6 +40,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace bc2n {
 
@@ -369,18 +380,40 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(Sample a) {
 // ---------------------------------------------------------------------------
 // A workgroup a row.
 constexpr int CANDIDATES = 1024;
+constexpr int RUNS = 2048;  // runs of a row's vectors whose maxima are kept
 template <int NT>
 struct Shared {
   u64 mass[BINS];
   uint32_t count[BINS];
-  u64 list_key[LIST];
-  u64 list_mass[LIST];
-  float x[CANDIDATES];
-  int j[CANDIDATES];
+  union {
+    struct {
+      u64 list_key[LIST];
+      u64 list_mass[LIST];
+    };
+    uint32_t live_runs[CANDIDATES];  // beside the steps' counts, which a cut of the row takes up
+  };
+  union {
+    struct {
+      float x[CANDIDATES];
+      int j[CANDIDATES];
+    };
+    float run_max[RUNS];  // until the candidates are collected
+  };
   u64 wave_a[NT / 64], wave_b[NT / 64];
   u64 out[4];
   uint32_t n, found;
 };
+
+// The larger of two (of a NaN and a number either), in one instruction: fmaxf takes
+// one more an operand, which signalling NaNs need.
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float row_below(float v) {
+  const int b = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, CTRL, ROWS, 0xF, false));
+}
 
 // over the workgroup, the result in every thread
 template <int NT, class F>
@@ -414,6 +447,7 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* waves) {  // exclusive
 template <class T, int NT>
 struct RowOf {
   static constexpr int E = Vec<T>::N;
+  typedef T Type;
   const T* x;
   int V;
 
@@ -423,46 +457,48 @@ struct RowOf {
 #pragma unroll 1
     for (int j = threadIdx.x; j < V; j += NT) f((float)x[j], j);
   }
-  // f(classes' values, index of the first, number of the vector) of a thread's
-  // vectors.  One that would pass the row's end is read ending there, and its
-  // classes that another thread has are -infinity.
+  __device__ __forceinline__ int count() const { return (V + E - 1) / E; }
+  // Vector q's place.  One that would pass the row's end is read ending there, and
+  // its classes that the one before has are -infinity.
+  __device__ __forceinline__ int first(int q) const { return min(q * E, V - E); }
+  __device__ __forceinline__ void values(u32x4 raw, int q, float (&v)[E]) const {
+    Vec<T>::unpack(raw, v);
+    const int twice = q * E - first(q);
+    if (twice) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = e < twice ? NEG_INF : v[e];
+    }
+  }
+  // f(classes' values, number, whether it may be past the last) of a thread's vectors,
+  // lanes next to each other having vectors next to each other; past the last all
+  // of them are -infinity.
   template <class F>
   __device__ __forceinline__ void vectors(F f) const {
-    constexpr int AT_ONCE = 4;
-    const int n = (V + NT * E - 1) / (NT * E);
-    auto first = [&](int i) { return min((i * NT + (int)threadIdx.x) * E, V - E); };
-    auto one = [&](u32x4 raw, int i, int u) __attribute__((always_inline)) {
+    constexpr int AT_ONCE = NT == 1024 ? 8 : 4;
+    const int n = (count() + NT - 1) / NT;
+    auto one = [&](u32x4 raw, int q, auto end) __attribute__((always_inline)) {
       float v[E];
-      Vec<T>::unpack(raw, v);
-      const int j = first(i), own = (i * NT + (int)threadIdx.x) * E;
-      if ((int64_t)(i + 1) * NT * E > V) {  // the same for all threads
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = j + e < own ? NEG_INF : v[e];
-      }
-      f(v, j, u);
+      if (decltype(end)::value) values(raw, q, v);
+      else Vec<T>::unpack(raw, v);
+      f(v, q, end);
     };
     int i = 0;
-    for (; i + AT_ONCE <= n; i += AT_ONCE) {
+    for (; i + AT_ONCE < n; i += AT_ONCE) {
       u32x4 raw[AT_ONCE];
 #pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) raw[u] = Vec<T>::load(x + first(i + u));
+      for (int u = 0; u < AT_ONCE; ++u) raw[u] = Vec<T>::load(x + (int64_t)((i + u) * NT + (int)threadIdx.x) * E);
 #pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) one(raw[u], i + u, u);
+      for (int u = 0; u < AT_ONCE; ++u) one(raw[u], (i + u) * NT + (int)threadIdx.x, std::false_type());
     }
-    for (; i < n; ++i) one(Vec<T>::load(x + first(i)), i, 0);
+    u32x4 raw[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+      if (i + u < n) raw[u] = Vec<T>::load(x + first((i + u) * NT + (int)threadIdx.x));
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+      if (i + u < n) one(raw[u], (i + u) * NT + (int)threadIdx.x, std::true_type());
   }
 };
-// The classes that a row's draw is among, where they are few: in LDS, in no order.
-template <int NT>
-struct Candidates {
-  Shared<NT>& sh;
-  int n;
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    for (int i = threadIdx.x; i < n; i += NT) f(sh.x[i], sh.j[i]);
-  }
-};
-
 template <int NT>
 struct Drawer {
   Shared<NT>& sh;
@@ -488,7 +524,7 @@ struct Drawer {
   // The last filled step whose forerunners, `before` and the steps before it,
   // weigh less than the end; `before` becomes what those weigh.
   template <bool MASS>
-  __device__ int last_step(u64 end, u64& before) {
+  __device__ __forceinline__ int last_step(u64 end, u64& before) {
     constexpr int PER = BINS / NT;
     u64 w = 0;
 #pragma unroll
@@ -517,7 +553,7 @@ struct Drawer {
   // Counts and (masses) masses of the classes of `from` in steps of distance, those
   // of rank keys >= least.
   template <class S_>
-  __device__ void fill(const S_& from, bool masses, u64 least) {
+  __device__ __forceinline__ void fill(const S_& from, bool masses, u64 least) {
     clear(masses);
     from.each([&](float x, int j) {
       if (!counts(x) || rank_key(x, j) < least) return;
@@ -528,7 +564,7 @@ struct Drawer {
     __syncthreads();
   }
   // The weight of all steps.
-  __device__ u64 filled_mass(int steps_) {
+  __device__ __forceinline__ u64 filled_mass(int steps_) {
     u64 w = 0;
     for (int b = threadIdx.x; b < steps_; b += NT) w += sh.mass[b];
     return block_fold<NT>(w, sh.wave_b, Sum());
@@ -540,7 +576,7 @@ struct Drawer {
   // mass of the classes up to that one, if the steps' masses are filled and tell
   // it, and false is left in `intact` where the steps were filled anew.
   template <bool MASS, class S_>
-  __device__ u64 last_before(const S_& from, u64 end, u64 least, bool& intact, u64* kept = nullptr) {
+  __device__ __forceinline__ u64 last_before(const S_& from, u64 end, u64 least, bool& intact, u64* kept = nullptr) {
     u64 lo = 0, hi = ~u64(0), before = 0;
     int shift = -1;  // -1: steps of distance
     for (;;) {
@@ -604,26 +640,49 @@ struct Drawer {
     }
   }
 
-  // The first CANDIDATES of the classes that are at least `low` to LDS; how many
-  // there are.
+  // The classes that are at least `low` to LDS, from the runs of 2^shift vectors
+  // that have one; how many there are, more than CANDIDATES where not all fit.
   template <class R>
-  __device__ int collect(const R& row, float low) {
-    row.vectors([&](const float (&v)[R::E], int j, int) {
-      float top = v[0];
+  __device__ __forceinline__ int collect(const R& row, float low, int runs, int shift) {
+    if (threadIdx.x == 0) sh.n = sh.found = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < runs; i += NT) {
+      if (sh.run_max[i] >= low) {
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < CANDIDATES) sh.live_runs[at] = i;
+      }
+    }
+    __syncthreads();
+    const int live = (int)sh.n, n = min(live, CANDIDATES) << shift;
+    __syncthreads();  // what follows may clear it
+    if (live > CANDIDATES) return live;
+    constexpr int AT_ONCE = 4;
+    for (int i0 = threadIdx.x; i0 < n; i0 += AT_ONCE * NT) {
+      u32x4 raw[AT_ONCE];
+      int q[AT_ONCE];
 #pragma unroll
-      for (int e = 1; e < R::E; ++e) top = fmaxf(top, v[e]);
-      if (top < low) return;
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = min(i0 + u * NT, n - 1);
+        q[u] = ((int)sh.live_runs[i >> shift] << shift) + (i & ((1 << shift) - 1));
+        raw[u] = Vec<typename R::Type>::load(row.x + row.first(q[u]));
+      }
 #pragma unroll
-      for (int e = 0; e < R::E; ++e) {
-        if (v[e] >= low) {
-          const uint32_t at = atomicAdd(&sh.found, 1u);
-          if (at < CANDIDATES) {
-            sh.x[at] = v[e];
-            sh.j[at] = j + e;
+      for (int u = 0; u < AT_ONCE; ++u) {
+        if (i0 + u * NT >= n || q[u] >= row.count()) continue;
+        float v[R::E];
+        row.values(raw[u], q[u], v);
+#pragma unroll
+        for (int e = 0; e < R::E; ++e) {
+          if (v[e] >= low) {
+            const uint32_t at = atomicAdd(&sh.found, 1u);
+            if (at < CANDIDATES) {
+              sh.x[at] = v[e];
+              sh.j[at] = row.first(q[u]) + e;
+            }
           }
         }
       }
-    });
+    }
     __syncthreads();
     return (int)sh.found;
   }
@@ -638,7 +697,7 @@ struct Drawer {
   // by index from comparing each with all, sums of forerunners by scans in
   // their orders.
   template <class ST>
-  __device__ void draw_few(const Sample& a, int64_t r, int n, const ST& s, u64 whole) {
+  __device__ __forceinline__ void draw_few(const Sample& a, int64_t r, int n, const ST& s, u64 whole) {
     const int lane = threadIdx.x;
     const float x = lane < n ? sh.x[lane] : NEG_INF;
     const int j = lane < n ? sh.j[lane] : 0x7fffffff;
@@ -672,34 +731,119 @@ struct Drawer {
     if (w && before <= target && before + w > target) write(a, r, j, log_share(t, mass, S));
   }
 
-  // The class of `from` at which the kept masses' running sum by index passes u of
-  // the whole: written.  bits: of an index.
-  template <class KEPT>
-  __device__ void draw(const Sample& a, int64_t r, const Candidates<NT>& from, float u, int bits, KEPT kept) {
-    clear(true);
-    const int shift = max(bits - 11, 0);  // 2048 runs of indexes
-    u64 mine = 0;
-    from.each([&](float x, int j) {
-      const u64 w = kept(x, j);
-      mine += w;
-      if (w) {
-        atomicAdd(&sh.mass[j >> shift], w);
-        atomicAdd(&sh.count[j >> shift], 1u);
+  // The same of up to CANDIDATES by the workgroup: in buckets by distance (least: the
+  // candidates' least value) and in buckets by index, and only those of its own are
+  // compared with a class.
+  template <class ST>
+  __device__ __forceinline__ void draw_some(const Sample& a, int64_t r, int n, float least, const ST& s, u64 whole) {
+    constexpr int U = CANDIDATES / NT, BUCKETS = 256, PER = BUCKETS / 64;
+    const int t = threadIdx.x, lane = t & 63;
+    int shift = 0;
+    while ((a.V - 1) >> shift >= BUCKETS) ++shift;
+    const float f = fminf((BUCKETS - 1) / fminf(m - least, range), 3e38f);
+    auto bucket = [&](float x) { return (int)fminf((m - x) * f, (float)(BUCKETS - 1)); };
+    uint32_t *count = sh.count, *start = sh.count + 2 * BUCKETS;  // by value, then by index
+    for (int i = t; i < 2 * BUCKETS; i += NT) count[i] = 0;
+    __syncthreads();
+    float x[U];
+    int j[U], slot[U], rank[U], place[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = t + u * NT;
+      x[u] = c < n ? sh.x[c] : NEG_INF;
+      j[u] = c < n ? sh.j[c] : 0;
+      if (c < n)
+        slot[u] = (int)(atomicAdd(&count[bucket(x[u])], 1u) |
+                        atomicAdd(&count[BUCKETS + (j[u] >> shift)], 1u) << 16);
+    }
+    __syncthreads();
+    if (t < 128) {  // a wave for each
+      const uint32_t* from = count + (t >> 6) * BUCKETS + lane * PER;
+      uint32_t own = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) own += from[i];
+      uint32_t run = (uint32_t)wave_scan((u64)own, Sum()) - own;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        start[(t >> 6) * BUCKETS + lane * PER + i] = run;
+        run += from[i];
       }
-    });
-    const u64 whole = block_fold<NT>(mine, sh.wave_b, Sum()), target = target_of(u, whole);
-    // the last run whose forerunners weigh at most the target
-    u64 before = 0;
-    const int run = last_step<true>(target + 1, before);
-    from.each([&](float x, int j) {
-      if (j >> shift != run) return;
-      const u64 w = kept(x, j);
-      u64 f = before;
-      if (sh.count[run] > 1 && w)
-        for (int i = 0; i < from.n; ++i)
-          if (sh.j[i] < j && sh.j[i] >> shift == run) f += kept(sh.x[i], sh.j[i]);
-      if (w && f <= target && f + w > target) write(a, r, j, log_share(distance(x), whole, S));
-    });
+    }
+    __syncthreads();
+    float* by_value = reinterpret_cast<float*>(sh.mass);  // values, and their indexes
+    int* index_of = reinterpret_cast<int*>(by_value + CANDIDATES);
+    int* by_index = index_of + CANDIDATES;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u * NT >= n) continue;
+      const int at = (int)start[bucket(x[u])] + (slot[u] & 0xffff);
+      by_value[at] = x[u];
+      index_of[at] = j[u];
+      by_index[start[BUCKETS + (j[u] >> shift)] + (slot[u] >> 16)] = j[u];
+    }
+    __syncthreads();
+    u64 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = 0;
+      rank[u] = place[u] = 0;
+      if (t + u * NT >= n) continue;
+      int b = bucket(x[u]), i = (int)start[b], end = i + (int)count[b];
+      rank[u] = i;
+      for (; i < end; ++i) {
+        const float y = by_value[i];
+        rank[u] += y > x[u] || (y == x[u] && index_of[i] < j[u]);
+      }
+      b = BUCKETS + (j[u] >> shift);
+      i = (int)start[b];
+      end = i + (int)count[b];
+      place[u] = i;
+      for (; i < end; ++i) place[u] += by_index[i] < j[u];
+      if (counts(x[u]) && !(s.k && rank[u] >= s.k)) w[u] = mass(x[u]);
+    }
+    // what the forerunners weigh, in the order that `at` numbers
+    auto forerunners = [&](const int (&at)[U], u64 (&v)[U]) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (t + u * NT < n) sh.mass[at[u]] = w[u];
+      __syncthreads();
+      u64 own = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) own += t * U + u < n ? sh.mass[t * U + u] : 0;
+      u64 run = block_scan<NT>(own, sh.wave_a);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (t * U + u >= n) continue;
+        sh.mass[CANDIDATES + t * U + u] = run;
+        run += sh.mass[t * U + u];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = t + u * NT < n ? sh.mass[CANDIDATES + at[u]] : 0;
+    };
+    auto all = [&] {
+      u64 sum = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum += w[u];
+      return block_fold<NT>(sum, sh.wave_b, Sum());
+    };
+    u64 before[U];
+    if (s.p < 1.0) {
+      if (s.k) whole = all();
+      const u64 end = share_of(s.p, whole);
+      forerunners(rank, before);
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = before[u] >= end ? 0 : w[u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = distance(x[u]) < s.floor ? 0 : w[u];
+    const u64 sum = all(), target = target_of(s.u, sum);
+    forerunners(place, before);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (w[u] && before[u] <= target && before[u] + w[u] > target)
+        write(a, r, j[u], log_share(distance(x[u]), sum, S));
   }
 };
 
@@ -712,18 +856,53 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   typedef RowOf<T, NT> R;
   const R row{reinterpret_cast<const T*>(a.x) + r * a.ld, a.V};
   const Settings s = settings_of(a, r);
-  if (threadIdx.x == 0) sh.found = 0;
-  // maxima of four parts of a thread's vectors
-  float part[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+  // Maxima of runs of 2^shift vectors, as short as there is room for (up to 8, and
+  // from 64 on): later passes over few classes read their runs alone.
+  int shift = 0;
+  while (((row.count() - 1) >> shift) >= RUNS) shift += shift == 3 ? 3 : 1;
+  const int runs = ((row.count() - 1) >> shift) + 1;
+  float hi = NEG_INF;
   bool nan = false;
-  row.vectors([&](const float (&v)[R::E], int, int u) {
+  auto maxima = [&](auto lanes) __attribute__((always_inline)) {
+    constexpr int L = decltype(lanes)::value;
+    const bool last = (lane & (L - 1)) == L - 1;  // has its run's maximum
+    row.vectors([&](const float (&v)[R::E], int q, auto end) __attribute__((always_inline)) {
+      float g = v[0];
 #pragma unroll
-    for (int e = 0; e < R::E; ++e) {
-      nan |= v[e] != v[e];
-      part[u] = fmaxf(part[u], v[e]);
-    }
-  });
-  const float hi = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+      for (int e = 0; e < R::E; e += 2) {
+        nan |= __builtin_isunordered(v[e], v[e + 1]);
+        if (e) g = larger(g, v[e]);
+        g = larger(g, v[e + 1]);
+      }
+      hi = larger(hi, g);
+      if (L >= 2) g = larger(g, dpp_mov<DPP_QUAD_1032>(g));
+      if (L >= 4) g = larger(g, dpp_mov<DPP_QUAD_2301>(g));
+      if (L >= 8) g = larger(g, dpp_mov<DPP_ROW_HALF_MIRROR>(g));
+      if (L == 64) {
+        g = larger(g, dpp_mov<DPP_ROW_MIRROR>(g));
+        g = larger(g, row_below<ROW_BCAST15, 0xA>(g));
+        g = larger(g, row_below<ROW_BCAST31, 0xC>(g));
+      }
+      const int run = q >> shift;
+      if (last && (!decltype(end)::value || run < runs)) {
+        if (L < 64 || shift == 6) sh.run_max[run] = g;
+        else __hip_atomic_fetch_max(&sh.run_max[run], g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      }
+    });
+  };
+  if (shift == 0) {
+    maxima(std::integral_constant<int, 1>());
+  } else if (shift == 1) {
+    maxima(std::integral_constant<int, 2>());
+  } else if (shift == 2) {
+    maxima(std::integral_constant<int, 4>());
+  } else if (shift == 3) {
+    maxima(std::integral_constant<int, 8>());
+  } else {
+    for (int i = threadIdx.x; i < runs; i += NT) sh.run_max[i] = NEG_INF;
+    __syncthreads();
+    maxima(std::integral_constant<int, 64>());
+  }
   const u64 top = block_fold<NT>(nan ? ~u64(0) : (u64)key_of(hi), sh.wave_a, Max());
   const uint32_t bits = (uint32_t)top;
   const float m = __builtin_bit_cast(float, bits & 0x80000000u ? bits & 0x7fffffffu : ~bits);
@@ -733,13 +912,21 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   }
   if (s.greedy) {
     u64 first = ~u64(0);
-    row.vectors([&](const float (&v)[R::E], int j, int) {
+    for (int i = threadIdx.x; i < runs; i += NT)
+      if (sh.run_max[i] == m) first = min(first, (u64)i);
+    first = block_fold<NT>(first, sh.wave_b, Min());
+    u64 at = ~u64(0);
+    for (int i = threadIdx.x; i < 1 << shift; i += NT) {
+      const int q = ((int)first << shift) + i;
+      if (q >= row.count()) break;
+      float v[R::E];
+      row.values(Vec<T>::load(row.x + row.first(q)), q, v);
 #pragma unroll
       for (int e = 0; e < R::E; ++e)
-        if (v[e] == m) first = min(first, (u64)(j + e));
-    });
-    first = block_fold<NT>(first, sh.wave_b, Min());
-    if (threadIdx.x == 0) write(a, r, (int)first, 0.f);
+        if (v[e] == m) at = min(at, (u64)(row.first(q) + e));
+    }
+    at = block_fold<NT>(at, sh.wave_a, Min());
+    if (threadIdx.x == 0) write(a, r, (int)at, 0.f);
     return;
   }
   Drawer<NT> d{sh, m, 0.f, 0.f, s.inv, mass_bits(a.V)};
@@ -748,75 +935,82 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   d.steps = fminf((float)(BINS - 1) / d.range, 3e38f);
 
   u64 least = 0, whole = 0;
-  // The candidates: with top-k, what is at least the k-th of the maxima of the
-  // threads' parts, but for a coarse step, which the k-th class is; with top-p
-  // alone, what is within the step in which the mass passes it.
+  // The candidates: with top-k, what is at least the k-th of the runs' maxima,
+  // but for a coarse step, which the k-th class is, or where that is too many (1.9 k
+  // of random rows with 4/3 k runs, more with fewer) what is within the k-th
+  // class's step; with top-p alone, what is within the step in which the mass
+  // passes it; with min-p alone, what is that large.
   int n = CANDIDATES + 1;
-  const bool by_k = s.k && s.k <= 2 * NT && s.k <= CANDIDATES / 2;
-  if (by_k) {
+  float low = NEG_INF;
+  if (s.k && 4 * s.k <= 3 * runs && s.k <= CANDIDATES / 2) {
     constexpr int COARSE = 4, BINS_K = BINS / COARSE, PER = BINS_K / 64;
     for (int i = threadIdx.x; i < BINS_K; i += NT) sh.count[i] = 0;
     __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (d.counts(part[u])) atomicAdd(&sh.count[d.step_of(part[u]) / COARSE], 1u);
+    for (int i = threadIdx.x; i < runs; i += NT) {
+      const float x = sh.run_max[i];
+      if (d.counts(x)) atomicAdd(&sh.count[d.step_of(x) / COARSE], 1u);
+    }
     __syncthreads();
     // each wave for itself
     uint32_t own = 0, c[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) own += c[i] = sh.count[lane * PER + i];
     u64 run = wave_scan((u64)own, Sum()) - own;
-    int step = BINS_K;  // fewer than k parts that count: all classes that do
+    int step = BINS_K;  // fewer than k runs that count: all classes that do
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       if (run < (u64)s.k && run + c[i] >= (u64)s.k) step = lane * PER + i;
       run += c[i];
     }
     step = (int)wave_fold((u64)step, Min());
-    n = d.collect(row, d.lowest(min(step * COARSE + COARSE - 1, BINS - 1)));
+    low = d.lowest(min(step * COARSE + COARSE - 1, BINS - 1));
+  } else if (s.k && s.k < CANDIDATES) {
+    d.clear(false);
+    row.vectors([&](const float (&v)[R::E], int, auto) {
+#pragma unroll
+      for (int e = 0; e < R::E; ++e)
+        if (d.counts(v[e])) atomicAdd(&sh.count[d.step_of(v[e])], 1u);
+    });
+    __syncthreads();
+    u64 before = 0;
+    low = d.lowest(d.template last_step<false>((u64)s.k, before));
   } else if (!s.k && s.p < 1.0) {
     d.fill(row, true, 0);
     whole = d.filled_mass(BINS);
     u64 before = 0;
-    const int step = d.template last_step<true>(share_of(s.p, whole), before);
-    n = d.collect(row, d.lowest(step));
+    low = d.lowest(d.template last_step<true>(share_of(s.p, whole), before));
+  } else if (!s.k && s.floor > (double)NEG_INF) {
+    low = (float)((double)m + s.floor / s.inv);
+    low -= 1e-6f * (fabsf(low) + fabsf(m)) + 1e-37f;
   }
+  if (low > NEG_INF) n = d.collect(row, low, runs, shift);
   auto kept_mass = [&](float x, int j) -> u64 {
     if (!d.counts(x) || rank_key(x, j) < least) return 0;
     const double t = d.distance(x);
     return t < s.floor ? 0 : mass_of(t, d.S);
-  };
-  // The cuts, each by the steps that the one before has left where they tell it.
-  auto cut = [&](const auto& from, bool filled) {
-    const bool by_mass = s.p < 1.0;
-    bool intact = true;
-    if (s.k) {
-      d.fill(from, by_mass, 0);
-      least = d.template last_before<false>(from, (u64)s.k, 0, intact, by_mass ? &whole : nullptr);
-      if (by_mass && !intact) {
-        d.fill(from, true, least);
-        whole = d.filled_mass(BINS);
-        intact = true;
-      }
-    } else if (by_mass && !filled) {
-      d.fill(from, true, 0);
-    }
-    // steps beyond the k-th class weigh nothing here: what is before them is the whole
-    if (by_mass) least = d.template last_before<true>(from, share_of(s.p, whole), least, intact);
   };
   if (n <= 64) {
     if (wave == 0) d.draw_few(a, r, n, s, whole);
     return;
   }
   if (n <= CANDIDATES) {
-    const Candidates<NT> few{sh, n};
-    cut(few, false);
-    int index_bits = 0;
-    while ((int64_t(1) << index_bits) < a.V) ++index_bits;
-    d.draw(a, r, few, s.u, index_bits, kept_mass);
+    d.draw_some(a, r, n, low, s, whole);
     return;
   }
-  cut(row, !s.k && s.p < 1.0);
+  // The cuts, each by the steps that the one before has left where they tell it.
+  const bool by_mass = s.p < 1.0;
+  bool intact = true;
+  if (s.k) {
+    d.fill(row, by_mass, 0);
+    least = d.template last_before<false>(row, (u64)s.k, 0, intact, by_mass ? &whole : nullptr);
+    if (by_mass && !intact) {
+      d.fill(row, true, least);
+      whole = d.filled_mass(BINS);
+      intact = true;
+    }
+  }
+  // steps beyond the k-th class weigh nothing here: what is before them is the whole
+  if (by_mass) least = d.template last_before<true>(row, share_of(s.p, whole), least, intact);
 
   // the running sum over the whole row in tiles of OWN classes a thread: groups of
   // tiles, then the tiles of one group, then the waves of one tile
@@ -905,9 +1099,13 @@ void go(hipStream_t st, const Sample& a) {
     else if (a.V <= 256) sample_wave_kernel<T, 4><<<grid, 256, 0, st>>>(a);
     else if (a.V <= 512) sample_wave_kernel<T, 8><<<grid, 256, 0, st>>>(a);
     else sample_wave_kernel<T, 16><<<grid, 256, 0, st>>>(a);
-  } else if (a.V <= 16 * 256 * E) row_go<T, 256>(st, a);
-  else if (a.rows > device_cus()) row_go<T, 512>(st, a);
-  else row_go<T, 1024>(st, a);
+  } else if (a.V <= 16 * 256 * E) {
+    row_go<T, 256>(st, a);  // 16 vectors a thread at most: more workgroups a unit
+  } else if (a.rows > device_cus()) {
+    row_go<T, 512>(st, a);  // two a unit
+  } else {
+    row_go<T, 1024>(st, a);  // one: 64 rows of 131 k 99 us of 512 threads, 82 so
+  }
 }
 
 }  // namespace
