@@ -1589,12 +1589,26 @@ namespace {
 
 int padded(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : 128; }
 
+// Up to so many keys of all sequences one workgroup takes any sequence's.
+constexpr int64_t UNSPLIT = 4096;
+
 // Whether the rows go to the few-rows kernel: where a sequence has 32 rows or
-// fewer, or 128-row workgroups would leave compute units idle.
+// fewer, and where 128-row workgroups (`blocks` of them, each a sequence's keys
+// long) would leave so many compute units idle that the other's overheads cost
+// less.  A 128-row workgroup by itself on a unit takes 64 keys in 1.1 to 1.5 us;
+// the stretches of all rows take a unit's share of the same in 1.65 times that, and
+// their join some 20 us: they win where keys * (2/3 - blocks / units) is above 800
+// (one sequence, 4 heads: of 4000 tokens 25 against 48 us, of 7900 200 against
+// 133; three of 1800 61 against 34).  Without a join four waves share a
+// sequence's keys, which from 1024 on pays as long as units are idle (one of 3000, 8
+// heads 29 against 54 us; six of 512 25 against 16).
 bool few_rows(const PackedAttn& a) {
-  const int64_t rows = a.q_tokens * (a.heads / a.kv_heads);
-  const int64_t live = std::min<int64_t>(a.sequences, a.q_tokens);
-  return rows <= 32 * live || std::max((rows + 127) / 128, live) * a.kv_heads < device_cus();
+  const int64_t rows = a.q_tokens * (a.heads / a.kv_heads), cus = device_cus();
+  const int64_t live = std::max<int64_t>(1, std::min<int64_t>(a.sequences, a.q_tokens));
+  if (rows <= 32 * live) return true;
+  const int64_t blocks = std::max((rows + 127) / 128, live) * a.kv_heads, keys = a.k_tokens / live;
+  if (a.k_tokens <= UNSPLIT) return 8 * blocks < 5 * cus || (keys >= 1024 && blocks < cus);
+  return 3 * blocks < 2 * cus && keys * (2 * cus - 3 * blocks) > 3 * 800 * cus;
 }
 // Waves of it that the card holds, by their registers.
 int64_t few_grid(const PackedAttn&) { return (int64_t)device_cus() * 8; }
@@ -1612,8 +1626,6 @@ Split carve_split(const PackedAttn& a, char* p, size_t* bytes) {
   *bytes = z.off;
   return s;
 }
-// Up to so many keys of all sequences one workgroup takes any sequence's.
-constexpr int64_t UNSPLIT = 4096;
 bool may_split(const PackedAttn& a) { return a.q_tokens > 0 && few_rows(a) && a.k_tokens > UNSPLIT; }
 
 }  // namespace
@@ -1694,7 +1706,10 @@ void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
     const int64_t rows = a.q_tokens * G, live = std::max<int64_t>(1, std::min<int64_t>(a.sequences, a.q_tokens));
     const int64_t x = std::min(live + rows / 32, goal) * a.kv_heads;
     const int64_t y = std::min<int64_t>(32, (rows + live - 1) / live);
-    if (goal >= 32 * live)
+    // 16 waves a row where it has some 32 stretches (one sequence of 131 k, 8 rows a
+    // head of keys: 12 us), one where it has fewer (7974 rows of three heads, two or
+    // three stretches each: 592 us of 16 waves, 41 of one)
+    if (goal >= 32 * std::max(live, rows / 32))
       packattn_join_kernel<T, DP, 16><<<dim3((unsigned)x, (unsigned)y), 1024, 0, st>>>(a, goal, split);
     else
       packattn_join_kernel<T, DP, 1><<<dim3((unsigned)x, (unsigned)(y + 3) / 4), NT, 0, st>>>(a, goal, split);

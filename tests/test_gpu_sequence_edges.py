@@ -146,3 +146,19 @@ def test_refused_tensors(cuda):
         ops.Sampler(top_p=u[:5]).sample(x, u)
     with pytest.raises(NativeError, match="row stride"):
         ops.Sampler().sample(x[:1].expand(6, 50), u)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,heads,kv,d,causal", [(700, 9000, 2, 1, 64, True), (1200, 5000, 3, 1, 128, False),
+                                                   (2600, 2600, 2, 2, 32, True), (5100, 5100, 1, 1, 64, True),
+                                                   (6001, 6001, 2, 2, 40, True)])
+def test_few_long_sequences(cuda, m, n, heads, kv, d, causal, dtype):
+    """On both sides of the rules by which few workgroups of rows share the keys."""
+    q, g = rand(1, m, heads, d, dtype=dtype), rand(2, m, heads, d, dtype=dtype)
+    k, v = rand(3, n, kv, d, dtype=dtype), rand(4, n, kv, d, dtype=dtype)
+    op, qo, ko = ops.PackedAttention(causal), i32(0, m), i32(0, n)
+    out, lse = op.forward(q, k, v, qo, ko)
+    grads = op.backward(g, q, k, v, out, lse, qo, ko)
+    want = R.attention(q, k, v, causal, d ** -0.5, g)
+    for name, got in zip(("out", "lse", "d_q", "d_k", "d_v"), (out, lse, *grads)):
+        R.check(name, got, *want[name])
