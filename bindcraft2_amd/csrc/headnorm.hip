@@ -13,7 +13,9 @@
 // Every element is read once and written once (the gradient reads two), some
 // ten operations each, so memory bounds it: 16-byte loads, a head in the
 // registers of a few lanes, and the angles, which all heads of a token share,
-// made once for all of them.
+// made once for all of them.  16384 tokens of 40 heads of 128 bfloat16: 75 us, 4.5
+// TB/s (when it took 98: vectors of 8 bytes 114, stores past the caches 111); the
+// gradient of 8191 tokens of 20 heads of 64 f32 25 us, 5.0 TB/s, and 4 of its join.
 //
 // A lane holds units of two vectors of N elements that rotate into each other
 // (or, past R, two vectors side by side; interleaved, one run of 2 N), N the

@@ -622,6 +622,12 @@ struct Online {
 
 // Workgroup = 128 rows of one sequence and head of keys, 4 waves x 32 rows;
 // keys in tiles of 64, two buffers, one barrier a tile.
+//
+// Products and exponentials bound it: two workgroups a unit, one's products beside
+// the other's exponentials.  11 causal sequences of 16384 tokens, 32 heads over 8
+// of 128, bfloat16: 370 us, 835 TFLOP/s of what is seen, two thirds of what a
+// large library product reaches; with the operands read as they are needed
+// instead of up to eight ahead (the order below) 393.
 template <class T, int DP>
 __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64_t tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -694,8 +700,10 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
 // wave adds up all sequences' blocks, which gives the length of a stretch for
 // `goal` equal ones a head, and finds its own among them.  A wave has one
 // buffer of keys and one of values, and refills each as soon as it is read, so
-// that nearly all of the LDS is in flight nearly all of the time.  Rows of more
-// than one stretch go to packattn_join_kernel through memory.
+// that nearly all of the LDS is in flight nearly all of the time (64 sequences of
+// 11 .. 8192 keys, 8 heads of 128: 240 MB in 56 us, 4.3 TB/s; one of 131 k, 4 heads
+// of 64: 134 MB in 30).  Rows of more than one stretch go to packattn_join_kernel
+// through memory.
 // W = 4, few keys: all of a sequence's by one workgroup, every fourth block a
 // wave, joined in LDS: no second launch.
 struct Split {
@@ -931,7 +939,9 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
 }
 
 // The stretches of rows, RW waves a row: DP / 4 lanes a stretch, each lane group
-// with a reference of its own.
+// with a reference of its own.  Bound by its launch and one round of loads: 10 us
+// beside 56 of the stretches (64 sequences of 11 .. 8192 keys), 12 beside 30 (one of
+// 131 k).
 template <class T, int DP, int RW>
 __global__ __launch_bounds__(RW > 1 ? 64 * RW : NT) void packattn_join_kernel(PackedAttn a, int64_t goal, Split split) {
   constexpr int KN = block_keys(DP), LP = DP / 4, ROWS = RW > 1 ? 1 : WAVES, GROUPS = 64 * RW / LP;
@@ -1090,7 +1100,11 @@ struct Back {
 };
 
 constexpr int FEW_KEYS = 256;
-// dq, and D = sum (do o) of every row for the other kernel.
+// dq, and D = sum (do o) of every row for the other kernel.  The forward's layout
+// with a product more, and as it bound by products and exponentials.  The scores
+// are made in both kernels, so that neither adds to memory in an order of
+// chance: nine products for seven.  6 causal sequences of 10007 tokens, 32 heads
+// over 8 of 128, bfloat16: this 320 us (340 without the order of reads), the other 490.
 template <class T, int DP>
 __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_t tiles, Back back) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -1264,7 +1278,9 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
 //
 // dk and dv take half of a wave's registers, so two waves a SIMD, without which
 // the matrix cores wait for each exponential, leave no room for the keys' and
-// values' operands beside them: those are read from LDS, in operand order.
+// values' operands beside them: those are read from LDS, in operand order (one
+// wave a SIMD with them in registers 960 us, two 672, with the reads ahead of
+// their products and the heaviest tiles first 490).
 template <class T, int DP>
 __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, Back back) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -1523,6 +1539,7 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
 }
 
 constexpr int SUM_TOKENS = 4;  // of a workgroup
+// Bound by memory; 7 to 18 us where there are parts at all.
 // The parts' sums of a few tokens of one sequence: blockIdx.y 0 of dq, 1 of dk, 2 of dv.
 template <class T, int DP>
 __global__ __launch_bounds__(NT) void packattn_sum_kernel(PackedAttn a, Back back) {

@@ -572,11 +572,11 @@ struct Drawer {
 
   // The rank key of the last class of `from` whose forerunners, among those of
   // rank keys >= least, weigh less than `end`: by number, or (MASS) by mass.  The
-  // steps have to be filled, with those at least; `kept`, where given, gets the
-  // mass of the classes up to that one, if the steps' masses are filled and tell
-  // it, and false is left in `intact` where the steps were filled anew.
+  // steps have to be filled, with those at least.  False is left in `intact` where
+  // they were filled anew; else, with `tell` and the steps' masses filled, `kept`
+  // gets the mass of the classes up to that one.
   template <bool MASS, class S_>
-  __device__ __forceinline__ u64 last_before(const S_& from, u64 end, u64 least, bool& intact, u64* kept = nullptr) {
+  __device__ __forceinline__ u64 last_before(const S_& from, u64 end, u64 least, bool& intact, bool tell, u64& kept) {
     u64 lo = 0, hi = ~u64(0), before = 0;
     int shift = -1;  // -1: steps of distance
     for (;;) {
@@ -592,7 +592,7 @@ struct Drawer {
           if (c < least || c < lo || c > hi || bin_of(x, c) != bin) return;
           const uint32_t at = atomicAdd(&sh.n, 1u);
           sh.list_key[at] = c;
-          sh.list_mass[at] = MASS || kept ? mass(x) : 1;
+          sh.list_mass[at] = MASS || tell ? mass(x) : 1;
         });
         __syncthreads();
         const int n = (int)sh.n;
@@ -604,10 +604,10 @@ struct Drawer {
           if (f < end) key = min(key, c);
         }
         key = block_fold<NT>(key, sh.wave_a, Min());
-        if (kept && intact) {
+        if (tell && intact) {
           u64 w = 0;
           for (int i = threadIdx.x; i < n; i += NT) w += sh.list_key[i] >= key ? sh.list_mass[i] : 0;
-          *kept = filled_mass(bin) + block_fold<NT>(w, sh.wave_a, Sum());
+          kept = filled_mass(bin) + block_fold<NT>(w, sh.wave_a, Sum());
         }
         return key;
       }
@@ -1002,7 +1002,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
   bool intact = true;
   if (s.k) {
     d.fill(row, by_mass, 0);
-    least = d.template last_before<false>(row, (u64)s.k, 0, intact, by_mass ? &whole : nullptr);
+    least = d.template last_before<false>(row, (u64)s.k, 0, intact, by_mass, whole);
     if (by_mass && !intact) {
       d.fill(row, true, least);
       whole = d.filled_mass(BINS);
@@ -1010,7 +1010,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     }
   }
   // steps beyond the k-th class weigh nothing here: what is before them is the whole
-  if (by_mass) least = d.template last_before<true>(row, share_of(s.p, whole), least, intact);
+  if (by_mass) least = d.template last_before<true>(row, share_of(s.p, whole), least, intact, false, whole);
 
   // the running sum over the whole row in tiles of OWN classes a thread: groups of
   // tiles, then the tiles of one group, then the waves of one tile
