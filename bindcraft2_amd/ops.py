@@ -890,8 +890,9 @@ class LogProbs:
         return (logp, entropy), out
 
 
-def _heads(t, what, dtype=None, shape=None):
-    """(address, token stride, head stride) of [tokens, heads, width]."""
+def _heads(t, what, device, dtype=None, shape=None):
+    """(address, token stride, head stride) of [tokens, heads, width].  device: the
+    current one, asked for once a call (a fifth of a microsecond each time)."""
     if t is None:
         raise ValueError(f"{what}: missing")
     if t.dim() != 3 or (shape is not None and t.shape != shape):
@@ -899,7 +900,8 @@ def _heads(t, what, dtype=None, shape=None):
         raise ValueError(f"{what}: expected {want}, got {tuple(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
-    _current(t, what)
+    if t.get_device() != device:
+        _current(t, what)
     st, sh, e = t.stride()
     if e != 1 and t.shape[2] > 1:
         raise ValueError(f"{what}: a head's elements must be contiguous")
@@ -909,16 +911,19 @@ def _heads(t, what, dtype=None, shape=None):
 def _new_heads(t):
     """A new contiguous tensor like t, and its (address, token stride, head stride)."""
     out = torch.empty_like(t, memory_format=torch.contiguous_format)
-    return out, (out.data_ptr(), t.shape[1] * t.shape[2], t.shape[2])
+    st, sh, _ = out.stride()
+    return out, (out.data_ptr(), st, sh)
 
 
-def _vector(t, n, dtypes, what):
+def _vector(t, n, dtypes, what, device):
     """The address of a contiguous [n] on the current device."""
     if t is None:
         raise ValueError(f"{what}: missing")
     if t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes:
         raise ValueError(f"{what}: expected {', '.join(map(str, dtypes))} [{n}], got {t.dtype} {tuple(t.shape)}")
-    if not _current(t, what).is_contiguous():
+    if t.get_device() != device:
+        _current(t, what)
+    if not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous tensor")
     return t.data_ptr()
 
@@ -940,7 +945,7 @@ class HeadNormRotate:
             raise ValueError("eps must be finite and not negative")
         self.freq, self.eps, self.interleaved = freq, float(eps), int(bool(interleaved))
 
-    def _operands(self, q, k, positions, q_weight, k_weight):
+    def _operands(self, q, k, positions, q_weight, k_weight, device):
         """(the calls' operands before the tensors of heads, those after them)"""
         if q.dim() != 3 or q.dtype not in _DTYPES:
             raise ValueError(f"q: expected float32, float16 or bfloat16 [tokens, heads, width], got {q.dtype} "
@@ -949,29 +954,30 @@ class HeadNormRotate:
         if positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"positions: expected int32 or int64, got {positions.dtype}")
         pairs, wt = self.freq.shape[0], q_weight.dtype
-        at = _vector(positions, n, (positions.dtype,), "positions")
-        _current(self.freq, "freq")
-        qw, kw = _vector(q_weight, width, (torch.float32, q.dtype), "q_weight"), None
+        at = _vector(positions, n, (positions.dtype,), "positions", device)
+        if self.freq.get_device() != device:
+            _current(self.freq, "freq")
+        qw, kw = _vector(q_weight, width, (torch.float32, q.dtype), "q_weight", device), None
         if k is not None:
             if k.dim() != 3 or k.shape[0] != n or k.shape[2] != width:
                 raise ValueError(f"k: expected [{n}, heads, {width}], got {tuple(k.shape)}")
-            kw = _vector(k_weight, width, (wt,), "k_weight")
+            kw = _vector(k_weight, width, (wt,), "k_weight", device)
         return ((_DTYPES[q.dtype], n, heads, 0 if k is None else k.shape[1], width, 2 * pairs, self.interleaved),
                 (at, 64 if positions.dtype == torch.int64 else 32, self.freq.data_ptr(), qw, kw, _DTYPES[wt],
                  self.eps))
 
     @staticmethod
-    def _pair(q, k, like_q, like_k, what):
+    def _pair(q, k, like_q, like_k, what, device):
         """The six operands of queries and keys, checked against the inputs."""
-        a = _heads(q, what[0], like_q.dtype, like_q.shape)
+        a = _heads(q, what[0], device, like_q.dtype, like_q.shape)
         if like_k is None:
             return (*a, None, 0, 0)
-        return a + _heads(k, what[1], like_q.dtype, like_k.shape)
+        return a + _heads(k, what[1], device, like_q.dtype, like_k.shape)
 
-    def _results(self, out, q, k):
+    def _results(self, out, q, k, device):
         """(results, the calls' six operands of them)"""
         if out is not None:
-            return tuple(out), self._pair(*out, q, k, ("out", "out"))
+            return tuple(out), self._pair(*out, q, k, ("out", "out"), device)
         a, x = _new_heads(q)
         b, y = (None, (None, 0, 0)) if k is None else _new_heads(k)
         return (a, b), x + y
@@ -979,9 +985,10 @@ class HeadNormRotate:
     def forward(self, q, k, positions, q_weight, k_weight=None, out=None):
         """-> (q, k) normed and rotated, in new tensors or in out = (q, k), which
         may be the inputs; without k, k is None"""
-        first, last = self._operands(q, k, positions, q_weight, k_weight)
-        x = self._pair(q, k, q, k, ("q", "k"))
-        out, y = self._results(out, q, k)
+        device = torch.cuda.current_device()
+        first, last = self._operands(q, k, positions, q_weight, k_weight, device)
+        x = self._pair(q, k, q, k, ("q", "k"), device)
+        out, y = self._results(out, q, k, device)
         check(lib().bc2n_headnorm_fwd(_stream(), *first, *x, *last, *y))
         return out
 
@@ -989,10 +996,11 @@ class HeadNormRotate:
         """cts = (d_q, d_k), q and k the forward's inputs -> (d_q, d_k, d_q_weight,
         d_k_weight), the first two in out = (d_q, d_k) where given, the weights'
         f32"""
-        first, last = self._operands(q, k, positions, q_weight, k_weight)
-        x = self._pair(q, k, q, k, ("q", "k"))
-        d = self._pair(*cts, q, k, ("d_q", "d_k"))
-        out, y = self._results(out, q, k)
+        device = torch.cuda.current_device()
+        first, last = self._operands(q, k, positions, q_weight, k_weight, device)
+        x = self._pair(q, k, q, k, ("q", "k"), device)
+        d = self._pair(*cts, q, k, ("d_q", "d_k"), device)
+        out, y = self._results(out, q, k, device)
         width, dev = q.shape[2], q.device
         dw = torch.empty(2, width, dtype=torch.float32, device=dev)
         work = torch.empty(lib().bc2n_headnorm_work_bytes(q.shape[0], width), dtype=torch.uint8, device=dev)
@@ -1020,21 +1028,21 @@ class PackedAttention:
             raise ValueError("scale must be positive and finite")
         self.causal, self.scale = int(bool(causal)), scale
 
-    def _operands(self, q, k, v, q_offsets, k_offsets, k_lengths, q_lengths):
+    def _operands(self, q, k, v, q_offsets, k_offsets, k_lengths, q_lengths, device):
         if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"q: expected float16 or bfloat16 [tokens, heads, width], got {q.dtype} "
                              f"{tuple(q.shape)}")
         n, heads, width = q.shape
         if k.dim() != 3 or k.shape[2] != width or k.shape[1] == 0 or heads == 0 or heads % k.shape[1]:
             raise ValueError(f"k: expected [tokens, a divisor of {heads}, {width}], got {tuple(k.shape)}")
-        x = _heads(q, "q") + _heads(k, "k", q.dtype) + _heads(v, "v", q.dtype, k.shape)
+        x = _heads(q, "q", device) + _heads(k, "k", device, q.dtype) + _heads(v, "v", device, q.dtype, k.shape)
         i32 = (torch.int32,)
         count = q_offsets.shape[0] - 1 if q_offsets.dim() == 1 else -1
         if count < 0:
             raise ValueError("q_offsets: expected int32 [sequences + 1]")
-        offsets = [_vector(q_offsets, count + 1, i32, "q_offsets"),
-                   _vector(q_offsets if k_offsets is None else k_offsets, count + 1, i32, "k_offsets")]
-        lengths = [None if t is None else _vector(t, count, i32, what)
+        at = _vector(q_offsets, count + 1, i32, "q_offsets", device)
+        offsets = (at, at if k_offsets is None else _vector(k_offsets, count + 1, i32, "k_offsets", device))
+        lengths = [None if t is None else _vector(t, count, i32, what, device)
                    for t, what in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths"))]
         if k_offsets is None and k.shape[0] != n:
             raise ValueError(f"k_offsets: needed, q has {n} tokens and k {k.shape[0]}")
@@ -1045,12 +1053,13 @@ class PackedAttention:
     def forward(self, q, k, v, q_offsets, k_offsets=None, k_lengths=None, q_lengths=None, out=None):
         """-> (out like q, lse f32 [heads, q_tokens]), out in `out` where given.
         Without k_offsets the keys are the queries' tokens."""
-        sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths)
+        device = torch.cuda.current_device()
+        sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths, device)
         fill = out is None
         if fill:
             out, o = _new_heads(q)
         else:
-            o = _heads(out, "out", q.dtype, q.shape)
+            o = _heads(out, "out", device, q.dtype, q.shape)
         shape = (q.shape[1], q.shape[0])
         if fill:
             lse = torch.empty(shape, dtype=torch.float32, device=q.device)
@@ -1069,9 +1078,10 @@ class PackedAttention:
                  grads=None):
         """out and lse the forward's -> (d_q, d_k, d_v), in grads = (d_q, d_k, d_v)
         where given"""
-        sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths)
+        device = torch.cuda.current_device()
+        sizes, where, x = self._operands(q, k, v, q_offsets, k_offsets, k_lengths, q_lengths, device)
         shape = q.shape
-        g, o = _heads(d_out, "d_out", q.dtype, shape), _heads(out, "out", q.dtype, shape)
+        g, o = _heads(d_out, "d_out", device, q.dtype, shape), _heads(out, "out", device, q.dtype, shape)
         _f32(lse, (shape[1], shape[0]), "lse")
         if not _current(lse, "lse").is_contiguous():
             raise ValueError("lse: expected a contiguous tensor")
@@ -1079,7 +1089,7 @@ class PackedAttention:
         if fill:
             grads, d = zip(*map(_new_heads, (q, k, v)))
         else:
-            d = [_heads(t, what, q.dtype, like.shape)
+            d = [_heads(t, what, device, q.dtype, like.shape)
                  for t, like, what in zip(grads, (q, k, v), ("d_q", "d_k", "d_v"))]
         work = self._work(lib().bc2n_attention_bwd_work_bytes, sizes, q.device)
         check(lib().bc2n_attention_bwd(_stream(), *sizes, *where, *g, *x, *o, lse.data_ptr(), int(fill), *d[0],
@@ -1096,18 +1106,19 @@ class Sampler:
     temperature of 0 takes the first class."""
 
     def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-        self.settings = []
+        self.numbers, self.given = [], []  # a call's operands; (place, name, tensor) of the rows' own
         for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
             whole = name == "top_k"
             if torch.is_tensor(v):
                 if v.dtype != (torch.int32 if whole else torch.float32):
                     raise ValueError(f"{name}: expected {'int32' if whole else 'float32'}, got {v.dtype}")
-                self.settings.append((name, 0, v))
+                self.given.append((len(self.numbers) + 1, name, v))
+                self.numbers += (0, None)
                 continue
             v = min(int(v), 1 << 31) if whole else float(v)
             if not (0 <= v if name != "temperature" else 0 <= v < float("inf")):
                 raise ValueError(f"{name} must not be negative" + ("" if whole else ", infinite or NaN"))
-            self.settings.append((name, v, None))
+            self.numbers += (v, None)
 
     def sample(self, logits, uniforms):
         """logits [..., classes] f32, f16 or bf16, any row stride, uniforms f32 [...]
@@ -1119,14 +1130,13 @@ class Sampler:
                              f"{logits.dtype} {tuple(logits.shape)}")
         x, ld = LogProbs._rows(logits, "logits")
         _f32(uniforms, lead, "uniforms")
-        rows, own = uniforms.numel(), []
-        for name, v, t in self.settings:
-            at = None
-            if t is not None:
+        rows, own = uniforms.numel(), self.numbers
+        if self.given:
+            own = list(own)
+            for at, name, t in self.given:
                 if t.numel() != rows:
                     raise ValueError(f"{name}: expected a value for each of {rows} rows, got {t.numel()}")
-                at = LogProbs._given(t, name)
-            own += [v, at]
+                own[at] = LogProbs._given(t, name)
         index = torch.empty(lead, dtype=torch.int32, device=logits.device)
         logp = torch.empty(lead, dtype=torch.float32, device=logits.device)
         check(lib().bc2n_sample(_stream(), code, x, ld, rows, logits.shape[-1],

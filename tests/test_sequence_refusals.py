@@ -198,7 +198,7 @@ def test_sampler_settings():
         ops.Sampler(top_k=torch.zeros(3, dtype=torch.int64))
     with pytest.raises(ValueError, match="float32"):
         ops.Sampler(top_p=torch.zeros(3, dtype=torch.float64))
-    assert ops.Sampler(top_k=1 << 64).settings[1][1] == 1 << 31  # all classes, in 64 bits too
+    assert ops.Sampler(top_k=1 << 64).numbers[2] == 1 << 31  # all classes, in 64 bits too
 
 
 def test_settings_of_the_others():
