@@ -162,3 +162,26 @@ def test_few_long_sequences(cuda, m, n, heads, kv, d, causal, dtype):
     want = R.attention(q, k, v, causal, d ** -0.5, g)
     for name, got in zip(("out", "lse", "d_q", "d_k", "d_v"), (out, lse, *grads)):
         R.check(name, got, *want[name])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_graph_of_the_widest(cuda, dtype):
+    """Forward and gradient of heads of 128, captured where no call has been before."""
+    q, g = rand(1, 300, 4, 128, dtype=dtype), rand(2, 300, 4, 128, dtype=dtype)
+    k, v = rand(3, 300, 2, 128, dtype=dtype), rand(4, 300, 2, 128, dtype=dtype)
+    op, off = ops.PackedAttention(), i32(0, 120, 300)
+
+    def run():
+        out, lse = op.forward(q, k, v, off)
+        return out, lse, *op.backward(g, q, k, v, out, lse, off)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for _ in range(3):
+        q.mul_(0.9)
+        want = run()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
