@@ -1099,7 +1099,7 @@ struct Back {
   float *dk, *dv;       // [part][k_tokens][kv_heads][DP]
 };
 
-constexpr int FEW_KEYS = 256;
+constexpr int FEW_KEYS = 1024;
 // dq, and D = sum (do o) of every row for the other kernel.  The forward's layout
 // with a product more, and as it bound by products and exponentials.  The scores
 // are made in both kernels, so that neither adds to memory in an order of
@@ -1161,16 +1161,17 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   x.init(lds0, lane);
   // Rows of few keys: out, an average of few values, is as large as each of them,
   // and its rounding would weigh as much in dS as that of dS itself.  Their D is
-  // taken from the keys, sum P dP (224 keys, binary16: dq 1.56 times as far off
-  // as its own rounding with the rounded out, 1.46 so).
-  if (back.q_parts == 1 && nk <= FEW_KEYS / BN) {
+  // taken from the keys, sum P dP, by every part for itself (224 keys, binary16: dq
+  // 1.56 times as far off as its own rounding with the rounded out, 1.46 so; up to
+  // 1040 keys, bfloat16: 1.54 and 1.48).  It costs the packed prompts' gradient 3%.
+  if (every <= FEW_KEYS / BN && (part == 0 || kt0 < nk)) {
     tile.init(a, seq, at.head, 0, BN, wave, lane);
     float sum = 0.f;
-    for (int kt = 0; kt < nk; ++kt) {
+    for (int kt = 0; kt < every; ++kt) {
       if (kt == 0) tile.both(lds0);
       const unsigned here = (kt & 1) * 2 * TILE;
       wait_all_and_sync();
-      if (kt + 1 < nk) tile.both(lds0 + (~kt & 1) * 2 * TILE);
+      if (kt + 1 < every) tile.both(lds0 + (~kt & 1) * 2 * TILE);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         f32x16 p = {}, d = {};
