@@ -51,6 +51,7 @@ typedef unsigned long long u64;
 constexpr int BINS = 2048;
 constexpr int LIST = 256;  // classes ranked one against all
 constexpr float NEG_INF = -__builtin_inff();
+constexpr float MAX_F32 = 3.402823466e38f;
 
 // bits of a mass: V of them fit 62 bits
 __host__ __device__ constexpr int mass_bits(int V) {
@@ -342,8 +343,8 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(Sample a) {
     if (row.lane == 0) write(a, r, first, 0.f);
     return;
   }
-  // a value a little below the last with a mass
-  const float low = fmaxf(m - (float)fmin((S + 2) / s.inv * 1.0001, 3e38), -3e38f);
+  // a value a little below the last with a mass; no number is below the type's lowest
+  const float low = fmaxf(m - (float)fmin((S + 2) / s.inv * 1.0001, 3e38), -MAX_F32);
   u64 mine = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
