@@ -113,6 +113,12 @@ __device__ __forceinline__ Settings settings_of(const Sample& a, int64_t r) {
   s.inv = fmin(1.4426950408889634 / t, 1e300);
   return s;
 }
+// A value a little below the last with a mass beside a maximum of m: in 64 bits, so
+// that at temperatures about 1e37 the distance may pass f32's numbers, and no
+// lower than the lowest of those.
+__device__ __forceinline__ float last_with_mass(float m, double inv, int S) {
+  return (float)fmax((double)m - (S + 2) / inv * 1.0001, -(double)MAX_F32);
+}
 // the least sum of forerunners that ends top-p: p of the mass, at least 1
 __device__ __forceinline__ u64 share_of(double p, u64 mass) {
   const double x = ceil(fmax(p, 0.0) * (double)mass);
@@ -343,8 +349,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(Sample a) {
     if (row.lane == 0) write(a, r, first, 0.f);
     return;
   }
-  // a value a little below the last with a mass; no number is below the type's lowest
-  const float low = fmaxf(m - (float)fmin((S + 2) / s.inv * 1.0001, 3e38), -MAX_F32);
+  const float low = last_with_mass(m, s.inv, S);
   u64 mine = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -503,14 +508,14 @@ struct RowOf {
 template <int NT>
 struct Drawer {
   Shared<NT>& sh;
-  float m, range, steps;  // maximum, largest distance of a mass, steps a distance
+  float m, last, range, steps;  // maximum, lowest value with a mass, their distance, steps a distance
   double inv;
   int S;
 
   __device__ __forceinline__ double distance(float x) const { return ((double)x - (double)m) * inv; }
   __device__ __forceinline__ u64 mass(float x) const { return mass_of(distance(x), S); }
   // a class that can have a mass
-  __device__ __forceinline__ bool counts(float x) const { return m - x <= range; }
+  __device__ __forceinline__ bool counts(float x) const { return x >= last; }
   __device__ __forceinline__ int step_of(float x) const {
     return (int)fminf((m - x) * steps, (float)(BINS - 1));
   }
@@ -689,9 +694,9 @@ struct Drawer {
   }
   // a value that no class of the steps up to `step` is below
   __device__ __forceinline__ float lowest(int step) const {
-    if (step >= BINS - 1) return m - range;
+    if (step >= BINS - 1) return last;
     const float d = (float)(step + 1) / steps;  // of the next step's first, but for rounding
-    return m - fminf(d * 1.0001f, range) - 1e-6f * fabsf(m);
+    return fmaxf(m - d * 1.0001f - 1e-6f * fabsf(m), last);
   }
 
   // The same as cut and draw, of at most 64 candidates by one wave: ranks by value and
@@ -930,9 +935,10 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     if (threadIdx.x == 0) write(a, r, (int)at, 0.f);
     return;
   }
-  Drawer<NT> d{sh, m, 0.f, 0.f, s.inv, mass_bits(a.V)};
-  // a little past the last distance with a mass
-  d.range = (float)fmin((d.S + 2) / s.inv * 1.0001, 3e38);
+  Drawer<NT> d{sh, m, 0.f, 0.f, 0.f, s.inv, mass_bits(a.V)};
+  d.last = last_with_mass(m, s.inv, d.S);
+  // one that passes the numbers, as an infinite distance does, is in the last step
+  d.range = fminf(m - d.last, MAX_F32);
   d.steps = fminf((float)(BINS - 1) / d.range, 3e38f);
 
   u64 least = 0, whole = 0;
@@ -982,7 +988,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Sample a) {
     low = d.lowest(d.template last_step<true>(share_of(s.p, whole), before));
   } else if (!s.k && s.floor > (double)NEG_INF) {
     low = (float)((double)m + s.floor / s.inv);
-    low -= 1e-6f * (fabsf(low) + fabsf(m)) + 1e-37f;
+    low = fmaxf(low - 1e-6f * (fabsf(low) + fabsf(m)) - 1e-37f, d.last);
   }
   if (low > NEG_INF) n = d.collect(row, low, runs, shift);
   auto kept_mass = [&](float x, int j) -> u64 {
