@@ -33,6 +33,7 @@
 #include "packattn.h"
 
 #include "common.h"
+#include "packrows.h"
 #include "runtime.h"
 #include "vec.h"
 
@@ -1303,12 +1304,11 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   const bool stored = j < have, live = j < seq.lk;
   const int64_t token = seq.k0 + min(j, have - 1);
   const int lag = seq.lk - seq.lq;  // query i sees keys up to i + lag
-  // the first row that sees a key of the workgroup; without keys there is none
-  const int all = j0 < seq.lk ? seq.lq * G : 0;
-  const int first = a.causal ? min(max(j0 - lag, 0) * G / BN * BN, all) : 0;
-  const int sees = a.causal ? max(-lag, 0) * G : 0;  // rows before see no key: taken as zeros
-  const int per = ((all - first + BN - 1) / BN + back.k_parts - 1) / back.k_parts * BN;
-  const int part = blockIdx.y, from = min(first + part * per, all), rows = min(all, from + per);
+  const KeyRows seen = rows_of_keys(a.causal, j0, seq.lq, seq.lk, G, BN);
+  const int sees = seen.blind;  // rows before see no key: taken as zeros
+  const int part = blockIdx.y;
+  const Part range = part_of_rows(seen, back.k_parts, part, BN);
+  const int from = range.from, rows = range.to;
   const float ds = Half<T>::SCALED ? ds_scale(back.maxima, NORM_BLOCKS) : 1.f;
   // P is made 2^SHIFT times as large in binary16
   constexpr float SHIFT = 2 * Half<T>::SHIFT;
