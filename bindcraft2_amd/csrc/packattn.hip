@@ -460,6 +460,8 @@ __device__ __forceinline__ T* row_ptr(const HeadView& v, int64_t token, int head
   return (T*)v.p + token * v.st + (int64_t)head * v.sh;
 }
 
+__device__ __forceinline__ float finite_or_zero(float v) { return v < __builtin_inff() ? v : 0.f; }
+
 // Largest (or smallest) over the lanes of a wave
 __device__ __forceinline__ int wave_max(int v) {
 #pragma unroll
@@ -1029,63 +1031,60 @@ __global__ __launch_bounds__(RW > 1 ? 64 * RW : NT) void packattn_join_kernel(Pa
 
 // ----------------------------------------------------------------- backward
 // In binary16 a dS of many keys falls below the normal numbers, so it is made
-// 2^e times as large, e from the largest norms of a row of do and of v, which
-// bound it: |dS| <= 2 |do| |v|.  maxima [blocks][2]: partial maxima of the
-// squares, of queries' blocks and of keys'.
-template <class T>
-__global__ __launch_bounds__(NT) void packattn_norms_kernel(PackedAttn a, int64_t q_tiles, int64_t k_tiles,
-                                                            float* maxima) {
+// 2^e times as large, e from norms that bound it: |dS| <= 2 |do| max |v|.  dq has a
+// scale for every row, from its own |do| and the values that its workgroup goes over;
+// dk and dv one for a workgroup's keys, from the rows and values of their sequence
+// and group of heads.  So no sequence's, group's or row's accuracy hangs on what
+// others of the call hold; infinities and NaN are left out of the norms, and so are
+// rows that see no key.
+//
+// The values' part: largest squares of 64 keys, a workgroup a tile and head, 16
+// bytes a lane.
+constexpr int NORM_KEYS = 64;
+static_assert(NORM_KEYS == BN, "dq counts them by its tiles");
+template <class T, int DP>
+__global__ __launch_bounds__(NT) void packattn_norms_kernel(PackedAttn a, int64_t tiles, float* vmax) {
   __shared__ float best[WAVES];
-  constexpr int TOK = 64;
-  float top[2] = {0.f, 0.f};
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int chunks = (a.width + 7) / 8;
-  for (int64_t x = blockIdx.x; x < q_tiles + k_tiles; x += gridDim.x) {
-    const bool keys = x >= q_tiles;
+  constexpr int LR = DP / 8;  // lanes a row
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = threadIdx.x % LR * 8;
+  for (int64_t y = blockIdx.x; y < tiles * a.kv_heads; y += gridDim.x) {
+    const int64_t x = y / a.kv_heads;
+    const int head = (int)(y % a.kv_heads);
     int s;
-    const int64_t t = find_tile(keys ? a.k_off : a.q_off, a.sequences, keys ? a.k_tokens : a.q_tokens, 1,
-                            TOK, keys ? x - q_tiles : x, s);
-    const Seq seq = sequence(a, s, keys);
-    const int heads = keys ? a.kv_heads : a.heads;
-    const int n = t < 0 ? 0 : (int)min((int64_t)TOK, (keys ? seq.lk : seq.lq) - t * TOK) * heads;
+    const int64_t t = find_tile(a.k_off, a.sequences, a.k_tokens, 1, NORM_KEYS, x, s);
+    const Seq seq = sequence(a, s, true);
+    const int n = t < 0 ? 0 : (int)min((int64_t)NORM_KEYS, seq.lk - t * NORM_KEYS);
     float m = 0.f;
-    for (int r = threadIdx.x; r < n; r += NT) {
-      const int64_t token = (keys ? seq.k0 : seq.q0) + t * TOK + r / heads;
-      const T* row = row_ptr<const T>(keys ? a.v : a.d_o, token, r % heads);
-      float sq = 0.f;
-      for (int c = 0; c < chunks; ++c) {
-        float e[8];
-        Vec<T>::unpack(load8(row, 8 * c, a.width), e);
+    for (int r = threadIdx.x / LR; r < n; r += NT / LR) {
+      float v[8], sq = 0.f;
+      Vec<T>::unpack(load8(row_ptr<const T>(a.v, seq.k0 + t * NORM_KEYS + r, head), e, a.width), v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq = fmaf(e[i], e[i], sq);
-      }
-      m = fmaxf(m, sq);
+      for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+      sq = group_sum<LR>(sq);
+      m = fmaxf(m, finite_or_zero(sq));
     }
-    top[0] = keys ? top[0] : fmaxf(top[0], m);
-    top[1] = keys ? fmaxf(top[1], m) : top[1];
-  }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const float m = group_max<64>(top[k]);
+    m = group_max<64>(m);
+    __syncthreads();  // the tile before has been read
     if (lane == 0) best[wave] = m;
     __syncthreads();
     if (threadIdx.x == 0)
-      maxima[2 * blockIdx.x + k] = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-    __syncthreads();
+      vmax[head * tiles + x] = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
   }
 }
-constexpr int NORM_BLOCKS = 256;
+constexpr int NORM_BLOCKS = 2048;
 
-// the scale of dS from the partial maxima: a power of two, dS below 2^14
-__device__ __forceinline__ float ds_scale(const float* maxima, int blocks) {
-  const int lane = threadIdx.x & 63;
-  float d = 0.f, v = 0.f;
-  for (int i = lane; i < blocks; i += 64) {
-    d = fmaxf(d, maxima[2 * i]);
-    v = fmaxf(v, maxima[2 * i + 1]);
-  }
-  const float b = sqrtf(group_max<64>(d)) * sqrtf(group_max<64>(v));  // |dS| <= 2 b
-  if (!(b > 0.f && b < 3e38f)) return 1.f;
+// the largest of n squares, over a wave
+__device__ __forceinline__ float largest(const float* squares, int n) {
+  float m = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < n; i += 64) m = fmaxf(m, squares[i]);
+  return group_max<64>(m);
+}
+// the scale of dS from the largest squares of a row of do and of v: a power of two,
+// dS below 2^14
+__device__ __forceinline__ float ds_scale(float g, float v) {
+  const float b = sqrtf(g) * sqrtf(v);  // |dS| <= 2 b
+  if (!(b > 0.f)) return 1.f;
   return ldexpf(1.f, max(-100, min(100, 12 - (int)ceilf(log2f(b)))));
 }
 
@@ -1094,7 +1093,9 @@ __device__ __forceinline__ float ds_scale(const float* maxima, int blocks) {
 // parts, whose sums packattn_sum_kernel adds in their order.
 struct Back {
   float* delta;         // [heads][q_tokens]
-  const float* maxima;  // binary16: [NORM_BLOCKS][2]
+  // binary16: the largest squares of a row, over 64 keys of v and 32 rows of do
+  float *vmax, *gmax;  // [kv_heads][v_tiles], [kv_heads][4 * tiles of dq]
+  int64_t v_tiles, g_tiles;
   int q_parts, k_parts;
   float* dq;            // [part][q_tokens][heads][DP]
   float *dk, *dv;       // [part][k_tokens][kv_heads][DP]
@@ -1115,7 +1116,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   const int G = a.heads / a.kv_heads;
   int s;
   // from the last tile: a causal sequence's last rows see the most keys
-  const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, tiles - 1 - at.tile, s);
+  const int64_t number = tiles - 1 - at.tile, t = find_tile(a.q_off, a.sequences, a.q_tokens, G, BM, number, s);
   const Seq seq = lane_seq(sequence(a, s, false), 0);
   const int rows = (a.fill ? seq.have : seq.lq) * G;
   if (t < 0 || t * BM >= rows) return;
@@ -1130,13 +1131,14 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   if (a.fill && seq.lq < seq.have) far = seq.lk - 1;
   const int every = far < 0 ? 0 : far / BN + 1, per = (every + back.q_parts - 1) / back.q_parts;
   const int part = blockIdx.y, kt0 = part * per, nk = min(every, kt0 + per);
-  const float ds = Half<T>::SCALED ? ds_scale(back.maxima, NORM_BLOCKS) : 1.f;
+  float vmax = 0.f;
+  if (Half<T>::SCALED) vmax = largest(back.vmax + at.head * back.v_tiles + seq.k0 / NORM_KEYS + s, every);
 
   u32x4 q[KS], g[KS];
   const T* qrow = row_ptr<const T>(a.q, token, head);
   const T* grow = row_ptr<const T>(a.d_o, token, head);
   const T* orow = row_ptr<const T>(a.o, token, head);
-  float D = 0.f;
+  float D = 0.f, gg = 0.f;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
@@ -1145,9 +1147,20 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
     Vec<T>::unpack(g[ks], x);
     Vec<T>::unpack(load8(orow, 16 * ks + 8 * h, a.width), y);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) D = fmaf(x[i], y[i], D);
+    for (int i = 0; i < 8; ++i) {
+      D = fmaf(x[i], y[i], D);
+      if (Half<T>::SCALED) gg = fmaf(x[i], x[i], gg);
+    }
   }
   D = other_half_sum(D);
+  float ds = 1.f;
+  if (Half<T>::SCALED) {
+    gg = other_half_sum(gg);
+    gg = row.last < 0 ? 0.f : finite_or_zero(gg);
+    ds = ds_scale(gg, vmax);
+    const float m = group_max<64>(gg);
+    if (part == 0 && lane == 0) back.gmax[at.head * back.g_tiles + number * WAVES + wave] = m;
+  }
   float lse = a.lse[at_row] * LOG2E;
   if (lse == NEG_INF) lse = -NEG_INF;  // a row without a key: P = 0
   const float c = a.scale * LOG2E;
@@ -1309,7 +1322,14 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   const int part = blockIdx.y;
   const Part range = part_of_rows(seen, back.k_parts, part, BN);
   const int from = range.from, rows = range.to;
-  const float ds = Half<T>::SCALED ? ds_scale(back.maxima, NORM_BLOCKS) : 1.f;
+  float ds = 1.f;
+  if (Half<T>::SCALED) {  // rows 32 x on of the sequence are dq's wave 4 q0 G / 128 + 4 s + x
+    const int64_t wave0 = (seq.q0 * G / BK + s) * WAVES;
+    const float g = largest(back.gmax + at.head * back.g_tiles + wave0 + from / 32, (rows - from + 31) / 32);
+    const float v = largest(back.vmax + at.head * back.v_tiles + seq.k0 / NORM_KEYS + s,
+                            rows > from ? (seq.lk + NORM_KEYS - 1) / NORM_KEYS : 0);
+    ds = ds_scale(g, v);
+  }
   // P is made 2^SHIFT times as large in binary16
   constexpr float SHIFT = 2 * Half<T>::SHIFT;
 
@@ -1677,7 +1697,11 @@ Back carve_back(const PackedAttn& a, char* base, size_t* bytes) {
     return p;
   };
   b.delta = take(a.heads * a.q_tokens);
-  b.maxima = take(a.dtype == BC2N_F16 ? 2 * NORM_BLOCKS : 0);
+  const bool scaled = a.dtype == BC2N_F16;
+  b.v_tiles = tiles_of(a.k_tokens, 1, NORM_KEYS, a.sequences);
+  b.g_tiles = tiles_of(a.q_tokens, (int)G, 32 * WAVES, a.sequences) * WAVES;
+  b.vmax = take(scaled ? a.kv_heads * b.v_tiles : 0);
+  b.gmax = take(scaled ? a.kv_heads * b.g_tiles : 0);
   b.dq = take(b.q_parts > 1 ? b.q_parts * a.q_tokens * a.heads * DP : 0);
   b.dk = take(b.k_parts > 1 ? b.k_parts * a.k_tokens * a.kv_heads * DP : 0);
   b.dv = take(b.k_parts > 1 ? b.k_parts * a.k_tokens * a.kv_heads * DP : 0);
@@ -1744,10 +1768,13 @@ void packattn_bwd(hipStream_t st, const PackedAttn& a, void* work) {
     constexpr int DP = decltype(dp)::value;
     const int64_t q_tiles = tiles_of(a.q_tokens, a.heads / a.kv_heads, 32 * WAVES, a.sequences);
     const int64_t k_tiles = tiles_of(a.k_tokens, 1, 32 * WAVES, a.sequences);
-    if (a.dtype == BC2N_F16)
-      packattn_norms_kernel<T><<<NORM_BLOCKS, NT, 0, st>>>(a, tiles_of(a.q_tokens, 1, 64, a.sequences),
-                                                          tiles_of(a.k_tokens, 1, 64, a.sequences),
-                                                          const_cast<float*>(back.maxima));
+    if constexpr (Half<T>::SCALED) {
+      if (a.q_tokens && a.k_tokens) {
+        const int64_t items = back.v_tiles * a.kv_heads;
+        packattn_norms_kernel<T, DP><<<(unsigned)std::min<int64_t>(items, NORM_BLOCKS), NT, 0, st>>>(a, back.v_tiles,
+                                                                                                    back.vmax);
+      }
+    }
     if (a.q_tokens) {
       auto* dq = &packattn_dq_kernel<T, DP>;
       const size_t lds = 4 * BN * DP * 2;

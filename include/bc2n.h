@@ -730,8 +730,10 @@ int bc2n_headnorm_bwd(void* stream, int dtype, int64_t tokens, int heads, int kv
  * Products take the operands as they are, accumulate in f32 and round P and
  * its cotangent to the operands' type; maxima, sums and lse are f32, added in an
  * order that goes by the shapes and lengths alone.  In binary16 the
- * cotangent of S is scaled by a power of two from the largest norms of d_out
- * and v.
+ * cotangent of S is scaled by powers of two: for d_q one a row, from the norms of
+ * its d_out and of the v of its tiles of keys, for d_k one for 128 keys, from the
+ * largest norms of the rows that see them and of v in their sequence and head.
+ * Norms that are not finite, and rows that see no key, do not count.
  * work: bc2n_attention_*_work_bytes() bytes, 16-byte aligned, for the time of the
  * call (NULL where that is 0).  bwd takes the forward's out and lse, and
  * returns d_q, d_k and d_v (the group's sum), which overlap nothing.
