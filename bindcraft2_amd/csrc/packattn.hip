@@ -685,7 +685,9 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
     if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
   }
   const float sum = other_half_sum(st.sum);
-  const bool none = sum == 0.f;
+  // A row that sees keys has a sum of 0 where all its scores are -infinity: its
+  // softmax is NaN, as 0 / 0 here, and its lse log 0.
+  const bool none = row.last < 0;
   store_columns<T, DB>(st.o, none ? 0.f : 1.f / sum,
                        row.stored ? row_ptr<T>(a.o, token, head) : nullptr, a.width, lane);
   if (row.stored && h == 0)
@@ -903,7 +905,7 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
         f[w] = v.y == 0.f ? 0.f : exp2_f(v.x - top);
         l += v.y * f[w];
       }
-      const bool none = l == 0.f;
+      const bool none = mine.last < 0;
       const float inv = none ? 0.f : 1.f / l;
       if (mine.stored) {
         for (int e = part * 8; e < a.width; e += PER_ROW * 8) {
@@ -922,7 +924,7 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
       }
       __syncthreads();
     } else if (it.parts == 1) {
-      const bool none = sum == 0.f;
+      const bool none = row.last < 0;
       store_columns<T, DB>(st.o, none ? 0.f : 1.f / sum,
                            row.stored ? row_ptr<T>(a.o, token, head) : nullptr, a.width, lane);
       if (row.stored && h == 0)
@@ -1015,7 +1017,7 @@ __global__ __launch_bounds__(RW > 1 ? 64 * RW : NT) void packattn_join_kernel(Pa
         }
       }
       if (t < LP && row.stored) {
-        const bool none = sum == 0.f;
+        const bool none = row.last < 0;
         const float inv = none ? 0.f : 1.f / sum;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] *= inv;
@@ -1162,7 +1164,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
     if (part == 0 && lane == 0) back.gmax[at.head * back.g_tiles + number * WAVES + wave] = m;
   }
   float lse = a.lse[at_row] * LOG2E;
-  if (lse == NEG_INF) lse = -NEG_INF;  // a row without a key: P = 0
+  if (row.last < 0) lse = -NEG_INF;  // a row without a key: P = 0
   const float c = a.scale * LOG2E;
   f32x16 o[DB];
 #pragma unroll
@@ -1415,7 +1417,7 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   auto keep = [&](int buf) {
     if (wave == 0) {
       float* st = stats(buf);
-      st[lane] = n_lse == NEG_INF ? -NEG_INF : n_lse;  // a row without a key: P = 0
+      st[lane] = n_last < 0 ? -NEG_INF : n_lse;  // a row without a key: P = 0
       st[BN + lane] = n_delta;
       reinterpret_cast<int*>(st)[2 * BN + lane] = n_last;
     }

@@ -720,6 +720,7 @@ int bc2n_headnorm_bwd(void* stream, int dtype, int64_t tokens, int heads, int kv
  *   out = P v,  lse f32 [heads][q_tokens] = log sum e^S.
  *   - A query that sees no key has out 0, lse -inf and no gradient, whatever it
  *     and its cotangent hold.
+ *   - A query whose scores are all -inf has out and gradients NaN, lse -inf.
  *   - Tokens of no sequence (before the first, behind the last, past a
  *     length) may hold anything.  Their rows of the results are zeros (lse
  *     -inf) where `fill` is set and left as they were where it is not.
