@@ -711,9 +711,17 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
 // through memory.
 // W = 4, few keys: all of a sequence's by one workgroup, every fourth block a
 // wave, joined in LDS: no second launch.
+// Calls of more entries than a wave holds: sums over the entries before each, and
+// over all, made once a call and searched 64 at a time.  (Each wave adding up all
+// entries for each of its items: 5000 sequences of one query and four keys, 32 heads
+// over 8 of 128, 1408 us, 20 000 of 64 keys 16.8 ms.)
+struct Table {
+  int64_t *per, *items, *splits, *slots;  // [1], [entries + 1] each
+};
 struct Split {
   float* o;    // [slot][32 rows][DP], sums of exponents times values
   float2* ml;  // [slot][32]: reference in log 2, sum of exponents
+  Table table;  // of more entries than a wave holds, else null
 };
 // keys of a block: 16 KB of keys and values at the widths 64 and 128
 __host__ __device__ constexpr int block_keys(int DP) { return DP == 128 ? 32 : 64; }
@@ -728,16 +736,15 @@ struct Item {
 };
 // An entry (sequence, or the tokens outside) as one lane sees it.
 struct Entry {
-  Seq seq;
   int tiles, blocks;
 };
 template <int KN>
 __device__ __forceinline__ Entry entry_of(const PackedAttn& a, int e, int G) {
-  Entry r = {};
+  Entry r = {0, 0};
   if (e >= a.sequences + 2) return r;
-  r.seq = sequence(a, e, false);
-  r.tiles = (int)(((int64_t)(a.fill ? r.seq.have : r.seq.lq) * G + 31) / 32);
-  r.blocks = r.seq.lq > 0 ? (r.seq.lk + KN - 1) / KN : 0;
+  const Seq seq = sequence(a, e, false);
+  r.tiles = (int)(((int64_t)(a.fill ? seq.have : seq.lq) * G + 31) / 32);
+  r.blocks = seq.lq > 0 ? (seq.lk + KN - 1) / KN : 0;
   return r;
 }
 __device__ __forceinline__ int64_t wave_sum64(int64_t v) {
@@ -755,18 +762,97 @@ __device__ __forceinline__ int64_t wave_before(int64_t v, int lane) {
   }
   return run - v;
 }
-// The wave's view of all sequences: what the first 64 HELD entries come to stays
-// in its lanes, more are read again at each search.
+// Blocks of a stretch.  work: of all tiles; all: how many tiles there are.
 template <int KN>
+__device__ __forceinline__ int stretch_of(int64_t work, int64_t all, int64_t goal) {
+  // every tile may end in a short stretch: with those too one round of waves
+  // (64 sequences of 11 .. 8192 keys, 8 heads of 128: 70.5 -> 62 us)
+  if (all < goal / 2) goal -= all;
+  return (int)max((int64_t)(SHORTEST / KN), (work + goal - 1) / goal);
+}
+// Of an entry: items, tiles of more than one stretch, and those tiles' stretches.
+struct Counts {
+  int64_t items, splits, slots;
+};
+__device__ __forceinline__ Counts counts_of(int tiles, int parts) {
+  Counts c;
+  c.items = (int64_t)tiles * parts;
+  c.splits = parts > 1 ? tiles : 0;
+  c.slots = parts > 1 ? c.items : 0;
+  return c;
+}
+template <int KN>
+__global__ __launch_bounds__(1024) void packattn_table_kernel(PackedAttn a, int64_t goal, Table table) {
+  __shared__ int64_t sums[3][16];
+  const int G = a.heads / a.kv_heads, entries = a.sequences + 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // v of the threads before this one, and of all
+  auto scan = [&](int64_t v, int64_t* waves, int64_t& total) __attribute__((always_inline)) {
+    const int64_t before = wave_before(v, lane);
+    if (lane == 63) waves[wave] = before + v;
+    __syncthreads();
+    int64_t own = before;
+    total = 0;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      if (i < wave) own += waves[i];
+      total += waves[i];
+    }
+    return own;
+  };
+  int64_t work = 0, all = 0, of_items, of_splits, of_slots;
+  for (int e = threadIdx.x; e < entries; e += 1024) {
+    const Entry x = entry_of<KN>(a, e, G);
+    work += (int64_t)x.tiles * x.blocks;
+    all += x.tiles;
+  }
+  scan(work, sums[0], of_items);
+  scan(all, sums[1], of_splits);
+  const int per = stretch_of<KN>(of_items, of_splits, goal);
+  if (threadIdx.x == 0) *table.per = per;
+  Counts run = {};
+  for (int e0 = 0; e0 < entries; e0 += 1024) {
+    const int e = e0 + threadIdx.x;
+    const Entry x = entry_of<KN>(a, e, G);
+    const Counts c = counts_of(x.tiles, max(1, (x.blocks + per - 1) / per));
+    __syncthreads();  // the sums before have been read
+    const int64_t items = run.items + scan(c.items, sums[0], of_items);
+    const int64_t splits = run.splits + scan(c.splits, sums[1], of_splits);
+    const int64_t slots = run.slots + scan(c.slots, sums[2], of_slots);
+    if (e <= entries) {
+      table.items[e] = items;
+      table.splits[e] = splits;
+      table.slots[e] = slots;
+    }
+    run.items += of_items;
+    run.splits += of_splits;
+    run.slots += of_slots;
+  }
+  if (threadIdx.x == 0) {
+    table.items[entries] = run.items;
+    table.splits[entries] = run.splits;
+    table.slots[entries] = run.slots;
+  }
+}
+
+// The wave's view of all sequences: what up to 64 HELD entries come to lies in its
+// lanes, more (TABLE) in the call's table.
+constexpr int HELD = 4;
+template <int KN, bool TABLE>
 struct Stretches {
-  static constexpr int HELD = 4;
   int tiles[HELD], blocks[HELD];  // of entry 64 i + lane
   int per, G, lane, entries;
+  Table table;
 
-  __device__ __forceinline__ void init(const PackedAttn& a, int G_, int64_t goal) {
+  __device__ __forceinline__ void init(const PackedAttn& a, int G_, int64_t goal, const Table& t) {
     G = G_;
     lane = threadIdx.x & 63;
     entries = a.sequences + 2;
+    if constexpr (TABLE) {
+      table = t;
+      per = uniform((int)*table.per);
+      return;
+    }
     int64_t work = 0, all = 0;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
@@ -776,71 +862,97 @@ struct Stretches {
       work += (int64_t)x.tiles * x.blocks;
       all += x.tiles;
     }
-    for (int e = 64 * HELD + lane; e - lane < entries; e += 64) {
-      const Entry x = entry_of<KN>(a, e, G);
-      work += (int64_t)x.tiles * x.blocks;
-      all += x.tiles;
-    }
-    work = wave_sum64(work);
-    all = wave_sum64(all);
-    // every tile may end in a short stretch: with those too one round of waves
-    // (64 sequences of 11 .. 8192 keys, 8 heads of 128: 70.5 -> 62 us)
-    if (all < goal / 2) goal -= all;
-    per = uniform((int)max((int64_t)(SHORTEST / KN), (work + goal - 1) / goal));
+    per = uniform(stretch_of<KN>(wave_sum64(work), wave_sum64(all), goal));
+  }
+  __device__ __forceinline__ int parts_of(int blocks_) const { return max(1, (blocks_ + per - 1) / per); }
+  // tile or stretch y of entry e, whose stretches' slots begin at `slots`
+  template <bool SPLIT>
+  __device__ __forceinline__ void item(const PackedAttn& a, int e, int parts, int64_t y, int64_t slots, Item& r) const {
+    r.seq = lane_seq(sequence(a, e, false), 0);
+    r.parts = parts;
+    r.tile = uniform((int)(SPLIT ? y : y / parts));
+    r.part = SPLIT ? 0 : uniform((int)(y % parts));
+    r.slot = slots + (int64_t)r.tile * parts;
+    r.per = per;
   }
   // Item x of all (SPLIT: tile x of those with more stretches than one);
   // false past the last.
   template <bool SPLIT>
   __device__ __forceinline__ bool find(const PackedAttn& a, int64_t x, Item& r) const {
+    if constexpr (TABLE) {
+      const int64_t* from = SPLIT ? table.splits : table.items;
+      if (x >= from[entries]) return false;
+      int lo = 0, count = entries;  // the last entry that begins at x or before it
+      while (count > 1) {
+        const int step = (count + 63) / 64, i = lane * step;
+        const bool below = i < count && from[lo + min(i, count - 1)] <= x;
+        const int passed = max(__popcll(__ballot(below)) - 1, 0) * step;
+        lo += passed;
+        count = min(step, count - passed);
+      }
+      lo = uniform(lo);
+      const Entry m = entry_of<KN>(a, lo, G);
+      item<SPLIT>(a, lo, uniform(parts_of(m.blocks)), uniform64(x - from[lo]), uniform64(table.slots[lo]), r);
+      return true;
+    }
     int64_t slots = 0;
-    auto look = [&](int e0, int tiles_, int blocks_) {
-      const int parts = max(1, (blocks_ + per - 1) / per);
-      const int64_t n = SPLIT ? (parts > 1 ? tiles_ : 0) : (int64_t)tiles_ * parts;
-      const int64_t before = wave_before(n, lane), s = parts > 1 ? (int64_t)tiles_ * parts : 0;
+    auto look = [&](int i) {
+      const int parts = parts_of(blocks[i]);
+      const Counts c = counts_of(tiles[i], parts);
+      const int64_t n = SPLIT ? c.splits : c.items, before = wave_before(n, lane);
       const unsigned long long at = __ballot(before <= x && x < before + n);
       if (at) {
         const int l = uniform(__ffsll(at) - 1);
-        const int64_t y = x - lane64(before, l);
-        r.seq = lane_seq(sequence(a, e0 + l, false), 0);
-        r.parts = __builtin_amdgcn_readlane(parts, l);
-        r.tile = uniform((int)(SPLIT ? y : y / r.parts));
-        r.part = SPLIT ? 0 : uniform((int)(y % r.parts));
-        r.slot = slots + lane64(wave_before(s, lane), l) + (int64_t)r.tile * r.parts;
-        r.per = per;
+        item<SPLIT>(a, 64 * i + l, __builtin_amdgcn_readlane(parts, l), x - lane64(before, l),
+                    slots + lane64(wave_before(c.slots, lane), l), r);
         return true;
       }
       x -= wave_sum64(n);
-      slots += wave_sum64(s);
+      slots += wave_sum64(c.slots);
       return false;
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-      if (64 * i < entries && look(64 * i, tiles[i], blocks[i])) return true;
-    for (int e0 = 64 * HELD; e0 < entries; e0 += 64) {
-      const Entry m = entry_of<KN>(a, e0 + lane, G);
-      if (look(e0, m.tiles, m.blocks)) return true;
-    }
+      if (64 * i < entries && look(i)) return true;
     return false;
   }
 };
 
-template <class T, int DP, int W>
+template <class T, int DP, int W, bool TABLE>
 __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, int64_t goal, Split split) {
+  // goal: of equal stretches a head of keys; W = 4: tiles of 32 rows
   constexpr int KN = block_keys(DP), KS = DP / 16, DB = DP / 32, TILE = KN * DP * 2, LD = DP + 4;
   constexpr int JOIN = W > 1 ? W * 32 * (LD * 4 + 8) : 0;
   constexpr int LDS = W * 2 * TILE > JOIN ? W * 2 * TILE : JOIN;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[LDS];
   const int G = a.heads / a.kv_heads, lane = threadIdx.x & 63, h = lane >> 5;
   const int wave = W > 1 ? uniform(threadIdx.x >> 6) : 0;
-  Stretches<KN> all;
-  all.init(a, G, goal);
+  Stretches<KN, TABLE> all;
+  if (W == 1) all.init(a, G, goal, split.table);
+  // W = 4: every entry's keys whole, its tiles by their numbers
+  auto tile_of = [&](int64_t x, Item& r) __attribute__((always_inline)) {
+    int s;
+    const int64_t t = find_tile(a.q_off, a.sequences, a.q_tokens, G, 32, x, s);
+    r.seq = lane_seq(sequence(a, s, false), 0);
+    r.tile = (int)t;
+    r.part = 0;
+    r.parts = 1;
+    r.per = (r.seq.lk + KN - 1) / KN;
+    return t >= 0 && t * 32 < (int64_t)(a.fill ? r.seq.have : r.seq.lq) * G;
+  };
   const unsigned kb = lds_addr(smem) + wave * 2 * TILE, vb = kb + TILE;
   Operands<DP> ops;
   ops.init(kb, lane);
   const float c = a.scale * LOG2E;
   typedef KeyTiles<T, DP, KN, 1> Tiles;
   Item it;
-  for (int64_t x = blockIdx.x; all.template find<false>(a, x / a.kv_heads, it); x += gridDim.x) {
+  for (int64_t x = blockIdx.x;; x += gridDim.x) {
+    if constexpr (W > 1) {
+      if (x >= goal * a.kv_heads) break;
+      if (!tile_of(x / a.kv_heads, it)) continue;
+    } else {
+      if (!all.template find<false>(a, x / a.kv_heads, it)) break;
+    }
     const int kv = uniform((int)(x % a.kv_heads));
     const Seq& seq = it.seq;
     const Row row = row_of(a, seq, it.tile * 32 + (lane & 31), G);
@@ -947,14 +1059,14 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
 // with a reference of its own.  Bound by its launch and one round of loads: 10 us
 // beside 56 of the stretches (64 sequences of 11 .. 8192 keys), 12 beside 30 (one of
 // 131 k).
-template <class T, int DP, int RW>
+template <class T, int DP, int RW, bool TABLE>
 __global__ __launch_bounds__(RW > 1 ? 64 * RW : NT) void packattn_join_kernel(PackedAttn a, int64_t goal, Split split) {
   constexpr int KN = block_keys(DP), LP = DP / 4, ROWS = RW > 1 ? 1 : WAVES, GROUPS = 64 * RW / LP;
   __shared__ float so[ROWS][RW][DP];
   __shared__ float2 sml[ROWS][RW];
   const int G = a.heads / a.kv_heads;
-  Stretches<KN> all;
-  all.init(a, G, goal);
+  Stretches<KN, TABLE> all;
+  all.init(a, G, goal, split.table);
   const int mine = threadIdx.x / (64 * RW), t = threadIdx.x % (64 * RW);
   const int group = t / LP, e = t % LP * 4;
   Item it;
@@ -1663,6 +1775,15 @@ Split carve_split(const PackedAttn& a, char* p, size_t* bytes) {
   z.take<float>(rows * padded(a.width));
   s.ml = reinterpret_cast<float2*>(p + z.off);
   z.take<float2>(rows);
+  s.table = Table{};
+  const size_t entries = (size_t)a.sequences + 2;
+  if (entries > 64 * HELD) {
+    int64_t** at[] = {&s.table.per, &s.table.items, &s.table.splits, &s.table.slots};
+    for (int64_t** x : at) {
+      *x = reinterpret_cast<int64_t*>(p + z.off);
+      z.take<int64_t>(x == &s.table.per ? 1 : entries + 1);
+    }
+  }
   *bytes = z.off;
   return s;
 }
@@ -1737,7 +1858,7 @@ void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
     const int64_t tiles = tiles_of(a.q_tokens, G, 32, a.sequences);
     if (!may_split(a)) {
       const int64_t items = std::min(tiles * a.kv_heads, 4 * (int64_t)device_cus());
-      packattn_keys_kernel<T, DP, 4><<<(unsigned)items, 256, 0, st>>>(a, 1, Split{});
+      packattn_keys_kernel<T, DP, 4, false><<<(unsigned)items, 256, 0, st>>>(a, tiles, Split{});
       return;
     }
     size_t bytes = 0;
@@ -1745,18 +1866,27 @@ void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
     const int64_t goal = few_goal(a);
     // items: a tile's first stretch each, and the further ones
     const int64_t items = (tiles + goal) * a.kv_heads;
-    packattn_keys_kernel<T, DP, 1><<<(unsigned)std::min(items, few_grid(a)), 64, 0, st>>>(a, goal, split);
     // a row's share of the waves, and of the stretches, were all sequences alike
     const int64_t rows = a.q_tokens * G, live = std::max<int64_t>(1, std::min<int64_t>(a.sequences, a.q_tokens));
     const int64_t x = std::min(live + rows / 32, goal) * a.kv_heads;
     const int64_t y = std::min<int64_t>(32, (rows + live - 1) / live);
-    // 16 waves a row where it has some 32 stretches (one sequence of 131 k, 8 rows a
-    // head of keys: 12 us), one where it has fewer (7974 rows of three heads, two or
-    // three stretches each: 592 us of 16 waves, 41 of one)
-    if (goal >= 32 * std::max(live, rows / 32))
-      packattn_join_kernel<T, DP, 16><<<dim3((unsigned)x, (unsigned)y), 1024, 0, st>>>(a, goal, split);
-    else
-      packattn_join_kernel<T, DP, 1><<<dim3((unsigned)x, (unsigned)(y + 3) / 4), NT, 0, st>>>(a, goal, split);
+    auto launch = [&](auto table) {
+      constexpr bool TABLE = decltype(table)::value;
+      packattn_keys_kernel<T, DP, 1, TABLE><<<(unsigned)std::min(items, few_grid(a)), 64, 0, st>>>(a, goal, split);
+      // 16 waves a row where it has some 32 stretches (one sequence of 131 k, 8 rows a
+      // head of keys: 12 us), one where it has fewer (7974 rows of three heads, two or
+      // three stretches each: 592 us of 16 waves, 41 of one)
+      if (goal >= 32 * std::max(live, rows / 32))
+        packattn_join_kernel<T, DP, 16, TABLE><<<dim3((unsigned)x, (unsigned)y), 1024, 0, st>>>(a, goal, split);
+      else
+        packattn_join_kernel<T, DP, 1, TABLE><<<dim3((unsigned)x, (unsigned)(y + 3) / 4), NT, 0, st>>>(a, goal, split);
+    };
+    if (!split.table.per) {
+      launch(std::false_type());
+      return;
+    }
+    packattn_table_kernel<block_keys(DP)><<<1, 1024, 0, st>>>(a, goal, split.table);
+    launch(std::true_type());
   });
 }
 
