@@ -67,3 +67,14 @@ def test_no_key_is_another_matter(cuda, dtype):
     assert (out[:30] == 0).all() and (lse[:, :30] == -math.inf).all() and out[30:].isfinite().all()
     d_q, d_k, d_v = op.backward(g, q, k, v, out, lse, qo, ko)
     assert (d_q[:30] == 0).all() and all(t.isfinite().all() for t in (d_q, d_k, d_v))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_no_key_beside_scores_of_minus_infinity_in_stretches(cuda, dtype):
+    """6001 queries of 5000 keys, which are joined from stretches: 1001 rows see none, the
+    next 300 see keys of -infinity alone."""
+    q, k, v, g, (qo, ko) = problem(6001, 5000, 2, 2, 40, dtype)
+    k[:300, :, 0] = -math.inf
+    out, lse = ops.PackedAttention().forward(q, k, v, qo, ko)
+    assert (out[:1001] == 0).all() and (lse[:, :1301] == -math.inf).all()
+    assert out[1001:1301].isnan().all() and out[1301:].isfinite().all() and lse[:, 1301:].isfinite().all()
