@@ -69,6 +69,7 @@ struct Half<h16> {
   // normal numbers.
   static constexpr float SHIFT = 7.f;
   static constexpr bool SCALED = true;  // dS needs a scale (below)
+  static constexpr uint32_t EXPONENT = 0x7c00;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a),
                                                   __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
@@ -79,6 +80,7 @@ struct Half<bf16> {
   typedef bf16 V2 __attribute__((ext_vector_type(2)));
   static constexpr float SHIFT = 0.f;
   static constexpr bool SCALED = false;
+  static constexpr uint32_t EXPONENT = 0x7f80;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -395,6 +397,58 @@ struct Operands {
   }
 };
 
+// Infinities and NaN ("others") in masked places.  A tile's products multiply what a row
+// does not see by a weight of 0, which makes 0 of a number but NaN of others.  So
+// where some rows see less than a tile others in it are wiped, 0 in their place in
+// LDS, and what they make of the rows that see them is made apart.  The forward and dq
+// of 128 rows, whose sums tell whether there were any, look at those and go over
+// their tiles once more if so; a few rows' blocks, of which one or two are cut, are
+// wiped at once; dk and dv wipe rows whose lse or D tells of others.  Packed prompts
+// without any: forward 368 -> 372 us, with the gradient 1135 -> 1150.  (Cut tiles
+// wiped at once in the forward of 128 rows: 380.)
+//
+// The finite ones of two 16-bit numbers, 0 in the place of others
+template <class T>
+__device__ __forceinline__ uint32_t finite2(uint32_t v) {
+  constexpr uint32_t E = Half<T>::EXPONENT;
+  return ((v & E) == E ? 0 : v & 0xffff) | ((v >> 16 & E) == E ? 0 : v & 0xffff0000u);
+}
+// Wipes chunk `chunk` (16 bytes) of a tile at `lds`; whether there was something to wipe
+template <class T>
+__device__ __forceinline__ bool wipe(unsigned lds, int chunk) {
+  typedef __attribute__((address_space(3))) u32x4 lds_chunk;
+  const u32x4 v = *(lds_u32x4*)(lds + chunk * 16);
+  u32x4 w;
+  bool other = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = finite2<T>(v[i]);
+    other |= w[i] != v[i];
+  }
+  if (other) *(lds_chunk*)(lds + chunk * 16) = w;
+  return other;
+}
+template <int DB>
+__device__ __forceinline__ bool has_others(const f32x16 (&o)[DB]) {
+  float t[4] = {};
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i % 4] = fmaf(o[db][i], 0.f, t[i % 4]);
+  return !(t[0] + t[1] + t[2] + t[3] == 0.f);
+}
+// Whether a wave of the workgroup says so; `word`: 4 bytes of LDS a wave, for this alone
+constexpr int WORDS = 32;  // bytes of them
+template <int W>
+__device__ __forceinline__ bool any_wave(bool mine, int* word, int wave) {
+  if ((threadIdx.x & 63) == 0) word[wave] = mine;
+  __syncthreads();
+  int r = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) r |= word[i];
+  return uniform(r) != 0;
+}
+
 // 8 elements from element e of a head's row, zeros past the width
 template <class T>
 __device__ __forceinline__ u32x4 load8(const T* row, int e, int width) {
@@ -523,6 +577,31 @@ struct KeyTiles {
   }
 };
 
+// What the values of keys from .. to - 1 that are infinities or NaN make of the outputs
+// of a lane's row, whose last key is `last`: its weights are positive.
+template <class T, int DB>
+__device__ __forceinline__ void add_others(const PackedAttn& a, const Seq& s, int head, int from, int to, int last,
+                                           f32x16 (&o)[DB], int lane) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll 1
+  for (int key = from; key < to; ++key) {
+    const T* v = row_ptr<const T>(a.v, s.k0 + key, head) + 4 * (lane >> 5);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (32 * db + 8 * i >= a.width) continue;
+        const t4 x = *global_ptr<const t4>(v + 32 * db + 8 * i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float y = (float)x[k];
+          if (!(fabsf(y) < __builtin_inff()) && key <= last) o[db][4 * i + k] += y;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // in few registers
+      }
+  }
+}
+
 // ------------------------------------------------------------------ forward
 // A wave's 32 rows over tiles of 32 NB keys: outputs, sums and exponents'
 // references of a lane's row.
@@ -532,9 +611,12 @@ struct Online {
   f32x16 o[DB];
   float ref, mc, sum;  // mc: ref times c; sum: of a lane's own keys
 
-  __device__ __forceinline__ void init() {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+  }
+  __device__ __forceinline__ void init() {
+    clear();
     ref = NEG_INF;
     mc = sum = 0.f;
   }
@@ -662,17 +744,20 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
   for (int ks = 0; ks < KS; ++ks) q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
   const float c = a.scale * LOG2E;
   Online<T, DP, 2> st;
-  st.init();
   const unsigned lds0 = lds_addr(smem);
   KeyTiles<T, DP, BN, WAVES> tile;
-  tile.init(a, seq, at.head, 0, BN, wave, lane);
-  if (nk > 0) tile.both(lds0);
-
   Operands<DP> x;
   x.init(lds0, lane);
+  // the first key that not all rows see, once others have to be wiped from there on
+  int wiped = 0x7fffffff;
   auto step = [&](int kt, unsigned here, unsigned next) __attribute__((always_inline)) {
     const int k0 = kt * BN;
     wait_all_and_sync();
+    if (k0 + BN > wiped) {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < TILE / 16; i += NT) wipe<T>(lds0 + here + TILE, i);
+      __syncthreads();
+    }
     if (kt + 1 < nk) tile.both(lds0 + next);
     if (k0 > most) return;
     f32x16 p[2];
@@ -680,14 +765,29 @@ __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64
     st.weights(p, c, row.last - k0 - 4 * h, k0 + BN - 1 > least);
     st.values(p, c, x, here + TILE);
   };
-  for (int kt = 0; kt < nk; kt += 2) {  // the two buffers at constant places
-    step(kt, 0, 2 * TILE);
-    if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
+  for (;;) {
+    st.init();
+    tile.init(a, seq, at.head, 0, BN, wave, lane);
+    if (nk > 0) tile.both(lds0);
+    for (int kt = 0; kt < nk; kt += 2) {  // the two buffers at constant places
+      step(kt, 0, 2 * TILE);
+      if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
+    }
+    if (!a.causal) break;
+    if (wiped < 0x7fffffff) {
+      add_others<T>(a, seq, at.head, wiped / BN * BN, most + 1, row.last, st.o, lane);
+      break;
+    }
+    // others in a row that does not see all of its wave's last tile
+    const bool others = row.last >= 0 && row.last < min(most / BN * BN + BN, seq.lk) - 1 && has_others(st.o);
+    if (!any_wave<WAVES>(__any(others), reinterpret_cast<int*>(smem + 4 * TILE), wave)) break;
+    wiped = uniform(row_of(a, seq, r0, G).last) + 1;
   }
   const float sum = other_half_sum(st.sum);
   // A row that sees keys has a sum of 0 where all its scores are -infinity: its
   // softmax is NaN, as 0 / 0 here, and its lse log 0.
   const bool none = row.last < 0;
+  if (none) st.clear();
   store_columns<T, DB>(st.o, none ? 0.f : 1.f / sum,
                        row.stored ? row_ptr<T>(a.o, token, head) : nullptr, a.width, lane);
   if (row.stored && h == 0)
@@ -964,6 +1064,10 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
     const T* qrow = row_ptr<const T>(a.q, token, head);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[ks] = load8(qrow, 16 * ks + 8 * h, a.width);
+    // The first key that not all rows see.  Few blocks have one (those of single tokens
+    // none), and are wiped at once.
+    const int sure = a.causal ? uniform(row_of(a, seq, it.tile * 32, G).last) + 1 : seq.lk;
+    bool dirty = false;
     Online<T, DP, KN / 32> st;
     st.init();
     Tiles tile;
@@ -982,10 +1086,19 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
       st.weights(p, c, row.last - b * KN - 4 * h, b * KN + KN - 1 > least);
       if (more) wait_copies<Tiles::C::PER>();
       else wait_copies<0>();
+      if (min(b * KN + KN, seq.lk) > sure) {
+#pragma unroll 1
+        for (int i = lane; i < TILE / 16; i += 64) dirty |= wipe<T>(vb, i);
+        wait_reads();
+      }
       st.values(p, c, ops, TILE);
       wait_reads();
       if (more) tile.values(vb);
     }
+    if (__any(dirty))
+      for (b = b0 + wave; b < b1; b += W)
+        if (min(b * KN + KN, seq.lk) > sure)
+          add_others<T>(a, seq, kv, b * KN, min(b * KN + KN, most + 1), row.last, st.o, lane);
     const float sum = other_half_sum(st.sum);
     if constexpr (W > 1) {
       // the waves' sums of a row, relative to the largest reference
@@ -1018,7 +1131,7 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
         l += v.y * f[w];
       }
       const bool none = mine.last < 0;
-      const float inv = none ? 0.f : 1.f / l;
+      const float inv = 1.f / l;
       if (mine.stored) {
         for (int e = part * 8; e < a.width; e += PER_ROW * 8) {
           float v[8] = {};
@@ -1027,7 +1140,7 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = fmaf(so[(w * 32 + r) * LD + e + i], f[w], v[i]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= inv;
+          for (int i = 0; i < 8; ++i) v[i] = none ? 0.f : v[i] * inv;
           Vec<T>::store(row_ptr<T>(a.o, my_token, my_head) + e, Vec<T>::pack(v));
         }
         if (part == 0)
@@ -1037,6 +1150,7 @@ __global__ __launch_bounds__(64 * W, 2) void packattn_keys_kernel(PackedAttn a, 
       __syncthreads();
     } else if (it.parts == 1) {
       const bool none = row.last < 0;
+      if (none) st.clear();
       store_columns<T, DB>(st.o, none ? 0.f : 1.f / sum,
                            row.stored ? row_ptr<T>(a.o, token, head) : nullptr, a.width, lane);
       if (row.stored && h == 0)
@@ -1135,9 +1249,9 @@ __global__ __launch_bounds__(RW > 1 ? 64 * RW : NT) void packattn_join_kernel(Pa
       }
       if (t < LP && row.stored) {
         const bool none = blind && sum == 0.f;
-        const float inv = none ? 0.f : 1.f / sum;
+        const float inv = 1.f / sum;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] *= inv;
+        for (int k = 0; k < 4; ++k) v[k] = none ? 0.f : v[k] * inv;
         const float w[4] = {v[0], v[1], v[2], v[3]};
         if (e < a.width) Few<T, 4>::template store<false>(row_ptr<T>(a.o, it.seq.q0 + row.i, kv * G + row.g) + e, w);
         if (t == 0)
@@ -1284,8 +1398,6 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   if (row.last < 0) lse = -NEG_INF;  // a row without a key: P = 0
   const float c = a.scale * LOG2E;
   f32x16 o[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db) o[db] = f32x16{};
   const unsigned lds0 = lds_addr(smem);
   // what was loaded above is here before the first copy is issued
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1324,11 +1436,22 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
   }
   if (row.last < 0) D = 0.f;  // no gradient, whatever do holds
   if (row.stored && row.i < seq.lq && h == 0 && part == 0) back.delta[at_row] = D;
-  tile.init(a, seq, at.head, kt0 * BN, BN, wave, lane);
-  if (kt0 < nk) tile.both(lds0);
+  // The first key that not all rows see, once others have to be wiped from there on;
+  // marks: NaN for keys that had some, whose scores are NaN then where they are seen.
+  int wiped = 0x7fffffff;
+  float* marks = reinterpret_cast<float*>(smem + 4 * TILE + WORDS);  // [BN]
   auto step = [&](int kt, unsigned here, unsigned next) __attribute__((always_inline)) {
     const int k0 = kt * BN;
     wait_all_and_sync();
+    const bool wiping = k0 + BN > wiped;
+    if (wiping) {
+      if (threadIdx.x < BN) marks[threadIdx.x] = 0.f;
+      __syncthreads();
+#pragma unroll 1
+      for (int i = threadIdx.x; i < TILE / 16; i += NT)
+        if (wipe<T>(lds0 + here, i)) marks[i / (DP / 8)] = __builtin_nanf("");
+      __syncthreads();
+    }
     if (kt + 1 < nk) tile.both(lds0 + next);
     if (k0 > most) return;
 #pragma unroll
@@ -1352,6 +1475,10 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
           order<LDS_READ, 1>();
         }
         order<MFMA, AHEAD>();
+      }
+      if (wiping) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] += marks[32 * b + 8 * (i / 4) + 4 * h + i % 4];
       }
       const int last = row.last - k0 - 4 * h;
       if (k0 + 32 * b + 31 > least) {  // a dP of NaN in a masked place stays there
@@ -1389,9 +1516,19 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
       order<MFMA, DB>();
     }
   };
-  for (int kt = kt0; kt < nk; kt += 2) {
-    step(kt, 0, 2 * TILE);
-    if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
+  for (;;) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+    tile.init(a, seq, at.head, kt0 * BN, BN, wave, lane);
+    if (kt0 < nk) tile.both(lds0);
+    for (int kt = kt0; kt < nk; kt += 2) {
+      step(kt, 0, 2 * TILE);
+      if (kt + 1 < nk) step(kt + 1, 2 * TILE, 0);
+    }
+    if (!a.causal || wiped < 0x7fffffff) break;
+    const bool others = row.last >= 0 && row.last < min(most / BN * BN + BN, seq.lk) - 1 && has_others(o);
+    if (!any_wave<WAVES>(__any(others), reinterpret_cast<int*>(smem + 4 * TILE), wave)) break;
+    wiped = uniform(row_of(a, seq, r0, G).last) + 1;
   }
   if (row.last < 0) {
 #pragma unroll
@@ -1447,7 +1584,7 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
     const float g = largest(back.gmax + at.head * back.g_tiles + wave0 + from / 32, (rows - from + 31) / 32);
     const float v = largest(back.vmax + at.head * back.v_tiles + seq.k0 / NORM_KEYS + s,
                             rows > from ? (seq.lk + NORM_KEYS - 1) / NORM_KEYS : 0);
-    ds = ds_scale(g, v);
+    ds = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, ds_scale(g, v))));
   }
   // P is made 2^SHIFT times as large in binary16
   constexpr float SHIFT = 2 * Half<T>::SHIFT;
@@ -1468,6 +1605,7 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
   const float c = a.scale * LOG2E;
 
+  int* others = reinterpret_cast<int*>(smem + 2 * BUF + 8 * OPERANDS);  // of a tile's rows, by buffer
   auto stats = [&](int buf) { return reinterpret_cast<float*>(smem + buf * BUF + 2 * TILE); };
   // Where 64 rows are whole tokens, the next tile's lie as this one's, so many
   // tokens on; elsewhere each tile divides its rows anew.
@@ -1537,6 +1675,9 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
       st[lane] = n_last < 0 ? -NEG_INF : n_lse;  // a row without a key: P = 0
       st[BN + lane] = n_delta;
       reinterpret_cast<int*>(st)[2 * BN + lane] = n_last;
+      // a row of others in q or do has an lse or a D of them
+      const bool other = n_last >= 0 && !(fabsf(n_delta) < -NEG_INF && n_lse == n_lse);
+      if (a.causal) others[buf] = __any(other);
     }
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1549,6 +1690,14 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   auto step = [&](int r0, auto buf_) __attribute__((always_inline)) {
     constexpr int buf = decltype(buf_)::value;
     wait_all_and_sync();
+    // Where some rows of the tile do not see all keys: others in rows that have any are
+    // wiped, and P and dS of such a row are NaN where it sees.
+    if (a.causal && r0 / G + lag < j0 + BK - 1 && uniform(others[buf])) {
+#pragma unroll 1
+      for (int i = 64 * wave + lane; i < 2 * TILE / 16; i += 2 * NT)
+        if (wipe<T>(lds0 + buf * BUF, i)) stats(buf)[i % (TILE / 16) / (DP / 8)] = __builtin_nanf("");
+      __syncthreads();
+    }
     if (r0 + BN < rows) issue(r0 + BN, buf ^ 1);
     const int mine = r0 + 32 * half;  // the wave's rows of the tile
     // its last row sees the most keys, its first the fewest
@@ -1590,15 +1739,15 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
         lse[x] = *(lds_f32x4*)at_row;
         D[x] = *(lds_f32x4*)(at_row + BN * 4);
       }
-      if (cut) {  // a dP of NaN in a masked place stays there
+      if (cut) {  // what a row holds that does not see the key stays there: P = dS = 0
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const u32x4 last = *(lds_u32x4*)(sb + (8 * x + 4 * h) * 4 + 2 * BN * 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (j > (int)last[i]) {
-              p[4 * x + i] = NEG_INF;
-              d[4 * x + i] = 0.f;
+              p[4 * x + i] = d[4 * x + i] = D[x][i] = 0.f;
+              lse[x][i] = -NEG_INF;
             }
         }
       }
@@ -1855,7 +2004,7 @@ void packattn_fwd(hipStream_t st, const PackedAttn& a, void* work) {
     if (!few_rows(a)) {
       const int64_t tiles = tiles_of(a.q_tokens, G, 32 * WAVES, a.sequences);
       auto* kernel = &packattn_fwd_kernel<T, DP>;
-      const size_t lds = 4 * BN * DP * 2;
+      const size_t lds = 4 * BN * DP * 2 + WORDS;
       with_lds(kernel, lds);
       kernel<<<place_grid(a.kv_heads, tiles), NT, lds, st>>>(a, tiles);
       return;
@@ -1914,13 +2063,13 @@ void packattn_bwd(hipStream_t st, const PackedAttn& a, void* work) {
     }
     if (a.q_tokens) {
       auto* dq = &packattn_dq_kernel<T, DP>;
-      const size_t lds = 4 * BN * DP * 2;
+      const size_t lds = 4 * BN * DP * 2 + WORDS + BN * 4;
       with_lds(dq, lds);
       dq<<<dim3(place_grid(a.kv_heads, q_tiles), back.q_parts), NT, lds, st>>>(a, q_tiles, back);
     }
     if (a.k_tokens) {
       auto* dkv = &packattn_dkv_kernel<T, DP>;
-      const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4) + 2 * 32 * WAVES * DP * 2;
+      const size_t lds = 2 * (2 * BN * DP * 2 + 3 * BN * 4) + 2 * 32 * WAVES * DP * 2 + WORDS;
       with_lds(dkv, lds);
       dkv<<<dim3(place_grid(a.kv_heads, k_tiles), back.k_parts), 2 * NT, lds, st>>>(a, k_tiles, back);
     }

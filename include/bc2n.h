@@ -724,10 +724,10 @@ int bc2n_headnorm_bwd(void* stream, int dtype, int64_t tokens, int heads, int kv
  *   - Tokens of no sequence (before the first, behind the last, past a
  *     length) may hold anything.  Their rows of the results are zeros (lse
  *     -inf) where `fill` is set and left as they were where it is not.
- *   - A NaN or an infinity in a key reaches the rows that see it; in a value
- *     of a causal sequence it may also reach rows up to 63 tokens before it, as
- *     0 * NaN in a product of tiles, and so may one in a key, a query or a
- *     cotangent reach gradients up to 127 tokens from those it belongs to.
+ *   - A NaN or an infinity in a key or a value reaches the queries that see it and
+ *     no others, one in a query or its cotangent the gradients of the keys that it
+ *     sees.  A row of a gradient that it reaches may be NaN as a whole where the
+ *     formula has an infinity or a number.
  * Products take the operands as they are, accumulate in f32 and round P and
  * its cotangent to the operands' type; maxima, sums and lse are f32, added in an
  * order that goes by the shapes and lengths alone.  In binary16 the
