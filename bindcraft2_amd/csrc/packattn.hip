@@ -403,9 +403,10 @@ struct Operands {
 // LDS, and what they make of the rows that see them is made apart.  The forward and dq
 // of 128 rows, whose sums tell whether there were any, look at those and go over
 // their tiles once more if so; a few rows' blocks, of which one or two are cut, are
-// wiped at once; dk and dv wipe rows whose lse or D tells of others.  Packed prompts
-// without any: forward 368 -> 372 us, with the gradient 1135 -> 1150.  (Cut tiles
-// wiped at once in the forward of 128 rows: 380.)
+// wiped at once; dk and dv wipe rows whose lse or D tells of others.  Without any, on
+// packed prompts, that costs the forward 1% (371 -> 375 us), dq 1%, dk and dv what a
+// third division a tile did (below).  (Cut tiles wiped at once in the forward of 128
+// rows: 4%.)
 //
 // The finite ones of two 16-bit numbers, 0 in the place of others
 template <class T>
@@ -1687,12 +1688,17 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
   }
   Operands<DP> ops;
   ops.init(lds0 + half * (32 * DP * 2), lane);
+  // the first rows that see the first of the wave's keys, all of them, all of the workgroup's
+  // (a division by G a tile for each comparison: 478 us, with a third one 488, so 469)
+  const int some = j0 + 32 * group < seq.lk ? first_row(a.causal, j0 + 32 * group, seq.lq, seq.lk, G) : 0x7fffffff;
+  const int every = first_row(a.causal, j0 + 32 * group + 31, seq.lq, seq.lk, G);
+  const int whole = first_row(a.causal, j0 + BK - 1, seq.lq, seq.lk, G);
   auto step = [&](int r0, auto buf_) __attribute__((always_inline)) {
     constexpr int buf = decltype(buf_)::value;
     wait_all_and_sync();
     // Where some rows of the tile do not see all keys: others in rows that have any are
     // wiped, and P and dS of such a row are NaN where it sees.
-    if (a.causal && r0 / G + lag < j0 + BK - 1 && uniform(others[buf])) {
+    if (r0 < whole && uniform(others[buf])) {
 #pragma unroll 1
       for (int i = 64 * wave + lane; i < 2 * TILE / 16; i += 2 * NT)
         if (wipe<T>(lds0 + buf * BUF, i)) stats(buf)[i % (TILE / 16) / (DP / 8)] = __builtin_nanf("");
@@ -1700,11 +1706,10 @@ __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, i
     }
     if (r0 + BN < rows) issue(r0 + BN, buf ^ 1);
     const int mine = r0 + 32 * half;  // the wave's rows of the tile
-    // its last row sees the most keys, its first the fewest
-    const bool any = mine < rows && (!a.causal || (mine + 31) / G + lag >= j0 + 32 * group);
+    const bool any = mine < rows && mine + 31 >= some;
     if (any) {
       const unsigned sb = lds0 + buf * BUF + 2 * TILE + 128 * half;
-      const bool cut = a.causal && mine / G + lag < j0 + 32 * group + 31;
+      const bool cut = mine < every;
       constexpr unsigned qb = buf * BUF, gb = qb + TILE;
       f32x16 p = {}, d = {};
       {

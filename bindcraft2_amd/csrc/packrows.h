@@ -5,6 +5,13 @@
 
 namespace bc2n {
 
+// The first row that sees key j, or the last key for one past it.  (Compared with a row
+// this needs no division by the group's heads for each.)
+__host__ __device__ constexpr int first_row(bool causal, int j, int lq, int lk, int G) {
+  const int i = (j < lk ? j : lk - 1) - (lk - lq);  // below lq
+  return causal && i > 0 ? i * G : 0;
+}
+
 struct KeyRows {
   int all = 0;    // the sequence's rows
   int first = 0;  // the first that sees a key from j0 on, down to a multiple of the tile
@@ -18,7 +25,7 @@ __host__ __device__ constexpr KeyRows rows_of_keys(bool causal, int j0, int lq, 
   r.all = lq * G;
   if (!causal) return r;
   const int lag = lk - lq;  // query i sees keys up to i + lag
-  r.first = (j0 > lag ? j0 - lag : 0) * G / tile * tile;
+  r.first = first_row(causal, j0, lq, lk, G) / tile * tile;
   r.blind = (lag < 0 ? -lag : 0) * G;
   return r;
 }

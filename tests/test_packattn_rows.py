@@ -26,6 +26,7 @@ constexpr bool counted(bool causal, int lq, int lk, int G, int capacity) {
       if (last >= j0) first = row;
       if (last < 0) ++blind;
     }
+    if (first_row(causal, j0, lq, lk, G) != first) return false;
     if (r.all != lq * G || r.blind != blind || r.first % TILE || r.first > first || r.first + TILE <= first)
       return false;
     for (int parts = 1; parts < 6; ++parts) {
@@ -54,6 +55,10 @@ constexpr bool fits(bool causal, int G, int lq, int lk, int capacity) {
     const int j0 = (j < 0 ? 0 : j) / 128 * 128;
     const KeyRows r = rows_of_keys(causal, j0, lq, lk, G, TILE);
     if (r.first < 0 || r.first > r.all + TILE || r.blind < 0) return false;
+    for (int on : {0, 31, 127}) {
+      const int x = first_row(causal, j0 + on, lq, lk, G);
+      if (x < 0 || x > lq * G) return false;
+    }
     for (int parts : {1, 2, 7, 64})
       for (int p = 0; p < parts; ++p) {
         const Part x = part_of_rows(r, parts, p, TILE);
