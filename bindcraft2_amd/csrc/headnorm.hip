@@ -13,7 +13,7 @@
 // Every element is read once and written once (the gradient reads two), some
 // ten operations each, so memory bounds it: 16-byte loads, a head in the
 // registers of a few lanes, and the angles, which all heads of a token share,
-// made once for all of them.  16384 tokens of 40 heads of 128 bfloat16: 75 us, 4.5
+// made once for all of them.  16384 tokens of 40 heads of 128 bfloat16: 76 us, 4.4
 // TB/s (when it took 98: vectors of 8 bytes 114, stores past the caches 111); the
 // gradient of 8191 tokens of 20 heads of 64 f32 25 us, 5.0 TB/s, and 4 of its join.
 //
@@ -86,9 +86,11 @@ __device__ __forceinline__ Unit unit_of(const HeadNorm& p, int u) {
   return r;
 }
 
-// cos and sin of position * freq.  The product is taken in 64 bits (exact for
-// positions below 2^29; one of 10^6 would lose a tenth of a radian in 32), in
-// turns, and whole turns leave there; the rest is good to 2^-26 of one.  Then
+// cos and sin of position * freq.  The product is taken in 64 bits (at a position of
+// 10^6 one of 32 would lose a tenth of a radian), in turns: the frequency in turns and
+// its product with the position round to 53 bits each, 2^-52 of the turns with the
+// constant's own rounding.  Whole turns leave there; the rest, in f32, is good to 2^-26
+// of one.  Then
 // quarters of a turn, and the series of both for an eighth at most, which end
 // below 2^-29 (a library call for both, with its own reductions, takes twice the
 // instructions).

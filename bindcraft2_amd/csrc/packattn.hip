@@ -25,6 +25,12 @@
 // the other operand, a column of the row-major tile in LDS, is read in the same
 // order with two ds_read_b64_tr_b16.
 //
+// P and dS are rounded to the operands' type, which the second products' instructions
+// take: half a step of a term, as the result's own rounding is of the sum.  Outputs of
+// prompts are 2.1e-3 off 64 bits with it, 1.6e-3 with their own rounding alone, gradients
+// 2.4e-3 and 1.7e-3 (bfloat16; binary16 an eighth); P and dS as two halves each would
+// double those products.  Scores, maxima, sums, lse, D and all sums of products are f32.
+//
 // Tiles are copied global -> LDS directly through buffer descriptors whose
 // bounds turn what lies past a sequence or past the width into zeros.  A copy
 // fills LDS in lane order, so the source address carries the swizzle (fswz)
@@ -711,9 +717,9 @@ struct Online {
 //
 // Products and exponentials bound it: two workgroups a unit, one's products beside
 // the other's exponentials.  11 causal sequences of 16384 tokens, 32 heads over 8
-// of 128, bfloat16: 370 us, 835 TFLOP/s of what is seen, two thirds of what a
+// of 128, bfloat16: 373 us, 828 TFLOP/s of what is seen, two thirds of what a
 // large library product reaches; with the operands read as they are needed
-// instead of up to eight ahead (the order below) 393.
+// instead of up to eight ahead (the order below) 6% more.
 template <class T, int DP>
 __global__ __launch_bounds__(NT, 2) void packattn_fwd_kernel(PackedAttn a, int64_t tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -1339,8 +1345,9 @@ constexpr int FEW_KEYS = 1024;
 // dq, and D = sum (do o) of every row for the other kernel.  The forward's layout
 // with a product more, and as it bound by products and exponentials.  The scores
 // are made in both kernels, so that neither adds to memory in an order of
-// chance: nine products for seven.  6 causal sequences of 10007 tokens, 32 heads
-// over 8 of 128, bfloat16: this 320 us (340 without the order of reads), the other 490.
+// chance: nine products for seven, and for rows of up to 1024 keys eleven (below).
+// 6 causal sequences of 10007 tokens, 32 heads over 8 of 128, bfloat16: this 371 us
+// (the order of reads saved 6%), the other 469.
 template <class T, int DP>
 __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_t tiles, Back back) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -1552,7 +1559,7 @@ __global__ __launch_bounds__(NT, 2) void packattn_dq_kernel(PackedAttn a, int64_
 // the matrix cores wait for each exponential, leave no room for the keys' and
 // values' operands beside them: those are read from LDS, in operand order (one
 // wave a SIMD with them in registers 960 us, two 672, with the reads ahead of
-// their products and the heaviest tiles first 490).
+// their products and the heaviest tiles first 478, without divisions a tile 469).
 template <class T, int DP>
 __global__ __launch_bounds__(2 * NT, 2) void packattn_dkv_kernel(PackedAttn a, int64_t tiles, Back back) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
