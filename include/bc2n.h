@@ -664,7 +664,8 @@ int bc2n_logprobs_grad(void* stream, int dtype, const void* logits, int64_t ld, 
  * q [tokens][heads][width] and k [tokens][kv_heads][width] of BC2N_F32,
  * BC2N_F16 or BC2N_BF16, each with a token stride and a head stride in
  * elements (slices of one projection, or heads first; of one token or one head
- * any), a head's elements contiguous; either may have 0 heads.  With x a head's row and w its weight
+ * any), a head's elements contiguous; either may have 0 heads.  Below 2^26
+ * tokens, 2^16 heads at most.  With x a head's row and w its weight
  * [width] (BC2N_F32 or the operands' type):
  *   y = x (mean x^2 + eps)^-1/2 w
  * and the pairs of its first `rotated` elements -- (i, i + rotated / 2), or
@@ -764,8 +765,9 @@ int bc2n_attention_bwd(void* stream, int dtype, int causal, int sequences, int64
  * A class a row of logits by a given uniform number (next to the
  * log-probabilities: acids for designed positions, the next token of running
  * sequences).  No reference counterpart.
- * logits [rows][classes] of BC2N_F32, BC2N_F16 or BC2N_BF16, row stride ld;
- * uniforms f32 [rows] in [0, 1) (others are taken to the nearer end).  The
+ * logits [rows][classes] of BC2N_F32, BC2N_F16 or BC2N_BF16, row stride ld, below
+ * 2^31 rows and 2^28 classes at most; uniforms f32 [rows] in [0, 1) (others are
+ * taken to the nearer end).  The
  * settings are one value for all rows, or f32 (top_ks i32) [rows] on the device
  * where the array is not NULL.  With m the row's maximum, classes ranked by
  * logit, ties to the lowest index, and e = exp((x - m) / temperature):
